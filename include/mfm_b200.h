@@ -44,6 +44,9 @@ extern "C" {
  * keeps float64 parameters for the whole fit in F32_F64, as the reference
  * does (python/modern_fm/_backend.py:116-130). */
 enum { MFM_DTYPE_F64 = 0, MFM_DTYPE_F32 = 1, MFM_DTYPE_F32_F64 = 2 };
+/* Storage types of the embedding and preference entry points only (float32
+ * arithmetic, results rounded once); every other entry point rejects them. */
+enum { MFM_DTYPE_BF16 = 3, MFM_DTYPE_F16 = 4 };
 enum { MFM_MODEL_FM = 0, MFM_MODEL_FFM = 1, MFM_MODEL_FWFM = 2 };
 enum { MFM_LOSS_LOGISTIC = 0, MFM_LOSS_SQUARED = 1 };
 enum { MFM_OPT_SGD = 0, MFM_OPT_ADAGRAD = 1, MFM_OPT_ADAM = 2, MFM_OPT_FTRL = 3 };
@@ -416,6 +419,123 @@ int mfm_fit_csr_dp(mfm_dp* dp, int dtype, int model, int64_t n_classes, const mf
                    const double* y, const int64_t* ycls, const double* sample_weight,
                    const int64_t* field_ids, int64_t n_fields, const mfm_train* tr, int64_t k,
                    mfm_group* w0, mfm_group* w, mfm_group* v, mfm_group* r);
+
+/* ---- latent rows as outputs: embedding lookup and its gradient -------------
+ * No reference counterpart (its latent rows never leave the kernels that score
+ * with them). Every array is DEVICE memory on `device`; calls run on `stream`
+ * (a cudaStream_t), allocate nothing, do not synchronise, and may be captured.
+ *
+ * n_entries ids (int32, or int64 with ids64 = 1) select rows of a table
+ * (n_rows, d) with row pitch ld_table elements. An id outside [0, n_rows) is
+ * padding: a zero row, no gradient. `scale` (one value per entry, NULL = 1) and
+ * alpha multiply the rows. With indptr = NULL entry t is output row t
+ * (n_out = n_entries); otherwise output row b is the sum over the entries
+ * [indptr[b], indptr[b+1]) (int64, n_out + 1, non-decreasing; bounds are
+ * limited to [0, n_entries], and entries of no row count as padding).
+ *
+ * dtype: MFM_DTYPE_F64, _F32, _BF16, _F16: table, output rows and gradient
+ * rows of that type, scale float64 for F64 and float32 otherwise, sums in
+ * float64 / float32. MFM_DTYPE_F32_F64: float32 table, everything else and the
+ * arithmetic float64. Sums have a fixed order: results are bitwise
+ * reproducible. n_entries, n_out, n_rows and d < 2^31; their products are not
+ * limited. out must not overlap the inputs. */
+
+/* out[t] = alpha scale[t] table[ids[t]], or its row sums; out (n_out, d) with
+ * row pitch ld_out. */
+int mfm_embedding_lookup_device(int dtype, int device, int ids64, const void* ids,
+                                int64_t n_entries, const int64_t* indptr, int64_t n_out,
+                                const void* scale, double alpha, const void* table,
+                                int64_t n_rows, int64_t d, int64_t ld_table, void* out,
+                                int64_t ld_out, void* stream);
+
+/* Gradient of the lookup by sorted ids, grad (n_out, d) with row pitch ld_grad:
+ *   d_table[i] = alpha sum over entries t with ids[t] = i of scale[t] grad[row(t)]
+ *   d_scale[t] = alpha <grad[row(t)], table[ids[t]]>   (0 for padding)
+ * Exactly one of two results:
+ *   d_table (n_rows, d) contiguous: every row written (keys, rows, count NULL);
+ *   keys (the id type), rows (d wide, contiguous), count (int64): the touched
+ *     ids in ascending order and their rows, in arrays of min(n_entries,
+ *     n_rows) places; *count of them are used, keys are -1 and rows 0 behind
+ *     them (d_table NULL).
+ * Their element type is out_dtype: the gradient's type (MFM_DTYPE_F64 for
+ * F32_F64), or MFM_DTYPE_F32 for BF16 / F16. d_scale (n_entries, the scale
+ * type) is written when it and `table` are given. `workspace` (256-byte
+ * aligned) holds at least mfm_embedding_grad_workspace_bytes(...) bytes; a call
+ * owns it until its work on the stream is done. */
+int64_t mfm_embedding_grad_workspace_bytes(int dtype, int64_t n_entries, int64_t n_rows,
+                                           int64_t d);
+int mfm_embedding_grad_device(int dtype, int out_dtype, int device, int ids64, const void* ids,
+                              int64_t n_entries, const int64_t* indptr, int64_t n_out,
+                              const void* scale, double alpha, const void* grad,
+                              int64_t ld_grad, const void* table, int64_t ld_table,
+                              int64_t n_rows, int64_t d, void* d_table, void* keys, void* rows,
+                              int64_t* count, void* d_scale, void* workspace,
+                              int64_t workspace_bytes, void* stream);
+
+/* ---- losses of class scores by label log-probabilities ---------------------
+ * No reference counterpart (its softmax loss exists only inside fit). Every
+ * array is DEVICE memory on `device`; calls run on `stream`, allocate nothing,
+ * do not synchronise, and may be captured.
+ *
+ * logits (n_tokens, n_classes), row pitch ld elements, of type dtype
+ * (MFM_DTYPE_F64, _F32, _BF16, _F16): one row of class scores per token, e.g.
+ * the C logits per row of mfm_model_predict_device. labels: int32, or int64 with
+ * labels64 = 1; a label outside [0, n_classes) masks its token
+ * (log-probability 0, gradient 0), and so does a row whose every score is
+ * -infinity. Everything else is in the arithmetic type: float64 for F64, else
+ * float32. Sums over tokens and pairs run in float64 in a fixed order. */
+
+/* logprobs[t] = logits[t, labels[t]] - lse[t], lse[t] = log sum exp logits[t]
+ * (written for masked tokens too). sums (n_seq; NULL = not wanted): the sum of
+ * logprobs over tokens [indptr[s], indptr[s+1]) (int64, n_seq + 1, limited to
+ * [0, n_tokens]). */
+int mfm_label_logprobs_device(int dtype, int device, const void* logits, int64_t ld,
+                              int64_t n_tokens, int64_t n_classes, int labels64,
+                              const void* labels, const int64_t* indptr, int64_t n_seq,
+                              void* logprobs, void* lse, void* sums, void* stream);
+
+/* d_logits[t, c] = grad[t] ([c = labels[t]] - exp(logits[t, c] - lse[t])), of the
+ * logits' type, row pitch ld_out; must not overlap logits. */
+int mfm_label_logprobs_grad_device(int dtype, int device, const void* logits, int64_t ld,
+                                   int64_t n_tokens, int64_t n_classes, int labels64,
+                                   const void* labels, const void* grad, const void* lse,
+                                   void* d_logits, int64_t ld_out, void* stream);
+
+/* Paired preference loss. 2 n_pairs sequences of tokens by indptr: sequence p is
+ * the preferred one of pair p, sequence n_pairs + p the other. With S the
+ * sequences' summed log-probabilities and R = reference (2 n_pairs):
+ *   z[p] = beta ((S[p] - R[p]) - (S[n_pairs + p] - R[n_pairs + p]))
+ *   loss = sum w[p] (-(1 - e) log sigmoid(z[p]) - e log sigmoid(-z[p])) / sum w[p]
+ * with e = label_smoothing and w = sample_weight (NULL = 1). Pairs of weight 0
+ * are left out; weights that sum to 0 give loss and gradient 0. Writes loss (1), margins z (n_pairs), seq_logprobs
+ * S (2 n_pairs) and, unless NULL, d_logits (as above; tokens of no sequence get
+ * 0). workspace: mfm_preference_workspace_bytes(...) bytes, 256-byte aligned. */
+int64_t mfm_preference_workspace_bytes(int dtype, int64_t n_tokens, int64_t n_pairs);
+int mfm_preference_loss_device(int dtype, int device, const void* logits, int64_t ld,
+                               int64_t n_tokens, int64_t n_classes, int labels64,
+                               const void* labels, const int64_t* indptr, int64_t n_pairs,
+                               const void* reference, double beta, double label_smoothing,
+                               const void* sample_weight, void* loss, void* margins,
+                               void* seq_logprobs, void* d_logits, int64_t ld_out,
+                               void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Clipped policy loss with a KL term. Per token, with lp its log-probability,
+ * r = exp(lp - old_logprobs) and u = reference - lp:
+ *   l = -min(r A, clamp(r, 1 - clip_low, 1 + clip_high) A) + kl_coef (exp(u) - u - 1)
+ * with A = advantages (reference NULL: no KL term). loss = sum w l / sum w over the
+ * unmasked tokens, w = sample_weight (NULL = 1); tokens of weight 0 are left out,
+ * and weights that sum to 0 give 0.
+ * stats (3): the loss, the mean of exp(u) - u - 1, and the share of tokens whose
+ * clipped term is the smaller one. Writes logprobs (n_tokens) and, unless NULL,
+ * d_logits. workspace: mfm_policy_workspace_bytes(...) bytes, 256-byte aligned. */
+int64_t mfm_policy_workspace_bytes(int dtype, int64_t n_tokens);
+int mfm_policy_loss_device(int dtype, int device, const void* logits, int64_t ld,
+                           int64_t n_tokens, int64_t n_classes, int labels64,
+                           const void* labels, const void* old_logprobs,
+                           const void* advantages, const void* reference, double clip_low,
+                           double clip_high, double kl_coef, const void* sample_weight,
+                           void* stats, void* logprobs, void* d_logits, int64_t ld_out,
+                           void* workspace, int64_t workspace_bytes, void* stream);
 
 /* Device time (seconds, CUDA events) of the calling thread's last fit, by
  * phase: out[0] uploads and setup, out[1] the epochs' plans (sorts), out[2]

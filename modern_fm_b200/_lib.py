@@ -16,6 +16,7 @@ LIB_PATH = os.path.join(PKG, "libmfm_b200.so")
 MFM_OK = 0
 MFM_ERR_INVALID, MFM_ERR_UNSUPPORTED = -1, -2
 MFM_DTYPE_F64, MFM_DTYPE_F32, MFM_DTYPE_F32_F64 = 0, 1, 2
+MFM_DTYPE_BF16, MFM_DTYPE_F16 = 3, 4  # embedding and preference entry points only
 MFM_MODEL_FM, MFM_MODEL_FFM, MFM_MODEL_FWFM = 0, 1, 2
 DTYPES = {"float64": MFM_DTYPE_F64, "f64": MFM_DTYPE_F64, "float32": MFM_DTYPE_F32,
           "f32": MFM_DTYPE_F32, "float32-float64": MFM_DTYPE_F32_F64,
@@ -128,6 +129,32 @@ _SIGNATURES = {
     "mfm_libffm_info": (ct.c_int, [ct.c_void_p, i64p, i64p, i64p]),
     "mfm_libffm_arrays": (ct.c_int, [ct.c_void_p] + [ct.POINTER(ct.c_void_p)] * 5),
     "mfm_libffm_free": (None, [ct.c_void_p]),
+    "mfm_embedding_lookup_device": (ct.c_int, [
+        ct.c_int, ct.c_int, ct.c_int, ct.c_void_p, ct.c_int64, ct.c_void_p, ct.c_int64,
+        ct.c_void_p, ct.c_double, ct.c_void_p, ct.c_int64, ct.c_int64, ct.c_int64, ct.c_void_p,
+        ct.c_int64, ct.c_void_p]),
+    "mfm_embedding_grad_workspace_bytes": (ct.c_int64, [ct.c_int] + [ct.c_int64] * 3),
+    "mfm_embedding_grad_device": (ct.c_int, [
+        ct.c_int, ct.c_int, ct.c_int, ct.c_int, ct.c_void_p, ct.c_int64, ct.c_void_p, ct.c_int64,
+        ct.c_void_p, ct.c_double, ct.c_void_p, ct.c_int64, ct.c_void_p, ct.c_int64, ct.c_int64,
+        ct.c_int64, ct.c_void_p, ct.c_void_p, ct.c_void_p, ct.c_void_p, ct.c_void_p, ct.c_void_p,
+        ct.c_int64, ct.c_void_p]),
+    "mfm_label_logprobs_device": (ct.c_int, [
+        ct.c_int, ct.c_int, ct.c_void_p, ct.c_int64, ct.c_int64, ct.c_int64, ct.c_int, ct.c_void_p,
+        ct.c_void_p, ct.c_int64, ct.c_void_p, ct.c_void_p, ct.c_void_p, ct.c_void_p]),
+    "mfm_label_logprobs_grad_device": (ct.c_int, [
+        ct.c_int, ct.c_int, ct.c_void_p, ct.c_int64, ct.c_int64, ct.c_int64, ct.c_int, ct.c_void_p,
+        ct.c_void_p, ct.c_void_p, ct.c_void_p, ct.c_int64, ct.c_void_p]),
+    "mfm_preference_workspace_bytes": (ct.c_int64, [ct.c_int, ct.c_int64, ct.c_int64]),
+    "mfm_preference_loss_device": (ct.c_int, [
+        ct.c_int, ct.c_int, ct.c_void_p, ct.c_int64, ct.c_int64, ct.c_int64, ct.c_int, ct.c_void_p,
+        ct.c_void_p, ct.c_int64, ct.c_void_p, ct.c_double, ct.c_double, ct.c_void_p, ct.c_void_p,
+        ct.c_void_p, ct.c_void_p, ct.c_void_p, ct.c_int64, ct.c_void_p, ct.c_int64, ct.c_void_p]),
+    "mfm_policy_workspace_bytes": (ct.c_int64, [ct.c_int, ct.c_int64]),
+    "mfm_policy_loss_device": (ct.c_int, [
+        ct.c_int, ct.c_int, ct.c_void_p, ct.c_int64, ct.c_int64, ct.c_int64, ct.c_int, ct.c_void_p,
+        ct.c_void_p, ct.c_void_p, ct.c_void_p, ct.c_double, ct.c_double, ct.c_double, ct.c_void_p,
+        ct.c_void_p, ct.c_void_p, ct.c_void_p, ct.c_int64, ct.c_void_p, ct.c_int64, ct.c_void_p]),
     "mfm_fm_predict_device": (ct.c_int, [ct.c_int, ct.c_int, ct.c_void_p, ct.c_void_p,
                                          ct.c_void_p, ct.c_int64, ct.c_double, ct.c_void_p,
                                          ct.c_void_p, ct.c_int64, ct.c_void_p, ct.c_void_p]),
