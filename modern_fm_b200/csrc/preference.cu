@@ -4,6 +4,18 @@
 //
 // Per token row x of C scores with label y: lse = m + log sum exp(x - m), m = max x;
 // lp = x[y] - lse; a loss with derivative g in lp has d/dx[c] = g ([c = y] - exp(x[c] - lse)).
+//
+// All of it is a stream over the scores: bound by HBM where the rows are read
+// and written once (policy, forward, gradient), with one or two exponentials per
+// value (16 a clock and SM) close behind for 16-bit scores. Rows are worked on
+// in three ways:
+//  * up to kSmallC classes: a thread per row, rows staged through shared memory
+//    so that global accesses are whole vectors (small_rows_kernel);
+//  * rows of up to 4 KB: a warp holds the whole row in registers (at most eight
+//    16-byte vectors a lane), so it is read once for the maximum, the sum and the
+//    gradient (cached_rows_kernel);
+//  * longer rows: persistent blocks stream rows through a ring in shared memory
+//    that bulk copies fill ahead of the work (ring_rows_kernel).
 #include "vecio.cuh"
 
 #include <algorithm>
@@ -12,171 +24,908 @@ namespace mfm {
 namespace {
 
 constexpr int kNT = 256;
+constexpr int kSmallC = 32;
+constexpr int kSmallNT = 128;
+constexpr int kSmallPerSm = 8;  // blocks of 64 registers a thread
 
+// exp(d): the 32-bit form is one multiply and ex2 (2^-22 of the value), exact at 0.
 __device__ __forceinline__ float exp_of(float d) {
     float r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d * 1.4426950408889634f));
     return r;
 }
-__device__ __forceinline__ double exp_of(double d) { return exp(d); }
+// a call: its code is long, and unrolled loops hold many
+__device__ __noinline__ double exp_call(double d) { return exp(d); }
+__device__ __forceinline__ double exp_of(double d) { return exp_call(d); }
 __device__ __forceinline__ float log_of(float v) { return logf(v); }
 __device__ __forceinline__ double log_of(double v) { return log(v); }
+__device__ __forceinline__ float quotient(float a, float b) { return __fdividef(a, b); }  // 2 ulp
+__device__ __forceinline__ double quotient(double a, double b) { return a / b; }
+
+// sum + exp(v - off) over N values, and k exp(v - off) for each: two 32-bit lanes an
+// instruction (the f32x2 forms round each lane as the scalar ones do), since
+// 16-bit scores are otherwise bound by issue slots, not by bytes.
+__device__ __forceinline__ uint64_t pair_of(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void pair_to(uint64_t r, float& a, float& b) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(r));
+}
+__device__ __forceinline__ uint64_t pair_add(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t pair_mul(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t pair_exp(float a, float b, uint64_t minus_off) {
+    const uint64_t d = pair_mul(pair_add(pair_of(a, b), minus_off), pair_of(1.4426950408889634f, 1.4426950408889634f));
+    float p, q;
+    pair_to(d, p, q);
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(p) : "f"(p));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(q) : "f"(q));
+    return pair_of(p, q);
+}
+// Adds N values' exponentials to `acc`, a pair of partial sums.
+template <int N>
+__device__ __forceinline__ void add_exp(uint64_t& acc, const float (&v)[N], uint64_t minus_off) {
+#pragma unroll
+    for (int q = 0; q < N; q += 2) acc = pair_add(acc, pair_exp(v[q], v[q + 1], minus_off));
+}
+template <int N>
+__device__ __forceinline__ void scaled_exp(float (&v)[N], float k, uint64_t minus_off) {
+    const uint64_t kk = pair_of(k, k);
+#pragma unroll
+    for (int q = 0; q < N; q += 2) pair_to(pair_mul(pair_exp(v[q], v[q + 1], minus_off), kk), v[q], v[q + 1]);
+}
+template <class A>
+struct ExpSum {  // running sum of exp(v - off)
+    uint64_t acc = 0, moff;
+    __device__ __forceinline__ explicit ExpSum(float off) : moff(pair_of(-off, -off)) {}
+    template <int N>
+    __device__ __forceinline__ void add(const float (&v)[N]) { add_exp(acc, v, moff); }
+    __device__ __forceinline__ float sum() const {
+        float a, b;
+        pair_to(acc, a, b);
+        return a + b;
+    }
+    template <int N>
+    __device__ __forceinline__ void scaled(float (&v)[N], float k) const { scaled_exp(v, k, moff); }
+};
+template <>
+struct ExpSum<double> {
+    double acc = 0.0, off;
+    __device__ __forceinline__ explicit ExpSum(double o) : off(o) {}
+    template <int N>
+    __device__ __forceinline__ void add(const double (&v)[N]) {
+#pragma unroll
+        for (int q = 0; q < N; ++q) acc += exp_of(v[q] - off);
+    }
+    __device__ __forceinline__ double sum() const { return acc; }
+    template <int N>
+    __device__ __forceinline__ void scaled(double (&v)[N], double k) const {
+#pragma unroll
+        for (int q = 0; q < N; ++q) v[q] = k * exp_of(v[q] - off);
+    }
+};
 
 template <class A>
 __device__ __forceinline__ A minus_inf() { return (A)(-INFINITY); }
 
-// A running maximum m and s = sum of exp(x - m); m = -inf stands for an offset of 0
-// so that rows of -inf stay 0 and NaN stays NaN.
-template <class A>
-struct Softmax {
-    A m = minus_inf<A>(), s = A(0);
-    __device__ __forceinline__ A off() const { return m == minus_inf<A>() ? A(0) : m; }
-    template <int N>
-    __device__ __forceinline__ void add(const A (&x)[N]) {
-        A top = m;
-#pragma unroll
-        for (int j = 0; j < N; ++j) top = fmax(top, x[j]);
-        if (top > m) {
-            s *= exp_of(m - top);
-            m = top;
-        }
-        const A o = off();
-#pragma unroll
-        for (int j = 0; j < N; ++j) s += exp_of(x[j] - o);
+// Labels are int32 or int64 (one load per row: no type of its own in the kernels).
+struct Labels {
+    const void* p;
+    int is64;
+    // the label of token t, -1 for one outside [0, c)
+    __device__ __forceinline__ int in(int64_t t, int64_t c) const {
+        const int64_t y = is64 ? static_cast<const int64_t*>(p)[t] : (int64_t)static_cast<const int32_t*>(p)[t];
+        return y >= 0 && y < c ? (int)y : -1;
     }
-    __device__ __forceinline__ void join(A m2, A s2) {
-        const A top = fmax(m, m2);
-        if (top == minus_inf<A>()) {
-            s += s2;
+};
+
+// The offset subtracted before exp: the maximum, or 0 for a row of -inf, so that
+// such rows sum to 0 and NaN stays NaN.
+template <class A>
+__device__ __forceinline__ A offset_of(A m) { return m == minus_inf<A>() ? A(0) : m; }
+
+template <class A>
+struct RowStats {
+    A m, s;  // maximum, sum of exp(x - offset_of(m))
+};
+
+// The statistics of `width` neighbouring lanes joined, on each of them.
+template <class A>
+__device__ __forceinline__ void across(RowStats<A>& r, int width) {
+    const A was = r.m;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1)
+        if (o < width) r.m = fmax(r.m, __shfl_xor_sync(0xffffffffu, r.m, o));
+    if (r.m != minus_inf<A>()) r.s *= exp_of(was - r.m);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1)
+        if (o < width) r.s += __shfl_xor_sync(0xffffffffu, r.s, o);
+}
+
+template <class A, class Op>
+__device__ __forceinline__ A warp_reduce(A v, Op op) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v = op(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return v;
+}
+
+// What a row's loss needs, in global memory; which pointers are set goes by the mode.
+enum Mode { STATS, POLICY, GRAD };
+
+template <class A>
+struct RowArgs {
+    Labels labels;
+    int64_t n, c;
+    A* lp;
+    // STATS
+    A* lse;
+    A* zero;            // cleared per token, or NULL
+    unsigned* counter;  // cleared by the first block, or NULL
+    // POLICY
+    const A *old, *adv, *ref, *weight;
+    A clip_lo, clip_hi, kl_coef;  // ratio bounds
+    const double* wpart;          // partial sums of the weights
+    int n_wpart;
+    double* part;  // three sums per block
+    A* stats;
+    unsigned* done;  // blocks finished
+    // GRAD
+    const A *g, *lse_in;
+    const double* scale;  // factor of every g, NULL = 1
+    __device__ __forceinline__ A factor(int64_t t, int y, A l) const {
+        if (y < 0 || l == minus_inf<A>()) return A(0);
+        return scale ? (A)((double)g[t] * *scale) : g[t];
+    }
+};
+
+// em1 = exp(u) - 1 and kl = exp(u) - u - 1. Near 0 both by the series of kl, where the
+// differences would lose what is left: to u^8 / 8! below 1/4 in 32 bits (what is cut
+// off is 2^-33 of kl), to u^13 / 13! below 1/8 in 64 bits (2^-66).
+__device__ __forceinline__ void kl_terms(float u, float& em1, float& kl) {
+    if (fabsf(u) < 0.25f) {
+        float r = 1.0f / 40320;
+        r = r * u + 1.0f / 5040;
+        r = r * u + 1.0f / 720;
+        r = r * u + 1.0f / 120;
+        r = r * u + 1.0f / 24;
+        r = r * u + 1.0f / 6;
+        r = r * u + 0.5f;
+        kl = r * u * u;
+        em1 = u + kl;
+    } else {
+        em1 = exp_of(u) - 1.0f;
+        kl = em1 - u;
+    }
+}
+constexpr double inverse_factorial(int i) { return i < 2 ? 1.0 : inverse_factorial(i - 1) / i; }
+__device__ __forceinline__ void kl_terms(double u, double& em1, double& kl) {
+    em1 = expm1(u);
+    kl = em1 - u;
+    if (fabs(u) < 0.125) {
+        double r = 0.0;
+#pragma unroll
+        for (int i = 13; i >= 2; --i) r = r * u + inverse_factorial(i);
+        kl = r * u * u;
+    }
+}
+
+// A token's own inputs, loaded ahead of its row's statistics.
+template <class A>
+struct Token {
+    A w = A(0), adv = A(0), old = A(0), ref = A(0);
+    __device__ __forceinline__ void load(const RowArgs<A>& a, int64_t t) {
+        w = a.weight ? a.weight[t] : A(1);
+        adv = a.adv[t];
+        old = a.old[t];
+        if (a.ref) ref = a.ref[t];
+    }
+};
+
+// A token's derivative g, and its weighted loss terms e.
+template <class A>
+__device__ __forceinline__ A policy_terms(const RowArgs<A>& a, const Token<A>& k, A lp, bool live,
+                                          A inv_total, A (&e)[3]) {
+    e[0] = e[1] = e[2] = A(0);
+    // masked, or a token of weight 0: left out, whatever its ratio
+    if (!live || k.w == A(0)) return A(0);
+    const A ratio = exp_of(lp - k.old);
+    const A bent = fmin(fmax(ratio, a.clip_lo), a.clip_hi);
+    const bool cut = ratio * k.adv > bent * k.adv;
+    A slope = cut ? A(0) : -ratio * k.adv, kl = A(0);
+    if (a.ref) {
+        A em1;
+        kl_terms(k.ref - lp, em1, kl);
+        slope -= a.kl_coef * em1;
+    }
+    e[0] = k.w * (a.kl_coef * kl - (cut ? bent : ratio) * k.adv);
+    e[1] = k.w * kl;
+    e[2] = cut ? k.w : A(0);
+    return k.w * slope * inv_total;
+}
+
+// Sum over the block in a fixed order, on every thread.
+__device__ __forceinline__ double block_sum(double v, double* sm) {
+    v = warp_sum(v);
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) sm[threadIdx.x / 32] = v;
+    __syncthreads();
+    double t = 0.0;
+    for (int w = 0; w < (int)blockDim.x / 32; ++w) t += sm[w];
+    return t;
+}
+
+template <class A>
+__device__ __forceinline__ double weight_total(const RowArgs<A>& a) {  // on every lane
+    double total = 0.0;
+    for (int i = threadIdx.x & 31; i < a.n_wpart; i += 32) total += a.wpart[i];
+    return warp_sum(total);
+}
+
+// 1 / the sum of the weights; weights that sum to 0 give gradient 0.
+__device__ __forceinline__ double inverse(double total) { return total != 0.0 ? 1.0 / total : 0.0; }
+
+// The block's three sums to `part`; the block that finishes last adds all of
+// them, in block order, into the results.
+template <class A>
+__device__ __forceinline__ void policy_finish(const RowArgs<A>& a, const double (&e)[3],
+                                              double total, double* sm) {
+    __shared__ unsigned last;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < 3; ++i) a.part[3 * (int64_t)blockIdx.x + i] = e[i];
+        __threadfence();
+        last = atomicAdd(a.done, 1u) == gridDim.x - 1 ? 1u : 0u;
+    }
+    __syncthreads();
+    if (!last) return;
+    __threadfence();
+    for (int i = 0; i < 3; ++i) {
+        double v = 0.0;
+        for (int64_t b = threadIdx.x; b < gridDim.x; b += blockDim.x) v += __ldcg(a.part + 3 * b + i);
+        v = block_sum(v, sm);
+        if (threadIdx.x == 0) a.stats[i] = total != 0.0 ? (A)(v / total) : A(0);
+    }
+}
+
+// ------------------------------------------------------------ few classes --
+
+__device__ __forceinline__ uint4 load16(const void* p) { return *static_cast<const uint4*>(p); }
+
+// A warp works on tiles of 32 rows, a thread per row, and copies the next tile into
+// shared memory while it works on one. Tiles keep the scores' type and layout, so
+// whole 16-byte pieces come and go; the result takes its row's place there.
+constexpr int kTileRows = 32;
+
+// Copies a tile's elements: asynchronously where the rows are contiguous and
+// aligned (`whole`), one by one otherwise. The caller commits the group.
+template <class T>
+__device__ __forceinline__ void tile_fetch(const T* x, int64_t ld, int64_t t0, int rows, int c,
+                                           bool whole, T* tile) {
+    const int lane = threadIdx.x & 31, total = rows * c;
+    const T* at = x + t0 * ld;
+    if (whole) {
+        constexpr int V = Pack<T>::N;
+        const int vecs = total / V;
+        for (int i = lane; i < vecs; i += 32)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
+                             (uint32_t)__cvta_generic_to_shared(tile + i * V)),
+                         "l"(at + i * V)
+                         : "memory");
+        for (int i = vecs * V + lane; i < total; i += 32) tile[i] = at[i];
+    } else {
+        for (int i = lane; i < total; i += 32) tile[i] = at[(i / c) * ld + i % c];
+    }
+}
+
+template <class T>
+__device__ __forceinline__ void tile_put(T* out, int64_t ld, int64_t t0, int rows, int c, bool whole,
+                                         const T* tile) {
+    const int lane = threadIdx.x & 31, total = rows * c;
+    T* at = out + t0 * ld;
+    if (whole) {
+        constexpr int V = Pack<T>::N;
+        const int vecs = total / V;
+        for (int i = lane; i < vecs; i += 32) *reinterpret_cast<uint4*>(at + i * V) = load16(tile + i * V);
+        for (int i = vecs * V + lane; i < total; i += 32) at[i] = tile[i];
+    } else {
+        for (int i = lane; i < total; i += 32) at[(i / c) * ld + i % c] = tile[i];
+    }
+}
+
+// The column at which a thread begins its row, where c is a multiple of 4 (two
+// rows at most meet in a bank otherwise). Rows of c elements meet in the same
+// banks after 32 / gcd(c, 32) rows (64-bit values: of 16 lanes; 16-bit ones:
+// pairs); each such round of rows begins one column further on.
+template <class T>
+__device__ __forceinline__ int first_column(int c) {
+    const int lane = threadIdx.x & 31, g = c & -c;
+    if (sizeof(T) == 8) return (lane & 15) * (g < 16 ? g : 16) / 16 % c;
+    if (sizeof(T) == 2) return g == 1 ? 0 : 2 * (lane * (g / 2 < 32 ? g / 2 : 32) / 32) % c;
+    return lane * (g < 32 ? g : 32) / 32 % c;
+}
+
+// The thread's row of the gradient: k e with e = exp(x - off) in v, and g + k e at the
+// label (its e in ey), rounded once; 0 for a token without one, whatever its scores
+// are. TURN: the thread's first column is not 0.
+template <class T, class A, int CW, bool TURN>
+__device__ __forceinline__ void small_grad(T* row, const A (&v)[CW], int c, int first, A g, A k, A ey,
+                                           int y) {
+    int col = first;
+#pragma unroll
+    for (int j = 0; j < CW; ++j)
+        if (j < c) {
+            row[TURN ? col : j] = narrow<T>(g == A(0) ? A(0) : v[j] * k);
+            if (TURN) col = col + 1 == c ? 0 : col + 1;
+        }
+    if (g != A(0)) row[y] = narrow<T>(g + k * ey);
+}
+
+// c <= CW classes, a row in a thread's registers.
+template <class T, class A, int CW, bool TURN, Mode M>
+__global__ void __launch_bounds__(kSmallNT, IsF64<A>::value || CW > 16 ? 4 : kSmallPerSm)
+    small_rows_kernel(const T* __restrict__ x, int64_t ld, T* __restrict__ out, int64_t ld_out,
+                      RowArgs<A> a, bool whole_in, bool whole_out) {
+    extern __shared__ uint4 small_smem[];  // per warp two tiles of kTileRows x c
+    __shared__ double sm[kSmallNT / 32];
+    const int c = (int)a.c, lane = threadIdx.x & 31;
+    T* const tiles = reinterpret_cast<T*>(small_smem) + (threadIdx.x / 32) * (2 * kTileRows * c);
+    const int first = TURN ? first_column<T>(c) : 0;
+    const double total = M == POLICY ? weight_total(a) : 0.0, inv = inverse(total);
+    const double scale = M == GRAD && a.scale ? *a.scale : 1.0;
+    double e[3] = {0.0, 0.0, 0.0};
+    const int64_t n_tiles = ceil_div(a.n, (int64_t)kTileRows), step = (int64_t)gridDim.x * (kSmallNT / 32);
+    int64_t tile = (int64_t)blockIdx.x * (kSmallNT / 32) + threadIdx.x / 32;
+    // the gradient goes from the last row to the first: the forward that read the
+    // scores just before left the last ones in L2
+    auto begin = [&](int64_t i) { return (M == GRAD ? n_tiles - 1 - i : i) * kTileRows; };
+    auto rows_of = [&](int64_t t0) { return (int)(a.n - t0 < kTileRows ? a.n - t0 : kTileRows); };
+    Token<A> tok;
+    int y = -1;
+    auto inputs = [&](int64_t t0) {  // a thread's own inputs of the tile
+        y = -1;
+        tok = Token<A>();
+        if (lane >= rows_of(t0)) return;
+        y = a.labels.in(t0 + lane, a.c);
+        if (M == POLICY) tok.load(a, t0 + lane);
+        if (M == GRAD) {
+            tok.w = a.g[t0 + lane];
+            tok.old = a.lse_in[t0 + lane];
+        }
+    };
+    if (tile < n_tiles) {
+        tile_fetch(x, ld, begin(tile), rows_of(begin(tile)), c, whole_in, tiles);
+        inputs(begin(tile));
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    for (int buf = 0; tile < n_tiles; tile += step, buf ^= 1) {
+        const int64_t t0 = begin(tile), t = t0 + lane;
+        const int rows = rows_of(t0), y_now = y;
+        const Token<A> now = tok;
+        if (tile + step < n_tiles) {
+            const int64_t next = begin(tile + step);
+            tile_fetch(x, ld, next, rows_of(next), c, whole_in, tiles + (buf ^ 1) * (kTileRows * c));
+            inputs(next);
+        }
+        asm volatile("cp.async.commit_group;\ncp.async.wait_group 1;" ::: "memory");
+        __syncwarp();
+        T* row = tiles + buf * (kTileRows * c) + lane * c;
+        if (lane < rows) {
+            A v[CW];
+            A m = minus_inf<A>(), s = A(0);
+            const A at = y_now >= 0 ? widen<A>(row[y_now]) : A(0);
+            int col = first;
+#pragma unroll
+            for (int j = 0; j < CW; ++j) {
+                v[j] = minus_inf<A>();
+                if (j < c) {
+                    v[j] = widen<A>(row[TURN ? col : j]);
+                    if (TURN) col = col + 1 == c ? 0 : col + 1;
+                }
+                if (M != GRAD) m = fmax(m, v[j]);
+            }
+            const A off = M == GRAD ? now.old : offset_of(m);
+            if (M != GRAD) {
+#pragma unroll
+                for (int j = 0; j < CW; ++j) {
+                    v[j] = exp_of(v[j] - off);
+                    s += v[j];
+                }
+                const bool empty = m == minus_inf<A>() && s == A(0);
+                const A ls = log_of(s);
+                const bool live = y_now >= 0 && !empty;
+                const A lp = live ? (at - off) - ls : A(0);
+                a.lp[t] = lp;
+                if (M == STATS) {
+                    if (a.lse) a.lse[t] = empty ? minus_inf<A>() : off + ls;
+                    if (a.zero) a.zero[t] = A(0);
+                } else {
+                    A f[3];
+                    const A g = policy_terms(a, now, lp, live, (A)inv, f);
+                    for (int i = 0; i < 3; ++i) e[i] += (double)f[i];
+                    if (out) small_grad<T, A, CW, TURN>(row, v, c, first, g, quotient(-g, s), exp_of(at - off), y_now);
+                }
+            } else {
+                A g = y_now >= 0 && off != minus_inf<A>() ? now.w : A(0);
+                if (a.scale) g = (A)((double)g * scale);
+#pragma unroll
+                for (int j = 0; j < CW; ++j) v[j] = exp_of(v[j] - off);
+                small_grad<T, A, CW, TURN>(row, v, c, first, g, -g, exp_of(at - off), y_now);
+            }
+        }
+        __syncwarp();
+        if (M != STATS && out) tile_put(out, ld_out, t0, rows, c, whole_out, tiles + buf * (kTileRows * c));
+        __syncwarp();  // the tile's buffer is filled again
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    if (M == STATS) {
+        if (a.counter && blockIdx.x == 0 && threadIdx.x == 0) *a.counter = 0;
+    } else if (M == POLICY) {
+        for (int i = 0; i < 3; ++i) e[i] = block_sum(e[i], sm);
+        policy_finish(a, e, total, sm);
+    }
+}
+
+// ---------------------------------------------------------- rows at once --
+
+// Where a row's 16-byte vectors begin, how many there are, and the single
+// elements before and behind them (at most 2 (V - 1): one per lane).
+template <class T>
+struct RowShape {
+    static constexpr int V = 16 / sizeof(T);
+    int head, nv, edges;
+    __device__ __forceinline__ RowShape(const T* x, int c) {
+        const int h = (int)((16 - (uintptr_t)x % 16) % 16 / sizeof(T));
+        head = h < c ? h : c;
+        nv = (c - head) / V;
+        edges = c - nv * V;
+    }
+    __device__ __forceinline__ int edge(int i) const { return i < head ? i : i + nv * V; }
+};
+
+// Whether two rows have the same place within 16 bytes, so that their vectors do.
+__device__ __forceinline__ bool alike(const void* a, const void* b) {
+    return ((uintptr_t)a - (uintptr_t)b) % 16 == 0;
+}
+
+// The gradient's vector at column `at` from k exp(x - off): 0 for a token without one
+// (whatever its scores are), g more at the label.
+template <class A, int N>
+__device__ __forceinline__ void grad_vec(A (&p)[N], int at, int y, A g) {
+    if (g == A(0)) {
+#pragma unroll
+        for (int q = 0; q < N; ++q) p[q] = A(0);
+    } else if ((unsigned)(y - at) < (unsigned)N) {
+#pragma unroll
+        for (int q = 0; q < N; ++q)
+            if (at + q == y) p[q] += g;
+    }
+}
+
+// N values to `at`: as one vector, or one by one where the rows of scores and
+// gradient are not alike.
+template <class T, class A>
+__device__ __forceinline__ void store16(T* at, const A (&v)[Pack<T>::N], bool whole) {
+    if (whole) {
+        *reinterpret_cast<uint4*>(at) = Pack<T>::pack(v);
+    } else {
+#pragma unroll
+        for (int q = 0; q < Pack<T>::N; ++q) at[q] = narrow<T>(v[q]);
+    }
+}
+
+// Lane 0 of a group hands over the finished row: statistics, or loss terms and
+// the gradient's two factors: out[c] = k exp(x[c] - off), plus g at the label.
+template <class T, class A, Mode M>
+struct RowResult {
+    A g = A(0), k = A(0);
+    A e[3] = {A(0), A(0), A(0)};
+    __device__ __forceinline__ RowResult(const RowArgs<A>& a, const Token<A>& tok, int64_t t,
+                                         int y, T xy, A m, A s, double inv_total, bool first) {
+        const A off = offset_of(m);
+        const bool empty = m == minus_inf<A>() && s == A(0);
+        const bool live = y >= 0 && !empty;
+        const A ls = log_of(s);
+        const A lp = live ? (widen<A>(xy) - off) - ls : A(0);
+        if (first) a.lp[t] = lp;
+        if (M == STATS) {
+            if (first && a.lse) a.lse[t] = empty ? minus_inf<A>() : off + ls;
+            if (first && a.zero) a.zero[t] = A(0);
         } else {
-            s = s * exp_of(m - top) + s2 * exp_of(m2 - top);
-            m = top;
+            g = policy_terms(a, tok, lp, live, (A)inv_total, e);
+            k = quotient(-g, s);
         }
     }
 };
 
-// Group of L lanes working on one row; L = kNT is the whole block.
-template <class A, int L>
-__device__ __forceinline__ void group_join(Softmax<A>& r, A* sm) {
-    constexpr int W = L < 32 ? L : 32;
+// A warp per row, the row in its registers: K vectors a lane.
+template <class T, class A, int K, Mode M>
+__global__ void __launch_bounds__(kNT, IsF64<A>::value ? 2 : 4)
+    cached_rows_kernel(const T* __restrict__ x, int64_t ld, T* __restrict__ out, int64_t ld_out,
+                       RowArgs<A> a) {
+    constexpr int V = 16 / sizeof(T), L = 32, R = kNT / L;
+    __shared__ double sums[32];
+    const int lane = threadIdx.x % L;
+    const int64_t t = (int64_t)blockIdx.x * R + threadIdx.x / L;
+    const bool in = t < a.n;
+    const T* row = x + (in ? t : 0) * ld;
+    const RowShape<T> sh(row, in ? (int)a.c : 0);
+    uint4 v[K];
+    T edge = narrow<T>(minus_inf<A>());
 #pragma unroll
-    for (int o = W / 2; o > 0; o >>= 1) {
-        const A m2 = __shfl_xor_sync(0xffffffffu, r.m, o);
-        const A s2 = __shfl_xor_sync(0xffffffffu, r.s, o);
-        r.join(m2, s2);
+    for (int i = 0; i < K; ++i) {
+        const int j = lane + i * L;
+        v[i] = j < sh.nv ? load16(row + sh.head + j * V) : Pack<T>::minus_inf();
     }
-    if (L > 32) {
-        const int warp = threadIdx.x / 32;
-        if ((threadIdx.x & 31) == 0) {
-            sm[2 * warp] = r.m;
-            sm[2 * warp + 1] = r.s;
+    if (lane < sh.edges) edge = row[sh.edge(lane)];
+    const int y = in ? a.labels.in(t, a.c) : -1;
+    const T xy = row[y >= 0 ? y : 0];  // the label's score, on its way with the row
+    Token<A> tok;
+    if (M == POLICY && in) tok.load(a, t);
+    const double total = M == POLICY ? weight_total(a) : 0.0, inv = inverse(total);
+    A m = widen<A>(edge);
+#pragma unroll
+    for (int i = 0; i < K; ++i)
+        if (i * L < sh.nv) m = fmax(m, Pack<T>::top(v[i]));
+    m = warp_reduce(m, [](A p, A q) { return fmax(p, q); });
+    const A off = offset_of(m);
+    ExpSum<A> ex(off);
+#pragma unroll
+    for (int i = 0; i < K; ++i)
+        if (i * L < sh.nv) {
+            A p[V];
+            Pack<T>::unpack(v[i], p);
+            ex.add(p);
+        }
+    const A s = warp_sum(exp_of(widen<A>(edge) - off) + ex.sum());
+    double e[3] = {0.0, 0.0, 0.0};
+    if (in) {
+        const RowResult<T, A, M> r(a, tok, t, y, xy, m, s, inv, lane == 0);
+        if (M == POLICY && lane == 0)
+            for (int i = 0; i < 3; ++i) e[i] = (double)r.e[i];
+        if (M == POLICY && out) {
+            T* to = out + t * ld_out;
+            const bool whole = alike(row, to), none = r.g == A(0);
+            if (lane < sh.edges) {
+                const int j = sh.edge(lane);
+                to[j] = none ? narrow<T>(A(0))
+                             : narrow<T>((j == y ? r.g : A(0)) + r.k * exp_of(widen<A>(edge) - off));
+            }
+#pragma unroll
+            for (int i = 0; i < K; ++i) {
+                const int j = lane + i * L;
+                if (j < sh.nv) {
+                    const int at = sh.head + j * V;
+                    A p[V];
+                    Pack<T>::unpack(v[i], p);
+                    ex.scaled(p, r.k);
+                    grad_vec(p, at, y, r.g);
+                    store16<T, A>(to + at, p, whole);
+                }
+            }
+        }
+    }
+    if (M == STATS) {
+        if (a.counter && blockIdx.x == 0 && threadIdx.x == 0) *a.counter = 0;
+    } else {
+        for (int i = 0; i < 3; ++i) e[i] = block_sum(e[i], sums);
+        policy_finish(a, e, total, sums);
+    }
+}
+
+// ------------------------------------------- long rows, statistics alone --
+
+// Rows read once with a running maximum: L lanes a row, U vectors a lane in
+// flight. The fewest lanes that still fill the GPU: what a row costs besides its
+// values (reductions, log) is paid once a warp.
+template <class T, class A, int L>
+__global__ void __launch_bounds__(kNT, IsF64<A>::value ? 2 : 4)
+    scan_rows_kernel(const T* __restrict__ x, int64_t ld, RowArgs<A> a) {
+    constexpr int V = 16 / sizeof(T), U = 8, W = L / 32;
+    __shared__ A sm_m[kNT / 32], sm_s[kNT / 32];
+    const int lane = threadIdx.x % L, warp = threadIdx.x / 32;
+    const int64_t t = (int64_t)blockIdx.x * (kNT / L) + threadIdx.x / L;
+    const bool in = t < a.n;
+    const T* row = x + (in ? t : 0) * ld;
+    const RowShape<T> sh(row, in ? (int)a.c : 0);
+    const int y = in ? a.labels.in(t, a.c) : -1;
+    const T edge = lane < sh.edges ? row[sh.edge(lane)] : narrow<T>(minus_inf<A>());
+    RowStats<A> r{widen<A>(edge), A(0)};
+    r.s = exp_of(r.m - offset_of(r.m));
+    const T* at = row + sh.head;
+    for (int j0 = lane; j0 < sh.nv; j0 += L * U) {
+        uint4 v[U];
+        A top = r.m;
+#pragma unroll
+        for (int u = 0; u < U; ++u) v[u] = j0 + u * L < sh.nv ? load16(at + (j0 + u * L) * V) : Pack<T>::minus_inf();
+#pragma unroll
+        for (int u = 0; u < U; ++u) top = fmax(top, Pack<T>::top(v[u]));
+        if (top > r.m) {
+            r.s *= exp_of(r.m - top);
+            r.m = top;
+        }
+        ExpSum<A> ex(offset_of(r.m));
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            A p[V];
+            Pack<T>::unpack(v[u], p);
+            ex.add(p);
+        }
+        r.s += ex.sum();
+    }
+    const T xy = row[y >= 0 ? y : 0];
+    across(r, 32);
+    if (W > 1) {
+        if ((lane & 31) == 0) {
+            sm_m[warp] = r.m;
+            sm_s[warp] = r.s;
         }
         __syncthreads();
-        Softmax<A> t;
+        r.m = sm_m[warp / W * W + (lane & (W - 1))];
+        r.s = sm_s[warp / W * W + (lane & (W - 1))];
+        across(r, W);
+    }
+    if (in) RowResult<T, A, STATS>(a, Token<A>(), t, y, xy, r.m, r.s, 0.0, lane == 0);
+    if (a.counter && blockIdx.x == 0 && threadIdx.x == 0) *a.counter = 0;
+}
+
+// ------------------------------------------------------------- long rows --
+
+// mbarriers and bulk copies. Every wait ends: after kWaitLimit polls it raises the
+// block's flag, which ends all later waits at once; the block then runs to its
+// end on whatever is in shared memory and reports NaN.
+constexpr int kWaitLimit = 1 << 24;
+
+__device__ __forceinline__ uint32_t smem_at(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void bar_init(uint64_t* b, unsigned count) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_at(b)), "r"(count) : "memory");
+}
+__device__ __forceinline__ void bar_arrive(uint64_t* b) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_at(b)) : "memory");
+}
+__device__ __forceinline__ void bar_expect(uint64_t* b, unsigned bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_at(b)), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ bool bar_try(uint64_t* b, unsigned parity) {
+    unsigned ok;
+    asm volatile(
+        "{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+        "selp.u32 %0, 1, 0, p;\n}"
+        : "=r"(ok)
+        : "r"(smem_at(b)), "r"(parity)
+        : "memory");
+    return ok;
+}
+__device__ __forceinline__ void bar_wait(uint64_t* b, unsigned parity, volatile int* stop) {
+    for (int i = 0; !bar_try(b, parity); ++i) {
+        if (*stop) return;
+        if (i >= kWaitLimit) {
+            *stop = 1;
+            return;
+        }
+    }
+}
+// 16-byte aligned addresses, bytes a multiple of 16.
+__device__ __forceinline__ void bulk_copy(void* to, const void* from, unsigned bytes, uint64_t* b) {
+    asm volatile("cp.async.bulk.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                 ::"r"(smem_at(to)), "l"(from), "r"(bytes), "r"(smem_at(b))
+                 : "memory");
+}
+
+// Rows streamed through a ring of shared-memory chunks by bulk copies: one warp
+// keeps copies of the rows ahead in flight while L threads work, so the loads do
+// not stop for a row's reductions or its gradient. A row that fits the ring is
+// kept there until its gradient is written; a longer one is read twice, the
+// second time mostly from L2. A chunk is kRingVecs vectors a thread.
+constexpr int kRingVecs = 4;
+constexpr int kRingMost = 512;  // lanes of the longest rows, one block per SM
+constexpr int ring_blocks(int L) { return kRingMost / L; }
+constexpr int ring_slots(int L) { return 200704 / ring_blocks(L) / (L * kRingVecs * 16); }
+
+template <class T, class A, int L>
+__global__ void __launch_bounds__(L + 32, ring_blocks(L))
+    ring_rows_kernel(const T* __restrict__ x, int64_t ld, T* __restrict__ out, int64_t ld_out,
+                     RowArgs<A> a) {
+    constexpr int V = 16 / sizeof(T), S = ring_slots(L), CV = L * kRingVecs, W = L / 32;
+    extern __shared__ uint4 ring[];  // S x CV
+    __shared__ uint64_t full[S], empty[S];
+    __shared__ A sm_m[2][W], sm_s[2][W];
+    __shared__ double sums[32];
+    __shared__ int stop_flag;
+    volatile int* stop = &stop_flag;
+    if (threadIdx.x == 0) {
+        stop_flag = 0;
+        for (int i = 0; i < S; ++i) {
+            bar_init(&full[i], 1);
+            bar_init(&empty[i], W);
+        }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    __syncthreads();
+    const bool grad = out != nullptr;
+    double e[3] = {0.0, 0.0, 0.0}, total = 0.0;
+    if (threadIdx.x >= L) {
+        if (threadIdx.x == L) {
+            unsigned seq = 0;
+            for (int64_t t = blockIdx.x; t < a.n; t += gridDim.x) {
+                const T* row = x + t * ld;
+                const RowShape<T> sh(row, (int)a.c);
+                const int chunks = (sh.nv + CV - 1) / CV;
+                for (int pass = grad && chunks > S ? 2 : 1; pass > 0; --pass)
+                    for (int c = 0; c < chunks; ++c, ++seq) {
+                        const unsigned slot = seq % S;
+                        bar_wait(&empty[slot], (seq / S + 1) & 1, stop);
+                        if (*stop) break;
+                        const int left = sh.nv - c * CV;
+                        const unsigned bytes = (unsigned)(left < CV ? left : CV) * 16;
+                        bar_expect(&full[slot], bytes);
+                        bulk_copy(ring + slot * CV, row + sh.head + (int64_t)c * CV * V, bytes, &full[slot]);
+                    }
+            }
+            // copies in flight end before the block does
+            for (unsigned q = seq > S ? seq - S : 0; q < seq; ++q)
+                for (int i = 0; i < kWaitLimit && !bar_try(&full[q % S], (q / S) & 1); ++i) {}
+        }
+        __syncwarp();
+    } else {
+        const int lane = threadIdx.x, warp = lane / 32;
+        unsigned seq = 0;
+        int64_t t = blockIdx.x;
+        int y = t < a.n ? a.labels.in(t, a.c) : -1;
+        total = weight_total(a);
+        const double inv = inverse(total);
+        for (int it = 0; t < a.n; t += gridDim.x, ++it) {
+            const T* row = x + t * ld;
+            const RowShape<T> sh(row, (int)a.c);
+            const int chunks = (sh.nv + CV - 1) / CV;
+            const bool keep = grad && chunks <= S;
+            const T edge = lane < sh.edges ? row[sh.edge(lane)] : narrow<T>(minus_inf<A>());
+            const T xy = row[y >= 0 ? y : 0];
+            Token<A> tok;
+            tok.load(a, t);
+            const int64_t tn = t + gridDim.x;
+            const int y_next = tn < a.n ? a.labels.in(tn, a.c) : -1;
+            RowStats<A> r{widen<A>(edge), A(0)};
+            r.s = exp_of(r.m - offset_of(r.m));
+            const unsigned first = seq;
+            for (int c = 0; c < chunks; ++c, ++seq) {
+                const unsigned slot = seq % S;
+                bar_wait(&full[slot], (seq / S) & 1, stop);
+                const uint4* at = ring + slot * CV + lane;
+                const int left = sh.nv - c * CV - lane;
+                uint4 v[kRingVecs];
+                A top = r.m;
 #pragma unroll
-        for (int w = 0; w < L / 32; ++w) t.join(sm[2 * w], sm[2 * w + 1]);
-        r = t;
-        __syncthreads();
-    }
-}
-
-// Elements before the first 16-byte boundary of a row (all of them when the row is short).
-template <class T, int VEC>
-__device__ __forceinline__ int64_t head_of(const T* x, int64_t c) {
-    if (VEC == 1) return 0;
-    const int64_t h = (int64_t)((16 - (uintptr_t)x % 16) % 16 / sizeof(T));
-    return h < c ? h : c;
-}
-
-template <class T, class A, int VEC, int L>
-__device__ __forceinline__ Softmax<A> row_softmax(const T* x, int64_t c, int lane, A* sm) {
-    Softmax<A> r;
-    const int64_t h = head_of<T, VEC>(x, c), nv = (c - h) / VEC;
-    for (int64_t j = lane; j < h; j += L) {
-        const A v[1] = {widen<A>(x[j])};
-        r.add(v);
-    }
-    for (int64_t j = lane; j < nv; j += L) {
-        const Vec<T, VEC> p = ldg_vec<T, VEC>(x + h + j * VEC);
-        A v[VEC];
+                for (int u = 0; u < kRingVecs; ++u) v[u] = u * L < left ? at[u * L] : Pack<T>::minus_inf();
+                if (!keep) {  // the chunk is in registers
+                    __syncwarp();
+                    if ((lane & 31) == 0) bar_arrive(&empty[slot]);
+                }
 #pragma unroll
-        for (int q = 0; q < VEC; ++q) v[q] = widen<A>(p.v[q]);
-        r.add(v);
-    }
-    for (int64_t j = h + nv * VEC + lane; j < c; j += L) {
-        const A v[1] = {widen<A>(x[j])};
-        r.add(v);
-    }
-    group_join<A, L>(r, sm);
-    return r;
-}
-
-// out = g ([c = y] - exp(x - lse)); x and out have the same place within 16 bytes when VEC > 1.
-template <class T, class A, int VEC, int L>
-__device__ __forceinline__ void row_grad(const T* x, T* out, int64_t c, int64_t y, A g, A lse,
-                                         int lane) {
-    const int64_t h = head_of<T, VEC>(x, c), nv = (c - h) / VEC;
-    auto one = [&](T v, int64_t j) {
-        return g == A(0) ? narrow<T>(A(0))
-                         : narrow<T>(g * ((j == y ? A(1) : A(0)) - exp_of(widen<A>(v) - lse)));
-    };
-    for (int64_t j = lane; j < h; j += L) out[j] = one(x[j], j);
-    for (int64_t j = lane; j < nv; j += L) {
-        const int64_t at = h + j * VEC;
-        Vec<T, VEC> p = ldg_vec<T, VEC>(x + at);
+                for (int u = 0; u < kRingVecs; ++u) top = fmax(top, Pack<T>::top(v[u]));
+                if (top > r.m) {
+                    r.s *= exp_of(r.m - top);
+                    r.m = top;
+                }
+                ExpSum<A> ex(offset_of(r.m));
 #pragma unroll
-        for (int q = 0; q < VEC; ++q) p.v[q] = one(p.v[q], at + q);
-        *reinterpret_cast<Vec<T, VEC>*>(out + at) = p;
+                for (int u = 0; u < kRingVecs; ++u) {
+                    A p[V];
+                    Pack<T>::unpack(v[u], p);
+                    ex.add(p);
+                }
+                r.s += ex.sum();
+            }
+            // (m, s) over the warp, then over the block: one barrier a row
+            across(r, 32);
+            if ((lane & 31) == 0) {
+                sm_m[it & 1][warp] = r.m;
+                sm_s[it & 1][warp] = r.s;
+            }
+            asm volatile("bar.sync 1, %0;" ::"n"(L) : "memory");
+            r.m = (lane & 31) < W ? sm_m[it & 1][lane & 31] : minus_inf<A>();
+            r.s = (lane & 31) < W ? sm_s[it & 1][lane & 31] : A(0);
+            across(r, 32);
+            const RowResult<T, A, POLICY> res(a, tok, t, y, xy, r.m, r.s, inv, lane == 0);
+            for (int i = 0; i < 3; ++i) e[i] += (double)res.e[i];
+            if (grad) {
+                T* to = out + t * ld_out;
+                const bool whole = alike(row, to), none = res.g == A(0);
+                const A off = offset_of(r.m);
+                const ExpSum<A> ex(off);
+                if (lane < sh.edges) {
+                    const int j = sh.edge(lane);
+                    to[j] = none ? narrow<T>(A(0))
+                                 : narrow<T>((j == y ? res.g : A(0)) + res.k * exp_of(widen<A>(edge) - off));
+                }
+                if (keep) seq = first;
+                for (int c = 0; c < chunks; ++c, ++seq) {
+                    const unsigned slot = seq % S;
+                    if (!keep) bar_wait(&full[slot], (seq / S) & 1, stop);
+                    const uint4* at = ring + slot * CV + lane;
+                    const int left = sh.nv - c * CV - lane;
+                    uint4 v[kRingVecs];
+#pragma unroll
+                    for (int u = 0; u < kRingVecs; ++u)
+                        if (u * L < left) v[u] = at[u * L];
+                    __syncwarp();
+                    if ((lane & 31) == 0) bar_arrive(&empty[slot]);
+#pragma unroll
+                    for (int u = 0; u < kRingVecs; ++u)
+                        if (u * L < left) {
+                            const int j = sh.head + (c * CV + u * L + lane) * V;
+                            A p[V];
+                            Pack<T>::unpack(v[u], p);
+                            ex.scaled(p, res.k);
+                            grad_vec(p, j, y, res.g);
+                            store16<T, A>(to + j, p, whole);
+                        }
+                }
+            }
+            if (*stop && lane == 0) {
+                a.lp[t] = (A)NAN;
+                e[0] = e[1] = e[2] = NAN;
+            }
+            y = y_next;
+        }
     }
-    for (int64_t j = h + nv * VEC + lane; j < c; j += L) out[j] = one(x[j], j);
+    __syncthreads();
+    total = weight_total(a);  // the copying warp too
+    policy_finish(a, e, total, sums);
 }
 
-// (lse, label's log-probability, unmasked) of a finished row.
-template <class T, class A>
-__device__ __forceinline__ void finish_row(const Softmax<A>& r, const T* x, int64_t c, int64_t y,
-                                           A& lse, A& lp, bool& live) {
-    const bool empty = r.m == minus_inf<A>() && r.s == A(0);
-    const A ls = log_of(r.s);
-    lse = empty ? minus_inf<A>() : r.off() + ls;
-    live = y >= 0 && y < c && !empty;
-    lp = live ? (widen<A>(x[y]) - r.off()) - ls : A(0);
-}
+// ---------------------------------------------------------------- gradient --
 
-template <class T, class A, class I, int VEC, int L>
+// out = f ([c = y] - exp(x - lse)), f = g times *scale. Elementwise once lse is known. Rows
+// are walked from the last to the first: the forward that read them just before
+// left the last ones in L2.
+template <class T, class A, int L>
 __global__ void __launch_bounds__(kNT)
-    label_stats_kernel(const T* __restrict__ x, int64_t ld, int64_t n, int64_t c,
-                       const I* __restrict__ labels, A* __restrict__ lp, A* __restrict__ lse,
-                       A* __restrict__ zero) {
-    __shared__ A sm[2 * kNT / 32];
+    label_grad_kernel(const T* __restrict__ x, int64_t ld, T* __restrict__ out, int64_t ld_out,
+                      RowArgs<A> a) {
+    constexpr int V = 16 / sizeof(T), U = 4;
     const int lane = threadIdx.x % L;
-    const int64_t t = (int64_t)blockIdx.x * (kNT / L) + threadIdx.x / L;
-    const bool in = t < n;
-    const T* row = x + (in ? t : 0) * ld;
-    const Softmax<A> r = row_softmax<T, A, VEC, L>(row, in ? c : 0, lane, sm);
-    if (in && lane == 0) {
-        A s, p;
-        bool live;
-        finish_row(r, row, c, (int64_t)labels[t], s, p, live);
-        lp[t] = p;
-        if (lse) lse[t] = s;
-        if (zero) zero[t] = A(0);
+    const int64_t t = a.n - 1 - ((int64_t)blockIdx.x * (kNT / L) + threadIdx.x / L);
+    if (t < 0) return;
+    const T* row = x + t * ld;
+    T* to = out + t * ld_out;
+    const RowShape<T> sh(row, (int)a.c);
+    const bool whole = alike(row, to);
+    const int y = a.labels.in(t, a.c);
+    const A l = a.lse_in[t], f = a.factor(t, y, l);
+    auto one = [&](A v) { return f == A(0) ? A(0) : -f * exp_of(v - l); };
+    if (lane < sh.edges) {
+        const int j = sh.edge(lane);
+        to[j] = narrow<T>(one(widen<A>(row[j])) + (j == y ? f : A(0)));
     }
-}
-
-// scale: factor of every g (NULL = 1), on the device.
-template <class T, class A, class I, int VEC, int L>
-__global__ void __launch_bounds__(kNT)
-    label_grad_kernel(const T* __restrict__ x, int64_t ld, int64_t n, int64_t c,
-                      const I* __restrict__ labels, const A* __restrict__ g,
-                      const double* __restrict__ scale, const A* __restrict__ lse,
-                      T* __restrict__ out, int64_t ld_out) {
-    const int lane = threadIdx.x % L;
-    const int64_t t = (int64_t)blockIdx.x * (kNT / L) + threadIdx.x / L;
-    if (t >= n) return;
-    const int64_t y = (int64_t)labels[t];
-    A f = y >= 0 && y < c && lse[t] != minus_inf<A>() ? g[t] : A(0);
-    if (scale) f = (A)((double)f * *scale);
-    row_grad<T, A, VEC, L>(x + t * ld, out + t * ld_out, c, y, f, lse[t], lane);
+    for (int j0 = lane; j0 < sh.nv; j0 += L * U) {
+        uint4 v[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (j0 + u * L < sh.nv) v[u] = load16(row + sh.head + (j0 + u * L) * V);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (j0 + u * L < sh.nv) {
+                const int at = sh.head + (j0 + u * L) * V;
+                A p[V];
+                Pack<T>::unpack(v[u], p);
+#pragma unroll
+                for (int q = 0; q < V; ++q) p[q] = one(p[q]);
+                if (y >= at && y < at + V) {
+#pragma unroll
+                    for (int q = 0; q < V; ++q)
+                        if (at + q == y) p[q] += f;
+                }
+                store16<T, A>(to + at, p, whole);
+            }
+    }
 }
 
 // Sums of v over [indptr[s], indptr[s+1]), one warp each, in float64.
@@ -207,60 +956,55 @@ __global__ void __launch_bounds__(kNT)
     if ((threadIdx.x & 31) == 0) sums[s] = (A)a;
 }
 
-// One warp per pair: sums, margin, the pair's weighted loss and its unnormalised
-// derivative, written to every token of the two sequences.
-template <class A>
+// One group of W threads per pair: sums, margin, the pair's weighted loss and its
+// unnormalised derivative, written to every token of the two sequences. The block
+// that finishes last adds the losses and the weights, in a fixed order.
+template <class A, int W>
 __global__ void __launch_bounds__(kNT)
     pair_kernel(const A* __restrict__ lp, int64_t n, const int64_t* __restrict__ indptr,
                 int64_t n_pairs, const A* __restrict__ reference, double beta, double eps,
                 const A* __restrict__ weight, A* __restrict__ margins, A* __restrict__ sums,
-                double* __restrict__ pair_loss, A* __restrict__ g) {
-    const int64_t p = (int64_t)blockIdx.x * (kNT / 32) + threadIdx.x / 32;
-    const int lane = threadIdx.x & 31;
-    if (p >= n_pairs) return;
-    int64_t lo[2], hi[2];
-    double s[2];
-    for (int i = 0; i < 2; ++i) {
-        seq_bounds(indptr, p + i * n_pairs, n, lo[i], hi[i]);
-        s[i] = warp_seq_sum(lp, lo[i], hi[i]);
+                double* __restrict__ pair_loss, A* __restrict__ g, unsigned* __restrict__ done,
+                A* __restrict__ loss, double* __restrict__ scale) {
+    __shared__ double sm[kNT / 32];
+    __shared__ unsigned last;
+    const int64_t p = (int64_t)blockIdx.x * (kNT / W) + threadIdx.x / W;
+    const int lane = threadIdx.x % W;
+    if (p < n_pairs) {  // uniform over the group
+        int64_t lo[2], hi[2];
+        double s[2];
+        for (int i = 0; i < 2; ++i) {
+            seq_bounds(indptr, p + i * n_pairs, n, lo[i], hi[i]);
+            s[i] = 0.0;
+            for (int64_t t = lo[i] + lane; t < hi[i]; t += W) s[i] += (double)lp[t];
+            s[i] = W == 32 ? warp_sum(s[i]) : block_sum(s[i], sm);
+        }
+        const double z = beta * ((s[0] - (double)reference[p]) - (s[1] - (double)reference[n_pairs + p]));
+        const double w = weight ? (double)weight[p] : 1.0;
+        const double up = 1.0 / (1.0 + exp(-z)), down = 1.0 / (1.0 + exp(z));
+        // a pair of weight 0 is left out, whatever its margin
+        const double slope = w == 0.0 ? 0.0 : -beta * w * ((1.0 - eps) * down - eps * up);
+        if (lane == 0) {
+            margins[p] = (A)z;
+            sums[p] = (A)s[0];
+            sums[n_pairs + p] = (A)s[1];
+            const double soft = log1p(exp(-fabs(z)));
+            pair_loss[p] = w == 0.0 ? 0.0 : w * (soft + (1.0 - eps) * fmax(-z, 0.0) + eps * fmax(z, 0.0));
+        }
+        if (g)
+            for (int i = 0; i < 2; ++i)
+                for (int64_t t = lo[i] + lane; t < hi[i]; t += W) g[t] = (A)(i ? -slope : slope);
     }
-    const double z = beta * ((s[0] - (double)reference[p]) - (s[1] - (double)reference[n_pairs + p]));
-    const double w = weight ? (double)weight[p] : 1.0;
-    const double up = 1.0 / (1.0 + exp(-z)), down = 1.0 / (1.0 + exp(z));
-    // a pair of weight 0 is left out, whatever its margin
-    const double slope = w == 0.0 ? 0.0 : -beta * w * ((1.0 - eps) * down - eps * up);
-    if (lane == 0) {
-        margins[p] = (A)z;
-        sums[p] = (A)s[0];
-        sums[n_pairs + p] = (A)s[1];
-        const double soft = log1p(exp(-fabs(z)));
-        pair_loss[p] = w == 0.0 ? 0.0 : w * (soft + (1.0 - eps) * fmax(-z, 0.0) + eps * fmax(z, 0.0));
-    }
-    if (g)
-        for (int i = 0; i < 2; ++i)
-            for (int64_t t = lo[i] + lane; t < hi[i]; t += 32) g[t] = (A)(i ? -slope : slope);
-}
-
-// Sums of `width` interleaved columns and of the weights by one block in a fixed order.
-__device__ __forceinline__ double block_sum(double v, double* sm) {
-    v = warp_sum(v);
-    if ((threadIdx.x & 31) == 0) sm[threadIdx.x / 32] = v;
+    __threadfence();
     __syncthreads();
-    double t = 0.0;
-    for (int w = 0; w < (int)blockDim.x / 32; ++w) t += sm[w];
+    if (threadIdx.x == 0) last = atomicAdd(done, 1u) == gridDim.x - 1 ? 1u : 0u;
     __syncthreads();
-    return t;
-}
-
-template <class A>
-__global__ void __launch_bounds__(1024)
-    pair_finish_kernel(const double* __restrict__ pair_loss, const A* __restrict__ weight,
-                       int64_t n_pairs, A* __restrict__ loss, double* __restrict__ scale) {
-    __shared__ double sm[32];
+    if (!last) return;
+    __threadfence();
     double a = 0.0, b = 0.0;
-    for (int64_t p = threadIdx.x; p < n_pairs; p += 1024) {
-        a += pair_loss[p];
-        b += weight ? (double)weight[p] : 1.0;
+    for (int64_t q = threadIdx.x; q < n_pairs; q += kNT) {
+        a += __ldcg(pair_loss + q);
+        b += weight ? (double)weight[q] : 1.0;
     }
     a = block_sum(a, sm);
     b = block_sum(b, sm);
@@ -270,94 +1014,39 @@ __global__ void __launch_bounds__(1024)
     }
 }
 
-constexpr int kWeightBlocks = 128;
+template <class A>
+__global__ void zero_loss_kernel(A* v, int n) {  // nothing to take a mean of
+    if ((int)threadIdx.x < n) v[threadIdx.x] = A(0);
+}
 
-template <class A, class I>
+constexpr int kWeightBlocks = 512;
+
+// Partial sums of the unmasked tokens' weights; also clears the losses' block count.
+template <class A>
 __global__ void __launch_bounds__(kNT)
-    weight_kernel(const I* __restrict__ labels, int64_t c, const A* __restrict__ weight, int64_t n,
-                  double* __restrict__ part) {
+    weight_kernel(Labels labels, int64_t c, const A* __restrict__ weight, int64_t n,
+                  double* __restrict__ part, unsigned* __restrict__ done) {
     __shared__ double sm[kNT / 32];
     double a = 0.0;
-    for (int64_t t = (int64_t)blockIdx.x * kNT + threadIdx.x; t < n; t += (int64_t)gridDim.x * kNT) {
-        const int64_t y = (int64_t)labels[t];
-        if (y >= 0 && y < c) a += weight ? (double)weight[t] : 1.0;
+    constexpr int U = 8;  // tokens in flight per thread
+    for (int64_t t0 = (int64_t)blockIdx.x * kNT * U + threadIdx.x; t0 < n; t0 += (int64_t)gridDim.x * kNT * U) {
+        int y[U];
+        A w[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int64_t t = t0 + u * kNT;
+            y[u] = t < n ? labels.in(t, c) : -1;
+            w[u] = weight && t < n ? weight[t] : A(1);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (y[u] >= 0) a += (double)w[u];
     }
     a = block_sum(a, sm);
-    if (threadIdx.x == 0) part[blockIdx.x] = a;
-}
-
-struct PolicyArgs {
-    double clip_low, clip_high, kl_coef;
-};
-
-// One group per token: statistics, the token's loss terms and its gradient row.
-template <class T, class A, class I, int VEC, int L>
-__global__ void __launch_bounds__(kNT)
-    policy_kernel(const T* __restrict__ x, int64_t ld, int64_t n, int64_t c,
-                  const I* __restrict__ labels, const A* __restrict__ old,
-                  const A* __restrict__ adv, const A* __restrict__ ref, PolicyArgs k,
-                  const A* __restrict__ weight, const double* __restrict__ wpart, int n_wpart,
-                  double* __restrict__ part, A* __restrict__ lps, T* __restrict__ out,
-                  int64_t ld_out) {
-    __shared__ A sm[2 * kNT / 32];
-    __shared__ double terms[3][kNT / L];
-    const int lane = threadIdx.x % L, row_in = threadIdx.x / L;
-    const int64_t t = (int64_t)blockIdx.x * (kNT / L) + row_in;
-    const bool in = t < n;
-    const T* row = x + (in ? t : 0) * ld;
-    double total = 0.0;
-    for (int i = threadIdx.x & 31; i < n_wpart; i += 32) total += wpart[i];
-    total = warp_sum(total);
-    const Softmax<A> r = row_softmax<T, A, VEC, L>(row, in ? c : 0, lane, sm);
-    double e[3] = {0.0, 0.0, 0.0};
-    if (in) {
-        const int64_t y = (int64_t)labels[t];
-        A lse, lp;
-        bool live;
-        finish_row(r, row, c, y, lse, lp, live);
-        A g = A(0);
-        const double w = live && weight ? (double)weight[t] : 1.0;
-        if (live && w != 0.0) {  // a token of weight 0 is left out, whatever its ratio
-            const double a = (double)adv[t];
-            const double ratio = exp((double)lp - (double)old[t]);
-            const double bent = fmin(fmax(ratio, 1.0 - k.clip_low), 1.0 + k.clip_high);
-            const bool cut = ratio * a > bent * a;
-            double slope = cut ? 0.0 : -ratio * a, kl = 0.0;
-            if (ref) {
-                const double u = (double)ref[t] - (double)lp, eu = expm1(u);
-                kl = eu - u;
-                slope -= k.kl_coef * eu;
-            }
-            e[0] = w * (-(cut ? bent * a : ratio * a) + k.kl_coef * kl);
-            e[1] = w * kl;
-            e[2] = cut ? w : 0.0;
-            g = total != 0.0 ? (A)(w * slope / total) : A(0);
-        }
-        if (lane == 0) lps[t] = lp;
-        if (out) row_grad<T, A, VEC, L>(row, out + t * ld_out, c, y, g, lse, lane);
+    if (threadIdx.x == 0) {
+        part[blockIdx.x] = a;
+        if (blockIdx.x == 0) *done = 0;
     }
-    if (lane == 0)
-        for (int i = 0; i < 3; ++i) terms[i][row_in] = e[i];
-    __syncthreads();
-    if (threadIdx.x < 3) {
-        double a = 0.0;
-        for (int i = 0; i < kNT / L; ++i) a += terms[threadIdx.x][i];
-        part[3 * (int64_t)blockIdx.x + threadIdx.x] = a;
-    }
-}
-
-template <class A>
-__global__ void __launch_bounds__(1024)
-    policy_finish_kernel(const double* __restrict__ part, int64_t n_part,
-                         const double* __restrict__ wpart, int n_wpart, A* __restrict__ stats) {
-    __shared__ double sm[32];
-    double e[3] = {0.0, 0.0, 0.0}, w = 0.0;
-    for (int64_t p = threadIdx.x; p < n_part; p += 1024)
-        for (int i = 0; i < 3; ++i) e[i] += part[3 * p + i];
-    for (int i = 0; i < 3; ++i) e[i] = block_sum(e[i], sm);
-    for (int i = threadIdx.x; i < n_wpart; i += 1024) w += wpart[i];
-    w = block_sum(w, sm);
-    if (threadIdx.x < 3) stats[threadIdx.x] = w != 0.0 ? (A)(e[threadIdx.x] / w) : A(0);
 }
 
 // ------------------------------------------------------------- launchers --
@@ -386,48 +1075,123 @@ void with_score_types(int dtype, F&& f) {
     }
 }
 
-// f(VEC, L): 16-byte vectors where rows of scores and gradient have the same place
-// within 16 bytes; lanes per row by the number of classes.
-template <class T, class F>
-void with_shape(const void* x, int64_t ld, const void* out, int64_t ld_out, int64_t c, F&& f) {
-    constexpr int V = 16 / sizeof(T);
-    const bool alike = !out || (((uintptr_t)x - (uintptr_t)out) % 16 == 0 && (ld - ld_out) % V == 0);
-    auto lanes = [&](auto vec) {
-        if (c <= 32)
-            f(vec, std::integral_constant<int, 8>{});
-        else if (c <= 2048)
-            f(vec, std::integral_constant<int, 32>{});
-        else
-            f(vec, std::integral_constant<int, kNT>{});
+// Few classes: persistent warps over the tiles, whatever the mode.
+template <class T, class A, Mode M>
+void small_launch(int device, const T* x, int64_t ld, T* out, int64_t ld_out, const RowArgs<A>& a,
+                  cudaStream_t s) {
+    const size_t bytes = (size_t)(kSmallNT / 32) * 2 * kTileRows * a.c * sizeof(T);
+    // one wave: the blocks an SM holds, by registers or by shared memory
+    const int64_t fit = std::min<int64_t>(kSmallPerSm, (int64_t)(227 * 1024 / (bytes + 1280)));
+    const int64_t blocks = ceil_div(a.n, kTileRows * (kSmallNT / 32)), most = (int64_t)sm_count(device) * fit;
+    auto go = [&](auto w, auto turn) {
+        auto k = small_rows_kernel<T, A, decltype(w)::value, decltype(turn)::value, M>;
+        if (bytes > 48 * 1024)
+            MFM_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes), "class tile shared memory");
+        k<<<(unsigned)std::min(blocks, most), kSmallNT, bytes, s>>>(
+            x, ld, out, ld_out, a, ld == a.c && (uintptr_t)x % 16 == 0, ld_out == a.c && (uintptr_t)out % 16 == 0);
     };
-    if (alike && c > 32)
-        lanes(std::integral_constant<int, V>{});
+    auto width = [&](auto turn) {
+        if (a.c <= 4)
+            go(std::integral_constant<int, 4>{}, turn);
+        else if (a.c <= 8)
+            go(std::integral_constant<int, 8>{}, turn);
+        else if (a.c <= 12)
+            go(std::integral_constant<int, 12>{}, turn);
+        else if (a.c <= 16)
+            go(std::integral_constant<int, 16>{}, turn);
+        else
+            go(std::integral_constant<int, kSmallC>{}, turn);
+    };
+    if (a.c % 4 == 0)
+        width(std::true_type{});
     else
-        lanes(std::integral_constant<int, 1>{});
+        width(std::false_type{});
 }
 
-template <int L>
-unsigned row_blocks(int64_t n) { return (unsigned)ceil_div(n, kNT / L); }
+// Launches the row kernel for c classes of type T: by the row's bytes, the fewest
+// lanes that hold it in registers.
+template <class T, class A, Mode M>
+void rows_launch(int device, const T* x, int64_t ld, T* out, int64_t ld_out, const RowArgs<A>& a,
+                 cudaStream_t s) {
+    const int64_t n = a.n, nv = ceil_div(a.c * (int64_t)sizeof(T), 16);
+    auto cached = [&](auto k) {
+        constexpr int K = decltype(k)::value;
+        cached_rows_kernel<T, A, K, M><<<(unsigned)ceil_div(n, kNT / 32), kNT, 0, s>>>(x, ld, out, ld_out, a);
+    };
+    auto ring = [&](auto l) {
+        constexpr int L = decltype(l)::value, bytes = ring_slots(L) * L * kRingVecs * 16;
+        auto k = ring_rows_kernel<T, A, L>;
+        MFM_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes), "row ring shared memory");
+        const int64_t grid = (int64_t)sm_count(device) * ring_blocks(L);
+        k<<<(unsigned)(n < grid ? n : grid), L + 32, bytes, s>>>(x, ld, out, ld_out, a);
+    };
+    auto scan = [&]() {
+        const int64_t warps = (int64_t)sm_count(device) * 32;  // resident at once
+        auto go = [&](auto l) {
+            constexpr int L = decltype(l)::value;
+            scan_rows_kernel<T, A, L><<<(unsigned)ceil_div(n, kNT / L), kNT, 0, s>>>(x, ld, a);
+        };
+        if (n * 4 < warps)
+            go(std::integral_constant<int, kNT>{});
+        else if (nv >= 1024)
+            go(std::integral_constant<int, 128>{});
+        else if (nv >= 512)
+            go(std::integral_constant<int, 64>{});
+        else
+            go(std::integral_constant<int, 32>{});
+    };
+    using std::integral_constant;
+    if (a.c <= kSmallC)
+        small_launch<T, A, M>(device, x, ld, out, ld_out, a, s);
+    else if (nv <= 64)
+        cached(integral_constant<int, 2>{});
+    else if (nv <= 256)
+        cached(integral_constant<int, 8>{});
+    else if constexpr (M == STATS)
+        scan();
+    else if (nv <= 2560)
+        ring(integral_constant<int, kRingMost / 4>{});
+    else if (nv <= 5120)
+        ring(integral_constant<int, kRingMost / 2>{});
+    else
+        ring(integral_constant<int, kRingMost>{});
+}
 
-template <class T, class A, class I>
-void stats_launch(const T* x, int64_t ld, int64_t n, int64_t c, const I* labels, A* lp, A* lse,
-                  A* zero, cudaStream_t s) {
+template <class T, class A>
+void stats_launch(int device, const T* x, int64_t ld, int64_t n, int64_t c, Labels labels, A* lp, A* lse,
+                  A* zero, unsigned* counter, cudaStream_t s) {
     if (n == 0) return;
-    with_shape<T>(x, ld, nullptr, 0, c, [&](auto v, auto l) {
-        constexpr int V = decltype(v)::value, L = decltype(l)::value;
-        label_stats_kernel<T, A, I, V, L><<<row_blocks<L>(n), kNT, 0, s>>>(x, ld, n, c, labels, lp, lse, zero);
-    });
+    RowArgs<A> a{};
+    a.labels = labels;
+    a.n = n;
+    a.c = c;
+    a.lp = lp;
+    a.lse = lse;
+    a.zero = zero;
+    a.counter = counter;
+    rows_launch<T, A, STATS>(device, x, ld, nullptr, 0, a, s);
     MFM_CHECK_LAUNCH("label log-probabilities launch");
 }
 
-template <class T, class A, class I>
-void grad_launch(const T* x, int64_t ld, int64_t n, int64_t c, const I* labels, const A* g,
-                 const double* scale, const A* lse, T* out, int64_t ld_out, cudaStream_t s) {
+// The gradient for given g and lse: elementwise.
+template <class T, class A>
+void grad_launch(int device, const T* x, int64_t ld, int64_t n, int64_t c, Labels labels,
+                 const A* g, const double* scale, const A* lse, T* out, int64_t ld_out,
+                 cudaStream_t s) {
     if (n == 0) return;
-    with_shape<T>(x, ld, out, ld_out, c, [&](auto v, auto l) {
-        constexpr int V = decltype(v)::value, L = decltype(l)::value;
-        label_grad_kernel<T, A, I, V, L><<<row_blocks<L>(n), kNT, 0, s>>>(x, ld, n, c, labels, g, scale, lse, out, ld_out);
-    });
+    RowArgs<A> a{};
+    a.labels = labels;
+    a.n = n;
+    a.c = c;
+    a.g = g;
+    a.scale = scale;
+    a.lse_in = lse;
+    if (c <= kSmallC)
+        small_launch<T, A, GRAD>(device, x, ld, out, ld_out, a, s);
+    else if (c * (int64_t)sizeof(T) <= 4096)
+        label_grad_kernel<T, A, 32><<<(unsigned)ceil_div(n, kNT / 32), kNT, 0, s>>>(x, ld, out, ld_out, a);
+    else
+        label_grad_kernel<T, A, kNT><<<(unsigned)n, kNT, 0, s>>>(x, ld, out, ld_out, a);
     MFM_CHECK_LAUNCH("label gradient launch");
 }
 
@@ -464,11 +1228,8 @@ extern "C" int mfm_label_logprobs_device(int dtype, int device, const void* logi
         with_score_types(dtype, [&](auto* t) {
             using T = Elem<decltype(t)>;
             using A = typename Arith<T>::type;
-            with_index_type(labels64, [&](auto* i) {
-                using I = Elem<decltype(i)>;
-                stats_launch<T, A, I>((const T*)logits, ld, n_tokens, n_classes, (const I*)labels,
-                                      (A*)logprobs, (A*)lse, nullptr, s);
-            });
+            stats_launch<T, A>(device, (const T*)logits, ld, n_tokens, n_classes, Labels{labels, labels64},
+                               (A*)logprobs, (A*)lse, nullptr, nullptr, s);
             if (sums && n_seq > 0) {
                 seq_sums_kernel<A><<<(unsigned)ceil_div(n_seq, kNT / 32), kNT, 0, s>>>(
                     (const A*)logprobs, n_tokens, indptr, n_seq, (A*)sums);
@@ -492,18 +1253,15 @@ extern "C" int mfm_label_logprobs_grad_device(int dtype, int device, const void*
         with_score_types(dtype, [&](auto* t) {
             using T = Elem<decltype(t)>;
             using A = typename Arith<T>::type;
-            with_index_type(labels64, [&](auto* i) {
-                using I = Elem<decltype(i)>;
-                grad_launch<T, A, I>((const T*)logits, ld, n_tokens, n_classes, (const I*)labels,
-                                     (const A*)grad, nullptr, (const A*)lse, (T*)d_logits, ld_out,
-                                     (cudaStream_t)stream);
-            });
+            grad_launch<T, A>(device, (const T*)logits, ld, n_tokens, n_classes,
+                              Labels{labels, labels64}, (const A*)grad, nullptr, (const A*)lse,
+                              (T*)d_logits, ld_out, (cudaStream_t)stream);
         });
     });
 }
 
 namespace {
-struct PrefWs {  // log-probabilities, lse, token coefficients, pair losses, 1 / sum of weights
+struct PrefWs {  // log-probabilities, lse, token coefficients, pair losses, 1 / sum of weights and a block count
     size_t lse, g, pair, scale, bytes;
     PrefWs(int dtype, int64_t n, int64_t pairs) {
         const size_t a = up256((size_t)n * arith_size(dtype));
@@ -546,33 +1304,42 @@ extern "C" int mfm_preference_loss_device(int dtype, int device, const void* log
         char* ws = (char*)workspace;
         double* pair = (double*)(ws + W.pair);
         double* scale = (double*)(ws + W.scale);
+        unsigned* done = (unsigned*)(ws + W.scale + 8);
         with_score_types(dtype, [&](auto* t) {
             using T = Elem<decltype(t)>;
             using A = typename Arith<T>::type;
             A *lp = (A*)ws, *lse = (A*)(ws + W.lse), *coef = d_logits ? (A*)(ws + W.g) : nullptr;
-            with_index_type(labels64, [&](auto* i) {
-                using I = Elem<decltype(i)>;
-                stats_launch<T, A, I>((const T*)logits, ld, n_tokens, n_classes, (const I*)labels,
-                                      lp, lse, coef, s);
-                if (n_pairs > 0)
-                    pair_kernel<A><<<(unsigned)ceil_div(n_pairs, kNT / 32), kNT, 0, s>>>(
+            const Labels y{labels, labels64};
+            if (n_pairs == 0) zero_loss_kernel<A><<<1, 32, 0, s>>>((A*)loss, 1);
+            if (n_pairs == 0 || n_tokens == 0)
+                MFM_CUDA(cudaMemsetAsync(ws + W.scale, 0, 16, s), "memset");
+            stats_launch<T, A>(device, (const T*)logits, ld, n_tokens, n_classes, y, lp, lse, coef, done, s);
+            if (n_pairs > 0) {
+                auto pairs = [&](auto w) {
+                    constexpr int PW = decltype(w)::value;
+                    pair_kernel<A, PW><<<(unsigned)ceil_div(n_pairs, kNT / PW), kNT, 0, s>>>(
                         lp, n_tokens, indptr, n_pairs, (const A*)reference, beta, label_smoothing,
-                        (const A*)sample_weight, (A*)margins, (A*)seq_logprobs, pair, coef);
-                pair_finish_kernel<A><<<1, 1024, 0, s>>>(pair, (const A*)sample_weight, n_pairs, (A*)loss, scale);
-                MFM_CHECK_LAUNCH("preference loss launch");
-                if (d_logits)
-                    grad_launch<T, A, I>((const T*)logits, ld, n_tokens, n_classes,
-                                         (const I*)labels, coef, scale, lse, (T*)d_logits, ld_out, s);
-            });
+                        (const A*)sample_weight, (A*)margins, (A*)seq_logprobs, pair, coef, done,
+                        (A*)loss, scale);
+                };
+                if (n_tokens / (2 * n_pairs) >= 64)  // a block only where a warp would loop
+                    pairs(std::integral_constant<int, kNT>{});
+                else
+                    pairs(std::integral_constant<int, 32>{});
+            }
+            MFM_CHECK_LAUNCH("preference loss launch");
+            if (d_logits)
+                grad_launch<T, A>(device, (const T*)logits, ld, n_tokens, n_classes, y, coef, scale,
+                                  lse, (T*)d_logits, ld_out, s);
         });
     });
 }
 
 namespace {
-struct PolicyWs {  // partial weights, partial loss terms
+struct PolicyWs {  // partial weights and a block count, partial loss terms
     size_t part, bytes;
     explicit PolicyWs(int64_t n) {
-        part = up256(kWeightBlocks * 8);
+        part = up256(kWeightBlocks * 8 + 8);
         bytes = part + up256((size_t)n * 24);
     }
 };
@@ -607,26 +1374,34 @@ extern "C" int mfm_policy_loss_device(int dtype, int device, const void* logits,
         cudaStream_t s = (cudaStream_t)stream;
         char* ws = (char*)workspace;
         double *wpart = (double*)ws, *part = (double*)(ws + W.part);
-        const int nw = (int)std::min<int64_t>(kWeightBlocks, ceil_div(n_tokens, kNT));
+        unsigned* done = (unsigned*)(wpart + kWeightBlocks);
+        const int nw = (int)std::min<int64_t>(kWeightBlocks, ceil_div(n_tokens, 8 * kNT));
         with_score_types(dtype, [&](auto* t) {
             using T = Elem<decltype(t)>;
             using A = typename Arith<T>::type;
-            int64_t n_part = 0;
-            if (n_tokens > 0)
-                with_index_type(labels64, [&](auto* i) {
-                    using I = Elem<decltype(i)>;
-                    weight_kernel<A, I><<<nw, kNT, 0, s>>>((const I*)labels, n_classes, (const A*)sample_weight, n_tokens, wpart);
-                    with_shape<T>(logits, ld, d_logits, ld_out, n_classes, [&](auto v, auto l) {
-                        constexpr int V = decltype(v)::value, L = decltype(l)::value;
-                        n_part = row_blocks<L>(n_tokens);
-                        policy_kernel<T, A, I, V, L><<<(unsigned)n_part, kNT, 0, s>>>(
-                            (const T*)logits, ld, n_tokens, n_classes, (const I*)labels,
-                            (const A*)old_logprobs, (const A*)advantages, (const A*)reference,
-                            PolicyArgs{clip_low, clip_high, kl_coef}, (const A*)sample_weight,
-                            wpart, nw, part, (A*)logprobs, (T*)d_logits, ld_out);
-                    });
-                });
-            policy_finish_kernel<A><<<1, 1024, 0, s>>>(part, n_part, wpart, nw, (A*)stats);
+            if (n_tokens == 0) {
+                zero_loss_kernel<A><<<1, 32, 0, s>>>((A*)stats, 3);
+            } else {
+                RowArgs<A> a{};
+                a.labels = Labels{labels, labels64};
+                a.n = n_tokens;
+                a.c = n_classes;
+                a.lp = (A*)logprobs;
+                a.old = (const A*)old_logprobs;
+                a.adv = (const A*)advantages;
+                a.ref = (const A*)reference;
+                a.weight = (const A*)sample_weight;
+                a.clip_lo = (A)(1.0 - clip_low);
+                a.clip_hi = (A)(1.0 + clip_high);
+                a.kl_coef = (A)kl_coef;
+                a.wpart = wpart;
+                a.n_wpart = nw;
+                a.part = part;
+                a.stats = (A*)stats;
+                a.done = done;
+                weight_kernel<A><<<nw, kNT, 0, s>>>(a.labels, n_classes, a.weight, n_tokens, wpart, done);
+                rows_launch<T, A, POLICY>(device, (const T*)logits, ld, (T*)d_logits, ld_out, a, s);
+            }
             MFM_CHECK_LAUNCH("policy loss launch");
         });
     });
