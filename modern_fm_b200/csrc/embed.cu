@@ -1,6 +1,11 @@
 // embed.cu — latent rows as outputs: embedding lookup with scaling (single
 // rows, or summed over the entries of sparse rows) and its gradient by sorted
 // ids, over the whole table or the touched rows only.
+//
+// Everything here moves rows: a multiply and an add per value against 2 to 16
+// bytes, so HBM bounds the large calls and latency (ids, then rows) the small
+// ones. Rows are walked in 16-byte vectors by lane groups, several entries in
+// flight per lane.
 #include "embed_sort.cuh"
 
 #include <algorithm>
@@ -8,49 +13,129 @@
 namespace mfm {
 namespace {
 
+// ---------------------------------------------------------------- vectors --
+
+// N = 16 / sizeof(T) values, or one where rows are not 16-byte aligned, held raw.
+template <class T, bool WIDE>
+struct Lane {
+    static constexpr int N = WIDE ? 16 / (int)sizeof(T) : 1;
+    uint4 raw;
+    T one;
+    __device__ __forceinline__ void load(const T* p) {
+        if (WIDE)
+            raw = *reinterpret_cast<const uint4*>(p);
+        else
+            one = *p;
+    }
+    template <class A>
+    __device__ __forceinline__ void get(A (&v)[N]) const {
+        if constexpr (WIDE) {
+            typename Arith<T>::type w[N];
+            Pack<T>::unpack(raw, w);
+#pragma unroll
+            for (int j = 0; j < N; ++j) v[j] = (A)w[j];
+        } else {
+            v[0] = widen<A>(one);
+        }
+    }
+};
+
+// N values to `to` (aligned to N of them), each rounded once.
+template <class O, class A, int N>
+__device__ __forceinline__ void put(O* to, const A (&v)[N]) {
+    constexpr int P = 16 / (int)sizeof(O);
+    if constexpr (N == 1) {
+        *to = narrow<O>(v[0]);
+    } else if constexpr (N < P) {
+        Vec<O, N> o;
+#pragma unroll
+        for (int j = 0; j < N; ++j) o.v[j] = narrow<O>(v[j]);
+        *reinterpret_cast<Vec<O, N>*>(to) = o;
+    } else {
+#pragma unroll
+        for (int k = 0; k < N / P; ++k) {
+            typename Arith<O>::type w[P];
+#pragma unroll
+            for (int j = 0; j < P; ++j) w[j] = v[k * P + j];
+            *reinterpret_cast<uint4*>(to + k * P) = Pack<O>::pack(w);
+        }
+    }
+}
+
 // ---------------------------------------------------------------- lookup --
 
-// out[t] = alpha scale[t] table[ids[t]]. One thread per vector of VEC elements,
-// U of them in flight.
-template <class T, class A, class O, class I, int VEC, int U>
+// out[t] = alpha scale[t] table[ids[t]], rows of at least 32 vectors: a warp per
+// (row, piece of 32 U vectors), U vectors a lane in flight.
+template <class T, class A, class O, class I, int U>
+__global__ void __launch_bounds__(256)
+    embed_wide_kernel(const I* __restrict__ ids, int64_t n, const A* __restrict__ scale, A alpha,
+                      const T* __restrict__ table, int64_t n_rows, int dv, int pieces, int64_t ld,
+                      O* __restrict__ out, int64_t ld_out) {
+    constexpr int N = Lane<T, true>::N;
+    const int64_t item = ((int64_t)blockIdx.x * 256 + threadIdx.x) / 32;
+    const int64_t t = item / pieces;
+    if (t >= n) return;
+    const int j0 = (int)(item - t * pieces) * (32 * U) + (threadIdx.x & 31);
+    const int64_t id = (int64_t)ids[t];
+    const bool live = id >= 0 && id < n_rows;
+    A f = alpha;
+    if (scale) f *= scale[t];
+    const T* from = table + (live ? id : 0) * ld;
+    O* to = out + t * ld_out;
+    Lane<T, true> v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+        if (live && j0 + u * 32 < dv) v[u].load(from + (int64_t)(j0 + u * 32) * N);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+        if (j0 + u * 32 < dv) {
+            A p[N];
+            v[u].get(p);
+#pragma unroll
+            for (int j = 0; j < N; ++j) p[j] = live ? f * p[j] : A(0);
+            put(to + (int64_t)(j0 + u * 32) * N, p);
+        }
+}
+
+// The same for narrow or unaligned rows: one thread per vector (or value), U in
+// flight, 256 apart.
+template <class T, class A, class O, class I, bool WIDE, int U>
 __global__ void __launch_bounds__(256)
     embed_rows_kernel(const I* __restrict__ ids, int64_t n, const A* __restrict__ scale, A alpha,
                       const T* __restrict__ table, int64_t n_rows, uint32_t dv, int64_t ld,
                       O* __restrict__ out, int64_t ld_out) {
+    constexpr int N = Lane<T, WIDE>::N;
     const int64_t first = (int64_t)blockIdx.x * (256 * U);
     const int64_t row0 = first / dv;
     const uint32_t off0 = (uint32_t)(first - row0 * dv);
-    Vec<T, VEC> v[U];
+    Lane<T, WIDE> v[U];
     A f[U];
-    int64_t row[U];
-    uint32_t col[U];
+    bool live[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-        const uint32_t o = off0 + threadIdx.x + u * 256;
-        const uint32_t r = o / dv;
-        row[u] = row0 + r;
-        col[u] = (o - r * dv) * VEC;
-        f[u] = A(0);
-        if (row[u] < n) {
-            const int64_t id = (int64_t)ids[row[u]];
-            if (id >= 0 && id < n_rows) {
-                v[u] = ldg_vec<T, VEC>(table + id * ld + col[u]);
-                f[u] = alpha;
-                if (scale) f[u] *= scale[row[u]];
-            } else {
-#pragma unroll
-                for (int j = 0; j < VEC; ++j) v[u].v[j] = narrow<T>(A(0));
-            }
+        const uint32_t o = off0 + threadIdx.x + u * 256, r = o / dv;
+        const int64_t row = row0 + r;
+        live[u] = false;
+        f[u] = alpha;
+        if (row < n) {
+            const int64_t id = (int64_t)ids[row];
+            live[u] = id >= 0 && id < n_rows;
+            if (live[u]) v[u].load(table + id * ld + (int64_t)(o - r * dv) * N);
+            if (scale) f[u] *= scale[row];
         }
     }
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-        if (row[u] < n) {
-            Vec<O, VEC> o;
+    for (int u = 0; u < U; ++u) {
+        const uint32_t o = off0 + threadIdx.x + u * 256, r = o / dv;
+        const int64_t row = row0 + r;
+        if (row < n) {
+            A p[N];
+            v[u].get(p);
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) o.v[j] = narrow<O>(f[u] * widen<A>(v[u].v[j]));
-            *reinterpret_cast<Vec<O, VEC>*>(out + row[u] * ld_out + col[u]) = o;
+            for (int j = 0; j < N; ++j) p[j] = live[u] ? f[u] * p[j] : A(0);
+            put(out + row * ld_out + (int64_t)(o - r * dv) * N, p);
         }
+    }
 }
 
 // Bounds of a row's entries, limited to the entries there are.
@@ -62,233 +147,500 @@ __device__ __forceinline__ void row_bounds(const int64_t* indptr, int64_t b, int
     hi = hi < lo ? lo : (hi > n ? n : hi);
 }
 
-// out[b] = alpha sum_t scale[t] table[ids[t]]: LV lanes per row, each a vector of
-// VEC columns, four entries in flight; blockIdx.y walks the columns.
-template <class T, class A, class O, class I, int VEC, int LV>
-__global__ void __launch_bounds__(256)
+// out[b] = alpha sum_t scale[t] table[ids[t]]. EL x LV lanes per row: LV lanes hold
+// the columns (a vector each; blockIdx.y walks them), EL take every EL-th entry, U
+// entries a lane in flight; their parts are added by shuffles. Bound by the
+// latency of the rows' gathers: 131072 rows of 36 entries, 16 float32 each in
+// float64 arithmetic, 54 us (62 us with a round's ids fetched just before its rows;
+// 67 us with EL = 4, 84 us at five blocks per SM).
+template <class T, class A, class O, class I, bool WIDE, int LV, int EL>
+__global__ void __launch_bounds__(256, 4)
     embed_sums_kernel(const I* __restrict__ ids, int64_t n, const int64_t* __restrict__ indptr,
                       int64_t n_out, const A* __restrict__ scale, A alpha,
                       const T* __restrict__ table, int64_t n_rows, int64_t d, int64_t ld,
                       O* __restrict__ out, int64_t ld_out) {
-    constexpr int U = 4;
-    const int lane = threadIdx.x % LV;
-    const int64_t b = (int64_t)blockIdx.x * (256 / LV) + threadIdx.x / LV;
-    const int64_t col = ((int64_t)blockIdx.y * LV + lane) * VEC;
-    if (b >= n_out || col >= d) return;
-    int64_t lo, hi;
-    row_bounds(indptr, b, n, lo, hi);
-    A acc[VEC];
+    constexpr int U = 4, G = LV * EL, N = Lane<T, WIDE>::N;
+    const int lane = threadIdx.x % LV, el = threadIdx.x % G / LV;
+    const int64_t b = (int64_t)blockIdx.x * (256 / G) + threadIdx.x / G;
+    const int64_t col = ((int64_t)blockIdx.y * LV + lane) * N;
+    const bool in = b < n_out && col < d;
+    int64_t lo = 0, hi = 0;
+    if (in) row_bounds(indptr, b, n, lo, hi);
+    A acc[N];
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) acc[j] = A(0);
-    for (int64_t e = lo; e < hi; e += U) {
-        Vec<T, VEC> v[U];
-        A f[U];
+    for (int j = 0; j < N; ++j) acc[j] = A(0);
+    // the next round's ids and scales are on their way while a round's rows are
+    I id[U];
+    A f[U];
+    auto fetch = [&](int64_t e) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            id[u] = -1;
+            f[u] = A(1);
+            if (e + u * EL < hi) {
+                id[u] = ids[e + u * EL];
+                if (scale) f[u] = scale[e + u * EL];
+            }
+        }
+    };
+    fetch(lo + el);
+    for (int64_t e = lo + el; e < hi; e += U * EL) {
+        Lane<T, WIDE> v[U];
+        A w[U];
         bool live[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            live[u] = false;
-            f[u] = A(1);
-            if (e + u < hi) {
-                const int64_t id = (int64_t)ids[e + u];
-                live[u] = id >= 0 && id < n_rows;
-                if (scale) f[u] = scale[e + u];
-                if (live[u]) v[u] = ldg_vec<T, VEC>(table + id * ld + col);
-            }
+            live[u] = id[u] >= 0 && id[u] < n_rows;
+            if (live[u]) v[u].load(table + (int64_t)id[u] * ld + col);
+            w[u] = f[u];
         }
+        fetch(e + U * EL);
 #pragma unroll
         for (int u = 0; u < U; ++u)
-            if (live[u])
+            if (live[u]) {
+                A p[N];
+                v[u].get(p);
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) acc[j] += f[u] * widen<A>(v[u].v[j]);
+                for (int j = 0; j < N; ++j) acc[j] += w[u] * p[j];
+            }
     }
-    Vec<O, VEC> o;
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) o.v[j] = narrow<O>(alpha * acc[j]);
-    *reinterpret_cast<Vec<O, VEC>*>(out + b * ld_out + col) = o;
+    for (int o = G / 2; o >= LV; o >>= 1)
+#pragma unroll
+        for (int j = 0; j < N; ++j) acc[j] += __shfl_xor_sync(0xffffffffu, acc[j], o);
+    if (in && el == 0) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) acc[j] *= alpha;
+        put(out + b * ld_out + col, acc);
+    }
 }
 
 // -------------------------------------------------------------- gradient --
 
-constexpr int kChunk = 32;  // sorted entries per lane group
+// Sorted entries per lane group: short enough that a batch of a few thousand ids
+// fills the GPU, long enough that the parts of runs cut by chunk bounds (two rows
+// of sums a chunk) stay an eighth of the reading.
+constexpr int kChunk = 16;
+constexpr int kHeadTile = 4096;             // entries per block of chunk_heads_kernel
+constexpr int kTileChunks = kHeadTile / kChunk;
+constexpr int kMainNT = 128;
 
-// row_of[t] = the output row whose sum entry t belongs to, -1 for none.
-__global__ void entry_rows_kernel(const int64_t* __restrict__ indptr, int64_t n_out, int64_t n,
-                                  int32_t* __restrict__ row_of) {
-    const int64_t stride = (int64_t)gridDim.x * blockDim.x / 32;
-    for (int64_t b = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) / 32; b < n_out; b += stride) {
-        int64_t lo, hi;
-        row_bounds(indptr, b, n, lo, hi);
-        for (int64_t t = lo + (threadIdx.x & 31); t < hi; t += 32) row_of[t] = (int32_t)b;
-    }
-}
-
-// heads[c] = how many runs of equal real keys begin in chunk c.
-__global__ void chunk_heads_kernel(const uint32_t* __restrict__ keys, int64_t n, uint32_t pad_key,
-                                   int64_t n_chunks, uint32_t* __restrict__ heads) {
-    const int64_t c = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) / 32;
-    const int64_t e = c * kChunk + (threadIdx.x & 31);
-    bool head = false;
-    if (e < n) {
-        const uint32_t k = keys[e];
-        head = k != pad_key && (e == 0 || keys[e - 1] != k);
-    }
-    const unsigned m = __ballot_sync(0xffffffffu, head);
-    if ((threadIdx.x & 31) == 0 && c < n_chunks) heads[c] = (uint32_t)__popc(m);
-}
-
-template <class O, class I>
-struct GradOut {  // where a finished run goes
-    O* table;          // (n_rows, d), or
-    O* rows;           // (cap, d) by rank with
-    I* keys;           // the ids
-    const uint32_t* base;  // runs begun before each chunk
-};
-
-// One chunk of kChunk sorted entries x LV * VEC columns by one lane group: sums
-// of scale[pos] grad[row], run by run. A run that lies in the chunk is
-// written; the part of a run that began before goes to part_head[chunk], the
-// part of one that goes on behind to part_tail[chunk] (all of it to part_head
-// when both).
-template <class G, class A, class O, class I, int VEC, int LV>
-__global__ void __launch_bounds__(128)
-    embed_reduce_kernel(const uint32_t* __restrict__ keys, const uint32_t* __restrict__ pos,
-                        int64_t n, uint32_t pad_key, const int32_t* __restrict__ row_of,
-                        const A* __restrict__ scale, A alpha, const G* __restrict__ grad,
-                        int64_t ld, int64_t d, int64_t n_chunks, A* __restrict__ part_head,
-                        A* __restrict__ part_tail, GradOut<O, I> out) {
-    constexpr int U = 8;
-    const int lane = threadIdx.x % LV;
-    const int64_t c = (int64_t)blockIdx.x * (128 / LV) + threadIdx.x / LV;
-    const int64_t col = ((int64_t)blockIdx.y * LV + lane) * VEC;
-    if (c >= n_chunks || col >= d) return;
-    const int64_t e0 = c * kChunk, e1 = e0 + kChunk < n ? e0 + kChunk : n;
-    uint32_t cur = keys[e0];
-    bool begun_before = e0 > 0 && keys[e0 - 1] == cur;
-    uint32_t rank = out.rows ? out.base[c] - (begun_before ? 1u : 0u) : 0u;
-    A acc[VEC];
+// base[c] = how many runs of equal real keys begin before chunk c within its tile
+// of kHeadTile entries; tile_base[t] = how many before tile t, by the block that
+// finishes last, and *count = all of them.
+__global__ void __launch_bounds__(kTileChunks)
+    chunk_heads_kernel(const uint32_t* __restrict__ keys, int64_t n, uint32_t pad_key,
+                       int64_t n_chunks, uint32_t* __restrict__ base,
+                       uint32_t* __restrict__ tile_base, unsigned* __restrict__ done,
+                       int64_t* __restrict__ count) {
+    __shared__ uint32_t sm[kTileChunks / 32];
+    __shared__ unsigned last;
+    const int64_t c = (int64_t)blockIdx.x * kTileChunks + threadIdx.x, e0 = c * kChunk;
+    uint32_t heads = 0;
+    if (e0 < n) {
+        uint32_t prev = e0 > 0 ? keys[e0 - 1] : pad_key;  // pad_key is no run
+        uint32_t k[kChunk];
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) acc[j] = A(0);
-    auto put = [&](uint32_t key) {  // a run ends inside the chunk
-        if (begun_before) {
-            Vec<A, VEC> p;
+        for (int i = 0; i < kChunk; ++i) k[i] = e0 + i < n ? keys[e0 + i] : pad_key;
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) p.v[j] = acc[j];
-            *reinterpret_cast<Vec<A, VEC>*>(part_head + c * d + col) = p;
-        } else {
-            Vec<O, VEC> o;
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) o.v[j] = narrow<O>(alpha * acc[j]);
-            O* base = out.rows ? out.rows + (int64_t)rank * d : out.table + (int64_t)key * d;
-            *reinterpret_cast<Vec<O, VEC>*>(base + col) = o;
-        }
-        if (out.keys && !begun_before && col == 0) out.keys[rank] = (I)key;
-    };
-    for (int64_t e = e0; e < e1; e += U) {
-        uint32_t k[U];
-        A f[U];
-        Vec<G, VEC> v[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            k[u] = pad_key;
-            f[u] = A(1);
-            if (e + u < e1) k[u] = keys[e + u];
-            if (k[u] != pad_key) {
-                const uint32_t p = pos[e + u];
-                const int64_t row = row_of ? (int64_t)row_of[p] : (int64_t)p;
-                if (scale) f[u] = scale[p];
-                v[u] = ldg_vec<G, VEC>(grad + row * ld + col);
-            }
-        }
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            if (e + u >= e1) break;
-            if (k[u] != cur) {
-                put(cur);
-                cur = k[u];
-                begun_before = false;
-                ++rank;
-#pragma unroll
-                for (int j = 0; j < VEC; ++j) acc[j] = A(0);
-            }
-            if (cur == pad_key) return;  // padding sorts last
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) acc[j] += f[u] * widen<A>(v[u].v[j]);
+        for (int i = 0; i < kChunk; ++i) {
+            heads += k[i] != pad_key && k[i] != prev ? 1u : 0u;
+            prev = k[i];
         }
     }
-    if (e1 < n && keys[e1] == cur) {  // the run goes on behind the chunk
-        Vec<A, VEC> p;
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) p.v[j] = acc[j];
-        A* part = begun_before ? part_head : part_tail;
-        *reinterpret_cast<Vec<A, VEC>*>(part + c * d + col) = p;
-    } else {
-        put(cur);
+    uint32_t all;
+    const uint32_t ex = block_exclusive_scan<uint32_t, kTileChunks>(heads, sm, all);
+    if (c < n_chunks) base[c] = ex;
+    if (threadIdx.x == 0) {
+        tile_base[blockIdx.x] = all;
+        __threadfence();
+        last = atomicAdd(done, 1u) == gridDim.x - 1 ? 1u : 0u;
     }
+    __syncthreads();
+    if (!last) return;
+    __threadfence();
+    uint32_t carry = 0;
+    for (unsigned b = 0; b < gridDim.x; b += kTileChunks) {
+        const unsigned t = b + threadIdx.x;
+        const uint32_t v = t < gridDim.x ? __ldcg(tile_base + t) : 0u;
+        const uint32_t x = block_exclusive_scan<uint32_t, kTileChunks>(v, sm, all);
+        if (t < gridDim.x) tile_base[t] = carry + x;
+        carry += all;
+    }
+    if (threadIdx.x == 0) *count = carry;
 }
 
-// The runs that cross chunks: the lane group of the chunk where one begins adds
-// its parts in chunk order and writes the run.
-template <class A, class O, class I, int VEC, int LV>
-__global__ void __launch_bounds__(128)
-    embed_cross_kernel(const uint32_t* __restrict__ keys, int64_t n, uint32_t pad_key, A alpha,
-                       int64_t d, int64_t n_chunks, const A* __restrict__ part_head,
-                       const A* __restrict__ part_tail, GradOut<O, I> out) {
-    const int lane = threadIdx.x % LV;
-    const int64_t c = (int64_t)blockIdx.x * (128 / LV) + threadIdx.x / LV;
-    const int64_t col = ((int64_t)blockIdx.y * LV + lane) * VEC;
-    if (c + 1 >= n_chunks || col >= d) return;
-    const int64_t e0 = c * kChunk, e1 = e0 + kChunk;  // not the last chunk: e1 < n
-    const uint32_t key = keys[e1 - 1];
-    if (key == pad_key || keys[e1] != key) return;
-    if (e0 > 0 && keys[e0 - 1] == key) return;  // began before this chunk
-    int64_t lo = e1, hi = n;  // first entry behind the run
+// First place in the sorted keys whose key is at least k, in [lo, hi).
+__device__ __forceinline__ int64_t first_at_least(const uint32_t* keys, int64_t lo, int64_t hi,
+                                                  uint32_t k) {
     while (lo < hi) {
-        const int64_t mid = lo + (hi - lo) / 2;
-        if (keys[mid] > key)
+        const int64_t mid = (lo + hi) >> 1;
+        if (keys[mid] >= k)
             hi = mid;
         else
             lo = mid + 1;
     }
-    const int64_t last = (lo - 1) / kChunk;
-    Vec<A, VEC> acc = ldg_vec<A, VEC>(part_tail + c * d + col);
-#pragma unroll 8
-    for (int64_t k = c + 1; k <= last; ++k) {
-        const Vec<A, VEC> p = ldg_vec<A, VEC>(part_head + k * d + col);
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) acc.v[j] += p.v[j];
-    }
-    const int64_t at = out.rows ? (int64_t)out.base[c + 1] - 1 : (int64_t)key;
-    Vec<O, VEC> o;
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) o.v[j] = narrow<O>(alpha * acc.v[j]);
-    *reinterpret_cast<Vec<O, VEC>*>((out.rows ? out.rows : out.table) + at * d + col) = o;
-    if (out.keys && col == 0) out.keys[at] = (I)key;
+    return lo;
 }
 
-__global__ void run_count_kernel(const uint32_t* base, int64_t n_chunks, int64_t* count) {
-    *count = base[n_chunks];
-}
-
-// d_scale[t] = alpha <grad[row(t)], table[ids[t]]>: one warp per entry.
-template <class G, class T, class A, class I, int VEC>
-__global__ void __launch_bounds__(256)
-    embed_scale_kernel(const I* __restrict__ ids, int64_t n, const int32_t* __restrict__ row_of,
-                       A alpha, const G* __restrict__ grad, int64_t ld, const T* __restrict__ table,
-                       int64_t n_rows, int64_t ld_table, int64_t d, A* __restrict__ d_scale) {
+// The same for two keys k0 <= k1 by a whole warp: 32 probes a round for each.
+__device__ __forceinline__ void warp_range(const uint32_t* keys, int64_t n, uint32_t k0, uint32_t k1,
+                                           int64_t& first, int64_t& behind) {
     const int lane = threadIdx.x & 31;
-    const int64_t t = (int64_t)blockIdx.x * 8 + threadIdx.x / 32;
-    if (t >= n) return;
-    const int64_t id = (int64_t)ids[t], row = row_of ? (int64_t)row_of[t] : t;
-    A acc = A(0);
-    if (id >= 0 && id < n_rows && row >= 0)
-        for (int64_t c = (int64_t)lane * VEC; c < d; c += 32 * VEC) {
-            const Vec<G, VEC> g = ldg_vec<G, VEC>(grad + row * ld + c);
-            const Vec<T, VEC> v = ldg_vec<T, VEC>(table + id * ld_table + c);
+    int64_t lo0 = 0, lo1 = 0, len0 = n, len1 = n;  // the answers are in [lo, lo + len]
+    while (len0 > 0 || len1 > 0) {
+        const int64_t s0 = (len0 + 31) / 32, s1 = (len1 + 31) / 32;
+        const int64_t p0 = (lane + 1) * s0, p1 = (lane + 1) * s1;  // probes end the 32 parts
+        const bool less0 = len0 > 0 && p0 <= len0 && keys[lo0 + p0 - 1] < k0;
+        const bool less1 = len1 > 0 && p1 <= len1 && keys[lo1 + p1 - 1] < k1;
+        const int n0 = __popc(__ballot_sync(0xffffffffu, less0)), n1 = __popc(__ballot_sync(0xffffffffu, less1));
+        // n parts lie before the answer; it is in the next part, or at its last place
+        lo0 += n0 * s0;
+        lo1 += n1 * s1;
+        const int64_t r0 = len0 - n0 * s0, r1 = len1 - n1 * s1;
+        len0 = r0 < s0 - 1 ? (r0 > 0 ? r0 : 0) : s0 - 1;
+        len1 = r1 < s1 - 1 ? (r1 > 0 ? r1 : 0) : s1 - 1;
+        if (s0 == 0) len0 = 0;
+        if (s1 == 0) len1 = 0;
+    }
+    first = lo0;
+    behind = lo1;
+}
+
+template <class G, class T, class A, class O, class I>
+struct GradArgs {
+    Entries<I> in;
+    const A* scale;
+    A alpha;
+    const G* grad;
+    int64_t ld;
+    const T* table;
+    int64_t ld_table, d;
+    O *d_table, *rows;
+    I* keys_out;
+    int64_t* count;
+    A* d_scale;
+    // sorted entries
+    const uint32_t *keys, *pos;
+    const int32_t* row_of;
+    const uint32_t *base, *tile_base;
+    A *part_head, *part_tail;
+    int64_t n_chunks;
+    unsigned reduce_blocks, scale_blocks, fill_blocks;  // of the main kernel
+    int fill_per;                                       // rows per warp that fills
+    __device__ __forceinline__ int64_t runs_before(int64_t c) const {
+        return (int64_t)tile_base[c / kTileChunks] + base[c];
+    }
+};
+
+// One chunk of sorted entries x LV vectors of columns by one lane group: sums of
+// scale[pos] grad[row], run by run. A run that lies in the chunk is written; the
+// part of a run that began before goes to part_head[chunk], the part of one that
+// goes on behind to part_tail[chunk] (all of it to part_head when both).
+template <class G, class T, class A, class O, class I, bool WIDE, int LV>
+__device__ __forceinline__ void reduce_chunk(const GradArgs<G, T, A, O, I>& a, int64_t c, int64_t col,
+                                             bool first_lane) {
+    constexpr int U = 8, N = Lane<G, WIDE>::N;
+    const uint32_t pad_key = (uint32_t)a.in.n_rows;
+    const int64_t n = a.in.n, e0 = c * kChunk, e1 = e0 + kChunk < n ? e0 + kChunk : n;
+    uint32_t cur = a.keys[e0];
+    if (cur == pad_key) return;  // padding sorts last
+    bool before = e0 > 0 && a.keys[e0 - 1] == cur;
+    const bool behind = e1 < n;
+    const uint32_t next = behind ? a.keys[e1] : pad_key;
+    int64_t rank = a.rows ? a.runs_before(c) - (before ? 1 : 0) : 0;
+    A acc[N];
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) acc += widen<A>(g.v[j]) * widen<A>(v.v[j]);
+    for (int j = 0; j < N; ++j) acc[j] = A(0);
+    auto part = [&](A* to) {
+        Vec<A, N> p;
+#pragma unroll
+        for (int j = 0; j < N; ++j) p.v[j] = acc[j];
+        *reinterpret_cast<Vec<A, N>*>(to + c * a.d + col) = p;
+    };
+    auto finish = [&]() {  // a run ends inside the chunk
+        if (before) {
+            part(a.part_head);
+        } else {
+#pragma unroll
+            for (int j = 0; j < N; ++j) acc[j] *= a.alpha;
+            put((a.rows ? a.rows + rank * a.d : a.d_table + (int64_t)cur * a.d) + col, acc);
+            if (a.keys_out && first_lane) a.keys_out[rank] = (I)cur;
         }
-    acc = warp_sum(acc);
-    if (lane == 0) d_scale[t] = alpha * acc;
+    };
+#pragma unroll
+    for (int b = 0; b < kChunk; b += U) {
+        if (e0 + b >= e1) break;
+        uint32_t k[U];
+        A f[U];
+        Lane<G, WIDE> v[U];
+        uint32_t p[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const bool in = e0 + b + u < e1;
+            k[u] = in ? a.keys[e0 + b + u] : pad_key;
+            p[u] = in ? a.pos[e0 + b + u] : 0u;
+        }
+        int64_t row[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            row[u] = a.row_of && k[u] != pad_key ? (int64_t)a.row_of[p[u]] : (int64_t)p[u];
+            f[u] = a.scale && k[u] != pad_key ? a.scale[p[u]] : A(1);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (k[u] != pad_key) v[u].load(a.grad + row[u] * a.ld + col);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (e0 + b + u < e1 && cur != pad_key) {
+                if (k[u] != cur) {
+                    finish();
+                    cur = k[u];
+                    before = false;
+                    ++rank;
+#pragma unroll
+                    for (int j = 0; j < N; ++j) acc[j] = A(0);
+                }
+                if (cur != pad_key) {
+                    A w[N];
+                    v[u].get(w);
+#pragma unroll
+                    for (int j = 0; j < N; ++j) acc[j] += f[u] * w[j];
+                }
+            }
+        }
+    }
+    if (cur == pad_key) return;
+    if (behind && next == cur)  // the run goes on behind the chunk
+        part(before ? a.part_head : a.part_tail);
+    else
+        finish();
+}
+
+// Zeros for the rows of the result that no run writes: table rows without an
+// entry (a warp per `per` <= 32 rows, found by bisection among the sorted keys), or the
+// places behind the last touched row. Each row of the result is written once.
+template <class G, class T, class A, class O, class I>
+__device__ __forceinline__ void fill_rest(const GradArgs<G, T, A, O, I>& a, int per, int64_t warp,
+                                          int64_t n_warps) {
+    const int lane = threadIdx.x & 31;
+    auto clear = [&](O* row) {
+        const int64_t bytes = a.d * (int64_t)sizeof(O);
+        char* p = reinterpret_cast<char*>(row);
+        if (bytes % 16 == 0 && (uintptr_t)p % 16 == 0) {
+            for (int64_t i = lane; i < bytes / 16; i += 32) reinterpret_cast<uint4*>(p)[i] = make_uint4(0, 0, 0, 0);
+        } else {
+            for (int64_t i = lane; i < a.d; i += 32) row[i] = narrow<O>(A(0));
+        }
+    };
+    if (a.rows) {
+        const int64_t used = *a.count, cap = a.in.n < a.in.n_rows ? a.in.n : a.in.n_rows;
+        for (int64_t r0 = used + warp * per; r0 < cap; r0 += n_warps * per) {
+            const int m = (int)(cap - r0 < per ? cap - r0 : per);
+            if (lane < m) a.keys_out[r0 + lane] = (I)-1;
+            if (a.d * (int64_t)sizeof(O) >= 512) {
+                for (int i = 0; i < m; ++i) clear(a.rows + (r0 + i) * a.d);
+            } else {  // short rows: together one stretch
+                O* at = a.rows + r0 * a.d;
+                const int64_t total = m * a.d;
+                if (total * sizeof(O) % 16 == 0 && (uintptr_t)at % 16 == 0) {
+                    for (int64_t i = lane; i < total * (int64_t)sizeof(O) / 16; i += 32)
+                        reinterpret_cast<uint4*>(at)[i] = make_uint4(0, 0, 0, 0);
+                } else {
+                    for (int64_t i = lane; i < total; i += 32) at[i] = narrow<O>(A(0));
+                }
+            }
+        }
+    } else {
+        const int64_t n = a.in.n, n_rows = a.in.n_rows;
+        for (int64_t r0 = warp * per; r0 < n_rows; r0 += n_warps * per) {
+            // all these rows' entries lie between the first of r0 and the first of r0 + per
+            const int64_t end = r0 + per < n_rows ? r0 + per : n_rows;
+            int64_t lo, hi;
+            warp_range(a.keys, n, (uint32_t)r0, (uint32_t)end, lo, hi);
+            unsigned touched = 0;
+            if (hi - lo > 1024) {  // popular ids: a bisection per row
+                if (lane < end - r0) {
+                    const uint32_t r = (uint32_t)(r0 + lane);
+                    const int64_t at = first_at_least(a.keys, lo, hi, r);
+                    if (at < hi && a.keys[at] == r) touched = 1u << lane;
+                }
+            } else {
+#pragma unroll 4
+                for (int64_t i = lo + lane; i < hi; i += 32) touched |= 1u << (a.keys[i] - (uint32_t)r0);
+            }
+            touched = __reduce_or_sync(0xffffffffu, touched);
+            unsigned m = ~touched & (end - r0 == 32 ? 0xffffffffu : (1u << (end - r0)) - 1u);
+            if (m == 0xffffffffu && a.d * (int64_t)sizeof(O) < 512 && a.d * sizeof(O) % 16 == 0 &&
+                (uintptr_t)(a.d_table + r0 * a.d) % 16 == 0) {
+                uint4* at = reinterpret_cast<uint4*>(a.d_table + r0 * a.d);
+                for (int i = lane; i < (int)(a.d * sizeof(O) * 2); i += 32) at[i] = make_uint4(0, 0, 0, 0);
+            } else {
+                for (; m; m &= m - 1) clear(a.d_table + (r0 + __ffs(m) - 1) * a.d);
+            }
+        }
+    }
+}
+
+// d_scale[t] = alpha <grad[row(t)], table[ids[t]]>: LV lanes per entry.
+template <class G, class T, class A, class O, class I, bool WIDE, int LV>
+__device__ __forceinline__ void scale_entry(const GradArgs<G, T, A, O, I>& a, int64_t t, int lane) {
+    constexpr int N = Lane<G, WIDE>::N;
+    A acc = A(0);
+    if (t < a.in.n) {
+        const int64_t id = (int64_t)a.in.ids[t], row = a.row_of ? (int64_t)a.row_of[t] : t;
+        if (id >= 0 && id < a.in.n_rows && row >= 0) {
+            const G* g = a.grad + row * a.ld;
+            const T* v = a.table + id * a.ld_table;
+#pragma unroll 4
+            for (int64_t c = (int64_t)lane * N; c < a.d; c += LV * N) {
+                Lane<G, WIDE> x;
+                x.load(g + c);
+                A p[N], q[N];
+                x.get(p);
+                if constexpr (sizeof(T) == sizeof(G)) {
+                    Lane<T, WIDE> y;
+                    y.load(v + c);
+                    y.get(q);
+                } else {  // a float32 table with float64 gradients: half a vector
+                    const Vec<T, N> y = ldg_vec<T, N>(v + c);
+#pragma unroll
+                    for (int j = 0; j < N; ++j) q[j] = widen<A>(y.v[j]);
+                }
+#pragma unroll
+                for (int j = 0; j < N; ++j) acc += p[j] * q[j];
+            }
+        }
+    }
+#pragma unroll
+    for (int o = LV / 2; o > 0; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
+    if (lane == 0 && t < a.in.n) a.d_scale[t] = a.alpha * acc;
+}
+
+// The gradient in one launch of three independent parts: blocks that sum chunks,
+// blocks that take the scales' gradient, and blocks that fill. Filling is bound
+// by HBM and the others by latency, so its blocks alternate with theirs.
+template <class G, class T, class A, class O, class I, bool WIDE, int LV>
+__global__ void __launch_bounds__(kMainNT)
+    embed_main_kernel(const GradArgs<G, T, A, O, I> a, int slabs) {
+    constexpr int N = Lane<G, WIDE>::N, GR = kMainNT / LV;
+    const int lane = threadIdx.x % LV, group = threadIdx.x / LV;
+    const unsigned work = a.reduce_blocks + a.scale_blocks;
+    const unsigned both = 2 * (work < a.fill_blocks ? work : a.fill_blocks);
+    unsigned b = blockIdx.x;
+    bool fill = false;
+    if (b < both) {
+        fill = b & 1;
+        b >>= 1;
+    } else {
+        b -= both / 2;
+        fill = work <= a.fill_blocks;
+    }
+    if (fill) {
+        fill_rest(a, a.fill_per, (int64_t)b * (kMainNT / 32) + threadIdx.x / 32,
+                  (int64_t)a.fill_blocks * (kMainNT / 32));
+    } else if (b < a.reduce_blocks) {
+        const int64_t c = (int64_t)(b / slabs) * GR + group;
+        const int64_t col = ((int64_t)(b % slabs) * LV + lane) * N;
+        if (c < a.n_chunks && col < a.d) reduce_chunk<G, T, A, O, I, WIDE, LV>(a, c, col, col == 0);
+    } else {
+        scale_entry<G, T, A, O, I, WIDE, LV>(a, (int64_t)(b - a.reduce_blocks) * GR + group, lane);
+    }
+}
+
+// The runs that cross chunks: the lane group of the chunk where one begins adds
+// its parts in chunk order and writes the run; the block's groups share a run of
+// more than kLongRun parts (ids that occur in every row: one part per 16 rows).
+constexpr int kLongRun = 16;
+
+template <class G, class T, class A, class O, class I, bool WIDE, int LV>
+__global__ void __launch_bounds__(256)
+    embed_cross_kernel(const GradArgs<G, T, A, O, I> a) {
+    constexpr int N = Lane<G, WIDE>::N, GR = 256 / LV;
+    __shared__ int64_t run_last[GR];  // last chunk of the run begun in the group's chunk, -1: none
+    __shared__ A shared_part[256 * N];
+    const int lane = threadIdx.x % LV, group = threadIdx.x / LV;
+    const int64_t c0 = (int64_t)blockIdx.x * GR, c = c0 + group, n = a.in.n;
+    const int64_t col = ((int64_t)blockIdx.y * LV + lane) * N;
+    const uint32_t pad_key = (uint32_t)a.in.n_rows;
+    if (lane == 0) {
+        int64_t last = -1;
+        if (c + 1 < a.n_chunks) {
+            const int64_t e0 = c * kChunk, e1 = e0 + kChunk;  // not the last chunk: e1 < n
+            const uint32_t key = a.keys[e1 - 1];
+            if (key != pad_key && a.keys[e1] == key && !(e0 > 0 && a.keys[e0 - 1] == key)) {
+                // most runs end within a few chunks: their first keys, all in flight
+                bool same[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) same[i] = c + 2 + i < a.n_chunks && a.keys[(c + 2 + i) * kChunk] == key;
+                last = c + 1;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) last += last == c + 1 + i && same[i] ? 1 : 0;
+                if (last == c + 9) last = (first_at_least(a.keys, last * kChunk, n, key + 1) - 1) / kChunk;
+            }
+        }
+        run_last[group] = last;
+    }
+    __syncthreads();
+    auto write = [&](int64_t chunk, A (&acc)[N]) {
+        const uint32_t key = a.keys[chunk * kChunk + kChunk - 1];
+        const int64_t at = a.rows ? a.runs_before(chunk + 1) - 1 : (int64_t)key;
+#pragma unroll
+        for (int j = 0; j < N; ++j) acc[j] *= a.alpha;
+        put((a.rows ? a.rows : a.d_table) + at * a.d + col, acc);
+        if (a.keys_out && col == 0) a.keys_out[at] = (I)key;
+    };
+    const bool in = col < a.d;
+    const int64_t mine = run_last[group];
+    if (mine >= 0 && mine - c <= kLongRun && in) {
+        Vec<A, N> p = ldg_vec<A, N>(a.part_tail + c * a.d + col);
+        A acc[N];
+#pragma unroll
+        for (int j = 0; j < N; ++j) acc[j] = p.v[j];
+#pragma unroll 4
+        for (int64_t k = c + 1; k <= mine; ++k) {
+            p = ldg_vec<A, N>(a.part_head + k * a.d + col);
+#pragma unroll
+            for (int j = 0; j < N; ++j) acc[j] += p.v[j];
+        }
+        write(c, acc);
+    }
+    for (int g = 0; g < GR; ++g) {  // uniform over the block
+        const int64_t last = run_last[g], from = c0 + g;
+        if (last < 0 || last - from <= kLongRun) continue;
+        A acc[N];
+#pragma unroll
+        for (int j = 0; j < N; ++j) acc[j] = A(0);
+        if (in) {
+#pragma unroll 4
+            for (int64_t k = from + 1 + group; k <= last; k += GR) {
+                const Vec<A, N> p = ldg_vec<A, N>(a.part_head + k * a.d + col);
+#pragma unroll
+                for (int j = 0; j < N; ++j) acc[j] += p.v[j];
+            }
+            if (group == 0) {
+                const Vec<A, N> p = ldg_vec<A, N>(a.part_tail + from * a.d + col);
+#pragma unroll
+                for (int j = 0; j < N; ++j) acc[j] += p.v[j];
+            }
+        }
+        // the groups' sums by a tree in shared memory
+#pragma unroll
+        for (int j = 0; j < N; ++j) shared_part[threadIdx.x * N + j] = acc[j];
+        for (int w = GR / 2; w > 0; w >>= 1) {
+            __syncthreads();
+            if (group < w) {
+#pragma unroll
+                for (int j = 0; j < N; ++j) shared_part[threadIdx.x * N + j] += shared_part[(threadIdx.x + w * LV) * N + j];
+            }
+        }
+        if (group == 0 && in) {
+#pragma unroll
+            for (int j = 0; j < N; ++j) acc[j] = shared_part[threadIdx.x * N + j];
+            write(from, acc);
+        }
+        __syncthreads();
+    }
 }
 
 // ------------------------------------------------------------- launchers --
@@ -328,7 +680,7 @@ void with_embed_types(int dtype, F&& f) {
     }
 }
 
-// f(integral constant): lanes per row for dv vectors.
+// f(LV): lanes per row for dv vectors.
 template <class F>
 void with_lanes(int64_t dv, F&& f) {
     if (dv <= 1)
@@ -344,28 +696,45 @@ void with_lanes(int64_t dv, F&& f) {
 }
 
 template <class P>
-using Elem = std::remove_pointer_t<std::remove_reference_t<P>>;
+using Elem = std::remove_const_t<std::remove_pointer_t<std::remove_reference_t<P>>>;
 
-template <class T, class A, class O, class I, int VEC>
-void lookup_launch(int device, const I* ids, int64_t n, const int64_t* indptr, int64_t n_out,
-                   const A* scale, A alpha, const T* table, int64_t n_rows, int64_t d, int64_t ld,
-                   O* out, int64_t ld_out, cudaStream_t s) {
-    const int64_t dv = d / VEC;
-    if (!indptr) {
-        const int64_t total = n * dv;
-        if (total <= (int64_t)sm_count(device) * 2048)
-            embed_rows_kernel<T, A, O, I, VEC, 1><<<(unsigned)ceil_div(total, 256), 256, 0, s>>>(
-                ids, n, scale, alpha, table, n_rows, (uint32_t)dv, ld, out, ld_out);
-        else
-            embed_rows_kernel<T, A, O, I, VEC, 4><<<(unsigned)ceil_div(total, 1024), 256, 0, s>>>(
-                ids, n, scale, alpha, table, n_rows, (uint32_t)dv, ld, out, ld_out);
-    } else {
+template <class T, class A, class O, class I, bool WIDE>
+void lookup_launch(int device, const Entries<I>& in, const A* scale, A alpha, const T* table,
+                   int64_t d, int64_t ld, O* out, int64_t ld_out, cudaStream_t s) {
+    constexpr int N = Lane<T, WIDE>::N;
+    const int64_t dv = d / N, n = in.n;
+    const int64_t fill = (int64_t)sm_count(device) * 2048;  // threads at once
+    if (in.indptr) {
         with_lanes(dv, [&](auto lv) {
-            constexpr int LV = decltype(lv)::value;
-            const dim3 g((unsigned)ceil_div(n_out, 256 / LV), (unsigned)ceil_div(dv, LV));
-            embed_sums_kernel<T, A, O, I, VEC, LV><<<g, 256, 0, s>>>(
-                ids, n, indptr, n_out, scale, alpha, table, n_rows, d, ld, out, ld_out);
+            constexpr int LV = decltype(lv)::value, EL = LV >= 8 ? 1 : 8 / LV;
+            const dim3 g((unsigned)ceil_div(in.n_out, 256 / (LV * EL)), (unsigned)ceil_div(dv, LV));
+            embed_sums_kernel<T, A, O, I, WIDE, LV, EL><<<g, 256, 0, s>>>(
+                in.ids, n, in.indptr, in.n_out, scale, alpha, table, in.n_rows, d, ld, out, ld_out);
         });
+    } else if (WIDE && dv >= 32) {
+        if constexpr (WIDE) {
+            auto wide = [&](auto unroll) {
+                constexpr int U = decltype(unroll)::value;
+                const int64_t pieces = ceil_div(dv, 32 * U);
+                embed_wide_kernel<T, A, O, I, U><<<(unsigned)ceil_div(n * pieces, 8), 256, 0, s>>>(
+                    in.ids, n, scale, alpha, table, in.n_rows, (int)dv, (int)pieces, ld, out, ld_out);
+            };
+            // fewer vectors a lane while the lanes do not fill the GPU
+            if (n * dv >= 4 * fill && dv >= 128)
+                wide(std::integral_constant<int, 4>{});
+            else if (n * dv >= 2 * fill && dv >= 64)
+                wide(std::integral_constant<int, 2>{});
+            else
+                wide(std::integral_constant<int, 1>{});
+        }
+    } else {
+        const int64_t total = n * dv;
+        if (total <= fill)
+            embed_rows_kernel<T, A, O, I, WIDE, 1><<<(unsigned)ceil_div(total, 256), 256, 0, s>>>(
+                in.ids, n, scale, alpha, table, in.n_rows, (uint32_t)dv, ld, out, ld_out);
+        else
+            embed_rows_kernel<T, A, O, I, WIDE, 4><<<(unsigned)ceil_div(total, 1024), 256, 0, s>>>(
+                in.ids, n, scale, alpha, table, in.n_rows, (uint32_t)dv, ld, out, ld_out);
     }
     MFM_CHECK_LAUNCH("embedding lookup launch");
 }
@@ -374,105 +743,81 @@ void lookup_launch(int device, const I* ids, int64_t n, const int64_t* indptr, i
 struct GradWs {
     IdSortPlan sort;
     int64_t n_chunks = 0;
-    size_t off_row = 0, off_base = 0, off_sums = 0, off_head = 0, off_tail = 0, bytes = 0;
+    size_t off_row = 0, off_base = 0, off_tile = 0, off_head = 0, off_tail = 0, bytes = 0;
     GradWs(int dtype, int64_t n, int64_t n_rows, int64_t d) : sort(n, n_rows) {
         auto up = [](size_t b) { return (b + 255) / 256 * 256; };
         const size_t a = dtype == MFM_DTYPE_F64 || dtype == MFM_DTYPE_F32_F64 ? 8 : 4;
         n_chunks = ceil_div(n, kChunk);
-        off_row = up((size_t)sort.words * 4);
+        off_row = up((size_t)sort.words * 4 + 4);  // the block count is the last word
         off_base = off_row + up((size_t)n * 4);
-        off_sums = off_base + up((size_t)(n_chunks + 1) * 4);
-        off_head = off_sums + up((size_t)(ceil_div(n_chunks, kScanTile) + 2) * 4);
+        off_tile = off_base + up((size_t)n_chunks * 4);
+        off_head = off_tile + up((size_t)ceil_div(n_chunks, kTileChunks) * 4);
         off_tail = off_head + up((size_t)n_chunks * d * a);
         bytes = off_tail + up((size_t)n_chunks * d * a);
     }
 };
 
-template <class G, class T, class A, class O, class I>
-struct GradArgs {
-    int device;
-    const I* ids;
-    int64_t n;
-    const int64_t* indptr;
-    int64_t n_out;
-    const A* scale;
-    A alpha;
-    const G* grad;
-    int64_t ld;
-    const T* table;
-    int64_t ld_table, n_rows, d;
-    O *d_table, *rows;
-    I* keys;
-    int64_t* count;
-    A* d_scale;
-    char* ws;
-    cudaStream_t s;
-};
-
-template <class G, class T, class A, class O, class I, int VEC>
-void grad_launch(const GradArgs<G, T, A, O, I>& a, const GradWs& W) {
-    const uint32_t pad = (uint32_t)a.n_rows;
-    int32_t* row_of = nullptr;
-    if (a.indptr) {
-        row_of = reinterpret_cast<int32_t*>(a.ws + W.off_row);
-        MFM_CUDA(cudaMemsetAsync(row_of, 0xff, (size_t)a.n * 4, a.s), "memset");
-        if (a.n_out > 0)
-            entry_rows_kernel<<<warp_grid(a.device, a.n_out, 8, 8), 256, 0, a.s>>>(a.indptr, a.n_out, a.n, row_of);
-    }
-    if (a.d_scale) {
-        const bool ok = vec_ok(a.table, a.ld_table, sizeof(T), VEC);
-        const unsigned g = (unsigned)ceil_div(a.n, 8);
-        if (ok)
-            embed_scale_kernel<G, T, A, I, VEC><<<g, 256, 0, a.s>>>(a.ids, a.n, row_of, a.alpha, a.grad, a.ld, a.table, a.n_rows, a.ld_table, a.d, a.d_scale);
-        else
-            embed_scale_kernel<G, T, A, I, 1><<<g, 256, 0, a.s>>>(a.ids, a.n, row_of, a.alpha, a.grad, a.ld, a.table, a.n_rows, a.ld_table, a.d, a.d_scale);
-    }
-    const IdSorted S = sort_ids(W.sort, a.ids, row_of, a.n_rows, reinterpret_cast<uint32_t*>(a.ws), a.s);
-    GradOut<O, I> out{a.d_table, a.rows, a.keys, nullptr};
-    const int64_t nc = W.n_chunks;
+template <class G, class T, class A, class O, class I, bool WIDE>
+void grad_launch(int device, GradArgs<G, T, A, O, I>& a, const GradWs& W, char* ws, cudaStream_t s) {
+    constexpr int N = Lane<G, WIDE>::N;
+    const int64_t n = a.in.n, nc = W.n_chunks, dv = a.d / N;
+    uint32_t* words = reinterpret_cast<uint32_t*>(ws);
+    unsigned* done = words + W.sort.words;
+    int32_t* row_of = a.in.indptr ? reinterpret_cast<int32_t*>(ws + W.off_row) : nullptr;
+    const IdSorted S = sort_ids(W.sort, a.in, row_of, done, words, s);
+    a.keys = S.keys;
+    a.pos = S.pos;
+    a.row_of = row_of;
+    a.n_chunks = nc;
+    a.part_head = reinterpret_cast<A*>(ws + W.off_head);
+    a.part_tail = reinterpret_cast<A*>(ws + W.off_tail);
     if (a.rows) {
-        uint32_t* base = reinterpret_cast<uint32_t*>(a.ws + W.off_base);
-        uint32_t* sums = reinterpret_cast<uint32_t*>(a.ws + W.off_sums);
-        chunk_heads_kernel<<<(unsigned)ceil_div(nc, 8), 256, 0, a.s>>>(S.keys, a.n, pad, nc, base);
-        const int64_t nb = ceil_div(nc, kScanTile);
-        scan_reduce_kernel<uint32_t, uint32_t><<<(unsigned)nb, kScanNT, 0, a.s>>>(base, nc, sums);
-        scan_sums_kernel<uint32_t><<<1, kScanNT, 0, a.s>>>(sums, nb);
-        scan_apply_kernel<uint32_t, uint32_t><<<(unsigned)nb, kScanNT, 0, a.s>>>(base, nc, sums, base);
-        run_count_kernel<<<1, 1, 0, a.s>>>(base, nc, a.count);
-        out.base = base;
+        uint32_t* base = reinterpret_cast<uint32_t*>(ws + W.off_base);
+        uint32_t* tiles = reinterpret_cast<uint32_t*>(ws + W.off_tile);
+        chunk_heads_kernel<<<(unsigned)ceil_div(nc, kTileChunks), kTileChunks, 0, s>>>(
+            S.keys, n, (uint32_t)a.in.n_rows, nc, base, tiles, done, a.count);
+        a.base = base;
+        a.tile_base = tiles;
     }
-    A* head = reinterpret_cast<A*>(a.ws + W.off_head);
-    A* tail = reinterpret_cast<A*>(a.ws + W.off_tail);
-    with_lanes(a.d / VEC, [&](auto lv) {
+    with_lanes(dv, [&](auto lv) {
         constexpr int LV = decltype(lv)::value;
-        const dim3 g((unsigned)ceil_div(nc, 128 / LV), (unsigned)ceil_div(a.d / VEC, LV));
-        embed_reduce_kernel<G, A, O, I, VEC, LV><<<g, 128, 0, a.s>>>(
-            S.keys, S.pos, a.n, pad, row_of, a.scale, a.alpha, a.grad, a.ld, a.d, nc, head, tail, out);
-        embed_cross_kernel<A, O, I, VEC, LV><<<g, 128, 0, a.s>>>(S.keys, a.n, pad, a.alpha, a.d, nc, head, tail, out);
+        const int64_t slabs = ceil_div(dv, LV), sm = sm_count(device);
+        a.reduce_blocks = (unsigned)(ceil_div(nc, kMainNT / LV) * slabs);
+        a.scale_blocks = a.d_scale ? (unsigned)ceil_div(n, kMainNT / LV) : 0u;
+        const int64_t rest = a.rows ? std::min(n, a.in.n_rows) : a.in.n_rows;
+        // a warp fills 32 rows, or fewer where the rows are long
+        a.fill_per = (int)std::min<int64_t>(32, std::max<int64_t>(4, 32768 / (a.d * (int64_t)sizeof(O))));
+        a.fill_blocks = (unsigned)std::min<int64_t>(ceil_div(rest, (int64_t)a.fill_per * (kMainNT / 32)), sm * 16);
+        embed_main_kernel<G, T, A, O, I, WIDE, LV>
+            <<<a.reduce_blocks + a.scale_blocks + a.fill_blocks, kMainNT, 0, s>>>(a, (int)slabs);
+        if (nc > 1) {
+            const dim3 g((unsigned)ceil_div(nc, 256 / LV), (unsigned)slabs);
+            embed_cross_kernel<G, T, A, O, I, WIDE, LV><<<g, 256, 0, s>>>(a);
+        }
     });
     MFM_CHECK_LAUNCH("embedding gradient launch");
 }
 
 template <class G, class T, class A, class O, class I>
-void grad_entry(const GradArgs<G, T, A, O, I>& a, const GradWs& W) {
-    // rows of the result that nothing touches
-    const int64_t cap = std::min(a.n, a.n_rows);
-    if (a.d_table) MFM_CUDA(cudaMemsetAsync(a.d_table, 0, (size_t)a.n_rows * a.d * sizeof(O), a.s), "memset");
-    if (a.keys) {
-        MFM_CUDA(cudaMemsetAsync(a.keys, 0xff, (size_t)cap * sizeof(I), a.s), "memset");
-        MFM_CUDA(cudaMemsetAsync(a.rows, 0, (size_t)cap * a.d * sizeof(O), a.s), "memset");
-        MFM_CUDA(cudaMemsetAsync(a.count, 0, sizeof(int64_t), a.s), "memset");
-    }
-    if (a.n == 0) return;
-    if (a.n_rows == 0 || a.n_out == 0) {  // nothing to add up
-        if (a.d_scale) MFM_CUDA(cudaMemsetAsync(a.d_scale, 0, (size_t)a.n * sizeof(A), a.s), "memset");
+void grad_entry(int device, GradArgs<G, T, A, O, I>& a, const GradWs& W, char* ws, cudaStream_t s) {
+    const int64_t cap = std::min(a.in.n, a.in.n_rows);
+    if (a.in.n == 0 || a.in.n_rows == 0 || a.in.n_out == 0) {  // nothing to add up
+        if (a.d_table) MFM_CUDA(cudaMemsetAsync(a.d_table, 0, (size_t)a.in.n_rows * a.d * sizeof(O), s), "memset");
+        if (a.keys_out) {
+            MFM_CUDA(cudaMemsetAsync(a.keys_out, 0xff, (size_t)cap * sizeof(I), s), "memset");
+            MFM_CUDA(cudaMemsetAsync(a.rows, 0, (size_t)cap * a.d * sizeof(O), s), "memset");
+            MFM_CUDA(cudaMemsetAsync(a.count, 0, sizeof(int64_t), s), "memset");
+        }
+        if (a.d_scale) MFM_CUDA(cudaMemsetAsync(a.d_scale, 0, (size_t)a.in.n * sizeof(A), s), "memset");
         return;
     }
-    constexpr int VEC = 16 / sizeof(G);
-    if (vec_ok(a.grad, a.ld, sizeof(G), VEC) && vec_ok(a.d_table ? a.d_table : a.rows, a.d, sizeof(O), VEC))
-        grad_launch<G, T, A, O, I, VEC>(a, W);
+    constexpr int N = Lane<G, true>::N;
+    const O* result = a.d_table ? a.d_table : a.rows;
+    const bool table_ok = !a.d_scale || vec_ok(a.table, a.ld_table, sizeof(T), N);
+    if (a.d % N == 0 && vec_ok(a.grad, a.ld, sizeof(G), N) && (uintptr_t)result % 16 == 0 && table_ok)
+        grad_launch<G, T, A, O, I, true>(device, a, W, ws, s);
     else
-        grad_launch<G, T, A, O, I, 1>(a, W);
+        grad_launch<G, T, A, O, I, false>(device, a, W, ws, s);
 }
 
 }  // namespace
@@ -498,17 +843,19 @@ extern "C" int mfm_embedding_lookup_device(int dtype, int device, int ids64, con
             using A = Elem<decltype(a)>;
             using O = Elem<decltype(o)>;
             with_index_type(ids64, [&](auto* i) {
-                using I = std::remove_const_t<Elem<decltype(i)>>;
-                constexpr int VEC = 16 / sizeof(T);
-                auto go = [&](auto vec) {
-                    lookup_launch<T, A, O, I, decltype(vec)::value>(
-                        device, (const I*)ids, n_entries, indptr, n_out, (const A*)scale, (A)alpha,
-                        (const T*)table, n_rows, d, ld_table, (O*)out, ld_out, (cudaStream_t)stream);
+                using I = Elem<decltype(i)>;
+                constexpr int N = Lane<T, true>::N;
+                const Entries<I> in{(const I*)ids, n_entries, indptr, n_out, n_rows};
+                auto go = [&](auto wide) {
+                    lookup_launch<T, A, O, I, decltype(wide)::value>(
+                        device, in, (const A*)scale, (A)alpha, (const T*)table, d, ld_table, (O*)out,
+                        ld_out, (cudaStream_t)stream);
                 };
-                if (d % VEC == 0 && vec_ok(table, ld_table, sizeof(T), VEC) && vec_ok(out, ld_out, sizeof(O), VEC))
-                    go(std::integral_constant<int, VEC>{});
+                // vectors of 16 bytes of the table, and the results' vectors whole
+                if (d % N == 0 && vec_ok(table, ld_table, sizeof(T), N) && vec_ok(out, ld_out, sizeof(O), std::min<int>(N, 16 / sizeof(O))))
+                    go(std::true_type{});
                 else
-                    go(std::integral_constant<int, 1>{});
+                    go(std::false_type{});
             });
         });
     });
@@ -557,15 +904,24 @@ extern "C" int mfm_embedding_grad_device(int dtype, int out_dtype, int device, i
             using A = Elem<decltype(a)>;
             using G = Elem<decltype(o)>;
             with_index_type(ids64, [&](auto* i) {
-                using I = std::remove_const_t<Elem<decltype(i)>>;
+                using I = Elem<decltype(i)>;
                 auto go = [&](auto* r) {
                     using O = Elem<decltype(r)>;
-                    GradArgs<G, T, A, O, I> x{device, (const I*)ids, n_entries, indptr, n_out,
-                                              (const A*)scale, (A)alpha, (const G*)grad, ld_grad,
-                                              (const T*)table, ld_table, n_rows, d, (O*)d_table,
-                                              (O*)rows, (I*)keys, count, (A*)d_scale,
-                                              (char*)workspace, (cudaStream_t)stream};
-                    grad_entry(x, W);
+                    GradArgs<G, T, A, O, I> x{};
+                    x.in = Entries<I>{(const I*)ids, n_entries, indptr, n_out, n_rows};
+                    x.scale = (const A*)scale;
+                    x.alpha = (A)alpha;
+                    x.grad = (const G*)grad;
+                    x.ld = ld_grad;
+                    x.table = (const T*)table;
+                    x.ld_table = ld_table;
+                    x.d = d;
+                    x.d_table = (O*)d_table;
+                    x.rows = (O*)rows;
+                    x.keys_out = (I*)keys;
+                    x.count = count;
+                    x.d_scale = (A*)d_scale;
+                    grad_entry(device, x, W, (char*)workspace, (cudaStream_t)stream);
                 };
                 if constexpr (sizeof(G) == 2) {
                     if (out_dtype == MFM_DTYPE_F32) {

@@ -15,6 +15,8 @@
 // Up to kSmallSort ids one block does every pass in shared memory.
 #pragma once
 
+#include <type_traits>
+
 #include "scan.cuh"
 #include "vecio.cuh"
 
@@ -24,36 +26,97 @@ constexpr int kETileNT = 256;
 constexpr int kETileItems = 8;
 constexpr int kETile = kETileNT * kETileItems;
 constexpr int kFuseTiles = 192;
-constexpr int kSmallNT = 1024;
-constexpr int kSmallItems = 8;
-constexpr int64_t kSmallSort = (int64_t)kSmallNT * kSmallItems;
+constexpr int64_t kSmallSort = 2048;
 
-// The key of entry q: its id, or n_rows for padding (an id outside the table, or
-// an entry of no row).
+// The entries of a batch: their ids and, where they are summed by rows, the rows'
+// bounds (indptr, n_out + 1; NULL: every entry is a row of its own).
 template <class I>
-__device__ __forceinline__ uint32_t id_key(const I* ids, const int32_t* row_of, int64_t q,
-                                           int64_t n_rows) {
-    const I id = ids[q];
-    const bool live = id >= 0 && (int64_t)id < n_rows && (!row_of || row_of[q] >= 0);
-    return live ? (uint32_t)id : (uint32_t)n_rows;
-}
+struct Entries {
+    const I* ids;
+    int64_t n;
+    const int64_t* indptr;
+    int64_t n_out, n_rows;
+    // The rows that M x 32 consecutive entries belong to, one warp, lane l's i-th
+    // being q0 + 32 i + l; -1 for none: the first row whose end is behind the entry,
+    // if it begins at or before it. The warp finds the first entry's row (32 probes
+    // a round), takes the ends of the 32 rows from there, one a lane, and looks
+    // its entries up among them; entries behind all of those bisect the rest. Any
+    // bounds give an answer in [-1, n_out), decreasing ones too.
+    template <int M>
+    __device__ __forceinline__ void rows(int64_t q0, int32_t (&r)[M]) const {
+        if (!indptr) {
+#pragma unroll
+            for (int i = 0; i < M; ++i) r[i] = 0;
+            return;
+        }
+        const int lane = threadIdx.x & 31;
+        int32_t base = 0, len = (int32_t)n_out;  // the first row is in [base, base + len]
+        while (len > 0) {
+            const int32_t step = (len + 31) / 32;
+            const int64_t p = (int64_t)(lane + 1) * step;
+            const bool ends = p <= len && indptr[base + p] <= q0;
+            const int n = __popc(__ballot_sync(0xffffffffu, ends));
+            base += n * step;
+            const int32_t rest = len - n * step;
+            len = rest < step - 1 ? (rest > 0 ? rest : 0) : step - 1;
+        }
+        const int64_t end = base + lane < n_out ? indptr[base + lane + 1] : INT64_MAX;
+#pragma unroll
+        for (int i = 0; i < M; ++i) {
+            const int64_t q = q0 + 32 * i + lane;
+            int32_t k = 0;  // how many of the 32 rows end at or before q
+#pragma unroll
+            for (int w = 16; w > 0; w >>= 1)
+                if (__shfl_sync(0xffffffffu, end, k + w - 1) <= q) k += w;
+            if (__shfl_sync(0xffffffffu, end, k) <= q) ++k;
+            int64_t lo = (int64_t)base + k;
+            if (k == 32) {
+                int64_t hi = n_out;
+                while (lo < hi) {
+                    const int64_t mid = (lo + hi) >> 1;
+                    if (indptr[mid + 1] > q)
+                        hi = mid;
+                    else
+                        lo = mid + 1;
+                }
+            }
+            r[i] = lo < n_out && indptr[lo] <= q ? (int32_t)lo : -1;
+        }
+    }
+    // The sort key of entry q: its id, or n_rows for padding (an id outside the
+    // table, or an entry of no row).
+    __device__ __forceinline__ uint32_t key(int64_t q, int32_t row) const {
+        const I id = ids[q];
+        return id >= 0 && (int64_t)id < n_rows && row >= 0 ? (uint32_t)id : (uint32_t)n_rows;
+    }
+};
 
-// Digit counts of the first pass by tile, and zeros for the passes after it.
+// Keys and rows of all entries, digit counts of the first pass by tile, and zeros
+// for the passes after it and for the block count of the kernels behind the sort.
 template <class I>
 __global__ void __launch_bounds__(kETileNT)
-    id_count_kernel(const I* __restrict__ ids, const int32_t* __restrict__ row_of, int64_t n,
-                    int64_t n_rows, int passes,
-                    int64_t n_tiles, uint32_t* __restrict__ counts) {
+    id_count_kernel(Entries<I> in, int passes, int64_t n_tiles, uint32_t* __restrict__ keys,
+                    int32_t* __restrict__ row_of, uint32_t* __restrict__ counts,
+                    unsigned* __restrict__ done) {
     __shared__ uint32_t h[256];
     const int t = threadIdx.x;
     const int64_t tile = blockIdx.x, lo = tile * kETile;
     h[t] = 0;
+    if (tile == 0 && t == 0) *done = 0;
     for (int p = 1; p < passes; ++p) counts[(p * n_tiles + tile) * 256 + t] = 0;
     __syncthreads();
+    const int64_t q0 = lo + (t / 32) * (32 * kETileItems);
+    int32_t r[kETileItems];
+    in.rows(q0, r);
 #pragma unroll
     for (int i = 0; i < kETileItems; ++i) {
-        const int64_t q = lo + t + i * kETileNT;
-        if (q < n) atomicAdd(&h[id_key(ids, row_of, q, n_rows) & 255u], 1u);
+        const int64_t q = q0 + 32 * i + (t & 31);
+        if (q < in.n) {
+            if (in.indptr) row_of[q] = r[i];
+            const uint32_t k = in.key(q, r[i]);
+            keys[q] = k;
+            atomicAdd(&h[k & 255u], 1u);
+        }
     }
     __syncthreads();
     counts[tile * 256 + t] = h[t];
@@ -78,17 +141,15 @@ __global__ void __launch_bounds__(256)
     if (threadIdx.x == 0) totals[d] = run;
 }
 
-// One pass of one tile. FIRST: keys come from the ids, values are positions.
+// One pass of one tile. FIRST: the values are the positions.
 // FUSED: `counts` holds digit counts and the tile adds up those before it;
 // otherwise it holds their prefix over the tiles, and `totals` the digits' sums.
 // next != NULL: the next pass's counts.
-template <class I, bool FIRST, bool FUSED>
+template <bool FIRST, bool FUSED>
 __global__ void __launch_bounds__(kETileNT)
-    id_scatter_kernel(const I* __restrict__ ids, const int32_t* __restrict__ row_of,
-                      const uint32_t* __restrict__ kin,
-                      const uint32_t* __restrict__ vin, uint32_t* __restrict__ kout,
-                      uint32_t* __restrict__ vout, int64_t n, int64_t n_rows, int64_t n_tiles,
-                      int shift, const uint32_t* __restrict__ counts,
+    id_scatter_kernel(const uint32_t* __restrict__ kin, const uint32_t* __restrict__ vin,
+                      uint32_t* __restrict__ kout, uint32_t* __restrict__ vout, int64_t n,
+                      int64_t n_tiles, int shift, const uint32_t* __restrict__ counts,
                       const uint32_t* __restrict__ totals, uint32_t* __restrict__ next) {
     constexpr int NW = kETileNT / 32;
     __shared__ uint32_t cnt[NW][256];
@@ -107,17 +168,22 @@ __global__ void __launch_bounds__(kETileNT)
         key[i] = 0;
         val[i] = 0;
         if (q < m) {
-            key[i] = FIRST ? id_key(ids, row_of, lo + q, n_rows) : kin[lo + q];
+            key[i] = kin[lo + q];
             val[i] = FIRST ? (uint32_t)(lo + q) : vin[lo + q];
         }
     }
     uint32_t dtotal = 0, before = 0, all;
     if (FUSED) {
-#pragma unroll 8
-        for (int64_t b = 0; b < n_tiles; ++b) {
-            const uint32_t c = counts[b * 256 + t];
-            dtotal += c;
-            before += b < tile ? c : 0u;
+        constexpr int F = 32;  // tiles' counts in flight
+        for (int b0 = 0; b0 < (int)n_tiles; b0 += F) {
+            uint32_t c[F];
+#pragma unroll
+            for (int f = 0; f < F; ++f) c[f] = b0 + f < (int)n_tiles ? counts[(b0 + f) * 256 + t] : 0u;
+#pragma unroll
+            for (int f = 0; f < F; ++f) {
+                dtotal += c[f];
+                before += b0 + f < tile ? c[f] : 0u;
+            }
         }
     } else {
         dtotal = totals[t];
@@ -183,8 +249,10 @@ __global__ void __launch_bounds__(kETileNT)
 // All passes of up to NT * ITEMS ids in one block.
 template <class I, int NT, int ITEMS>
 __global__ void __launch_bounds__(NT)
-    id_sort_small_kernel(const I* __restrict__ ids, const int32_t* __restrict__ row_of, int n, int64_t n_rows, int key_bits,
-                         uint32_t* __restrict__ kout, uint32_t* __restrict__ vout) {
+    id_sort_small_kernel(Entries<I> in, int key_bits, uint32_t* __restrict__ kout,
+                         uint32_t* __restrict__ vout, int32_t* __restrict__ row_of,
+                         unsigned* __restrict__ done) {
+    const int n = (int)in.n;
     constexpr int NW = NT / 32;
     extern __shared__ uint32_t dyn[];
     uint32_t(*cnt)[256] = reinterpret_cast<uint32_t(*)[256]>(dyn);  // NW x 256
@@ -193,12 +261,19 @@ __global__ void __launch_bounds__(NT)
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
     const int q0 = warp * (32 * ITEMS) + lane;
     uint32_t key[ITEMS], val[ITEMS], rank[ITEMS];
+    int32_t r[ITEMS];
+    in.rows(q0 - lane, r);
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i) {
         const int q = q0 + i * 32;
-        key[i] = q < n ? id_key(ids, row_of, q, n_rows) : 0u;
+        key[i] = 0u;
         val[i] = (uint32_t)q;
+        if (q < n) {
+            if (in.indptr) row_of[q] = r[i];
+            key[i] = in.key(q, r[i]);
+        }
     }
+    if (t == 0) *done = 0;
     const unsigned lt = (1u << lane) - 1u;
     for (int shift = 0; shift < key_bits; shift += 8) {
         for (int i = t; i < NW * 256; i += NT) (&cnt[0][0])[i] = 0;
@@ -286,41 +361,51 @@ struct IdSorted {
     const uint32_t* pos;
 };
 
+// Sorts the batch's keys; writes row_of (with indptr) and clears *done.
 template <class I>
-IdSorted sort_ids(const IdSortPlan& P, const I* ids, const int32_t* row_of, int64_t n_rows,
+IdSorted sort_ids(const IdSortPlan& P, const Entries<I>& in, int32_t* row_of, unsigned* done,
                   uint32_t* ws, cudaStream_t s) {
     const int64_t n = P.n;
     uint32_t *k0 = ws, *v0 = ws + n, *k1 = ws + 2 * n, *v1 = ws + 3 * n, *counts = ws + 4 * n;
     if (n <= kSmallSort) {
-        if (n <= 1024) {
-            constexpr int NT = 256, IT = 4, SM = (NT / 32) * 1024 + NT * IT * 8;
-            id_sort_small_kernel<I, NT, IT><<<1, NT, SM, s>>>(ids, row_of, (int)n, n_rows, P.key_bits, k0, v0);
-        } else {
-            constexpr int SM = (kSmallNT / 32) * 1024 + (int)kSmallSort * 8;
-            auto k = id_sort_small_kernel<I, kSmallNT, kSmallItems>;
-            MFM_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, SM), "id sort shared memory");
-            k<<<1, kSmallNT, SM, s>>>(ids, row_of, (int)n, n_rows, P.key_bits, k0, v0);
-        }
+        auto small = [&](auto nt, auto items) {
+            constexpr int NT = decltype(nt)::value, IT = decltype(items)::value;
+            constexpr int SM = (NT / 32) * 1024 + NT * IT * 8;
+            auto k = id_sort_small_kernel<I, NT, IT>;
+            static_assert(SM <= 48 * 1024, "id sort shared memory");
+            k<<<1, NT, SM, s>>>(in, P.key_bits, k0, v0, row_of, done);
+        };
+        using std::integral_constant;
+        if (n <= 256)
+            small(integral_constant<int, 256>{}, integral_constant<int, 1>{});
+        else if (n <= 512)
+            small(integral_constant<int, 512>{}, integral_constant<int, 1>{});
+        else
+            small(integral_constant<int, 512>{}, integral_constant<int, 4>{});
         MFM_CHECK_LAUNCH("id sort launch");
         return {k0, v0};
     }
     const unsigned g = (unsigned)P.n_tiles;
     const bool fused = P.n_tiles <= kFuseTiles;
     uint32_t* totals = counts + (int64_t)P.passes * P.n_tiles * 256;
-    id_count_kernel<I><<<g, kETileNT, 0, s>>>(ids, row_of, n, n_rows, P.passes, P.n_tiles, counts);
+    id_count_kernel<I><<<g, kETileNT, 0, s>>>(in, P.passes, P.n_tiles, k1, row_of, counts, done);
     uint32_t *ki = k1, *vi = v1, *ko = k0, *vo = v0;
     for (int p = 0; p < P.passes; ++p) {
         uint32_t* c = counts + (int64_t)p * P.n_tiles * 256;
         uint32_t* next = p + 1 < P.passes ? c + P.n_tiles * 256 : nullptr;
         if (!fused) id_prefix_kernel<<<256, 256, 0, s>>>(c, P.n_tiles, totals);
+        auto pass = [&](auto first, auto whole) {
+            id_scatter_kernel<decltype(first)::value, decltype(whole)::value>
+                <<<g, kETileNT, 0, s>>>(ki, vi, ko, vo, n, P.n_tiles, 8 * p, c, totals, next);
+        };
         if (p == 0 && fused)
-            id_scatter_kernel<I, true, true><<<g, kETileNT, 0, s>>>(ids, row_of, ki, vi, ko, vo, n, n_rows, P.n_tiles, 8 * p, c, totals, next);
+            pass(std::true_type{}, std::true_type{});
         else if (p == 0)
-            id_scatter_kernel<I, true, false><<<g, kETileNT, 0, s>>>(ids, row_of, ki, vi, ko, vo, n, n_rows, P.n_tiles, 8 * p, c, totals, next);
+            pass(std::true_type{}, std::false_type{});
         else if (fused)
-            id_scatter_kernel<I, false, true><<<g, kETileNT, 0, s>>>(ids, row_of, ki, vi, ko, vo, n, n_rows, P.n_tiles, 8 * p, c, totals, next);
+            pass(std::false_type{}, std::true_type{});
         else
-            id_scatter_kernel<I, false, false><<<g, kETileNT, 0, s>>>(ids, row_of, ki, vi, ko, vo, n, n_rows, P.n_tiles, 8 * p, c, totals, next);
+            pass(std::false_type{}, std::false_type{});
         std::swap(ki, ko);
         std::swap(vi, vo);
     }
