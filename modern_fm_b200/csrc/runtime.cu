@@ -29,6 +29,10 @@ static constexpr int kMaxDevices = 64;
 
 DeviceGuard::DeviceGuard(int device) {
     if (cudaGetDevice(&prev) != cudaSuccess) prev = -1;
+    if (prev == device && prev >= 0) {  // already there: nothing to set or restore
+        prev = -1;
+        return;
+    }
     int n = device_count();
     if (n <= 0) fail(MFM_ERR_NO_DEVICE, "no CUDA device available");
     if (device < 0 || device >= n)

@@ -37,16 +37,16 @@ class EmbeddingRows(NamedTuple):
     scale: Optional[object]
 
 
-_STORAGE = None
+_STORAGE = {}
 
 
 def _storage():
-    global _STORAGE
-    if _STORAGE is None:
+    if not _STORAGE:
         import torch
 
-        _STORAGE = {torch.float64: _lib.MFM_DTYPE_F64, torch.float32: _lib.MFM_DTYPE_F32,
-                    torch.bfloat16: _lib.MFM_DTYPE_BF16, torch.float16: _lib.MFM_DTYPE_F16}
+        _STORAGE.update({
+            torch.float64: _lib.MFM_DTYPE_F64, torch.float32: _lib.MFM_DTYPE_F32,
+            torch.bfloat16: _lib.MFM_DTYPE_BF16, torch.float16: _lib.MFM_DTYPE_F16})
     return _STORAGE
 
 
@@ -57,52 +57,34 @@ def _fail(rc):
         raise RuntimeError(_lib.last_error())
 
 
-def _one_device(tensors):
-    """The device index all tensors share; ValueError otherwise."""
-    dev = None
-    for name, t in tensors:
-        if t is None:
-            continue
-        if not t.is_cuda:
-            raise ValueError(f"{name} must be a CUDA tensor")
-        if dev is None:
-            dev = t.get_device()
-        elif t.get_device() != dev:
-            raise ValueError(f"{name} is on another device")
+def _one_device(first, *rest):
+    """The device index that all tensors (None: not given) share."""
+    if not first.is_cuda:
+        raise ValueError("every tensor must be a CUDA tensor")
+    dev = first.get_device()
+    for t in rest:
+        if t is not None and t.get_device() != dev:
+            raise ValueError("every tensor must be a CUDA tensor on one device")
     return dev
 
 
 def _matrix(name, t):
-    """(pointer, row pitch) of a matrix with contiguous rows that do not overlap."""
-    if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):
+    """(pointer, rows, columns, row pitch) of a matrix with contiguous rows that do not overlap."""
+    if t.dim() != 2:
         raise ValueError(f"{name} must be a matrix with contiguous rows")
-    pitch = t.stride(0) if t.shape[0] > 1 else max(t.shape[1], 1)
-    if pitch < t.shape[1]:
+    n, d = t.shape
+    pitch, step = t.stride()
+    if d > 1 and step != 1:
+        raise ValueError(f"{name} must be a matrix with contiguous rows")
+    if n <= 1:
+        pitch = max(d, 1)
+    if pitch < d:
         raise ValueError(f"the rows of {name} must not overlap")
-    return t.data_ptr(), pitch
+    return t.data_ptr(), n, d, pitch
 
 
 def _ptr(t):
     return None if t is None else t.data_ptr()
-
-
-def _on(stream, dev):
-    """(stream handle, context that allocates on it)."""
-    import torch
-
-    if stream is None:
-        return torch.cuda.current_stream(dev).cuda_stream, None
-    if stream.device.index != dev:
-        raise ValueError("stream belongs to another device")
-    return stream.cuda_stream, torch.cuda.stream(stream)
-
-
-def _hold(stream, *tensors):
-    """Keeps the memory of inputs of another stream until `stream` is done with them."""
-    if stream is not None:
-        for t in tensors:
-            if t is not None:
-                t.record_stream(stream)
 
 
 class _Nothing:
@@ -114,6 +96,25 @@ class _Nothing:
 
 
 _NOTHING = _Nothing()
+
+
+def _on(stream, dev):
+    """(stream handle, context that allocates on it)."""
+    import torch
+
+    if stream is None:
+        return torch._C._cuda_getCurrentRawStream(dev), _NOTHING
+    if stream.device.index != dev:
+        raise ValueError("stream belongs to another device")
+    return stream.cuda_stream, torch.cuda.stream(stream)
+
+
+def _hold(stream, *tensors):
+    """Keeps the memory of inputs of another stream until `stream` is done with them."""
+    if stream is not None:
+        for t in tensors:
+            if t is not None:
+                t.record_stream(stream)
 
 
 def _entries(ids, scale, indptr, wide):
@@ -161,25 +162,24 @@ def embedding_lookup(table, ids, scale=None, indptr=None, alpha: float = 1.0, ou
     if scale is not None and table.dtype == torch.float32 and scale.dtype == torch.float64:
         code, wide, kind = _lib.MFM_DTYPE_F32_F64, torch.float64, torch.float64
     ids64 = _entries(ids, scale, indptr, wide)
-    tp, ld = _matrix("table", table)
-    n_rows, d = table.shape
+    tp, n_rows, d, ld = _matrix("table", table)
     if d < 1:
         raise ValueError("embedding width must be >= 1")
-    dev = _one_device((("table", table), ("ids", ids), ("scale", scale), ("indptr", indptr),
-                       ("out", out)))
+    dev = _one_device(table, ids, scale, indptr, out)
     n = ids.numel()
     n_out = n if indptr is None else indptr.numel() - 1
     s, ctx = _on(stream, dev)
     _hold(stream, table, ids, scale, indptr, out)
     if out is None:
-        with ctx or _NOTHING:
-            out = torch.empty((n_out, d), dtype=kind, device=table.device)
+        with ctx:
+            out = table.new_empty((n_out, d), dtype=kind)
+        op, ld_out = out.data_ptr(), d
         result = out if ids.dim() == 1 else out.view(ids.shape + (d,))
     else:
         if out.dtype != kind or tuple(out.shape) != (n_out, d):
             raise ValueError(f"out must be {kind} of shape {(n_out, d)}")
         result = out
-    op, ld_out = _matrix("out", out)
+        op, _, _, ld_out = _matrix("out", out)
     _fail(_lib.lib().mfm_embedding_lookup_device(
         code, dev, ids64, ids.data_ptr(), n, _ptr(indptr), n_out, _ptr(scale), float(alpha), tp,
         n_rows, d, ld, op, ld_out, s))
@@ -206,11 +206,10 @@ def _grad(grad, ids, n_rows, scale, indptr, alpha, table, dtype, stream, by_rows
     n_out = n if indptr is None else indptr.numel() - 1
     if grad.dim() != 2:
         grad = grad.reshape(-1, grad.shape[-1]) if grad.dim() > 2 else grad
-    gp, ld = _matrix("grad", grad)
-    d = grad.shape[1]
+    gp, given, d, ld = _matrix("grad", grad)
     if d < 1:
         raise ValueError("embedding width must be >= 1")
-    if grad.shape[0] != n_out:
+    if given != n_out:
         raise ValueError(f"grad must have one row per {'id' if indptr is None else 'CSR row'}")
     tp, ld_table = None, d
     if table is not None:
@@ -220,26 +219,24 @@ def _grad(grad, ids, n_rows, scale, indptr, alpha, table, dtype, stream, by_rows
             code = _lib.MFM_DTYPE_F32_F64
         elif table.dtype != grad.dtype:
             raise ValueError("table must have grad's type (or be float32 with a float64 grad)")
-        tp, ld_table = _matrix("table", table)
-    dev = _one_device((("grad", grad), ("ids", ids), ("scale", scale), ("indptr", indptr),
-                       ("table", table)))
+        tp, _, _, ld_table = _matrix("table", table)
+    dev = _one_device(grad, ids, scale, indptr, table)
     L = _lib.lib()
     nbytes = L.mfm_embedding_grad_workspace_bytes(code, n, n_rows, d)
     s, ctx = _on(stream, dev)
     _hold(stream, grad, ids, scale, indptr, table)
-    device = grad.device
     keys = rows = count = whole = d_scale = None
-    with ctx or _NOTHING:
-        ws = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=device)
+    with ctx:
+        ws = grad.new_empty(max(nbytes, 1), dtype=torch.uint8)
         if by_rows:
             cap = min(n, n_rows)
-            keys = torch.empty(cap, dtype=ids.dtype, device=device)
-            rows = torch.empty((cap, d), dtype=kind, device=device)
-            count = torch.empty((), dtype=torch.int64, device=device)
+            keys = ids.new_empty(cap)
+            rows = grad.new_empty((cap, d), dtype=kind)
+            count = grad.new_empty((), dtype=torch.int64)
         else:
-            whole = torch.empty((n_rows, d), dtype=kind, device=device)
+            whole = grad.new_empty((n_rows, d), dtype=kind)
         if table is not None:
-            d_scale = torch.empty(ids.shape, dtype=wide, device=device)
+            d_scale = grad.new_empty(ids.shape, dtype=wide)
     # empty tensors have no address; the ABI tells its two results apart by theirs
     at = lambda t: None if t is None else (t.data_ptr() or ws.data_ptr())  # noqa: E731
     _fail(L.mfm_embedding_grad_device(

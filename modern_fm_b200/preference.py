@@ -24,7 +24,7 @@ from __future__ import annotations
 from typing import NamedTuple, Optional
 
 from . import _lib
-from .embedding import _NOTHING, _fail, _hold, _matrix, _on, _one_device, _ptr, _storage
+from .embedding import _fail, _hold, _matrix, _on, _one_device, _ptr, _storage
 
 
 class LabelLogprobs(NamedTuple):
@@ -55,20 +55,21 @@ class PolicyLoss(NamedTuple):
 
 
 def _scores(logits, labels):
-    """(dtype code, arithmetic type, pointer, pitch, labels64) of the class scores."""
+    """(dtype code, arithmetic type, pointer, rows, classes, pitch, labels64) of the scores."""
     import torch
 
     code = _storage().get(logits.dtype)
     if code is None:
         raise ValueError("logits must be float64, float32, bfloat16 or float16")
-    p, ld = _matrix("logits", logits)
-    if logits.shape[1] < 1:
+    p, n, c, ld = _matrix("logits", logits)
+    if c < 1:
         raise ValueError("logits must have at least one class")
-    if labels.dtype not in (torch.int32, torch.int64):
+    kind = labels.dtype
+    if kind is not torch.int64 and kind is not torch.int32:
         raise ValueError("labels must be int32 or int64")
-    _vector("labels", labels, logits.shape[0], labels.dtype)
-    wide = torch.float64 if logits.dtype == torch.float64 else torch.float32
-    return code, wide, p, ld, 1 if labels.dtype == torch.int64 else 0
+    _vector("labels", labels, n, kind)
+    wide = torch.float64 if code == _lib.MFM_DTYPE_F64 else torch.float32
+    return code, wide, p, n, c, ld, 1 if kind is torch.int64 else 0
 
 
 def _vector(name, t, n, dtype):
@@ -93,16 +94,15 @@ def label_logprobs(logits, labels, indptr=None, stream=None) -> LabelLogprobs:
     as ``preference_loss`` takes its reference."""
     import torch
 
-    code, wide, p, ld, l64 = _scores(logits, labels)
+    code, wide, p, n, c, ld, l64 = _scores(logits, labels)
     n_seq = 0 if indptr is None else _bounds(indptr)
-    dev = _one_device((("logits", logits), ("labels", labels), ("indptr", indptr)))
-    n, c = logits.shape
+    dev = _one_device(logits, labels, indptr)
     s, ctx = _on(stream, dev)
     _hold(stream, logits, labels, indptr)
-    with ctx or _NOTHING:
-        lp = torch.empty(n, dtype=wide, device=logits.device)
-        lse = torch.empty(n, dtype=wide, device=logits.device)
-        sums = None if indptr is None else torch.empty(n_seq, dtype=wide, device=logits.device)
+    with ctx:
+        lp = logits.new_empty(n, dtype=wide)
+        lse = logits.new_empty(n, dtype=wide)
+        sums = None if indptr is None else logits.new_empty(n_seq, dtype=wide)
     _fail(_lib.lib().mfm_label_logprobs_device(
         code, dev, p, ld, n, c, l64, labels.data_ptr(), _ptr(indptr), n_seq, lp.data_ptr(),
         lse.data_ptr(), sums.data_ptr() if n_seq else None, s))
@@ -115,15 +115,14 @@ def label_logprobs_grad(grad, logits, labels, lse, stream=None):
     the logits' type. ``lse`` is the forward's."""
     import torch
 
-    code, wide, p, ld, l64 = _scores(logits, labels)
-    n, c = logits.shape
+    code, wide, p, n, c, ld, l64 = _scores(logits, labels)
     _vector("grad", grad, n, wide)
     _vector("lse", lse, n, wide)
-    dev = _one_device((("logits", logits), ("labels", labels), ("grad", grad), ("lse", lse)))
+    dev = _one_device(logits, labels, grad, lse)
     s, ctx = _on(stream, dev)
     _hold(stream, logits, labels, grad, lse)
-    with ctx or _NOTHING:
-        out = torch.empty((n, c), dtype=logits.dtype, device=logits.device)
+    with ctx:
+        out = logits.new_empty((n, c))
     _fail(_lib.lib().mfm_label_logprobs_grad_device(
         code, dev, p, ld, n, c, l64, labels.data_ptr(), grad.data_ptr(), lse.data_ptr(),
         out.data_ptr(), c, s))
@@ -146,26 +145,23 @@ def preference_loss(logits, labels, indptr, reference, beta: float = 0.1,
     """
     import torch
 
-    code, wide, p, ld, l64 = _scores(logits, labels)
+    code, wide, p, n, c, ld, l64 = _scores(logits, labels)
     n_seq = _bounds(indptr)
     if n_seq % 2:
         raise ValueError("indptr must bound an even number of sequences")
     n_pairs = n_seq // 2
-    n, c = logits.shape
     _vector("reference", reference, n_seq, wide)
     if sample_weight is not None:
         _vector("sample_weight", sample_weight, n_pairs, wide)
-    dev = _one_device((("logits", logits), ("labels", labels), ("indptr", indptr),
-                       ("reference", reference), ("sample_weight", sample_weight)))
+    dev = _one_device(logits, labels, indptr, reference, sample_weight)
     L = _lib.lib()
     nbytes = L.mfm_preference_workspace_bytes(code, n, n_pairs)
     s, ctx = _on(stream, dev)
     _hold(stream, logits, labels, indptr, reference, sample_weight)
-    device = logits.device
-    with ctx or _NOTHING:
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
-        out = torch.empty(1 + 3 * n_pairs, dtype=wide, device=device)
-        grad = torch.empty((n, c), dtype=logits.dtype, device=device) if with_grad else None
+    with ctx:
+        ws = logits.new_empty(nbytes, dtype=torch.uint8)
+        out = logits.new_empty(1 + 3 * n_pairs, dtype=wide)
+        grad = logits.new_empty((n, c)) if with_grad else None
     at, size = out.data_ptr(), out.element_size()
     _fail(L.mfm_preference_loss_device(
         code, dev, p, ld, n, c, l64, labels.data_ptr(), indptr.data_ptr(), n_pairs,
@@ -190,27 +186,23 @@ def policy_loss(logits, labels, old_logprobs, advantages, reference=None, clip_l
     """
     import torch
 
-    code, wide, p, ld, l64 = _scores(logits, labels)
-    n, c = logits.shape
+    code, wide, p, n, c, ld, l64 = _scores(logits, labels)
     _vector("old_logprobs", old_logprobs, n, wide)
     _vector("advantages", advantages, n, wide)
     if reference is not None:
         _vector("reference", reference, n, wide)
     if sample_weight is not None:
         _vector("sample_weight", sample_weight, n, wide)
-    dev = _one_device((("logits", logits), ("labels", labels), ("old_logprobs", old_logprobs),
-                       ("advantages", advantages), ("reference", reference),
-                       ("sample_weight", sample_weight)))
+    dev = _one_device(logits, labels, old_logprobs, advantages, reference, sample_weight)
     L = _lib.lib()
     nbytes = L.mfm_policy_workspace_bytes(code, n)
     s, ctx = _on(stream, dev)
     _hold(stream, logits, labels, old_logprobs, advantages, reference, sample_weight)
-    device = logits.device
-    with ctx or _NOTHING:
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
-        stats = torch.empty(3, dtype=wide, device=device)
-        lp = torch.empty(n, dtype=wide, device=device)
-        grad = torch.empty((n, c), dtype=logits.dtype, device=device) if with_grad else None
+    with ctx:
+        ws = logits.new_empty(nbytes, dtype=torch.uint8)
+        stats = logits.new_empty(3, dtype=wide)
+        lp = logits.new_empty(n, dtype=wide)
+        grad = logits.new_empty((n, c)) if with_grad else None
     _fail(L.mfm_policy_loss_device(
         code, dev, p, ld, n, c, l64, labels.data_ptr(), old_logprobs.data_ptr(),
         advantages.data_ptr(), _ptr(reference), float(clip_low), float(clip_high), float(kl_coef),
