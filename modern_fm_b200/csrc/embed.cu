@@ -320,9 +320,10 @@ struct GradArgs {
     I* keys_out;
     int64_t* count;
     A* d_scale;
-    // sorted entries
-    const uint32_t *keys, *pos;
-    const int32_t* row_of;
+    // sorted entries, padded to whole chunks: key, gradient row, scale
+    const uint32_t *keys, *srows;
+    const A* scales;
+    const int32_t* row_of;  // by position
     const uint32_t *base, *tile_base;
     A *part_head, *part_tail;
     int64_t n_chunks;
@@ -334,7 +335,7 @@ struct GradArgs {
 };
 
 // One chunk of sorted entries x LV vectors of columns by one lane group: sums of
-// scale[pos] grad[row], run by run. A run that lies in the chunk is written; the
+// scale grad[row], run by run. A run that lies in the chunk is written; the
 // part of a run that began before goes to part_head[chunk], the part of one that
 // goes on behind to part_tail[chunk] (all of it to part_head when both).
 template <class G, class T, class A, class O, class I, bool WIDE, int LV>
@@ -342,12 +343,26 @@ __device__ __forceinline__ void reduce_chunk(const GradArgs<G, T, A, O, I>& a, i
                                              bool first_lane) {
     constexpr int U = 8, N = Lane<G, WIDE>::N;
     const uint32_t pad_key = (uint32_t)a.in.n_rows;
-    const int64_t n = a.in.n, e0 = c * kChunk, e1 = e0 + kChunk < n ? e0 + kChunk : n;
-    uint32_t cur = a.keys[e0];
-    if (cur == pad_key) return;  // padding sorts last
-    bool before = e0 > 0 && a.keys[e0 - 1] == cur;
+    const int64_t n = a.in.n, e0 = c * kChunk, e1 = e0 + kChunk;
+    uint32_t k[kChunk], row[kChunk];
+#pragma unroll
+    for (int i = 0; i < kChunk / 4; ++i) {
+        const uint4 x = reinterpret_cast<const uint4*>(a.keys + e0)[i], y = reinterpret_cast<const uint4*>(a.srows + e0)[i];
+        k[4 * i] = x.x;
+        k[4 * i + 1] = x.y;
+        k[4 * i + 2] = x.z;
+        k[4 * i + 3] = x.w;
+        row[4 * i] = y.x;
+        row[4 * i + 1] = y.y;
+        row[4 * i + 2] = y.z;
+        row[4 * i + 3] = y.w;
+    }
+    const uint32_t last = e0 > 0 ? a.keys[e0 - 1] : pad_key;
     const bool behind = e1 < n;
     const uint32_t next = behind ? a.keys[e1] : pad_key;
+    uint32_t cur = k[0];
+    if (cur == pad_key) return;  // padding sorts last
+    bool before = e0 > 0 && last == cur;
     int64_t rank = a.rows ? a.runs_before(c) - (before ? 1 : 0) : 0;
     A acc[N];
 #pragma unroll
@@ -370,32 +385,20 @@ __device__ __forceinline__ void reduce_chunk(const GradArgs<G, T, A, O, I>& a, i
     };
 #pragma unroll
     for (int b = 0; b < kChunk; b += U) {
-        if (e0 + b >= e1) break;
-        uint32_t k[U];
-        A f[U];
+        if (b > 0 && k[b] == pad_key) break;
         Lane<G, WIDE> v[U];
-        uint32_t p[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const bool in = e0 + b + u < e1;
-            k[u] = in ? a.keys[e0 + b + u] : pad_key;
-            p[u] = in ? a.pos[e0 + b + u] : 0u;
-        }
-        int64_t row[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            row[u] = a.row_of && k[u] != pad_key ? (int64_t)a.row_of[p[u]] : (int64_t)p[u];
-            f[u] = a.scale && k[u] != pad_key ? a.scale[p[u]] : A(1);
-        }
+        A f[U];
 #pragma unroll
         for (int u = 0; u < U; ++u)
-            if (k[u] != pad_key) v[u].load(a.grad + row[u] * a.ld + col);
+            if (k[b + u] != pad_key) v[u].load(a.grad + (int64_t)row[b + u] * a.ld + col);
+#pragma unroll
+        for (int u = 0; u < U; ++u) f[u] = a.scales ? a.scales[e0 + b + u] : A(1);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            if (e0 + b + u < e1 && cur != pad_key) {
-                if (k[u] != cur) {
+            if (cur != pad_key) {
+                if (k[b + u] != cur) {
                     finish();
-                    cur = k[u];
+                    cur = k[b + u];
                     before = false;
                     ++rank;
 #pragma unroll
@@ -558,11 +561,14 @@ __global__ void __launch_bounds__(256)
     embed_cross_kernel(const GradArgs<G, T, A, O, I> a) {
     constexpr int N = Lane<G, WIDE>::N, GR = 256 / LV;
     __shared__ int64_t run_last[GR];  // last chunk of the run begun in the group's chunk, -1: none
+    __shared__ int long_groups[GR], n_long;
     __shared__ A shared_part[256 * N];
     const int lane = threadIdx.x % LV, group = threadIdx.x / LV;
     const int64_t c0 = (int64_t)blockIdx.x * GR, c = c0 + group, n = a.in.n;
     const int64_t col = ((int64_t)blockIdx.y * LV + lane) * N;
     const uint32_t pad_key = (uint32_t)a.in.n_rows;
+    if (threadIdx.x == 0) n_long = 0;
+    __syncthreads();
     if (lane == 0) {
         int64_t last = -1;
         if (c + 1 < a.n_chunks) {
@@ -580,6 +586,8 @@ __global__ void __launch_bounds__(256)
             }
         }
         run_last[group] = last;
+        // which group's run is added first does not change any sum
+        if (last - c > kLongRun) long_groups[atomicAdd(&n_long, 1)] = group;
     }
     __syncthreads();
     auto write = [&](int64_t chunk, A (&acc)[N]) {
@@ -605,9 +613,9 @@ __global__ void __launch_bounds__(256)
         }
         write(c, acc);
     }
-    for (int g = 0; g < GR; ++g) {  // uniform over the block
+    for (int i = 0; i < n_long; ++i) {
+        const int g = long_groups[i];
         const int64_t last = run_last[g], from = c0 + g;
-        if (last < 0 || last - from <= kLongRun) continue;
         A acc[N];
 #pragma unroll
         for (int j = 0; j < N; ++j) acc[j] = A(0);
@@ -743,13 +751,14 @@ void lookup_launch(int device, const Entries<I>& in, const A* scale, A alpha, co
 struct GradWs {
     IdSortPlan sort;
     int64_t n_chunks = 0;
-    size_t off_row = 0, off_base = 0, off_tile = 0, off_head = 0, off_tail = 0, bytes = 0;
+    size_t off_row = 0, off_scale = 0, off_base = 0, off_tile = 0, off_head = 0, off_tail = 0, bytes = 0;
     GradWs(int dtype, int64_t n, int64_t n_rows, int64_t d) : sort(n, n_rows) {
         auto up = [](size_t b) { return (b + 255) / 256 * 256; };
         const size_t a = dtype == MFM_DTYPE_F64 || dtype == MFM_DTYPE_F32_F64 ? 8 : 4;
         n_chunks = ceil_div(n, kChunk);
         off_row = up((size_t)sort.words * 4 + 4);  // the block count is the last word
-        off_base = off_row + up((size_t)n * 4);
+        off_scale = off_row + up((size_t)n * 4);
+        off_base = off_scale + up((size_t)(n + kSortPad) * a);
         off_tile = off_base + up((size_t)n_chunks * 4);
         off_head = off_tile + up((size_t)ceil_div(n_chunks, kTileChunks) * 4);
         off_tail = off_head + up((size_t)n_chunks * d * a);
@@ -764,9 +773,13 @@ void grad_launch(int device, GradArgs<G, T, A, O, I>& a, const GradWs& W, char* 
     uint32_t* words = reinterpret_cast<uint32_t*>(ws);
     unsigned* done = words + W.sort.words;
     int32_t* row_of = a.in.indptr ? reinterpret_cast<int32_t*>(ws + W.off_row) : nullptr;
-    const IdSorted S = sort_ids(W.sort, a.in, row_of, done, words, s);
-    a.keys = S.keys;
-    a.pos = S.pos;
+    SortedOut<A> sorted{};
+    sorted.scale = a.scale;
+    sorted.scales = reinterpret_cast<A*>(ws + W.off_scale);
+    sort_ids(W.sort, a.in, row_of, done, words, sorted, s);
+    a.keys = sorted.keys;
+    a.srows = sorted.rows;
+    a.scales = a.scale ? sorted.scales : nullptr;
     a.row_of = row_of;
     a.n_chunks = nc;
     a.part_head = reinterpret_cast<A*>(ws + W.off_head);
@@ -775,7 +788,7 @@ void grad_launch(int device, GradArgs<G, T, A, O, I>& a, const GradWs& W, char* 
         uint32_t* base = reinterpret_cast<uint32_t*>(ws + W.off_base);
         uint32_t* tiles = reinterpret_cast<uint32_t*>(ws + W.off_tile);
         chunk_heads_kernel<<<(unsigned)ceil_div(nc, kTileChunks), kTileChunks, 0, s>>>(
-            S.keys, n, (uint32_t)a.in.n_rows, nc, base, tiles, done, a.count);
+            a.keys, n, (uint32_t)a.in.n_rows, nc, base, tiles, done, a.count);
         a.base = base;
         a.tile_base = tiles;
     }

@@ -1,18 +1,21 @@
-// embed_sort.cuh — stable radix sort of one batch's ids with their positions,
-// into a workspace of the caller: no allocation, no host round trip, no block
-// waits for another, so a call can be captured and its launches replayed.
+// embed_sort.cuh — stable radix sort of one batch's ids with what the gradient
+// reads by them, into a workspace of the caller: no allocation, no host round
+// trip, no block waits for another, so a call can be captured and replayed.
 //
 // Ids outside the table get the key n_rows and sort behind every real id. Least
-// significant digit first, 8 bits a pass, in the tiles of segsort.cuh's
-// scatter: a tile is ranked by match_any per warp, reordered in shared memory
-// and written in runs. Two things differ from the training plan's sort, because
-// one batch of some 10^5 ids is bound by its launches, not by its bytes:
+// significant digit first, in tiles of 2048 entries that are ranked by
+// match_any per warp, reordered in shared memory and written in runs. One
+// batch of 10^4 to 10^6 ids is bound by its launches and their latencies, not by
+// its bytes, which decides the rest:
+//  * digits of up to 12 bits where that saves a pass (17 to 24 bits: two passes
+//    instead of three, 302k click ids of 23 bits: 52 -> 38 us), of 8 bits otherwise;
 //  * a pass's scatter counts the next pass's digits while it writes (integer
 //    adds, grouped per warp), so only the first pass has a counting launch;
-//  * up to kFuseTiles tiles, each tile sums the counts before it by itself
-//    (at most 192 KB of L2 reads), which saves the prefix launch; more
-//    tiles take one prefix launch a pass.
-// Up to kSmallSort ids one block does every pass in shared memory.
+//  * 8-bit digits of up to kFuseTiles tiles: each tile sums the counts before it
+//    by itself (at most 192 KB of L2 reads); else one prefix launch a pass;
+//  * the last pass leaves, beside the sorted keys, each entry's gradient row and
+//    scale instead of its position, so the sums read them in order;
+//  * up to kSmallSort ids one block does every pass in shared memory.
 #pragma once
 
 #include <type_traits>
@@ -26,7 +29,9 @@ constexpr int kETileNT = 256;
 constexpr int kETileItems = 8;
 constexpr int kETile = kETileNT * kETileItems;
 constexpr int kFuseTiles = 192;
+constexpr int kWideBits = 12;
 constexpr int64_t kSmallSort = 2048;
+constexpr int kSortPad = 16;  // places behind the last entry: key n_rows, row 0, scale 0
 
 // The entries of a batch: their ids and, where they are summed by rows, the rows'
 // bounds (indptr, n_out + 1; NULL: every entry is a row of its own).
@@ -91,19 +96,43 @@ struct Entries {
     }
 };
 
+// What the last pass writes beside a key: the row and scale of the entry at
+// position p (row_of NULL: the position itself; scale NULL: none).
+template <class A>
+struct SortedOut {
+    uint32_t* keys;
+    uint32_t* rows;
+    A* scales;
+    const int32_t* row_of;
+    const A* scale;
+    uint32_t pad_key;
+    __device__ __forceinline__ void load(uint32_t p, uint32_t& row, A& s) const {
+        row = row_of ? (uint32_t)row_of[p] : p;
+        s = scale ? scale[p] : A(1);
+    }
+    __device__ __forceinline__ void store(int64_t at, uint32_t k, uint32_t row, A s) const {
+        keys[at] = k;
+        rows[at] = row;
+        if (scale) scales[at] = s;
+    }
+};
+
 // Keys and rows of all entries, digit counts of the first pass by tile, and zeros
 // for the passes after it and for the block count of the kernels behind the sort.
-template <class I>
+template <class I, int BITS>
 __global__ void __launch_bounds__(kETileNT)
-    id_count_kernel(Entries<I> in, int passes, int64_t n_tiles, uint32_t* __restrict__ keys,
-                    int32_t* __restrict__ row_of, uint32_t* __restrict__ counts,
-                    unsigned* __restrict__ done) {
-    __shared__ uint32_t h[256];
+    id_count_kernel(Entries<I> in, int passes, uint32_t mask, int64_t n_tiles,
+                    uint32_t* __restrict__ keys, int32_t* __restrict__ row_of,
+                    uint32_t* __restrict__ counts, unsigned* __restrict__ done) {
+    constexpr int D = 1 << BITS;
+    __shared__ uint32_t h[D];
     const int t = threadIdx.x;
     const int64_t tile = blockIdx.x, lo = tile * kETile;
-    h[t] = 0;
+    for (int d = t; d < D; d += kETileNT) {
+        h[d] = 0;
+        for (int p = 1; p < passes; ++p) counts[(p * n_tiles + tile) * D + d] = 0;
+    }
     if (tile == 0 && t == 0) *done = 0;
-    for (int p = 1; p < passes; ++p) counts[(p * n_tiles + tile) * 256 + t] = 0;
     __syncthreads();
     const int64_t q0 = lo + (t / 32) * (32 * kETileItems);
     int32_t r[kETileItems];
@@ -115,152 +144,243 @@ __global__ void __launch_bounds__(kETileNT)
             if (in.indptr) row_of[q] = r[i];
             const uint32_t k = in.key(q, r[i]);
             keys[q] = k;
-            atomicAdd(&h[k & 255u], 1u);
+            atomicAdd(&h[k & mask], 1u);
         }
     }
     __syncthreads();
-    counts[tile * 256 + t] = h[t];
+    for (int d = t; d < D; d += kETileNT) counts[tile * D + d] = h[d];
 }
 
-// For batches of more than kFuseTiles tiles: block d turns digit d's counts into
-// their prefix over the tiles, in place, and writes the digit's total.
+// Turns each digit's counts into their prefix over the tiles, in place, and writes
+// its total: a block takes 32 digits, 8 threads each a stretch of the tiles.
 __global__ void __launch_bounds__(256)
-    id_prefix_kernel(uint32_t* __restrict__ counts, int64_t n_tiles,
+    id_prefix_kernel(uint32_t* __restrict__ counts, int64_t n_tiles, int digits,
                      uint32_t* __restrict__ totals) {
-    __shared__ uint32_t sm[8];
-    const int d = blockIdx.x;
-    uint32_t run = 0;
-    for (int64_t b = 0; b < n_tiles; b += 256) {
-        const int64_t t = b + threadIdx.x;
-        const uint32_t c = t < n_tiles ? counts[t * 256 + d] : 0u;
-        uint32_t all;
-        const uint32_t ex = block_exclusive_scan<uint32_t, 256>(c, sm, all);
-        if (t < n_tiles) counts[t * 256 + d] = run + ex;
-        run += all;
+    constexpr int F = 20;  // counts in flight
+    __shared__ uint32_t part[8][33];
+    const int lane = threadIdx.x & 31, g = threadIdx.x / 32, d = blockIdx.x * 32 + lane;
+    const int64_t per = ceil_div(n_tiles, (int64_t)8), t0 = g * per;
+    const int64_t t1 = t0 + per < n_tiles ? t0 + per : n_tiles;
+    uint32_t sum = 0, c[F];
+    for (int64_t b = t0; b < t1; b += F) {
+#pragma unroll
+        for (int f = 0; f < F; ++f) c[f] = b + f < t1 ? counts[(b + f) * digits + d] : 0u;
+#pragma unroll
+        for (int f = 0; f < F; ++f) sum += c[f];
     }
-    if (threadIdx.x == 0) totals[d] = run;
+    part[g][lane] = sum;
+    __syncthreads();
+    uint32_t run = 0, all = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        if (i < g) run += part[i][lane];
+        all += part[i][lane];
+    }
+    if (g == 0) totals[d] = all;
+    for (int64_t b = t0; b < t1; b += F) {
+        if (per > F) {  // one stretch of F is still in registers
+#pragma unroll
+            for (int f = 0; f < F; ++f) c[f] = b + f < t1 ? counts[(b + f) * digits + d] : 0u;
+        }
+#pragma unroll
+        for (int f = 0; f < F; ++f)
+            if (b + f < t1) {
+                counts[(b + f) * digits + d] = run;
+                run += c[f];
+            }
+    }
 }
 
-// One pass of one tile. FIRST: the values are the positions.
-// FUSED: `counts` holds digit counts and the tile adds up those before it;
-// otherwise it holds their prefix over the tiles, and `totals` the digits' sums.
-// next != NULL: the next pass's counts.
-template <bool FIRST, bool FUSED>
+// A thread's ranks of its items among the equal digits of its warp, in order;
+// cnt: the warp's running counts (zero before).
+template <int ITEMS, class C>
+__device__ __forceinline__ void warp_ranks(const uint32_t (&digit)[ITEMS], C* cnt,
+                                           uint32_t (&rank)[ITEMS]) {
+    const int lane = threadIdx.x & 31;
+    const unsigned lt = (1u << lane) - 1u;
+    unsigned peers[ITEMS];
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) peers[i] = __match_any_sync(0xffffffffu, digit[i]);
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+        const int leader = __ffs(peers[i]) - 1;
+        uint32_t b = 0;
+        if (lane == leader && !(digit[i] & 0x80000000u)) {
+            b = cnt[digit[i]];
+            cnt[digit[i]] = (C)(b + (uint32_t)__popc(peers[i]));
+        }
+        b = __shfl_sync(0xffffffffu, b, leader);
+        rank[i] = b + (uint32_t)__popc(peers[i] & lt);
+        __syncwarp();
+    }
+}
+
+template <int BITS>
+constexpr int scatter_smem() {  // counts per warp (16 bits), offsets, the tile
+    return (kETileNT / 32) * (1 << BITS) * 2 + (1 << BITS) * 4 + kETile * 8;
+}
+
+// One pass of one tile. FIRST: the values are the positions. FUSED: `counts` holds
+// digit counts and the tile adds up those before it; otherwise it holds their
+// prefix over the tiles, and `totals` the digits' sums. next != NULL: the next
+// pass's counts; NULL: the last pass, which writes through `out`.
+template <class A, int BITS, bool FIRST, bool FUSED>
 __global__ void __launch_bounds__(kETileNT)
     id_scatter_kernel(const uint32_t* __restrict__ kin, const uint32_t* __restrict__ vin,
                       uint32_t* __restrict__ kout, uint32_t* __restrict__ vout, int64_t n,
-                      int64_t n_tiles, int shift, const uint32_t* __restrict__ counts,
-                      const uint32_t* __restrict__ totals, uint32_t* __restrict__ next) {
-    constexpr int NW = kETileNT / 32;
-    __shared__ uint32_t cnt[NW][256];
-    __shared__ uint32_t base[256];
+                      int64_t n_tiles, int shift, int bits, const uint32_t* __restrict__ counts,
+                      const uint32_t* __restrict__ totals, uint32_t* __restrict__ next,
+                      SortedOut<A> out) {
+    constexpr int NW = kETileNT / 32, D = 1 << BITS, PT = D / kETileNT;  // digits per thread
+    extern __shared__ uint4 scatter_mem[];
+    uint16_t(*cnt)[D] = reinterpret_cast<uint16_t(*)[D]>(scatter_mem);
+    uint32_t* base = reinterpret_cast<uint32_t*>(cnt + NW);
+    uint2* skv = reinterpret_cast<uint2*>(base + D);
     __shared__ uint32_t scan_sm[NW];
-    __shared__ uint2 skv[kETile];
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
     const int64_t tile = blockIdx.x, lo = tile * kETile;
     const int m = (int)(n - lo < kETile ? n - lo : kETile);
+    const uint32_t mask = (1u << bits) - 1u;
     const int q0 = warp * (32 * kETileItems) + lane;  // striped: a warp's items are in position order
-    for (int i = t; i < NW * 256; i += kETileNT) (&cnt[0][0])[i] = 0;
-    uint32_t key[kETileItems], val[kETileItems], rank[kETileItems];
+    for (int i = t; i < NW * D / 8; i += kETileNT) scatter_mem[i] = make_uint4(0, 0, 0, 0);
+    uint32_t key[kETileItems], val[kETileItems], digit[kETileItems], rank[kETileItems];
 #pragma unroll
     for (int i = 0; i < kETileItems; ++i) {
         const int q = q0 + i * 32;
-        key[i] = 0;
-        val[i] = 0;
-        if (q < m) {
-            key[i] = kin[lo + q];
-            val[i] = FIRST ? (uint32_t)(lo + q) : vin[lo + q];
-        }
+        key[i] = q < m ? kin[lo + q] : 0u;
+        val[i] = FIRST ? (uint32_t)(lo + q) : (q < m ? vin[lo + q] : 0u);
     }
-    uint32_t dtotal = 0, before = 0, all;
+    // this thread's digits are PT t .. PT t + PT - 1: their places in the output
+    uint32_t total[PT], before[PT];
     if (FUSED) {
         constexpr int F = 32;  // tiles' counts in flight
+        static_assert(!FUSED || PT == 1, "summed by the tile: one digit a thread");
+        total[0] = before[0] = 0;
         for (int b0 = 0; b0 < (int)n_tiles; b0 += F) {
             uint32_t c[F];
 #pragma unroll
-            for (int f = 0; f < F; ++f) c[f] = b0 + f < (int)n_tiles ? counts[(b0 + f) * 256 + t] : 0u;
+            for (int f = 0; f < F; ++f) c[f] = b0 + f < (int)n_tiles ? counts[(b0 + f) * D + t] : 0u;
 #pragma unroll
             for (int f = 0; f < F; ++f) {
-                dtotal += c[f];
-                before += b0 + f < tile ? c[f] : 0u;
+                total[0] += c[f];
+                before[0] += b0 + f < tile ? c[f] : 0u;
             }
         }
     } else {
-        dtotal = totals[t];
-        before = counts[tile * 256 + t];
-    }
-    const uint32_t goff = block_exclusive_scan<uint32_t, kETileNT>(dtotal, scan_sm, all) + before;
-    const unsigned lt = (1u << lane) - 1u;
 #pragma unroll
-    for (int i = 0; i < kETileItems; ++i) {
-        const bool valid = q0 + i * 32 < m;
-        const uint32_t d = valid ? (key[i] >> shift) & 255u : 256u + (uint32_t)lane;
-        const unsigned peers = __match_any_sync(0xffffffffu, d);
-        const int leader = __ffs(peers) - 1;
-        uint32_t b = 0;
-        if (valid && lane == leader) {
-            b = cnt[warp][d];
-            cnt[warp][d] = b + (uint32_t)__popc(peers);
+        for (int k = 0; k < PT; ++k) {
+            total[k] = totals[t * PT + k];
+            before[k] = counts[tile * D + t * PT + k];
         }
-        b = __shfl_sync(0xffffffffu, b, leader);
-        rank[i] = b + (uint32_t)__popc(peers & lt);
-        __syncwarp();
     }
+    uint32_t sum = 0, all;
+#pragma unroll
+    for (int k = 0; k < PT; ++k) sum += total[k];
+    uint32_t at = block_exclusive_scan<uint32_t, kETileNT>(sum, scan_sm, all);  // its barriers end the zeroing
+#pragma unroll
+    for (int k = 0; k < PT; ++k) {
+        before[k] += at;
+        at += total[k];
+    }
+#pragma unroll
+    for (int i = 0; i < kETileItems; ++i)
+        digit[i] = q0 + i * 32 < m ? (key[i] >> shift) & mask : 0x80000000u + (uint32_t)lane;
+    warp_ranks<kETileItems>(digit, cnt[warp], rank);
     __syncthreads();
-    uint32_t tot = 0;
+    // the warps' counts -> their prefix over the warps; two 16-bit counts a word
+    // (at most 2048 each: no carry)
+    uint32_t mine[PT];
+    if (PT > 1) {
+        uint32_t run[PT / 2 + 1];
 #pragma unroll
-    for (int w = 0; w < NW; ++w) {
-        const uint32_t c = cnt[w][t];
-        cnt[w][t] = tot;
-        tot += c;
+        for (int k = 0; k < PT / 2; ++k) run[k] = 0;
+#pragma unroll
+        for (int w = 0; w < NW; ++w) {
+            uint32_t* row = reinterpret_cast<uint32_t*>(cnt[w] + t * PT);
+#pragma unroll
+            for (int k = 0; k < PT / 2; ++k) {
+                const uint32_t c = row[k];
+                row[k] = run[k];
+                run[k] += c;
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < PT; ++k) mine[k] = (run[k / 2] >> (k & 1 ? 16 : 0)) & 0xffffu;
+    } else {
+        uint32_t run = 0;
+#pragma unroll
+        for (int w = 0; w < NW; ++w) {
+            const uint32_t c = cnt[w][t];
+            cnt[w][t] = (uint16_t)run;
+            run += c;
+        }
+        mine[0] = run;
     }
-    const uint32_t dstart = block_exclusive_scan<uint32_t, kETileNT>(tot, scan_sm, all);
+    sum = 0;
 #pragma unroll
-    for (int w = 0; w < NW; ++w) cnt[w][t] += dstart;
-    base[t] = goff - dstart;
+    for (int k = 0; k < PT; ++k) sum += mine[k];
+    uint32_t start = block_exclusive_scan<uint32_t, kETileNT>(sum, scan_sm, all);
+    uint32_t first[PT];
+#pragma unroll
+    for (int k = 0; k < PT; ++k) {
+        first[k] = start;
+        base[t * PT + k] = start;
+        start += mine[k];
+    }
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < kETileItems; ++i)
-        if (q0 + i * 32 < m) {
-            const uint32_t d = (key[i] >> shift) & 255u;
-            skv[cnt[warp][d] + rank[i]] = make_uint2(key[i], val[i]);
-        }
+        if (q0 + i * 32 < m) skv[base[digit[i]] + cnt[warp][digit[i]] + rank[i]] = make_uint2(key[i], val[i]);
     __syncthreads();
+#pragma unroll
+    for (int k = 0; k < PT; ++k) base[t * PT + k] = before[k] - first[k];  // output place less tile place
+    __syncthreads();
+    uint32_t dst[kETileItems];
+    uint2 e[kETileItems];
 #pragma unroll
     for (int u = 0; u < kETileItems; ++u) {
         const int j = t + u * kETileNT;
-        const bool valid = j < m;
-        uint32_t bin = 0xffffffffu;
-        if (valid) {
-            const uint2 e = skv[j];
-            const uint32_t dst = base[(e.x >> shift) & 255u] + (uint32_t)j;
-            kout[dst] = e.x;
-            vout[dst] = e.y;
-            // n < 2^31 entries: at most 2^20 tiles, so tile and digit fit 28 bits
-            bin = (dst / kETile) * 256u + ((e.x >> (shift + 8)) & 255u);
-        }
-        if (next) {  // uniform over the block
+        e[u] = j < m ? skv[j] : make_uint2(0, 0);
+        dst[u] = base[(e[u].x >> shift) & mask] + (uint32_t)j;
+    }
+    if (next) {
+#pragma unroll
+        for (int u = 0; u < kETileItems; ++u) {
+            const bool valid = t + u * kETileNT < m;
+            // n < 2^31 entries: at most 2^20 tiles of at most 2^12 digits
+            const uint32_t bin = valid ? (dst[u] / kETile) * D + ((e[u].x >> (shift + bits)) & mask) : 0xffffffffu;
+            if (valid) {
+                kout[dst[u]] = e[u].x;
+                vout[dst[u]] = e[u].y;
+            }
             const unsigned peers = __match_any_sync(0xffffffffu, bin);
             if (valid && lane == __ffs(peers) - 1) atomicAdd(next + bin, (uint32_t)__popc(peers));
         }
+    } else {
+        uint32_t row[kETileItems];
+        A s[kETileItems];
+#pragma unroll
+        for (int u = 0; u < kETileItems; ++u)
+            if (t + u * kETileNT < m) out.load(e[u].y, row[u], s[u]);
+#pragma unroll
+        for (int u = 0; u < kETileItems; ++u)
+            if (t + u * kETileNT < m) out.store(dst[u], e[u].x, row[u], s[u]);
+        if (tile == 0 && t < kSortPad) out.store(n + t, out.pad_key, 0u, A(0));
     }
 }
 
 // All passes of up to NT * ITEMS ids in one block.
-template <class I, int NT, int ITEMS>
+template <class A, class I, int NT, int ITEMS>
 __global__ void __launch_bounds__(NT)
-    id_sort_small_kernel(Entries<I> in, int key_bits, uint32_t* __restrict__ kout,
-                         uint32_t* __restrict__ vout, int32_t* __restrict__ row_of,
-                         unsigned* __restrict__ done) {
-    const int n = (int)in.n;
+    id_sort_small_kernel(Entries<I> in, int key_bits, int32_t* row_of,
+                         unsigned* __restrict__ done, SortedOut<A> out) {
     constexpr int NW = NT / 32;
-    extern __shared__ uint32_t dyn[];
-    uint32_t(*cnt)[256] = reinterpret_cast<uint32_t(*)[256]>(dyn);  // NW x 256
-    uint2* skv = reinterpret_cast<uint2*>(dyn + NW * 256);          // NT * ITEMS
+    __shared__ uint32_t cnt[NW][256];
+    __shared__ uint2 skv[NT * ITEMS];
     __shared__ uint32_t scan_sm[NW];
-    const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+    const int t = threadIdx.x, lane = t & 31, warp = t >> 5, n = (int)in.n;
     const int q0 = warp * (32 * ITEMS) + lane;
-    uint32_t key[ITEMS], val[ITEMS], rank[ITEMS];
+    uint32_t key[ITEMS], val[ITEMS], digit[ITEMS], rank[ITEMS];
     int32_t r[ITEMS];
     in.rows(q0 - lane, r);
 #pragma unroll
@@ -274,25 +394,13 @@ __global__ void __launch_bounds__(NT)
         }
     }
     if (t == 0) *done = 0;
-    const unsigned lt = (1u << lane) - 1u;
     for (int shift = 0; shift < key_bits; shift += 8) {
         for (int i = t; i < NW * 256; i += NT) (&cnt[0][0])[i] = 0;
         __syncthreads();
 #pragma unroll
-        for (int i = 0; i < ITEMS; ++i) {
-            const bool valid = q0 + i * 32 < n;
-            const uint32_t d = valid ? (key[i] >> shift) & 255u : 256u + (uint32_t)lane;
-            const unsigned peers = __match_any_sync(0xffffffffu, d);
-            const int leader = __ffs(peers) - 1;
-            uint32_t b = 0;
-            if (valid && lane == leader) {
-                b = cnt[warp][d];
-                cnt[warp][d] = b + (uint32_t)__popc(peers);
-            }
-            b = __shfl_sync(0xffffffffu, b, leader);
-            rank[i] = b + (uint32_t)__popc(peers & lt);
-            __syncwarp();
-        }
+        for (int i = 0; i < ITEMS; ++i)
+            digit[i] = q0 + i * 32 < n ? (key[i] >> shift) & 255u : 0x80000000u + (uint32_t)lane;
+        warp_ranks<ITEMS>(digit, cnt[warp], rank);
         __syncthreads();
         uint32_t tot = 0;
         if (t < 256)
@@ -310,30 +418,27 @@ __global__ void __launch_bounds__(NT)
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < ITEMS; ++i)
-            if (q0 + i * 32 < n) {
-                const uint32_t d = (key[i] >> shift) & 255u;
-                skv[cnt[warp][d] + rank[i]] = make_uint2(key[i], val[i]);
-            }
+            if (q0 + i * 32 < n) skv[cnt[warp][digit[i]] + rank[i]] = make_uint2(key[i], val[i]);
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < ITEMS; ++i) {
             const int q = q0 + i * 32;
             if (q < n) {
-                const uint2 e = skv[q];
-                key[i] = e.x;
-                val[i] = e.y;
+                key[i] = skv[q].x;
+                val[i] = skv[q].y;
             }
         }
         __syncthreads();
     }
+    uint32_t row[ITEMS];
+    A s[ITEMS];
 #pragma unroll
-    for (int i = 0; i < ITEMS; ++i) {
-        const int q = q0 + i * 32;
-        if (q < n) {
-            kout[q] = key[i];
-            vout[q] = val[i];
-        }
-    }
+    for (int i = 0; i < ITEMS; ++i)  // row_of was written by this block, before a barrier
+        if (q0 + i * 32 < n) out.load(val[i], row[i], s[i]);
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i)
+        if (q0 + i * 32 < n) out.store(q0 + i * 32, key[i], row[i], s[i]);
+    if (t < kSortPad) out.store(n + t, out.pad_key, 0u, A(0));
 }
 
 inline int id_key_bits(int64_t n_rows) {  // keys 0 .. n_rows
@@ -342,40 +447,44 @@ inline int id_key_bits(int64_t n_rows) {  // keys 0 .. n_rows
     return b;
 }
 
-// Workspace of a sort of n ids, in 32-bit words: two key / value pairs and the
-// passes' counts.
+// How n ids are sorted, and the workspace in 32-bit words: two key / value pairs,
+// the passes' counts and the digits' totals.
 struct IdSortPlan {
-    int64_t n = 0, n_tiles = 0;
-    int key_bits = 1, passes = 1;
+    int64_t n = 0, n_tiles = 0, pitch = 0;  // pitch: of the four arrays, with the padding
+    int key_bits = 1, passes = 1, bits = 8;
+    bool wide = false;
     int64_t words = 0;
     IdSortPlan(int64_t n_, int64_t n_rows) : n(n_) {
         key_bits = id_key_bits(n_rows);
-        passes = (key_bits + 7) / 8;
+        const int narrow = (key_bits + 7) / 8, few = (key_bits + kWideBits - 1) / kWideBits;
+        wide = few < narrow;
+        passes = wide ? few : narrow;
+        bits = wide ? (key_bits + passes - 1) / passes : 8;
         n_tiles = ceil_div(n, kETile);
-        words = 4 * n + (n > kSmallSort ? ((int64_t)passes * n_tiles + 1) * 256 : 0);
+        pitch = ceil_div(n + kSortPad, (int64_t)64) * 64;
+        const int64_t digits = wide ? 1 << kWideBits : 256;
+        words = 4 * pitch + (n > kSmallSort ? ((int64_t)passes * n_tiles + 1) * digits : 0);
     }
 };
 
-struct IdSorted {
-    const uint32_t* keys;
-    const uint32_t* pos;
-};
-
-// Sorts the batch's keys; writes row_of (with indptr) and clears *done.
-template <class I>
-IdSorted sort_ids(const IdSortPlan& P, const Entries<I>& in, int32_t* row_of, unsigned* done,
-                  uint32_t* ws, cudaStream_t s) {
+// Sorts the batch's keys into out.keys with the entries' rows and scales (out's
+// keys and rows are set here, in the workspace); writes row_of (with indptr) and
+// clears *done.
+template <class A, class I>
+void sort_ids(const IdSortPlan& P, const Entries<I>& in, int32_t* row_of, unsigned* done,
+              uint32_t* ws, SortedOut<A>& out, cudaStream_t s) {
     const int64_t n = P.n;
-    uint32_t *k0 = ws, *v0 = ws + n, *k1 = ws + 2 * n, *v1 = ws + 3 * n, *counts = ws + 4 * n;
+    uint32_t* counts = ws + 4 * P.pitch;
+    out.keys = ws;
+    out.rows = ws + P.pitch;
+    out.row_of = in.indptr ? row_of : nullptr;
+    out.pad_key = (uint32_t)in.n_rows;
+    using std::integral_constant;
     if (n <= kSmallSort) {
         auto small = [&](auto nt, auto items) {
             constexpr int NT = decltype(nt)::value, IT = decltype(items)::value;
-            constexpr int SM = (NT / 32) * 1024 + NT * IT * 8;
-            auto k = id_sort_small_kernel<I, NT, IT>;
-            static_assert(SM <= 48 * 1024, "id sort shared memory");
-            k<<<1, NT, SM, s>>>(in, P.key_bits, k0, v0, row_of, done);
+            id_sort_small_kernel<A, I, NT, IT><<<1, NT, 0, s>>>(in, P.key_bits, row_of, done, out);
         };
-        using std::integral_constant;
         if (n <= 256)
             small(integral_constant<int, 256>{}, integral_constant<int, 1>{});
         else if (n <= 512)
@@ -383,34 +492,45 @@ IdSorted sort_ids(const IdSortPlan& P, const Entries<I>& in, int32_t* row_of, un
         else
             small(integral_constant<int, 512>{}, integral_constant<int, 4>{});
         MFM_CHECK_LAUNCH("id sort launch");
-        return {k0, v0};
+        return;
     }
+    // keys and values go back and forth between the two pairs and end in `out`
+    uint32_t *k0 = out.keys, *v0 = out.rows, *k1 = ws + 2 * P.pitch, *v1 = ws + 3 * P.pitch;
     const unsigned g = (unsigned)P.n_tiles;
-    const bool fused = P.n_tiles <= kFuseTiles;
-    uint32_t* totals = counts + (int64_t)P.passes * P.n_tiles * 256;
-    id_count_kernel<I><<<g, kETileNT, 0, s>>>(in, P.passes, P.n_tiles, k1, row_of, counts, done);
-    uint32_t *ki = k1, *vi = v1, *ko = k0, *vo = v0;
-    for (int p = 0; p < P.passes; ++p) {
-        uint32_t* c = counts + (int64_t)p * P.n_tiles * 256;
-        uint32_t* next = p + 1 < P.passes ? c + P.n_tiles * 256 : nullptr;
-        if (!fused) id_prefix_kernel<<<256, 256, 0, s>>>(c, P.n_tiles, totals);
-        auto pass = [&](auto first, auto whole) {
-            id_scatter_kernel<decltype(first)::value, decltype(whole)::value>
-                <<<g, kETileNT, 0, s>>>(ki, vi, ko, vo, n, P.n_tiles, 8 * p, c, totals, next);
-        };
-        if (p == 0 && fused)
-            pass(std::true_type{}, std::true_type{});
-        else if (p == 0)
-            pass(std::true_type{}, std::false_type{});
-        else if (fused)
-            pass(std::false_type{}, std::true_type{});
-        else
-            pass(std::false_type{}, std::false_type{});
-        std::swap(ki, ko);
-        std::swap(vi, vo);
-    }
+    auto run = [&](auto width) {
+        constexpr int BITS = decltype(width)::value, D = 1 << BITS, SM = scatter_smem<BITS>();
+        uint32_t* totals = counts + (int64_t)P.passes * P.n_tiles * D;
+        const bool fused = BITS == 8 && P.n_tiles <= kFuseTiles;
+        uint32_t *ki = P.passes % 2 ? k1 : k0, *vi = P.passes % 2 ? v1 : v0;
+        uint32_t *ko = P.passes % 2 ? k0 : k1, *vo = P.passes % 2 ? v0 : v1;
+        id_count_kernel<I, BITS><<<g, kETileNT, 0, s>>>(in, P.passes, (1u << P.bits) - 1u, P.n_tiles, ki, row_of, counts, done);
+        for (int p = 0; p < P.passes; ++p) {
+            uint32_t* c = counts + (int64_t)p * P.n_tiles * D;
+            uint32_t* next = p + 1 < P.passes ? c + P.n_tiles * D : nullptr;
+            if (!fused) id_prefix_kernel<<<D / 32, 256, 0, s>>>(c, P.n_tiles, D, totals);
+            auto pass = [&](auto first, auto whole) {
+                auto k = id_scatter_kernel<A, BITS, decltype(first)::value, decltype(whole)::value && BITS == 8>;
+                if (SM > 48 * 1024)
+                    MFM_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, SM), "id sort shared memory");
+                k<<<g, kETileNT, SM, s>>>(ki, vi, ko, vo, n, P.n_tiles, P.bits * p, P.bits, c, totals, next, out);
+            };
+            if (p == 0 && fused)
+                pass(std::true_type{}, std::true_type{});
+            else if (p == 0)
+                pass(std::true_type{}, std::false_type{});
+            else if (fused)
+                pass(std::false_type{}, std::true_type{});
+            else
+                pass(std::false_type{}, std::false_type{});
+            std::swap(ki, ko);
+            std::swap(vi, vo);
+        }
+    };
+    if (P.wide)
+        run(integral_constant<int, kWideBits>{});
+    else
+        run(integral_constant<int, 8>{});
     MFM_CHECK_LAUNCH("id sort launch");
-    return {ki, vi};
 }
 
 }  // namespace mfm
