@@ -133,6 +133,13 @@ struct Labels {
 template <class A>
 __device__ __forceinline__ A offset_of(A m) { return m == minus_inf<A>() ? A(0) : m; }
 
+// x - off - log s with nothing rounded to 32 bits: a sequence adds up hundreds of
+// them, and a margin is the difference of two such sums.
+template <class T, class A>
+__device__ __noinline__ double exact_logprob(T x, A off, A s) {
+    return (widen<double>(x) - (double)off) - log((double)s);
+}
+
 template <class A>
 struct RowStats {
     A m, s;  // maximum, sum of exp(x - offset_of(m))
@@ -165,7 +172,8 @@ template <class A>
 struct RowArgs {
     Labels labels;
     int64_t n, c;
-    A* lp;
+    A* lp;         // log-probabilities, or
+    double* lp64;  // the same unrounded, for sums over sequences
     // STATS
     A* lse;
     A* zero;            // cleared per token, or NULL
@@ -206,14 +214,22 @@ __device__ __forceinline__ void kl_terms(float u, float& em1, float& kl) {
         kl = em1 - u;
     }
 }
-constexpr double inverse_factorial(int i) { return i < 2 ? 1.0 : inverse_factorial(i - 1) / i; }
 __device__ __forceinline__ void kl_terms(double u, double& em1, double& kl) {
     em1 = expm1(u);
     kl = em1 - u;
     if (fabs(u) < 0.125) {
-        double r = 0.0;
-#pragma unroll
-        for (int i = 13; i >= 2; --i) r = r * u + inverse_factorial(i);
+        double r = 1.0 / 6227020800.0;
+        r = r * u + 1.0 / 479001600.0;
+        r = r * u + 1.0 / 39916800.0;
+        r = r * u + 1.0 / 3628800.0;
+        r = r * u + 1.0 / 362880.0;
+        r = r * u + 1.0 / 40320.0;
+        r = r * u + 1.0 / 5040.0;
+        r = r * u + 1.0 / 720.0;
+        r = r * u + 1.0 / 120.0;
+        r = r * u + 1.0 / 24.0;
+        r = r * u + 1.0 / 6.0;
+        r = r * u + 0.5;
         kl = r * u * u;
     }
 }
@@ -442,8 +458,9 @@ __global__ void __launch_bounds__(kSmallNT, IsF64<A>::value || CW > 16 ? 4 : kSm
                 const A ls = log_of(s);
                 const bool live = y_now >= 0 && !empty;
                 const A lp = live ? (at - off) - ls : A(0);
-                a.lp[t] = lp;
+                if (a.lp) a.lp[t] = lp;
                 if (M == STATS) {
+                    if (a.lp64) a.lp64[t] = live ? exact_logprob(at, off, s) : 0.0;
                     if (a.lse) a.lse[t] = empty ? minus_inf<A>() : off + ls;
                     if (a.zero) a.zero[t] = A(0);
                 } else {
@@ -495,18 +512,13 @@ __device__ __forceinline__ bool alike(const void* a, const void* b) {
     return ((uintptr_t)a - (uintptr_t)b) % 16 == 0;
 }
 
-// The gradient's vector at column `at` from k exp(x - off): 0 for a token without one
-// (whatever its scores are), g more at the label.
-template <class A, int N>
-__device__ __forceinline__ void grad_vec(A (&p)[N], int at, int y, A g) {
-    if (g == A(0)) {
-#pragma unroll
-        for (int q = 0; q < N; ++q) p[q] = A(0);
-    } else if ((unsigned)(y - at) < (unsigned)N) {
-#pragma unroll
-        for (int q = 0; q < N; ++q)
-            if (at + q == y) p[q] += g;
-    }
+// The lane that writes the vector with column y of a row (-1: an edge element or
+// none). It writes the label's element once more, by itself, behind its vectors:
+// the loops over vectors then carry no test for it.
+template <class T, int L>
+__device__ __forceinline__ int label_lane(const RowShape<T>& sh, int y) {
+    const unsigned j = (unsigned)(y - sh.head) / (unsigned)RowShape<T>::V;
+    return y >= sh.head && j < (unsigned)sh.nv ? (int)(j % (unsigned)L) : -1;
 }
 
 // N values to `at`: as one vector, or one by one where the rows of scores and
@@ -534,8 +546,9 @@ struct RowResult {
         const bool live = y >= 0 && !empty;
         const A ls = log_of(s);
         const A lp = live ? (widen<A>(xy) - off) - ls : A(0);
-        if (first) a.lp[t] = lp;
+        if (first && a.lp) a.lp[t] = lp;
         if (M == STATS) {
+            if (first && a.lp64) a.lp64[t] = live ? exact_logprob(xy, off, s) : 0.0;
             if (first && a.lse) a.lse[t] = empty ? minus_inf<A>() : off + ls;
             if (first && a.zero) a.zero[t] = A(0);
         } else {
@@ -602,14 +615,18 @@ __global__ void __launch_bounds__(kNT, IsF64<A>::value ? 2 : 4)
             for (int i = 0; i < K; ++i) {
                 const int j = lane + i * L;
                 if (j < sh.nv) {
-                    const int at = sh.head + j * V;
                     A p[V];
-                    Pack<T>::unpack(v[i], p);
-                    ex.scaled(p, r.k);
-                    grad_vec(p, at, y, r.g);
-                    store16<T, A>(to + at, p, whole);
+                    if (none) {  // uniform over the row
+#pragma unroll
+                        for (int q = 0; q < V; ++q) p[q] = A(0);
+                    } else {
+                        Pack<T>::unpack(v[i], p);
+                        ex.scaled(p, r.k);
+                    }
+                    store16<T, A>(to + sh.head + j * V, p, whole);
                 }
             }
+            if (!none && lane == label_lane<T, L>(sh, y)) to[y] = narrow<T>(r.g + r.k * exp_of(widen<A>(xy) - off));
         }
     }
     if (M == STATS) {
@@ -857,17 +874,22 @@ __global__ void __launch_bounds__(L + 32, ring_blocks(L))
                         if (u * L < left) v[u] = at[u * L];
                     __syncwarp();
                     if ((lane & 31) == 0) bar_arrive(&empty[slot]);
+                    T* at_out = to + sh.head + (c * CV + lane) * V;
 #pragma unroll
                     for (int u = 0; u < kRingVecs; ++u)
                         if (u * L < left) {
-                            const int j = sh.head + (c * CV + u * L + lane) * V;
                             A p[V];
-                            Pack<T>::unpack(v[u], p);
-                            ex.scaled(p, res.k);
-                            grad_vec(p, j, y, res.g);
-                            store16<T, A>(to + j, p, whole);
+                            if (none) {  // uniform over the row
+#pragma unroll
+                                for (int q = 0; q < V; ++q) p[q] = A(0);
+                            } else {
+                                Pack<T>::unpack(v[u], p);
+                                ex.scaled(p, res.k);
+                            }
+                            store16<T, A>(at_out + u * L * V, p, whole);
                         }
                 }
+                if (!none && lane == label_lane<T, L>(sh, y)) to[y] = narrow<T>(res.g + res.k * exp_of(widen<A>(xy) - off));
             }
             if (*stop && lane == 0) {
                 a.lp[t] = (A)NAN;
@@ -900,11 +922,13 @@ __global__ void __launch_bounds__(kNT)
     const bool whole = alike(row, to);
     const int y = a.labels.in(t, a.c);
     const A l = a.lse_in[t], f = a.factor(t, y, l);
-    auto one = [&](A v) { return f == A(0) ? A(0) : -f * exp_of(v - l); };
+    const T xy = row[y >= 0 ? y : 0];
+    const bool none = f == A(0);
     if (lane < sh.edges) {
         const int j = sh.edge(lane);
-        to[j] = narrow<T>(one(widen<A>(row[j])) + (j == y ? f : A(0)));
+        to[j] = narrow<T>(none ? A(0) : -f * exp_of(widen<A>(row[j]) - l) + (j == y ? f : A(0)));
     }
+    const ExpSum<A> ex(l);
     for (int j0 = lane; j0 < sh.nv; j0 += L * U) {
         uint4 v[U];
 #pragma unroll
@@ -913,19 +937,18 @@ __global__ void __launch_bounds__(kNT)
 #pragma unroll
         for (int u = 0; u < U; ++u)
             if (j0 + u * L < sh.nv) {
-                const int at = sh.head + (j0 + u * L) * V;
                 A p[V];
-                Pack<T>::unpack(v[u], p);
+                if (none) {  // uniform over the row
 #pragma unroll
-                for (int q = 0; q < V; ++q) p[q] = one(p[q]);
-                if (y >= at && y < at + V) {
-#pragma unroll
-                    for (int q = 0; q < V; ++q)
-                        if (at + q == y) p[q] += f;
+                    for (int q = 0; q < V; ++q) p[q] = A(0);
+                } else {
+                    Pack<T>::unpack(v[u], p);
+                    ex.scaled(p, -f);
                 }
-                store16<T, A>(to + at, p, whole);
+                store16<T, A>(to + sh.head + (j0 + u * L) * V, p, whole);
             }
     }
+    if (!none && lane == label_lane<T, L>(sh, y)) to[y] = narrow<T>(f - f * exp_of(widen<A>(xy) - l));
 }
 
 // Sums of v over [indptr[s], indptr[s+1]), one warp each, in float64.
@@ -961,7 +984,7 @@ __global__ void __launch_bounds__(kNT)
 // that finishes last adds the losses and the weights, in a fixed order.
 template <class A, int W>
 __global__ void __launch_bounds__(kNT)
-    pair_kernel(const A* __restrict__ lp, int64_t n, const int64_t* __restrict__ indptr,
+    pair_kernel(const double* __restrict__ lp, int64_t n, const int64_t* __restrict__ indptr,
                 int64_t n_pairs, const A* __restrict__ reference, double beta, double eps,
                 const A* __restrict__ weight, A* __restrict__ margins, A* __restrict__ sums,
                 double* __restrict__ pair_loss, A* __restrict__ g, unsigned* __restrict__ done,
@@ -976,7 +999,7 @@ __global__ void __launch_bounds__(kNT)
         for (int i = 0; i < 2; ++i) {
             seq_bounds(indptr, p + i * n_pairs, n, lo[i], hi[i]);
             s[i] = 0.0;
-            for (int64_t t = lo[i] + lane; t < hi[i]; t += W) s[i] += (double)lp[t];
+            for (int64_t t = lo[i] + lane; t < hi[i]; t += W) s[i] += lp[t];
             s[i] = W == 32 ? warp_sum(s[i]) : block_sum(s[i], sm);
         }
         const double z = beta * ((s[0] - (double)reference[p]) - (s[1] - (double)reference[n_pairs + p]));
@@ -1158,14 +1181,15 @@ void rows_launch(int device, const T* x, int64_t ld, T* out, int64_t ld_out, con
 }
 
 template <class T, class A>
-void stats_launch(int device, const T* x, int64_t ld, int64_t n, int64_t c, Labels labels, A* lp, A* lse,
-                  A* zero, unsigned* counter, cudaStream_t s) {
+void stats_launch(int device, const T* x, int64_t ld, int64_t n, int64_t c, Labels labels, A* lp,
+                  double* lp64, A* lse, A* zero, unsigned* counter, cudaStream_t s) {
     if (n == 0) return;
     RowArgs<A> a{};
     a.labels = labels;
     a.n = n;
     a.c = c;
     a.lp = lp;
+    a.lp64 = lp64;
     a.lse = lse;
     a.zero = zero;
     a.counter = counter;
@@ -1229,7 +1253,7 @@ extern "C" int mfm_label_logprobs_device(int dtype, int device, const void* logi
             using T = Elem<decltype(t)>;
             using A = typename Arith<T>::type;
             stats_launch<T, A>(device, (const T*)logits, ld, n_tokens, n_classes, Labels{labels, labels64},
-                               (A*)logprobs, (A*)lse, nullptr, nullptr, s);
+                               (A*)logprobs, nullptr, (A*)lse, nullptr, nullptr, s);
             if (sums && n_seq > 0) {
                 seq_sums_kernel<A><<<(unsigned)ceil_div(n_seq, kNT / 32), kNT, 0, s>>>(
                     (const A*)logprobs, n_tokens, indptr, n_seq, (A*)sums);
@@ -1265,9 +1289,9 @@ struct PrefWs {  // log-probabilities, lse, token coefficients, pair losses, 1 /
     size_t lse, g, pair, scale, bytes;
     PrefWs(int dtype, int64_t n, int64_t pairs) {
         const size_t a = up256((size_t)n * arith_size(dtype));
-        lse = a;
-        g = 2 * a;
-        pair = 3 * a;
+        lse = up256((size_t)n * 8);
+        g = lse + a;
+        pair = g + a;
         scale = pair + up256((size_t)pairs * 8);
         bytes = scale + 256;
     }
@@ -1308,12 +1332,13 @@ extern "C" int mfm_preference_loss_device(int dtype, int device, const void* log
         with_score_types(dtype, [&](auto* t) {
             using T = Elem<decltype(t)>;
             using A = typename Arith<T>::type;
-            A *lp = (A*)ws, *lse = (A*)(ws + W.lse), *coef = d_logits ? (A*)(ws + W.g) : nullptr;
+            double* lp = (double*)ws;
+            A *lse = (A*)(ws + W.lse), *coef = d_logits ? (A*)(ws + W.g) : nullptr;
             const Labels y{labels, labels64};
             if (n_pairs == 0) zero_loss_kernel<A><<<1, 32, 0, s>>>((A*)loss, 1);
             if (n_pairs == 0 || n_tokens == 0)
                 MFM_CUDA(cudaMemsetAsync(ws + W.scale, 0, 16, s), "memset");
-            stats_launch<T, A>(device, (const T*)logits, ld, n_tokens, n_classes, y, lp, lse, coef, done, s);
+            stats_launch<T, A>(device, (const T*)logits, ld, n_tokens, n_classes, y, nullptr, lp, lse, coef, done, s);
             if (n_pairs > 0) {
                 auto pairs = [&](auto w) {
                     constexpr int PW = decltype(w)::value;
