@@ -9,13 +9,15 @@
 // and written once (policy, forward, gradient), with one or two exponentials per
 // value (16 a clock and SM) close behind for 16-bit scores. Rows are worked on
 // in three ways:
-//  * up to kSmallC classes: a thread per row, rows staged through shared memory
-//    so that global accesses are whole vectors (small_rows_kernel);
-//  * rows of up to 4 KB: a warp holds the whole row in registers (at most eight
+//  * up to kSmallC classes: a thread per row, tiles of 32 rows copied through
+//    shared memory so that global accesses are whole vectors (small_rows_kernel);
+//  * rows of up to 8 KB: 8 to 32 lanes hold the row in registers (at most sixteen
 //    16-byte vectors a lane), so it is read once for the maximum, the sum and the
 //    gradient (cached_rows_kernel);
-//  * longer rows: persistent blocks stream rows through a ring in shared memory
-//    that bulk copies fill ahead of the work (ring_rows_kernel).
+//  * longer rows of the policy loss: persistent blocks stream rows through a ring
+//    in shared memory that bulk copies fill ahead of the work (ring_rows_kernel);
+//    the forward alone scans them (scan_rows_kernel), and the gradient for given
+//    statistics is elementwise (label_grad_kernel).
 #include "vecio.cuh"
 
 #include <algorithm>
@@ -156,13 +158,6 @@ __device__ __forceinline__ void across(RowStats<A>& r, int width) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1)
         if (o < width) r.s += __shfl_xor_sync(0xffffffffu, r.s, o);
-}
-
-template <class A, class Op>
-__device__ __forceinline__ A warp_reduce(A v, Op op) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v = op(v, __shfl_xor_sync(0xffffffffu, v, o));
-    return v;
 }
 
 // What a row's loss needs, in global memory; which pointers are set goes by the mode.
@@ -558,59 +553,90 @@ struct RowResult {
     }
 };
 
-// A warp per row, the row in its registers: K vectors a lane.
-template <class T, class A, int K, Mode M>
-__global__ void __launch_bounds__(kNT, IsF64<A>::value ? 2 : 4)
+// Blocks per SM by the registers that K vectors take.
+template <class A>
+constexpr int cached_blocks(int k) { return IsF64<A>::value || k > 8 ? 2 : 4; }
+
+// L lanes per row, the row in their registers: K vectors a lane. Persistent warps
+// walk the rows, so what a block adds up, it adds up once.
+template <class T, class A, int L, int K, Mode M>
+__global__ void __launch_bounds__(kNT, cached_blocks<A>(K))
     cached_rows_kernel(const T* __restrict__ x, int64_t ld, T* __restrict__ out, int64_t ld_out,
                        RowArgs<A> a) {
-    constexpr int V = 16 / sizeof(T), L = 32, R = kNT / L;
-    __shared__ double sums[32];
+    constexpr int V = 16 / sizeof(T), R = 32 / L;            // rows per warp
+    constexpr int E = (2 * (V - 1) + L - 1) / L;             // edge elements per lane
+    __shared__ double sums[kNT / 32];
     const int lane = threadIdx.x % L;
-    const int64_t t = (int64_t)blockIdx.x * R + threadIdx.x / L;
-    const bool in = t < a.n;
-    const T* row = x + (in ? t : 0) * ld;
-    const RowShape<T> sh(row, in ? (int)a.c : 0);
-    uint4 v[K];
-    T edge = narrow<T>(minus_inf<A>());
-#pragma unroll
-    for (int i = 0; i < K; ++i) {
-        const int j = lane + i * L;
-        v[i] = j < sh.nv ? load16(row + sh.head + j * V) : Pack<T>::minus_inf();
-    }
-    if (lane < sh.edges) edge = row[sh.edge(lane)];
-    const int y = in ? a.labels.in(t, a.c) : -1;
-    const T xy = row[y >= 0 ? y : 0];  // the label's score, on its way with the row
-    Token<A> tok;
-    if (M == POLICY && in) tok.load(a, t);
     const double total = M == POLICY ? weight_total(a) : 0.0, inv = inverse(total);
-    A m = widen<A>(edge);
-#pragma unroll
-    for (int i = 0; i < K; ++i)
-        if (i * L < sh.nv) m = fmax(m, Pack<T>::top(v[i]));
-    m = warp_reduce(m, [](A p, A q) { return fmax(p, q); });
-    const A off = offset_of(m);
-    ExpSum<A> ex(off);
-#pragma unroll
-    for (int i = 0; i < K; ++i)
-        if (i * L < sh.nv) {
-            A p[V];
-            Pack<T>::unpack(v[i], p);
-            ex.add(p);
-        }
-    const A s = warp_sum(exp_of(widen<A>(edge) - off) + ex.sum());
+    const double scale = M == GRAD && a.scale ? *a.scale : 1.0;
     double e[3] = {0.0, 0.0, 0.0};
-    if (in) {
-        const RowResult<T, A, M> r(a, tok, t, y, xy, m, s, inv, lane == 0);
-        if (M == POLICY && lane == 0)
-            for (int i = 0; i < 3; ++i) e[i] = (double)r.e[i];
-        if (M == POLICY && out) {
-            T* to = out + t * ld_out;
-            const bool whole = alike(row, to), none = r.g == A(0);
-            if (lane < sh.edges) {
-                const int j = sh.edge(lane);
-                to[j] = none ? narrow<T>(A(0))
-                             : narrow<T>((j == y ? r.g : A(0)) + r.k * exp_of(widen<A>(edge) - off));
+    const int64_t warps = (int64_t)gridDim.x * (kNT / 32);
+    for (int64_t t0 = ((int64_t)blockIdx.x * (kNT / 32) + threadIdx.x / 32) * R; t0 < a.n; t0 += warps * R) {
+        // the gradient goes from the last row to the first: the forward that read
+        // the scores just before left the last ones in L2
+        const int64_t at = t0 + threadIdx.x % 32 / L, t = M == GRAD ? a.n - 1 - at : at;
+        const bool in = at < a.n;
+        const T* row = x + (in ? t : 0) * ld;
+        const RowShape<T> sh(row, in ? (int)a.c : 0);
+        uint4 v[K];
+        A edge[E];
+#pragma unroll
+        for (int i = 0; i < K; ++i) {
+            const int j = lane + i * L;
+            v[i] = j < sh.nv ? load16(row + sh.head + j * V) : Pack<T>::minus_inf();
+        }
+#pragma unroll
+        for (int i = 0; i < E; ++i)
+            edge[i] = lane + i * L < sh.edges ? widen<A>(row[sh.edge(lane + i * L)]) : minus_inf<A>();
+        const int y = in ? a.labels.in(t, a.c) : -1;
+        const T xy = row[y >= 0 ? y : 0];  // the label's score, on its way with the row
+        Token<A> tok;
+        if (M == POLICY && in) tok.load(a, t);
+        A off, g = A(0), k = A(0);
+        if (M == GRAD) {
+            off = in ? a.lse_in[t] : A(0);
+            g = in && y >= 0 && off != minus_inf<A>() ? a.g[t] : A(0);
+            if (a.scale) g = (A)((double)g * scale);
+            k = -g;
+        } else {
+            A m = edge[0];
+#pragma unroll
+            for (int i = 1; i < E; ++i) m = fmax(m, edge[i]);
+#pragma unroll
+            for (int i = 0; i < K; ++i) m = fmax(m, Pack<T>::top(v[i]));
+#pragma unroll
+            for (int o = L / 2; o > 0; o >>= 1) m = fmax(m, __shfl_xor_sync(0xffffffffu, m, o));
+            off = offset_of(m);
+            ExpSum<A> ex(off);
+#pragma unroll
+            for (int i = 0; i < K; ++i) {
+                A p[V];
+                Pack<T>::unpack(v[i], p);
+                ex.add(p);
             }
+            A s = ex.sum();
+#pragma unroll
+            for (int i = 0; i < E; ++i) s += exp_of(edge[i] - off);
+#pragma unroll
+            for (int o = L / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+            if (in) {
+                const RowResult<T, A, M> r(a, tok, t, y, xy, m, s, inv, lane == 0);
+                g = r.g;
+                k = r.k;
+                if (M == POLICY && lane == 0)
+                    for (int i = 0; i < 3; ++i) e[i] += (double)r.e[i];
+            }
+        }
+        if (M != STATS && out && in) {
+            T* to = out + t * ld_out;
+            const bool whole = alike(row, to), none = g == A(0);
+            const ExpSum<A> ex(off);
+#pragma unroll
+            for (int i = 0; i < E; ++i)
+                if (lane + i * L < sh.edges) {
+                    const int j = sh.edge(lane + i * L);
+                    to[j] = narrow<T>(none ? A(0) : (j == y ? g : A(0)) + k * exp_of(edge[i] - off));
+                }
 #pragma unroll
             for (int i = 0; i < K; ++i) {
                 const int j = lane + i * L;
@@ -621,17 +647,17 @@ __global__ void __launch_bounds__(kNT, IsF64<A>::value ? 2 : 4)
                         for (int q = 0; q < V; ++q) p[q] = A(0);
                     } else {
                         Pack<T>::unpack(v[i], p);
-                        ex.scaled(p, r.k);
+                        ex.scaled(p, k);
                     }
                     store16<T, A>(to + sh.head + j * V, p, whole);
                 }
             }
-            if (!none && lane == label_lane<T, L>(sh, y)) to[y] = narrow<T>(r.g + r.k * exp_of(widen<A>(xy) - off));
+            if (!none && lane == label_lane<T, L>(sh, y)) to[y] = narrow<T>(g + k * exp_of(widen<A>(xy) - off));
         }
     }
     if (M == STATS) {
         if (a.counter && blockIdx.x == 0 && threadIdx.x == 0) *a.counter = 0;
-    } else {
+    } else if (M == POLICY) {
         for (int i = 0; i < 3; ++i) e[i] = block_sum(e[i], sums);
         policy_finish(a, e, total, sums);
     }
@@ -739,12 +765,22 @@ __device__ __forceinline__ void bulk_copy(void* to, const void* from, unsigned b
 // Rows streamed through a ring of shared-memory chunks by bulk copies: one warp
 // keeps copies of the rows ahead in flight while L threads work, so the loads do
 // not stop for a row's reductions or its gradient. A row that fits the ring is
-// kept there until its gradient is written; a longer one is read twice, the
-// second time mostly from L2. A chunk is kRingVecs vectors a thread.
+// kept there until its gradient is written; of a longer one the last chunks are,
+// and the others come a second time, from L2. A chunk is kRingVecs vectors a
+// thread. Two blocks of 256 threads an SM work on two rows: one's barrier and
+// statistics hide behind the other's values (4096 x 65536 bf16: 218 us with one
+// block of 512 that keeps whole rows, 217 us with two of 256 that keep half, 270 us
+// with four of 128 that keep a quarter; 239 us with one of 768). Shorter rows take
+// more and smaller blocks, since a row's statistics cost each of its warps about
+// 250 instructions (16384 x 16384 bf16: 271, 236, 226 us with 256, 128, 64 threads
+// a row; 8192 x 32000: 230 us with 256, 220 us with 128).
 constexpr int kRingVecs = 4;
-constexpr int kRingMost = 512;  // lanes of the longest rows, one block per SM
-constexpr int ring_blocks(int L) { return kRingMost / L; }
+constexpr int kRingLanes = 512;  // of an SM
+constexpr int ring_blocks(int L) { return kRingLanes / L; }
 constexpr int ring_slots(int L) { return 200704 / ring_blocks(L) / (L * kRingVecs * 16); }
+// How many of a row's chunks stay for its gradient: all, or as many as leave two
+// slots for the others to pass through.
+__host__ __device__ constexpr int kept_chunks(int chunks, int slots) { return chunks <= slots ? chunks : slots - 2; }
 
 template <class T, class A, int L>
 __global__ void __launch_bounds__(L + 32, ring_blocks(L))
@@ -775,16 +811,17 @@ __global__ void __launch_bounds__(L + 32, ring_blocks(L))
                 const T* row = x + t * ld;
                 const RowShape<T> sh(row, (int)a.c);
                 const int chunks = (sh.nv + CV - 1) / CV;
-                for (int pass = grad && chunks > S ? 2 : 1; pass > 0; --pass)
-                    for (int c = 0; c < chunks; ++c, ++seq) {
-                        const unsigned slot = seq % S;
-                        bar_wait(&empty[slot], (seq / S + 1) & 1, stop);
-                        if (*stop) break;
-                        const int left = sh.nv - c * CV;
-                        const unsigned bytes = (unsigned)(left < CV ? left : CV) * 16;
-                        bar_expect(&full[slot], bytes);
-                        bulk_copy(ring + slot * CV, row + sh.head + (int64_t)c * CV * V, bytes, &full[slot]);
-                    }
+                // the row, then for its gradient the chunks that were not kept
+                const int all = chunks + (grad ? chunks - kept_chunks(chunks, S) : 0);
+                for (int i = 0; i < all; ++i, ++seq) {
+                    const unsigned slot = seq % S;
+                    bar_wait(&empty[slot], (seq / S + 1) & 1, stop);
+                    if (*stop) break;
+                    const int c = i < chunks ? i : i - chunks, left = sh.nv - c * CV;
+                    const unsigned bytes = (unsigned)(left < CV ? left : CV) * 16;
+                    bar_expect(&full[slot], bytes);
+                    bulk_copy(ring + slot * CV, row + sh.head + (int64_t)c * CV * V, bytes, &full[slot]);
+                }
             }
             // copies in flight end before the block does
             for (unsigned q = seq > S ? seq - S : 0; q < seq; ++q)
@@ -802,7 +839,7 @@ __global__ void __launch_bounds__(L + 32, ring_blocks(L))
             const T* row = x + t * ld;
             const RowShape<T> sh(row, (int)a.c);
             const int chunks = (sh.nv + CV - 1) / CV;
-            const bool keep = grad && chunks <= S;
+            const int kept = grad ? kept_chunks(chunks, S) : 0, again = chunks - kept;
             const T edge = lane < sh.edges ? row[sh.edge(lane)] : narrow<T>(minus_inf<A>());
             const T xy = row[y >= 0 ? y : 0];
             Token<A> tok;
@@ -811,7 +848,6 @@ __global__ void __launch_bounds__(L + 32, ring_blocks(L))
             const int y_next = tn < a.n ? a.labels.in(tn, a.c) : -1;
             RowStats<A> r{widen<A>(edge), A(0)};
             r.s = exp_of(r.m - offset_of(r.m));
-            const unsigned first = seq;
             for (int c = 0; c < chunks; ++c, ++seq) {
                 const unsigned slot = seq % S;
                 bar_wait(&full[slot], (seq / S) & 1, stop);
@@ -821,7 +857,7 @@ __global__ void __launch_bounds__(L + 32, ring_blocks(L))
                 A top = r.m;
 #pragma unroll
                 for (int u = 0; u < kRingVecs; ++u) v[u] = u * L < left ? at[u * L] : Pack<T>::minus_inf();
-                if (!keep) {  // the chunk is in registers
+                if (c < again) {  // the chunk is in registers and not kept
                     __syncwarp();
                     if ((lane & 31) == 0) bar_arrive(&empty[slot]);
                 }
@@ -862,10 +898,12 @@ __global__ void __launch_bounds__(L + 32, ring_blocks(L))
                     to[j] = none ? narrow<T>(A(0))
                                  : narrow<T>((j == y ? res.g : A(0)) + res.k * exp_of(widen<A>(edge) - off));
                 }
-                if (keep) seq = first;
-                for (int c = 0; c < chunks; ++c, ++seq) {
-                    const unsigned slot = seq % S;
-                    if (!keep) bar_wait(&full[slot], (seq / S) & 1, stop);
+                // the kept chunks again, the row's last, and behind them the others
+                const unsigned kept_at = seq - (unsigned)kept;
+                for (int i = 0; i < chunks; ++i) {
+                    const int c = i < kept ? again + i : i - kept;
+                    const unsigned at_seq = kept_at + (unsigned)i, slot = at_seq % S;
+                    if (i >= kept) bar_wait(&full[slot], (at_seq / S) & 1, stop);
                     const uint4* at = ring + slot * CV + lane;
                     const int left = sh.nv - c * CV - lane;
                     uint4 v[kRingVecs];
@@ -889,6 +927,7 @@ __global__ void __launch_bounds__(L + 32, ring_blocks(L))
                             store16<T, A>(at_out + u * L * V, p, whole);
                         }
                 }
+                seq += (unsigned)again;
                 if (!none && lane == label_lane<T, L>(sh, y)) to[y] = narrow<T>(res.g + res.k * exp_of(widen<A>(xy) - off));
             }
             if (*stop && lane == 0) {
@@ -1131,16 +1170,39 @@ void small_launch(int device, const T* x, int64_t ld, T* out, int64_t ld_out, co
         width(std::false_type{});
 }
 
+// Rows of up to kCachedVecs vectors: the fewest lanes that hold one.
+constexpr int64_t kCachedVecs = 512;
+
+template <class T, class A, Mode M>
+void cached_launch(int device, const T* x, int64_t ld, T* out, int64_t ld_out, const RowArgs<A>& a,
+                   cudaStream_t s) {
+    const int64_t nv = a.c / Pack<T>::N;
+    auto go = [&](auto l, auto k) {
+        constexpr int L = decltype(l)::value, K = decltype(k)::value;
+        const int64_t blocks = ceil_div(a.n, (int64_t)kNT / L), most = (int64_t)sm_count(device) * cached_blocks<A>(K);
+        cached_rows_kernel<T, A, L, K, M><<<(unsigned)std::min(blocks, most), kNT, 0, s>>>(x, ld, out, ld_out, a);
+    };
+    using std::integral_constant;
+    if (nv <= 16)
+        go(integral_constant<int, 8>{}, integral_constant<int, 2>{});
+    else if (nv <= 32)
+        go(integral_constant<int, 8>{}, integral_constant<int, 4>{});
+    else if (nv <= 64)
+        go(integral_constant<int, 16>{}, integral_constant<int, 4>{});
+    else if (nv <= 128)
+        go(integral_constant<int, 32>{}, integral_constant<int, 4>{});
+    else if (nv <= 256)
+        go(integral_constant<int, 32>{}, integral_constant<int, 8>{});
+    else
+        go(integral_constant<int, 32>{}, integral_constant<int, 16>{});
+}
+
 // Launches the row kernel for c classes of type T: by the row's bytes, the fewest
 // lanes that hold it in registers.
 template <class T, class A, Mode M>
 void rows_launch(int device, const T* x, int64_t ld, T* out, int64_t ld_out, const RowArgs<A>& a,
                  cudaStream_t s) {
-    const int64_t n = a.n, nv = ceil_div(a.c * (int64_t)sizeof(T), 16);
-    auto cached = [&](auto k) {
-        constexpr int K = decltype(k)::value;
-        cached_rows_kernel<T, A, K, M><<<(unsigned)ceil_div(n, kNT / 32), kNT, 0, s>>>(x, ld, out, ld_out, a);
-    };
+    const int64_t n = a.n, nv = a.c / Pack<T>::N;  // a row's vectors, at most
     auto ring = [&](auto l) {
         constexpr int L = decltype(l)::value, bytes = ring_slots(L) * L * kRingVecs * 16;
         auto k = ring_rows_kernel<T, A, L>;
@@ -1166,18 +1228,16 @@ void rows_launch(int device, const T* x, int64_t ld, T* out, int64_t ld_out, con
     using std::integral_constant;
     if (a.c <= kSmallC)
         small_launch<T, A, M>(device, x, ld, out, ld_out, a, s);
-    else if (nv <= 64)
-        cached(integral_constant<int, 2>{});
-    else if (nv <= 256)
-        cached(integral_constant<int, 8>{});
+    else if (nv <= (M == STATS ? kCachedVecs / 2 : kCachedVecs))
+        cached_launch<T, A, M>(device, x, ld, out, ld_out, a, s);
     else if constexpr (M == STATS)
         scan();
     else if (nv <= 2560)
-        ring(integral_constant<int, kRingMost / 4>{});
+        ring(integral_constant<int, kRingLanes / 8>{});
     else if (nv <= 5120)
-        ring(integral_constant<int, kRingMost / 2>{});
+        ring(integral_constant<int, kRingLanes / 4>{});
     else
-        ring(integral_constant<int, kRingMost>{});
+        ring(integral_constant<int, kRingLanes / 2>{});
 }
 
 template <class T, class A>
@@ -1212,8 +1272,8 @@ void grad_launch(int device, const T* x, int64_t ld, int64_t n, int64_t c, Label
     a.lse_in = lse;
     if (c <= kSmallC)
         small_launch<T, A, GRAD>(device, x, ld, out, ld_out, a, s);
-    else if (c * (int64_t)sizeof(T) <= 4096)
-        label_grad_kernel<T, A, 32><<<(unsigned)ceil_div(n, kNT / 32), kNT, 0, s>>>(x, ld, out, ld_out, a);
+    else if (c / Pack<T>::N <= kCachedVecs)
+        cached_launch<T, A, GRAD>(device, x, ld, out, ld_out, a, s);
     else
         label_grad_kernel<T, A, kNT><<<(unsigned)n, kNT, 0, s>>>(x, ld, out, ld_out, a);
     MFM_CHECK_LAUNCH("label gradient launch");
