@@ -460,10 +460,10 @@ int mfm_embedding_lookup_device(int dtype, int device, int ids64, const void* id
  * Their element type is out_dtype: the gradient's type (MFM_DTYPE_F64 for
  * F32_F64), or MFM_DTYPE_F32 for BF16 / F16. d_scale (n_entries, the scale
  * type) is written when it and `table` are given. `workspace` (256-byte
- * aligned) holds at least mfm_embedding_grad_workspace_bytes(...) bytes; a call
- * owns it until its work on the stream is done. */
-int64_t mfm_embedding_grad_workspace_bytes(int dtype, int64_t n_entries, int64_t n_rows,
-                                           int64_t d);
+ * aligned) holds at least mfm_embedding_grad_workspace_bytes(...) bytes, by_rows = 1
+ * for (keys, rows, count); a call owns it until its work on the stream is done. */
+int64_t mfm_embedding_grad_workspace_bytes(int dtype, int by_rows, int64_t n_entries,
+                                           int64_t n_rows, int64_t d);
 int mfm_embedding_grad_device(int dtype, int out_dtype, int device, int ids64, const void* ids,
                               int64_t n_entries, const int64_t* indptr, int64_t n_out,
                               const void* scale, double alpha, const void* grad,

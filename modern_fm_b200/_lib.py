@@ -133,7 +133,7 @@ _SIGNATURES = {
         ct.c_int, ct.c_int, ct.c_int, ct.c_void_p, ct.c_int64, ct.c_void_p, ct.c_int64,
         ct.c_void_p, ct.c_double, ct.c_void_p, ct.c_int64, ct.c_int64, ct.c_int64, ct.c_void_p,
         ct.c_int64, ct.c_void_p]),
-    "mfm_embedding_grad_workspace_bytes": (ct.c_int64, [ct.c_int] + [ct.c_int64] * 3),
+    "mfm_embedding_grad_workspace_bytes": (ct.c_int64, [ct.c_int] * 2 + [ct.c_int64] * 3),
     "mfm_embedding_grad_device": (ct.c_int, [
         ct.c_int, ct.c_int, ct.c_int, ct.c_int, ct.c_void_p, ct.c_int64, ct.c_void_p, ct.c_int64,
         ct.c_void_p, ct.c_double, ct.c_void_p, ct.c_int64, ct.c_void_p, ct.c_int64, ct.c_int64,

@@ -131,6 +131,16 @@ void d2h(T* dst, const T* src, size_t count, cudaStream_t s, const char* what) {
 
 __host__ __device__ inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
+// Allows a kernel `bytes` of dynamic shared memory on `device`, asking the driver
+// once per kernel and device (K is the kernel's own type parameter: one flag set
+// per instantiation). The call costs as much as a launch.
+template <class K>
+void allow_smem(K kernel, int device, int bytes, bool (&asked)[64], const char* what) {
+    if (asked[device & 63]) return;
+    MFM_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes), what);
+    asked[device & 63] = true;  // two threads may both ask: the same answer
+}
+
 // Grid size for a warp-per-item kernel: enough blocks to fill the GPU
 // (a multiple of the SM count), never more than the work needs.
 inline unsigned warp_grid(int device, int64_t items, int warps_per_block, int blocks_per_sm) {

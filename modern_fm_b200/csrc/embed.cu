@@ -15,17 +15,20 @@ namespace {
 
 // ---------------------------------------------------------------- vectors --
 
-// N = 16 / sizeof(T) values, or one where rows are not 16-byte aligned, held raw.
-template <class T, bool WIDE>
+// B bytes of T: 16, 8, or one value, the largest that every row begins on; sixteen
+// are held raw.
+template <class T, int B>
 struct Lane {
-    static constexpr int N = WIDE ? 16 / (int)sizeof(T) : 1;
+    static constexpr int N = B > (int)sizeof(T) ? B / (int)sizeof(T) : 1;
+    static constexpr bool WIDE = N * sizeof(T) == 16;
+    using Few = Vec<T, WIDE ? 1 : N>;
     uint4 raw;
-    T one;
+    Few few;
     __device__ __forceinline__ void load(const T* p) {
-        if (WIDE)
+        if constexpr (WIDE)
             raw = *reinterpret_cast<const uint4*>(p);
         else
-            one = *p;
+            few = *reinterpret_cast<const Few*>(p);
     }
     template <class A>
     __device__ __forceinline__ void get(A (&v)[N]) const {
@@ -35,7 +38,8 @@ struct Lane {
 #pragma unroll
             for (int j = 0; j < N; ++j) v[j] = (A)w[j];
         } else {
-            v[0] = widen<A>(one);
+#pragma unroll
+            for (int j = 0; j < N; ++j) v[j] = widen<A>(few.v[j]);
         }
     }
 };
@@ -66,12 +70,12 @@ __device__ __forceinline__ void put(O* to, const A (&v)[N]) {
 
 // out[t] = alpha scale[t] table[ids[t]], rows of at least 32 vectors: a warp per
 // (row, piece of 32 U vectors), U vectors a lane in flight.
-template <class T, class A, class O, class I, int U>
+template <class T, class A, class O, class I, int B, int U>
 __global__ void __launch_bounds__(256)
     embed_wide_kernel(const I* __restrict__ ids, int64_t n, const A* __restrict__ scale, A alpha,
                       const T* __restrict__ table, int64_t n_rows, int dv, int pieces, int64_t ld,
                       O* __restrict__ out, int64_t ld_out) {
-    constexpr int N = Lane<T, true>::N;
+    constexpr int N = Lane<T, B>::N;
     const int64_t item = ((int64_t)blockIdx.x * 256 + threadIdx.x) / 32;
     const int64_t t = item / pieces;
     if (t >= n) return;
@@ -82,7 +86,7 @@ __global__ void __launch_bounds__(256)
     if (scale) f *= scale[t];
     const T* from = table + (live ? id : 0) * ld;
     O* to = out + t * ld_out;
-    Lane<T, true> v[U];
+    Lane<T, B> v[U];
 #pragma unroll
     for (int u = 0; u < U; ++u)
         if (live && j0 + u * 32 < dv) v[u].load(from + (int64_t)(j0 + u * 32) * N);
@@ -99,16 +103,16 @@ __global__ void __launch_bounds__(256)
 
 // The same for narrow or unaligned rows: one thread per vector (or value), U in
 // flight, 256 apart.
-template <class T, class A, class O, class I, bool WIDE, int U>
+template <class T, class A, class O, class I, int B, int U>
 __global__ void __launch_bounds__(256)
     embed_rows_kernel(const I* __restrict__ ids, int64_t n, const A* __restrict__ scale, A alpha,
                       const T* __restrict__ table, int64_t n_rows, uint32_t dv, int64_t ld,
                       O* __restrict__ out, int64_t ld_out) {
-    constexpr int N = Lane<T, WIDE>::N;
+    constexpr int N = Lane<T, B>::N;
     const int64_t first = (int64_t)blockIdx.x * (256 * U);
     const int64_t row0 = first / dv;
     const uint32_t off0 = (uint32_t)(first - row0 * dv);
-    Lane<T, WIDE> v[U];
+    Lane<T, B> v[U];
     A f[U];
     bool live[U];
 #pragma unroll
@@ -153,13 +157,13 @@ __device__ __forceinline__ void row_bounds(const int64_t* indptr, int64_t b, int
 // latency of the rows' gathers: 131072 rows of 36 entries, 16 float32 each in
 // float64 arithmetic, 54 us (62 us with a round's ids fetched just before its rows;
 // 67 us with EL = 4, 84 us at five blocks per SM).
-template <class T, class A, class O, class I, bool WIDE, int LV, int EL>
+template <class T, class A, class O, class I, int B, int LV, int EL>
 __global__ void __launch_bounds__(256, 4)
     embed_sums_kernel(const I* __restrict__ ids, int64_t n, const int64_t* __restrict__ indptr,
                       int64_t n_out, const A* __restrict__ scale, A alpha,
                       const T* __restrict__ table, int64_t n_rows, int64_t d, int64_t ld,
                       O* __restrict__ out, int64_t ld_out) {
-    constexpr int U = 4, G = LV * EL, N = Lane<T, WIDE>::N;
+    constexpr int U = 4, G = LV * EL, N = Lane<T, B>::N;
     const int lane = threadIdx.x % LV, el = threadIdx.x % G / LV;
     const int64_t b = (int64_t)blockIdx.x * (256 / G) + threadIdx.x / G;
     const int64_t col = ((int64_t)blockIdx.y * LV + lane) * N;
@@ -185,7 +189,7 @@ __global__ void __launch_bounds__(256, 4)
     };
     fetch(lo + el);
     for (int64_t e = lo + el; e < hi; e += U * EL) {
-        Lane<T, WIDE> v[U];
+        Lane<T, B> v[U];
         A w[U];
         bool live[U];
 #pragma unroll
@@ -270,20 +274,8 @@ __global__ void __launch_bounds__(kTileChunks)
     if (threadIdx.x == 0) *count = carry;
 }
 
-// First place in the sorted keys whose key is at least k, in [lo, hi).
-__device__ __forceinline__ int64_t first_at_least(const uint32_t* keys, int64_t lo, int64_t hi,
-                                                  uint32_t k) {
-    while (lo < hi) {
-        const int64_t mid = (lo + hi) >> 1;
-        if (keys[mid] >= k)
-            hi = mid;
-        else
-            lo = mid + 1;
-    }
-    return lo;
-}
-
-// The same for two keys k0 <= k1 by a whole warp: 32 probes a round for each.
+// First places in the sorted keys whose keys are at least k0 and k1, k0 <= k1, by a
+// whole warp: 32 probes a round for each.
 __device__ __forceinline__ void warp_range(const uint32_t* keys, int64_t n, uint32_t k0, uint32_t k1,
                                            int64_t& first, int64_t& behind) {
     const int lane = threadIdx.x & 31;
@@ -307,9 +299,20 @@ __device__ __forceinline__ void warp_range(const uint32_t* keys, int64_t n, uint
     behind = lo1;
 }
 
-template <class G, class T, class A, class O, class I>
+struct KeysOut {  // the touched ids, of the ids' type; p NULL: not wanted
+    void* p;
+    int is64;
+    __device__ __forceinline__ void put(int64_t at, int64_t key) const {
+        if (is64)
+            static_cast<int64_t*>(p)[at] = key;
+        else
+            static_cast<int32_t*>(p)[at] = (int32_t)key;
+    }
+};
+
+template <class G, class T, class A, class O>
 struct GradArgs {
-    Entries<I> in;
+    Entries in;
     const A* scale;
     A alpha;
     const G* grad;
@@ -317,13 +320,14 @@ struct GradArgs {
     const T* table;
     int64_t ld_table, d;
     O *d_table, *rows;
-    I* keys_out;
+    KeysOut keys_out;
     int64_t* count;
     A* d_scale;
     // sorted entries, padded to whole chunks: key, gradient row, scale
     const uint32_t *keys, *srows;
     const A* scales;
     const int32_t* row_of;  // by position
+    const uint32_t* touched;  // bits of the touched table rows, or NULL: search the keys
     const uint32_t *base, *tile_base;
     A *part_head, *part_tail;
     int64_t n_chunks;
@@ -338,10 +342,10 @@ struct GradArgs {
 // scale grad[row], run by run. A run that lies in the chunk is written; the
 // part of a run that began before goes to part_head[chunk], the part of one that
 // goes on behind to part_tail[chunk] (all of it to part_head when both).
-template <class G, class T, class A, class O, class I, bool WIDE, int LV>
-__device__ __forceinline__ void reduce_chunk(const GradArgs<G, T, A, O, I>& a, int64_t c, int64_t col,
+template <class G, class T, class A, class O, int B, int LV>
+__device__ __forceinline__ void reduce_chunk(const GradArgs<G, T, A, O>& a, int64_t c, int64_t col,
                                              bool first_lane) {
-    constexpr int U = 8, N = Lane<G, WIDE>::N;
+    constexpr int U = 8, N = Lane<G, B>::N;
     const uint32_t pad_key = (uint32_t)a.in.n_rows;
     const int64_t n = a.in.n, e0 = c * kChunk, e1 = e0 + kChunk;
     uint32_t k[kChunk], row[kChunk];
@@ -380,13 +384,13 @@ __device__ __forceinline__ void reduce_chunk(const GradArgs<G, T, A, O, I>& a, i
 #pragma unroll
             for (int j = 0; j < N; ++j) acc[j] *= a.alpha;
             put((a.rows ? a.rows + rank * a.d : a.d_table + (int64_t)cur * a.d) + col, acc);
-            if (a.keys_out && first_lane) a.keys_out[rank] = (I)cur;
+            if (a.keys_out.p && first_lane) a.keys_out.put(rank, cur);
         }
     };
 #pragma unroll
     for (int b = 0; b < kChunk; b += U) {
         if (b > 0 && k[b] == pad_key) break;
-        Lane<G, WIDE> v[U];
+        Lane<G, B> v[U];
         A f[U];
 #pragma unroll
         for (int u = 0; u < U; ++u)
@@ -421,10 +425,11 @@ __device__ __forceinline__ void reduce_chunk(const GradArgs<G, T, A, O, I>& a, i
 }
 
 // Zeros for the rows of the result that no run writes: table rows without an
-// entry (a warp per `per` <= 32 rows, found by bisection among the sorted keys), or the
-// places behind the last touched row. Each row of the result is written once.
-template <class G, class T, class A, class O, class I>
-__device__ __forceinline__ void fill_rest(const GradArgs<G, T, A, O, I>& a, int per, int64_t warp,
+// entry (a warp per `per` <= 32 rows; by the bits the sort left, or for a few ids by
+// a search among the sorted keys), or the places behind the last touched row.
+// Each row of the result is written once.
+template <class G, class T, class A, class O>
+__device__ __forceinline__ void fill_rest(const GradArgs<G, T, A, O>& a, int per, int64_t warp,
                                           int64_t n_warps) {
     const int lane = threadIdx.x & 31;
     auto clear = [&](O* row) {
@@ -440,7 +445,7 @@ __device__ __forceinline__ void fill_rest(const GradArgs<G, T, A, O, I>& a, int 
         const int64_t used = *a.count, cap = a.in.n < a.in.n_rows ? a.in.n : a.in.n_rows;
         for (int64_t r0 = used + warp * per; r0 < cap; r0 += n_warps * per) {
             const int m = (int)(cap - r0 < per ? cap - r0 : per);
-            if (lane < m) a.keys_out[r0 + lane] = (I)-1;
+            if (lane < m) a.keys_out.put(r0 + lane, -1);
             if (a.d * (int64_t)sizeof(O) >= 512) {
                 for (int i = 0; i < m; ++i) clear(a.rows + (r0 + i) * a.d);
             } else {  // short rows: together one stretch
@@ -455,78 +460,102 @@ __device__ __forceinline__ void fill_rest(const GradArgs<G, T, A, O, I>& a, int 
             }
         }
     } else {
-        const int64_t n = a.in.n, n_rows = a.in.n_rows;
+        const int64_t n = a.in.n, n_rows = a.in.n_rows, bytes = a.d * (int64_t)sizeof(O);
+        const bool vec = bytes % 16 == 0 && (uintptr_t)a.d_table % 16 == 0;
         for (int64_t r0 = warp * per; r0 < n_rows; r0 += n_warps * per) {
-            // all these rows' entries lie between the first of r0 and the first of r0 + per
-            const int64_t end = r0 + per < n_rows ? r0 + per : n_rows;
-            int64_t lo, hi;
-            warp_range(a.keys, n, (uint32_t)r0, (uint32_t)end, lo, hi);
+            const int rows = (int)(r0 + per < n_rows ? per : n_rows - r0);
             unsigned touched = 0;
-            if (hi - lo > 1024) {  // popular ids: a bisection per row
-                if (lane < end - r0) {
-                    const uint32_t r = (uint32_t)(r0 + lane);
-                    const int64_t at = first_at_least(a.keys, lo, hi, r);
-                    if (at < hi && a.keys[at] == r) touched = 1u << lane;
-                }
+            if (a.touched) {  // per divides 32
+                touched = a.touched[r0 / 32] >> (r0 & 31);
             } else {
-#pragma unroll 4
+                int64_t lo, hi;
+                warp_range(a.keys, n, (uint32_t)r0, (uint32_t)(r0 + rows), lo, hi);
                 for (int64_t i = lo + lane; i < hi; i += 32) touched |= 1u << (a.keys[i] - (uint32_t)r0);
+                touched = __reduce_or_sync(0xffffffffu, touched);
             }
-            touched = __reduce_or_sync(0xffffffffu, touched);
-            unsigned m = ~touched & (end - r0 == 32 ? 0xffffffffu : (1u << (end - r0)) - 1u);
-            if (m == 0xffffffffu && a.d * (int64_t)sizeof(O) < 512 && a.d * sizeof(O) % 16 == 0 &&
-                (uintptr_t)(a.d_table + r0 * a.d) % 16 == 0) {
-                uint4* at = reinterpret_cast<uint4*>(a.d_table + r0 * a.d);
-                for (int i = lane; i < (int)(a.d * sizeof(O) * 2); i += 32) at[i] = make_uint4(0, 0, 0, 0);
+            O* at = a.d_table + r0 * a.d;
+            if (vec && bytes <= 1024) {  // the rows' vectors as one stretch
+                const unsigned vr = (unsigned)(bytes / 16), total = (unsigned)rows * vr;
+                for (unsigned i = lane; i < total; i += 32)
+                    if (!(touched >> (i / vr) & 1u)) reinterpret_cast<uint4*>(at)[i] = make_uint4(0, 0, 0, 0);
             } else {
-                for (; m; m &= m - 1) clear(a.d_table + (r0 + __ffs(m) - 1) * a.d);
+                for (unsigned m = ~touched & (rows == 32 ? 0xffffffffu : (1u << rows) - 1u); m; m &= m - 1)
+                    clear(at + (__ffs(m) - 1) * a.d);
             }
         }
     }
 }
 
-// d_scale[t] = alpha <grad[row(t)], table[ids[t]]>: LV lanes per entry.
-template <class G, class T, class A, class O, class I, bool WIDE, int LV>
-__device__ __forceinline__ void scale_entry(const GradArgs<G, T, A, O, I>& a, int64_t t, int lane) {
-    constexpr int N = Lane<G, WIDE>::N;
-    A acc = A(0);
-    if (t < a.in.n) {
-        const int64_t id = (int64_t)a.in.ids[t], row = a.row_of ? (int64_t)a.row_of[t] : t;
-        if (id >= 0 && id < a.in.n_rows && row >= 0) {
-            const G* g = a.grad + row * a.ld;
-            const T* v = a.table + id * a.ld_table;
-#pragma unroll 4
-            for (int64_t c = (int64_t)lane * N; c < a.d; c += LV * N) {
-                Lane<G, WIDE> x;
-                x.load(g + c);
-                A p[N], q[N];
-                x.get(p);
-                if constexpr (sizeof(T) == sizeof(G)) {
-                    Lane<T, WIDE> y;
-                    y.load(v + c);
-                    y.get(q);
-                } else {  // a float32 table with float64 gradients: half a vector
-                    const Vec<T, N> y = ldg_vec<T, N>(v + c);
+// d_scale[t] = alpha <grad[row(t)], table[ids[t]]> for kScaleEntries entries LV lanes
+// apart, their loads in flight together.
+constexpr int kScaleEntries = 4;
+
+template <class G, class T, class A, class O, int B, int LV>
+__device__ __forceinline__ void scale_entries(const GradArgs<G, T, A, O>& a, int64_t t0, int stride,
+                                              int lane) {
+    constexpr int N = Lane<G, B>::N, U = kScaleEntries;
+    const T* v[U];
+    const G* g[U];
+    bool live[U];
+    A acc[U];
 #pragma unroll
-                    for (int j = 0; j < N; ++j) q[j] = widen<A>(y.v[j]);
+    for (int u = 0; u < U; ++u) {
+        const int64_t t = t0 + u * stride;
+        int64_t id = -1, row = -1;
+        if (t < a.in.n) {
+            id = a.in.ids[t];
+            row = a.row_of ? (int64_t)a.row_of[t] : t;
+        }
+        live[u] = id >= 0 && id < a.in.n_rows && row >= 0;
+        v[u] = a.table + (live[u] ? id : 0) * a.ld_table;
+        g[u] = a.grad + (live[u] ? row : 0) * a.ld;
+        acc[u] = A(0);
+    }
+    for (int64_t c = (int64_t)lane * N; c < a.d; c += LV * N) {
+        Lane<G, B> x[U];
+        // a float32 table with float64 gradients: half a vector
+        using Y = std::conditional_t<sizeof(T) == sizeof(G), Lane<T, B>, Vec<T, N>>;
+        Y y[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (live[u]) {
+                x[u].load(g[u] + c);
+                if constexpr (sizeof(T) == sizeof(G))
+                    y[u].load(v[u] + c);
+                else
+                    y[u] = ldg_vec<T, N>(v[u] + c);
+            }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (live[u]) {
+                A p[N], q[N];
+                x[u].get(p);
+                if constexpr (sizeof(T) == sizeof(G)) {
+                    y[u].get(q);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < N; ++j) q[j] = widen<A>(y[u].v[j]);
                 }
 #pragma unroll
-                for (int j = 0; j < N; ++j) acc += p[j] * q[j];
+                for (int j = 0; j < N; ++j) acc[u] += p[j] * q[j];
             }
-        }
     }
 #pragma unroll
-    for (int o = LV / 2; o > 0; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
-    if (lane == 0 && t < a.in.n) a.d_scale[t] = a.alpha * acc;
+    for (int u = 0; u < U; ++u) {
+#pragma unroll
+        for (int o = LV / 2; o > 0; o >>= 1) acc[u] += __shfl_xor_sync(0xffffffffu, acc[u], o);
+        const int64_t t = t0 + u * stride;
+        if (lane == 0 && t < a.in.n) a.d_scale[t] = a.alpha * acc[u];
+    }
 }
 
 // The gradient in one launch of three independent parts: blocks that sum chunks,
 // blocks that take the scales' gradient, and blocks that fill. Filling is bound
 // by HBM and the others by latency, so its blocks alternate with theirs.
-template <class G, class T, class A, class O, class I, bool WIDE, int LV>
+template <class G, class T, class A, class O, int B, int LV>
 __global__ void __launch_bounds__(kMainNT)
-    embed_main_kernel(const GradArgs<G, T, A, O, I> a, int slabs) {
-    constexpr int N = Lane<G, WIDE>::N, GR = kMainNT / LV;
+    embed_main_kernel(const GradArgs<G, T, A, O> a, int slabs) {
+    constexpr int N = Lane<G, B>::N, GR = kMainNT / LV;
     const int lane = threadIdx.x % LV, group = threadIdx.x / LV;
     const unsigned work = a.reduce_blocks + a.scale_blocks;
     const unsigned both = 2 * (work < a.fill_blocks ? work : a.fill_blocks);
@@ -545,21 +574,21 @@ __global__ void __launch_bounds__(kMainNT)
     } else if (b < a.reduce_blocks) {
         const int64_t c = (int64_t)(b / slabs) * GR + group;
         const int64_t col = ((int64_t)(b % slabs) * LV + lane) * N;
-        if (c < a.n_chunks && col < a.d) reduce_chunk<G, T, A, O, I, WIDE, LV>(a, c, col, col == 0);
+        if (c < a.n_chunks && col < a.d) reduce_chunk<G, T, A, O, B, LV>(a, c, col, col == 0);
     } else {
-        scale_entry<G, T, A, O, I, WIDE, LV>(a, (int64_t)(b - a.reduce_blocks) * GR + group, lane);
+        scale_entries<G, T, A, O, B, LV>(a, (int64_t)(b - a.reduce_blocks) * (GR * kScaleEntries) + group, GR, lane);
     }
 }
 
 // The runs that cross chunks: the lane group of the chunk where one begins adds
 // its parts in chunk order and writes the run; the block's groups share a run of
-// more than kLongRun parts (ids that occur in every row: one part per 16 rows).
-constexpr int kLongRun = 16;
+// more than kLongRun chunks (ids that occur in every row: one chunk per 16 rows).
+constexpr int kLongRun = 8;
 
-template <class G, class T, class A, class O, class I, bool WIDE, int LV>
+template <class G, class T, class A, class O, int B, int LV>
 __global__ void __launch_bounds__(256)
-    embed_cross_kernel(const GradArgs<G, T, A, O, I> a) {
-    constexpr int N = Lane<G, WIDE>::N, GR = 256 / LV;
+    embed_cross_kernel(const GradArgs<G, T, A, O> a) {
+    constexpr int N = Lane<G, B>::N, GR = 256 / LV;
     __shared__ int64_t run_last[GR];  // last chunk of the run begun in the group's chunk, -1: none
     __shared__ int long_groups[GR], n_long;
     __shared__ A shared_part[256 * N];
@@ -572,17 +601,17 @@ __global__ void __launch_bounds__(256)
     if (lane == 0) {
         int64_t last = -1;
         if (c + 1 < a.n_chunks) {
+            // the keys at the chunk's bounds and the first keys of the chunks behind
+            // it, where most runs end: all in flight
             const int64_t e0 = c * kChunk, e1 = e0 + kChunk;  // not the last chunk: e1 < n
-            const uint32_t key = a.keys[e1 - 1];
-            if (key != pad_key && a.keys[e1] == key && !(e0 > 0 && a.keys[e0 - 1] == key)) {
-                // most runs end within a few chunks: their first keys, all in flight
-                bool same[8];
+            const uint32_t key = a.keys[e1 - 1], next = a.keys[e1], prev = e0 > 0 ? a.keys[e0 - 1] : pad_key;
+            uint32_t ahead[8];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) same[i] = c + 2 + i < a.n_chunks && a.keys[(c + 2 + i) * kChunk] == key;
+            for (int i = 0; i < 8; ++i) ahead[i] = c + 2 + i < a.n_chunks ? a.keys[(c + 2 + i) * kChunk] : pad_key;
+            if (key != pad_key && next == key && prev != key) {
                 last = c + 1;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) last += last == c + 1 + i && same[i] ? 1 : 0;
-                if (last == c + 9) last = (first_at_least(a.keys, last * kChunk, n, key + 1) - 1) / kChunk;
+                for (int i = 0; i < 8; ++i) last += last == c + 1 + i && ahead[i] == key ? 1 : 0;
             }
         }
         run_last[group] = last;
@@ -596,7 +625,7 @@ __global__ void __launch_bounds__(256)
 #pragma unroll
         for (int j = 0; j < N; ++j) acc[j] *= a.alpha;
         put((a.rows ? a.rows : a.d_table) + at * a.d + col, acc);
-        if (a.keys_out && col == 0) a.keys_out[at] = (I)key;
+        if (a.keys_out.p && col == 0) a.keys_out.put(at, key);
     };
     const bool in = col < a.d;
     const int64_t mine = run_last[group];
@@ -615,12 +644,22 @@ __global__ void __launch_bounds__(256)
     }
     for (int i = 0; i < n_long; ++i) {
         const int g = long_groups[i];
-        const int64_t last = run_last[g], from = c0 + g;
+        const int64_t from = c0 + g;
+        // the run's last chunk: chunks are probed 256 a round by their first key
+        const uint32_t key = a.keys[from * kChunk + kChunk - 1];
+        int64_t last = run_last[g], end = a.n_chunks;  // in [last, end)
+        while (end - last > 1) {
+            const int64_t step = (end - last + 254) / 256;
+            const int64_t p = last + (threadIdx.x + 1) * step;
+            const int same = __syncthreads_count(p < end && a.keys[p * kChunk] == key);
+            last += same * step;
+            if (last + step < end) end = last + step;
+        }
         A acc[N];
 #pragma unroll
         for (int j = 0; j < N; ++j) acc[j] = A(0);
         if (in) {
-#pragma unroll 4
+#pragma unroll 8
             for (int64_t k = from + 1 + group; k <= last; k += GR) {
                 const Vec<A, N> p = ldg_vec<A, N>(a.part_head + k * a.d + col);
 #pragma unroll
@@ -706,53 +745,68 @@ void with_lanes(int64_t dv, F&& f) {
 template <class P>
 using Elem = std::remove_const_t<std::remove_pointer_t<std::remove_reference_t<P>>>;
 
-template <class T, class A, class O, class I, bool WIDE>
-void lookup_launch(int device, const Entries<I>& in, const A* scale, A alpha, const T* table,
-                   int64_t d, int64_t ld, O* out, int64_t ld_out, cudaStream_t s) {
-    constexpr int N = Lane<T, WIDE>::N;
-    const int64_t dv = d / N, n = in.n;
+template <class T, class A, class O, class I, int B>
+void lookup_launch(int device, const I* ids, int64_t n, const int64_t* indptr, int64_t n_out,
+                   const A* scale, A alpha, const T* table, int64_t n_rows, int64_t d, int64_t ld,
+                   O* out, int64_t ld_out, cudaStream_t s) {
+    constexpr int N = Lane<T, B>::N;
+    const int64_t dv = d / N;
     const int64_t fill = (int64_t)sm_count(device) * 2048;  // threads at once
-    if (in.indptr) {
+    if (indptr) {
         with_lanes(dv, [&](auto lv) {
             constexpr int LV = decltype(lv)::value, EL = LV >= 8 ? 1 : 8 / LV;
-            const dim3 g((unsigned)ceil_div(in.n_out, 256 / (LV * EL)), (unsigned)ceil_div(dv, LV));
-            embed_sums_kernel<T, A, O, I, WIDE, LV, EL><<<g, 256, 0, s>>>(
-                in.ids, n, in.indptr, in.n_out, scale, alpha, table, in.n_rows, d, ld, out, ld_out);
+            const dim3 g((unsigned)ceil_div(n_out, 256 / (LV * EL)), (unsigned)ceil_div(dv, LV));
+            embed_sums_kernel<T, A, O, I, B, LV, EL><<<g, 256, 0, s>>>(
+                ids, n, indptr, n_out, scale, alpha, table, n_rows, d, ld, out, ld_out);
         });
-    } else if (WIDE && dv >= 32) {
-        if constexpr (WIDE) {
-            auto wide = [&](auto unroll) {
-                constexpr int U = decltype(unroll)::value;
-                const int64_t pieces = ceil_div(dv, 32 * U);
-                embed_wide_kernel<T, A, O, I, U><<<(unsigned)ceil_div(n * pieces, 8), 256, 0, s>>>(
-                    in.ids, n, scale, alpha, table, in.n_rows, (int)dv, (int)pieces, ld, out, ld_out);
-            };
-            // fewer vectors a lane while the lanes do not fill the GPU
-            if (n * dv >= 4 * fill && dv >= 128)
-                wide(std::integral_constant<int, 4>{});
-            else if (n * dv >= 2 * fill && dv >= 64)
-                wide(std::integral_constant<int, 2>{});
-            else
-                wide(std::integral_constant<int, 1>{});
-        }
+    } else if (dv >= 32) {
+        auto wide = [&](auto unroll) {
+            constexpr int U = decltype(unroll)::value;
+            const int64_t pieces = ceil_div(dv, 32 * U);
+            embed_wide_kernel<T, A, O, I, B, U><<<(unsigned)ceil_div(n * pieces, 8), 256, 0, s>>>(
+                ids, n, scale, alpha, table, n_rows, (int)dv, (int)pieces, ld, out, ld_out);
+        };
+        // fewer vectors a lane while the lanes do not fill the GPU
+        if (n * dv >= 4 * fill && dv >= 128)
+            wide(std::integral_constant<int, 4>{});
+        else if (n * dv >= 2 * fill && dv >= 64)
+            wide(std::integral_constant<int, 2>{});
+        else
+            wide(std::integral_constant<int, 1>{});
     } else {
         const int64_t total = n * dv;
         if (total <= fill)
-            embed_rows_kernel<T, A, O, I, WIDE, 1><<<(unsigned)ceil_div(total, 256), 256, 0, s>>>(
-                in.ids, n, scale, alpha, table, in.n_rows, (uint32_t)dv, ld, out, ld_out);
+            embed_rows_kernel<T, A, O, I, B, 1><<<(unsigned)ceil_div(total, 256), 256, 0, s>>>(
+                ids, n, scale, alpha, table, n_rows, (uint32_t)dv, ld, out, ld_out);
         else
-            embed_rows_kernel<T, A, O, I, WIDE, 4><<<(unsigned)ceil_div(total, 1024), 256, 0, s>>>(
-                in.ids, n, scale, alpha, table, in.n_rows, (uint32_t)dv, ld, out, ld_out);
+            embed_rows_kernel<T, A, O, I, B, 4><<<(unsigned)ceil_div(total, 1024), 256, 0, s>>>(
+                ids, n, scale, alpha, table, n_rows, (uint32_t)dv, ld, out, ld_out);
     }
     MFM_CHECK_LAUNCH("embedding lookup launch");
+}
+
+// f(B) with the most bytes a lane that every row of T (and of a second type Q) begins on.
+template <class T, class F>
+void with_bytes(int64_t d, const void* p, int64_t ld, size_t q_size, const void* q, int64_t ld_q, F&& f) {
+    auto fits = [&](int bytes) {
+        const int n = bytes / (int)sizeof(T);
+        return n >= 1 && d % n == 0 && vec_ok(p, ld, sizeof(T), n) &&
+               vec_ok(q, ld_q, q_size, std::min<int>(n, 16 / (int)q_size));
+    };
+    if (fits(16))
+        f(std::integral_constant<int, 16>{});
+    else if (fits(8) && sizeof(T) < 8)
+        f(std::integral_constant<int, 8>{});
+    else
+        f(std::integral_constant<int, 1>{});
 }
 
 // Workspace layout of the gradient, 256-byte aligned pieces.
 struct GradWs {
     IdSortPlan sort;
     int64_t n_chunks = 0;
-    size_t off_row = 0, off_scale = 0, off_base = 0, off_tile = 0, off_head = 0, off_tail = 0, bytes = 0;
-    GradWs(int dtype, int64_t n, int64_t n_rows, int64_t d) : sort(n, n_rows) {
+    size_t off_row = 0, off_scale = 0, off_base = 0, off_tile = 0, off_head = 0, off_tail = 0, off_bits = 0, bytes = 0;
+    GradWs(int dtype, bool by_rows, int64_t n, int64_t n_rows, int64_t d) : sort(n, n_rows) {
         auto up = [](size_t b) { return (b + 255) / 256 * 256; };
         const size_t a = dtype == MFM_DTYPE_F64 || dtype == MFM_DTYPE_F32_F64 ? 8 : 4;
         n_chunks = ceil_div(n, kChunk);
@@ -762,13 +816,14 @@ struct GradWs {
         off_tile = off_base + up((size_t)n_chunks * 4);
         off_head = off_tile + up((size_t)ceil_div(n_chunks, kTileChunks) * 4);
         off_tail = off_head + up((size_t)n_chunks * d * a);
-        bytes = off_tail + up((size_t)n_chunks * d * a);
+        off_bits = off_tail + up((size_t)n_chunks * d * a);
+        bytes = off_bits + (by_rows || n <= kSmallSort ? 0 : up((size_t)ceil_div(n_rows, 32) * 4));
     }
 };
 
-template <class G, class T, class A, class O, class I, bool WIDE>
-void grad_launch(int device, GradArgs<G, T, A, O, I>& a, const GradWs& W, char* ws, cudaStream_t s) {
-    constexpr int N = Lane<G, WIDE>::N;
+template <class G, class T, class A, class O, int B>
+void grad_launch(int device, GradArgs<G, T, A, O>& a, const GradWs& W, char* ws, cudaStream_t s) {
+    constexpr int N = Lane<G, B>::N;
     const int64_t n = a.in.n, nc = W.n_chunks, dv = a.d / N;
     uint32_t* words = reinterpret_cast<uint32_t*>(ws);
     unsigned* done = words + W.sort.words;
@@ -776,7 +831,9 @@ void grad_launch(int device, GradArgs<G, T, A, O, I>& a, const GradWs& W, char* 
     SortedOut<A> sorted{};
     sorted.scale = a.scale;
     sorted.scales = reinterpret_cast<A*>(ws + W.off_scale);
-    sort_ids(W.sort, a.in, row_of, done, words, sorted, s);
+    if (a.d_table && n > kSmallSort) sorted.touched = reinterpret_cast<uint32_t*>(ws + W.off_bits);
+    a.touched = sorted.touched;
+    sort_ids(device, W.sort, a.in, row_of, done, words, sorted, s);
     a.keys = sorted.keys;
     a.srows = sorted.rows;
     a.scales = a.scale ? sorted.scales : nullptr;
@@ -796,41 +853,44 @@ void grad_launch(int device, GradArgs<G, T, A, O, I>& a, const GradWs& W, char* 
         constexpr int LV = decltype(lv)::value;
         const int64_t slabs = ceil_div(dv, LV), sm = sm_count(device);
         a.reduce_blocks = (unsigned)(ceil_div(nc, kMainNT / LV) * slabs);
-        a.scale_blocks = a.d_scale ? (unsigned)ceil_div(n, kMainNT / LV) : 0u;
+        a.scale_blocks = a.d_scale ? (unsigned)ceil_div(n, kMainNT / LV * kScaleEntries) : 0u;
         const int64_t rest = a.rows ? std::min(n, a.in.n_rows) : a.in.n_rows;
         // a warp fills 32 rows, or fewer where the rows are long
-        a.fill_per = (int)std::min<int64_t>(32, std::max<int64_t>(4, 32768 / (a.d * (int64_t)sizeof(O))));
+        a.fill_per = 32;
+        while (a.fill_per > 4 && a.fill_per * a.d * (int64_t)sizeof(O) > 32768) a.fill_per /= 2;
         a.fill_blocks = (unsigned)std::min<int64_t>(ceil_div(rest, (int64_t)a.fill_per * (kMainNT / 32)), sm * 16);
-        embed_main_kernel<G, T, A, O, I, WIDE, LV>
+        embed_main_kernel<G, T, A, O, B, LV>
             <<<a.reduce_blocks + a.scale_blocks + a.fill_blocks, kMainNT, 0, s>>>(a, (int)slabs);
         if (nc > 1) {
             const dim3 g((unsigned)ceil_div(nc, 256 / LV), (unsigned)slabs);
-            embed_cross_kernel<G, T, A, O, I, WIDE, LV><<<g, 256, 0, s>>>(a);
+            embed_cross_kernel<G, T, A, O, B, LV><<<g, 256, 0, s>>>(a);
         }
     });
     MFM_CHECK_LAUNCH("embedding gradient launch");
 }
 
-template <class G, class T, class A, class O, class I>
-void grad_entry(int device, GradArgs<G, T, A, O, I>& a, const GradWs& W, char* ws, cudaStream_t s) {
+template <class G, class T, class A, class O>
+void grad_entry(int device, GradArgs<G, T, A, O>& a, const GradWs& W, char* ws, cudaStream_t s) {
     const int64_t cap = std::min(a.in.n, a.in.n_rows);
     if (a.in.n == 0 || a.in.n_rows == 0 || a.in.n_out == 0) {  // nothing to add up
         if (a.d_table) MFM_CUDA(cudaMemsetAsync(a.d_table, 0, (size_t)a.in.n_rows * a.d * sizeof(O), s), "memset");
-        if (a.keys_out) {
-            MFM_CUDA(cudaMemsetAsync(a.keys_out, 0xff, (size_t)cap * sizeof(I), s), "memset");
+        if (a.keys_out.p) {
+            MFM_CUDA(cudaMemsetAsync(a.keys_out.p, 0xff, (size_t)cap * (a.keys_out.is64 ? 8 : 4), s), "memset");
             MFM_CUDA(cudaMemsetAsync(a.rows, 0, (size_t)cap * a.d * sizeof(O), s), "memset");
             MFM_CUDA(cudaMemsetAsync(a.count, 0, sizeof(int64_t), s), "memset");
         }
         if (a.d_scale) MFM_CUDA(cudaMemsetAsync(a.d_scale, 0, (size_t)a.in.n * sizeof(A), s), "memset");
         return;
     }
-    constexpr int N = Lane<G, true>::N;
     const O* result = a.d_table ? a.d_table : a.rows;
-    const bool table_ok = !a.d_scale || vec_ok(a.table, a.ld_table, sizeof(T), N);
-    if (a.d % N == 0 && vec_ok(a.grad, a.ld, sizeof(G), N) && (uintptr_t)result % 16 == 0 && table_ok)
-        grad_launch<G, T, A, O, I, true>(device, a, W, ws, s);
-    else
-        grad_launch<G, T, A, O, I, false>(device, a, W, ws, s);
+    with_bytes<G>(a.d, a.grad, a.ld, sizeof(O), result, a.d, [&](auto bytes) {
+        constexpr int B = decltype(bytes)::value, N = Lane<G, B>::N;
+        // the table's rows may begin elsewhere
+        if (N > 1 && a.d_scale && !vec_ok(a.table, a.ld_table, sizeof(T), N))
+            grad_launch<G, T, A, O, 1>(device, a, W, ws, s);
+        else
+            grad_launch<G, T, A, O, B>(device, a, W, ws, s);
+    });
 }
 
 }  // namespace
@@ -857,28 +917,21 @@ extern "C" int mfm_embedding_lookup_device(int dtype, int device, int ids64, con
             using O = Elem<decltype(o)>;
             with_index_type(ids64, [&](auto* i) {
                 using I = Elem<decltype(i)>;
-                constexpr int N = Lane<T, true>::N;
-                const Entries<I> in{(const I*)ids, n_entries, indptr, n_out, n_rows};
-                auto go = [&](auto wide) {
-                    lookup_launch<T, A, O, I, decltype(wide)::value>(
-                        device, in, (const A*)scale, (A)alpha, (const T*)table, d, ld_table, (O*)out,
-                        ld_out, (cudaStream_t)stream);
-                };
-                // vectors of 16 bytes of the table, and the results' vectors whole
-                if (d % N == 0 && vec_ok(table, ld_table, sizeof(T), N) && vec_ok(out, ld_out, sizeof(O), std::min<int>(N, 16 / sizeof(O))))
-                    go(std::true_type{});
-                else
-                    go(std::false_type{});
+                with_bytes<T>(d, table, ld_table, sizeof(O), out, ld_out, [&](auto bytes) {
+                    lookup_launch<T, A, O, I, decltype(bytes)::value>(
+                        device, (const I*)ids, n_entries, indptr, n_out, (const A*)scale, (A)alpha,
+                        (const T*)table, n_rows, d, ld_table, (O*)out, ld_out, (cudaStream_t)stream);
+                });
             });
         });
     });
 }
 
-extern "C" int64_t mfm_embedding_grad_workspace_bytes(int dtype, int64_t n_entries,
+extern "C" int64_t mfm_embedding_grad_workspace_bytes(int dtype, int by_rows, int64_t n_entries,
                                                       int64_t n_rows, int64_t d) {
     if (n_entries <= 0 || n_rows < 0 || d < 1 || n_entries > kMaxCount || n_rows > kMaxCount || d > kMaxCount)
         return 0;
-    return (int64_t)GradWs(dtype, n_entries, n_rows, d).bytes;
+    return (int64_t)GradWs(dtype, by_rows != 0, n_entries, n_rows, d).bytes;
 }
 
 extern "C" int mfm_embedding_grad_device(int dtype, int out_dtype, int device, int ids64,
@@ -907,7 +960,7 @@ extern "C" int mfm_embedding_grad_device(int dtype, int out_dtype, int device, i
             check_pitch("table", ld_table, d);
         }
         DeviceGuard g(device);
-        const GradWs W(dtype, n_entries, n_rows, d);
+        const GradWs W(dtype, by_rows, n_entries, n_rows, d);
         if (n_entries > 0 && (!workspace || workspace_bytes < (int64_t)W.bytes))
             fail(MFM_ERR_INVALID, fmt("workspace of %lld bytes, %lld needed", (long long)workspace_bytes,
                                       (long long)W.bytes));
@@ -916,34 +969,31 @@ extern "C" int mfm_embedding_grad_device(int dtype, int out_dtype, int device, i
             using T = Elem<decltype(t)>;
             using A = Elem<decltype(a)>;
             using G = Elem<decltype(o)>;
-            with_index_type(ids64, [&](auto* i) {
-                using I = Elem<decltype(i)>;
-                auto go = [&](auto* r) {
-                    using O = Elem<decltype(r)>;
-                    GradArgs<G, T, A, O, I> x{};
-                    x.in = Entries<I>{(const I*)ids, n_entries, indptr, n_out, n_rows};
-                    x.scale = (const A*)scale;
-                    x.alpha = (A)alpha;
-                    x.grad = (const G*)grad;
-                    x.ld = ld_grad;
-                    x.table = (const T*)table;
-                    x.ld_table = ld_table;
-                    x.d = d;
-                    x.d_table = (O*)d_table;
-                    x.rows = (O*)rows;
-                    x.keys_out = (I*)keys;
-                    x.count = count;
-                    x.d_scale = (A*)d_scale;
-                    grad_entry(device, x, W, (char*)workspace, (cudaStream_t)stream);
-                };
-                if constexpr (sizeof(G) == 2) {
-                    if (out_dtype == MFM_DTYPE_F32) {
-                        go((float*)nullptr);
-                        return;
-                    }
+            auto go = [&](auto* r) {
+                using O = Elem<decltype(r)>;
+                GradArgs<G, T, A, O> x{};
+                x.in = Entries{Ids{ids, ids64}, n_entries, indptr, n_out, n_rows};
+                x.scale = (const A*)scale;
+                x.alpha = (A)alpha;
+                x.grad = (const G*)grad;
+                x.ld = ld_grad;
+                x.table = (const T*)table;
+                x.ld_table = ld_table;
+                x.d = d;
+                x.d_table = (O*)d_table;
+                x.rows = (O*)rows;
+                x.keys_out = KeysOut{keys, ids64};
+                x.count = count;
+                x.d_scale = (A*)d_scale;
+                grad_entry(device, x, W, (char*)workspace, (cudaStream_t)stream);
+            };
+            if constexpr (sizeof(G) == 2) {
+                if (out_dtype == MFM_DTYPE_F32) {
+                    go((float*)nullptr);
+                    return;
                 }
-                go((G*)nullptr);
-            });
+            }
+            go((G*)nullptr);
         });
     });
 }

@@ -35,9 +35,16 @@ constexpr int kSortPad = 16;  // places behind the last entry: key n_rows, row 0
 
 // The entries of a batch: their ids and, where they are summed by rows, the rows'
 // bounds (indptr, n_out + 1; NULL: every entry is a row of its own).
-template <class I>
+struct Ids {  // int32 or int64
+    const void* p;
+    int is64;
+    __device__ __forceinline__ int64_t operator[](int64_t q) const {
+        return is64 ? static_cast<const int64_t*>(p)[q] : (int64_t)static_cast<const int32_t*>(p)[q];
+    }
+};
+
 struct Entries {
-    const I* ids;
+    Ids ids;
     int64_t n;
     const int64_t* indptr;
     int64_t n_out, n_rows;
@@ -91,8 +98,8 @@ struct Entries {
     // The sort key of entry q: its id, or n_rows for padding (an id outside the
     // table, or an entry of no row).
     __device__ __forceinline__ uint32_t key(int64_t q, int32_t row) const {
-        const I id = ids[q];
-        return id >= 0 && (int64_t)id < n_rows && row >= 0 ? (uint32_t)id : (uint32_t)n_rows;
+        const int64_t id = ids[q];
+        return id >= 0 && id < n_rows && row >= 0 ? (uint32_t)id : (uint32_t)n_rows;
     }
 };
 
@@ -106,6 +113,7 @@ struct SortedOut {
     const int32_t* row_of;
     const A* scale;
     uint32_t pad_key;
+    uint32_t* touched;  // one bit per table row, set for every real key; NULL: not wanted
     __device__ __forceinline__ void load(uint32_t p, uint32_t& row, A& s) const {
         row = row_of ? (uint32_t)row_of[p] : p;
         s = scale ? scale[p] : A(1);
@@ -118,12 +126,14 @@ struct SortedOut {
 };
 
 // Keys and rows of all entries, digit counts of the first pass by tile, and zeros
-// for the passes after it and for the block count of the kernels behind the sort.
-template <class I, int BITS>
+// for the passes after it, for the block count of the kernels behind the sort
+// and for the touched rows' bits.
+template <int BITS>
 __global__ void __launch_bounds__(kETileNT)
-    id_count_kernel(Entries<I> in, int passes, uint32_t mask, int64_t n_tiles,
+    id_count_kernel(Entries in, int passes, uint32_t mask, int64_t n_tiles,
                     uint32_t* __restrict__ keys, int32_t* __restrict__ row_of,
-                    uint32_t* __restrict__ counts, unsigned* __restrict__ done) {
+                    uint32_t* __restrict__ counts, unsigned* __restrict__ done,
+                    uint32_t* __restrict__ touched) {
     constexpr int D = 1 << BITS;
     __shared__ uint32_t h[D];
     const int t = threadIdx.x;
@@ -133,6 +143,8 @@ __global__ void __launch_bounds__(kETileNT)
         for (int p = 1; p < passes; ++p) counts[(p * n_tiles + tile) * D + d] = 0;
     }
     if (tile == 0 && t == 0) *done = 0;
+    if (touched)
+        for (int64_t i = tile * kETileNT + t; i * 32 < in.n_rows; i += n_tiles * kETileNT) touched[i] = 0;
     __syncthreads();
     const int64_t q0 = lo + (t / 32) * (32 * kETileItems);
     int32_t r[kETileItems];
@@ -364,15 +376,21 @@ __global__ void __launch_bounds__(kETileNT)
             if (t + u * kETileNT < m) out.load(e[u].y, row[u], s[u]);
 #pragma unroll
         for (int u = 0; u < kETileItems; ++u)
-            if (t + u * kETileNT < m) out.store(dst[u], e[u].x, row[u], s[u]);
+            if (t + u * kETileNT < m) {
+                const int j = t + u * kETileNT;
+                out.store(dst[u], e[u].x, row[u], s[u]);
+                // the tile holds equal keys together: one bit operation a run
+                if (out.touched && e[u].x != out.pad_key && (j == 0 || skv[j - 1].x != e[u].x))
+                    atomicOr(out.touched + e[u].x / 32, 1u << (e[u].x & 31));
+            }
         if (tile == 0 && t < kSortPad) out.store(n + t, out.pad_key, 0u, A(0));
     }
 }
 
 // All passes of up to NT * ITEMS ids in one block.
-template <class A, class I, int NT, int ITEMS>
+template <class A, int NT, int ITEMS>
 __global__ void __launch_bounds__(NT)
-    id_sort_small_kernel(Entries<I> in, int key_bits, int32_t* row_of,
+    id_sort_small_kernel(Entries in, int key_bits, int32_t* row_of,
                          unsigned* __restrict__ done, SortedOut<A> out) {
     constexpr int NW = NT / 32;
     __shared__ uint32_t cnt[NW][256];
@@ -470,8 +488,8 @@ struct IdSortPlan {
 // Sorts the batch's keys into out.keys with the entries' rows and scales (out's
 // keys and rows are set here, in the workspace); writes row_of (with indptr) and
 // clears *done.
-template <class A, class I>
-void sort_ids(const IdSortPlan& P, const Entries<I>& in, int32_t* row_of, unsigned* done,
+template <class A>
+void sort_ids(int device, const IdSortPlan& P, const Entries& in, int32_t* row_of, unsigned* done,
               uint32_t* ws, SortedOut<A>& out, cudaStream_t s) {
     const int64_t n = P.n;
     uint32_t* counts = ws + 4 * P.pitch;
@@ -483,7 +501,7 @@ void sort_ids(const IdSortPlan& P, const Entries<I>& in, int32_t* row_of, unsign
     if (n <= kSmallSort) {
         auto small = [&](auto nt, auto items) {
             constexpr int NT = decltype(nt)::value, IT = decltype(items)::value;
-            id_sort_small_kernel<A, I, NT, IT><<<1, NT, 0, s>>>(in, P.key_bits, row_of, done, out);
+            id_sort_small_kernel<A, NT, IT><<<1, NT, 0, s>>>(in, P.key_bits, row_of, done, out);
         };
         if (n <= 256)
             small(integral_constant<int, 256>{}, integral_constant<int, 1>{});
@@ -503,15 +521,15 @@ void sort_ids(const IdSortPlan& P, const Entries<I>& in, int32_t* row_of, unsign
         const bool fused = BITS == 8 && P.n_tiles <= kFuseTiles;
         uint32_t *ki = P.passes % 2 ? k1 : k0, *vi = P.passes % 2 ? v1 : v0;
         uint32_t *ko = P.passes % 2 ? k0 : k1, *vo = P.passes % 2 ? v0 : v1;
-        id_count_kernel<I, BITS><<<g, kETileNT, 0, s>>>(in, P.passes, (1u << P.bits) - 1u, P.n_tiles, ki, row_of, counts, done);
+        id_count_kernel<BITS><<<g, kETileNT, 0, s>>>(in, P.passes, (1u << P.bits) - 1u, P.n_tiles, ki, row_of, counts, done, out.touched);
         for (int p = 0; p < P.passes; ++p) {
             uint32_t* c = counts + (int64_t)p * P.n_tiles * D;
             uint32_t* next = p + 1 < P.passes ? c + P.n_tiles * D : nullptr;
             if (!fused) id_prefix_kernel<<<D / 32, 256, 0, s>>>(c, P.n_tiles, D, totals);
             auto pass = [&](auto first, auto whole) {
                 auto k = id_scatter_kernel<A, BITS, decltype(first)::value, decltype(whole)::value && BITS == 8>;
-                if (SM > 48 * 1024)
-                    MFM_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, SM), "id sort shared memory");
+                static bool asked[64];
+                if (SM > 48 * 1024) allow_smem(k, device, SM, asked, "id sort shared memory");
                 k<<<g, kETileNT, SM, s>>>(ki, vi, ko, vo, n, P.n_tiles, P.bits * p, P.bits, c, totals, next, out);
             };
             if (p == 0 && fused)

@@ -1147,8 +1147,8 @@ void small_launch(int device, const T* x, int64_t ld, T* out, int64_t ld_out, co
     const int64_t blocks = ceil_div(a.n, kTileRows * (kSmallNT / 32)), most = (int64_t)sm_count(device) * fit;
     auto go = [&](auto w, auto turn) {
         auto k = small_rows_kernel<T, A, decltype(w)::value, decltype(turn)::value, M>;
-        if (bytes > 48 * 1024)
-            MFM_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes), "class tile shared memory");
+        static bool asked[64];
+        if (bytes > 48 * 1024) allow_smem(k, device, 64 * 1024, asked, "class tile shared memory");
         k<<<(unsigned)std::min(blocks, most), kSmallNT, bytes, s>>>(
             x, ld, out, ld_out, a, ld == a.c && (uintptr_t)x % 16 == 0, ld_out == a.c && (uintptr_t)out % 16 == 0);
     };
@@ -1206,7 +1206,8 @@ void rows_launch(int device, const T* x, int64_t ld, T* out, int64_t ld_out, con
     auto ring = [&](auto l) {
         constexpr int L = decltype(l)::value, bytes = ring_slots(L) * L * kRingVecs * 16;
         auto k = ring_rows_kernel<T, A, L>;
-        MFM_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes), "row ring shared memory");
+        static bool asked[64];
+        allow_smem(k, device, bytes, asked, "row ring shared memory");
         const int64_t grid = (int64_t)sm_count(device) * ring_blocks(L);
         k<<<(unsigned)(n < grid ? n : grid), L + 32, bytes, s>>>(x, ld, out, ld_out, a);
     };

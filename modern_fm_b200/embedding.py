@@ -222,7 +222,7 @@ def _grad(grad, ids, n_rows, scale, indptr, alpha, table, dtype, stream, by_rows
         tp, _, _, ld_table = _matrix("table", table)
     dev = _one_device(grad, ids, scale, indptr, table)
     L = _lib.lib()
-    nbytes = L.mfm_embedding_grad_workspace_bytes(code, n, n_rows, d)
+    nbytes = L.mfm_embedding_grad_workspace_bytes(code, 1 if by_rows else 0, n, n_rows, d)
     s, ctx = _on(stream, dev)
     _hold(stream, grad, ids, scale, indptr, table)
     keys = rows = count = whole = d_scale = None
