@@ -311,6 +311,14 @@ int mfm_model_info(const mfm_model* m, int* dtype_used);
 int mfm_model_predict_csr(mfm_model* m, const mfm_csr* x, double* out);
 int mfm_model_predict_device(mfm_model* m, const int64_t* indptr, const int32_t* indices,
                              const void* data, int64_t n_rows, void* out, void* stream);
+/* mfm_model_factors_device: the rows' factor sums, out[b] = sum of x[b, j] V[j] over
+ *   the row's entries (no reference counterpart: its factors stay inside its
+ *   scores), from a DEVICE CSR as mfm_model_predict_device takes it, with nnz
+ *   entries; out (n_rows, k), multiclass (n_rows, C, k), FFM (n_rows, F, k) or
+ *   (n_rows, F, C, k), in data's type. */
+int mfm_model_factors_device(mfm_model* m, const int64_t* indptr, const int32_t* indices,
+                             const void* data, int64_t n_rows, int64_t nnz, void* out,
+                             void* stream);
 void mfm_model_free(mfm_model* m);
 
 /* ---- allocation-free FM scoring --------------------------------------------

@@ -124,6 +124,8 @@ _SIGNATURES = {
     "mfm_model_predict_csr": (ct.c_int, [ct.c_void_p, ct.POINTER(Csr), f64p]),
     "mfm_model_predict_device": (ct.c_int, [ct.c_void_p, ct.c_void_p, ct.c_void_p, ct.c_void_p,
                                             ct.c_int64, ct.c_void_p, ct.c_void_p]),
+    "mfm_model_factors_device": (ct.c_int, [ct.c_void_p, ct.c_void_p, ct.c_void_p, ct.c_void_p,
+                                            ct.c_int64, ct.c_int64, ct.c_void_p, ct.c_void_p]),
     "mfm_model_free": (None, [ct.c_void_p]),
     "mfm_libffm_read": (ct.c_int, [ct.c_char_p, ct.c_int, ct.POINTER(ct.c_void_p)]),
     "mfm_libffm_info": (ct.c_int, [ct.c_void_p, i64p, i64p, i64p]),

@@ -583,7 +583,7 @@ __global__ void __launch_bounds__(kMainNT)
 // The runs that cross chunks: the lane group of the chunk where one begins adds
 // its parts in chunk order and writes the run; the block's groups share a run of
 // more than kLongRun chunks (ids that occur in every row: one chunk per 16 rows).
-constexpr int kLongRun = 8;
+constexpr int kLongRun = 16;
 
 template <class G, class T, class A, class O, int B, int LV>
 __global__ void __launch_bounds__(256)
@@ -612,6 +612,12 @@ __global__ void __launch_bounds__(256)
                 last = c + 1;
 #pragma unroll
                 for (int i = 0; i < 8; ++i) last += last == c + 1 + i && ahead[i] == key ? 1 : 0;
+                for (int64_t r = c + 9; last == r && r - c <= kLongRun; r += 8) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) ahead[i] = r + 1 + i < a.n_chunks ? a.keys[(r + 1 + i) * kChunk] : pad_key;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) last += last == r + i && ahead[i] == key ? 1 : 0;
+                }
             }
         }
         run_last[group] = last;
@@ -619,9 +625,11 @@ __global__ void __launch_bounds__(256)
         if (last - c > kLongRun) long_groups[atomicAdd(&n_long, 1)] = group;
     }
     __syncthreads();
-    auto write = [&](int64_t chunk, A (&acc)[N]) {
-        const uint32_t key = a.keys[chunk * kChunk + kChunk - 1];
-        const int64_t at = a.rows ? a.runs_before(chunk + 1) - 1 : (int64_t)key;
+    // the row of the run that crosses the end of a chunk
+    auto place = [&](int64_t chunk, uint32_t key) {
+        return a.rows ? a.runs_before(chunk + 1) - 1 : (int64_t)key;
+    };
+    auto write = [&](int64_t at, uint32_t key, A (&acc)[N]) {
 #pragma unroll
         for (int j = 0; j < N; ++j) acc[j] *= a.alpha;
         put((a.rows ? a.rows : a.d_table) + at * a.d + col, acc);
@@ -630,23 +638,32 @@ __global__ void __launch_bounds__(256)
     const bool in = col < a.d;
     const int64_t mine = run_last[group];
     if (mine >= 0 && mine - c <= kLongRun && in) {
-        Vec<A, N> p = ldg_vec<A, N>(a.part_tail + c * a.d + col);
+        const uint32_t key = a.keys[c * kChunk + kChunk - 1];
+        const int64_t at = place(c, key);
+        const Vec<A, N> own = ldg_vec<A, N>(a.part_tail + c * a.d + col);
         A acc[N];
 #pragma unroll
-        for (int j = 0; j < N; ++j) acc[j] = p.v[j];
-#pragma unroll 4
-        for (int64_t k = c + 1; k <= mine; ++k) {
-            p = ldg_vec<A, N>(a.part_head + k * a.d + col);
+        for (int j = 0; j < N; ++j) acc[j] = own.v[j];
+        for (int64_t k0 = c + 1; k0 <= mine; k0 += 8) {  // eight parts in flight
+            Vec<A, N> p[8];
 #pragma unroll
-            for (int j = 0; j < N; ++j) acc[j] += p.v[j];
+            for (int k = 0; k < 8; ++k)
+                if (k0 + k <= mine) p[k] = ldg_vec<A, N>(a.part_head + (k0 + k) * a.d + col);
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                if (k0 + k <= mine) {
+#pragma unroll
+                    for (int j = 0; j < N; ++j) acc[j] += p[k].v[j];
+                }
         }
-        write(c, acc);
+        write(at, key, acc);
     }
     for (int i = 0; i < n_long; ++i) {
         const int g = long_groups[i];
         const int64_t from = c0 + g;
         // the run's last chunk: chunks are probed 256 a round by their first key
         const uint32_t key = a.keys[from * kChunk + kChunk - 1];
+        const int64_t at = place(from, key);
         int64_t last = run_last[g], end = a.n_chunks;  // in [last, end)
         while (end - last > 1) {
             const int64_t step = (end - last + 254) / 256;
@@ -684,7 +701,7 @@ __global__ void __launch_bounds__(256)
         if (group == 0 && in) {
 #pragma unroll
             for (int j = 0; j < N; ++j) acc[j] = shared_part[threadIdx.x * N + j];
-            write(from, acc);
+            write(at, key, acc);
         }
         __syncthreads();
     }

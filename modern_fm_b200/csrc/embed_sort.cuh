@@ -227,6 +227,35 @@ __device__ __forceinline__ void warp_ranks(const uint32_t (&digit)[ITEMS], C* cn
     }
 }
 
+// N neighbouring words, four at a time where there are that many.
+template <int N>
+__device__ __forceinline__ void load_many(const uint32_t* p, uint32_t (&v)[N]) {
+    if constexpr (N % 4 == 0) {
+#pragma unroll
+        for (int k = 0; k < N / 4; ++k) {
+            const uint4 x = reinterpret_cast<const uint4*>(p)[k];
+            v[4 * k] = x.x;
+            v[4 * k + 1] = x.y;
+            v[4 * k + 2] = x.z;
+            v[4 * k + 3] = x.w;
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < N; ++k) v[k] = p[k];
+    }
+}
+template <int N>
+__device__ __forceinline__ void store_many(uint32_t* p, const uint32_t (&v)[N]) {
+    if constexpr (N % 4 == 0) {
+#pragma unroll
+        for (int k = 0; k < N / 4; ++k)
+            reinterpret_cast<uint4*>(p)[k] = make_uint4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
+    } else {
+#pragma unroll
+        for (int k = 0; k < N; ++k) p[k] = v[k];
+    }
+}
+
 template <int BITS>
 constexpr int scatter_smem() {  // counts per warp (16 bits), offsets, the tile
     return (kETileNT / 32) * (1 << BITS) * 2 + (1 << BITS) * 4 + kETile * 8;
@@ -279,11 +308,8 @@ __global__ void __launch_bounds__(kETileNT)
             }
         }
     } else {
-#pragma unroll
-        for (int k = 0; k < PT; ++k) {
-            total[k] = totals[t * PT + k];
-            before[k] = counts[tile * D + t * PT + k];
-        }
+        load_many<PT>(totals + t * PT, total);
+        load_many<PT>(counts + tile * D + t * PT, before);
     }
     uint32_t sum = 0, all;
 #pragma unroll
@@ -299,25 +325,27 @@ __global__ void __launch_bounds__(kETileNT)
         digit[i] = q0 + i * 32 < m ? (key[i] >> shift) & mask : 0x80000000u + (uint32_t)lane;
     warp_ranks<kETileItems>(digit, cnt[warp], rank);
     __syncthreads();
-    // the warps' counts -> their prefix over the warps; two 16-bit counts a word
-    // (at most 2048 each: no carry)
+    // the warps' counts -> their prefix over the warps, and the digits' counts in
+    // the tile into base; two 16-bit counts a word (at most 2048 each: no carry),
+    // words 256 apart, so that no two lanes meet in a bank
     uint32_t mine[PT];
     if (PT > 1) {
-        uint32_t run[PT / 2 + 1];
+        constexpr int WT = PT > 1 ? PT / 2 : 1;  // words per thread
 #pragma unroll
-        for (int k = 0; k < PT / 2; ++k) run[k] = 0;
+        for (int k = 0; k < WT; ++k) {
+            const int word = t + k * kETileNT;
+            uint32_t run = 0;
 #pragma unroll
-        for (int w = 0; w < NW; ++w) {
-            uint32_t* row = reinterpret_cast<uint32_t*>(cnt[w] + t * PT);
-#pragma unroll
-            for (int k = 0; k < PT / 2; ++k) {
-                const uint32_t c = row[k];
-                row[k] = run[k];
-                run[k] += c;
+            for (int w = 0; w < NW; ++w) {
+                uint32_t* c = reinterpret_cast<uint32_t*>(cnt[w]) + word;
+                const uint32_t v = *c;
+                *c = run;
+                run += v;
             }
+            reinterpret_cast<uint2*>(base)[word] = make_uint2(run & 0xffffu, run >> 16);
         }
-#pragma unroll
-        for (int k = 0; k < PT; ++k) mine[k] = (run[k / 2] >> (k & 1 ? 16 : 0)) & 0xffffu;
+        __syncthreads();
+        load_many<PT>(base + t * PT, mine);
     } else {
         uint32_t run = 0;
 #pragma unroll
@@ -336,16 +364,17 @@ __global__ void __launch_bounds__(kETileNT)
 #pragma unroll
     for (int k = 0; k < PT; ++k) {
         first[k] = start;
-        base[t * PT + k] = start;
         start += mine[k];
     }
+    store_many<PT>(base + t * PT, first);
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < kETileItems; ++i)
         if (q0 + i * 32 < m) skv[base[digit[i]] + cnt[warp][digit[i]] + rank[i]] = make_uint2(key[i], val[i]);
     __syncthreads();
 #pragma unroll
-    for (int k = 0; k < PT; ++k) base[t * PT + k] = before[k] - first[k];  // output place less tile place
+    for (int k = 0; k < PT; ++k) before[k] -= first[k];  // output place less tile place
+    store_many<PT>(base + t * PT, before);
     __syncthreads();
     uint32_t dst[kETileItems];
     uint2 e[kETileItems];

@@ -1320,6 +1320,28 @@ extern "C" int mfm_model_predict_device(mfm_model* h, const int64_t* indptr,
     });
 }
 
+extern "C" int mfm_model_factors_device(mfm_model* h, const int64_t* indptr,
+                                        const int32_t* indices, const void* data, int64_t n_rows,
+                                        int64_t nnz, void* out, void* stream) {
+    return guarded([&] {
+        if (!h) fail(MFM_ERR_INVALID, "null model handle");
+        if (!h->ready) fail(MFM_ERR_INVALID, "model parameters are not set");
+        if (n_rows < 0 || nnz < 0) fail(MFM_ERR_INVALID, "negative CSR size");
+        if (n_rows == 0) return;
+        if (!indptr || !out || (nnz > 0 && (!indices || !data)))
+            fail(MFM_ERR_INVALID, "indptr, indices, data and out must be provided");
+        const DevModel& m = h->m;
+        const Mode md = mode_of(h->dtype, m);
+        // one row of the table per feature: every factor of every class (and field)
+        const int64_t d = m.C * m.k * (m.model == Model::FFM ? m.F : 1);
+        const int dtype = md == Mode::F32 ? MFM_DTYPE_F32 : md == Mode::F32_F64 ? MFM_DTYPE_F32_F64 : MFM_DTYPE_F64;
+        const void* v = md == Mode::F64 ? (const void*)m.v64.ptr : (const void*)m.v32.ptr;
+        const int rc = mfm_embedding_lookup_device(dtype, m.device, 0, indices, nnz, indptr, n_rows, data,
+                                                   1.0, v, m.n_features, d, d, out, d, stream);
+        if (rc != MFM_OK) fail(rc, mfm_last_error());
+    });
+}
+
 extern "C" void mfm_model_free(mfm_model* h) {
     if (!h) return;
     DeviceGuard guard(h->m.device);

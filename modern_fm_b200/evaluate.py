@@ -7,7 +7,9 @@ and FwFM estimators (python/modern_fm/ffm.py:210-212,
 python/modern_fm/fwfm.py:157-161), metric from python/modern_fm/losses.py.
 ``fm_eval_device`` / ``ffm_eval_device`` / ``fwfm_eval_device`` compute the
 same value from a device-resident validation CSR and device-resident
-parameters; only the scalar loss leaves the GPU.
+parameters; only the scalar loss leaves the GPU. ``preference_eval_device`` and
+``policy_eval_device`` do so for a resident softmax model (``DeviceModel``) and the
+losses of ``preference``.
 """
 
 from __future__ import annotations
@@ -139,3 +141,43 @@ def fwfm_eval_device(indptr, indices, data, field_ids, w0: float, w, v, r, y,
         sample_weight.data_ptr() if sample_weight is not None else None,
         _lib.LOSSES[loss], float(label_smoothing), ct.byref(out), _stream(stream, dev))
     return _finish(rc, out)
+
+
+def preference_eval_device(model, indptr, indices, data, labels, bounds, reference,
+                           beta: float = 0.1, label_smoothing: float = 0.0, sample_weight=None,
+                           stream=None) -> float:
+    """Preference loss of a resident softmax model on a validation set: the class
+    scores of a canonical device CSR (``DeviceModel.scores_device``) and
+    ``preference.preference_loss`` over the sequences of rows that ``bounds`` gives,
+    without the gradient; arguments as there."""
+    from .preference import preference_loss
+
+    scores = _class_scores(model, indptr, indices, data, stream)
+    r = preference_loss(scores, labels, bounds, reference, beta, label_smoothing, sample_weight,
+                        with_grad=False, stream=stream)
+    return _value(r.loss, stream)
+
+
+def policy_eval_device(model, indptr, indices, data, labels, old_logprobs, advantages,
+                       reference=None, clip_low: float = 0.2, clip_high: float = 0.2,
+                       kl_coef: float = 0.0, sample_weight=None, stream=None) -> float:
+    """Clipped policy loss of a resident softmax model on logged rows, as
+    ``preference_eval_device``; arguments as in ``preference.policy_loss``."""
+    from .preference import policy_loss
+
+    scores = _class_scores(model, indptr, indices, data, stream)
+    r = policy_loss(scores, labels, old_logprobs, advantages, reference, clip_low, clip_high,
+                    kl_coef, sample_weight, with_grad=False, stream=stream)
+    return _value(r.loss, stream)
+
+
+def _class_scores(model, indptr, indices, data, stream):
+    if model.n_classes < 2:
+        raise ValueError("these losses need a model with n_classes >= 2")
+    return model.scores_device(indptr, indices, data, stream)
+
+
+def _value(loss, stream):
+    if stream is not None:
+        stream.synchronize()
+    return float(loss)

@@ -114,6 +114,66 @@ class DeviceModel:
                                                    s.cuda_stream))
         return out
 
+    def _device_csr(self, indptr, indices, data):
+        """The torch dtype of scores and factors; checks a device CSR of the compute layout."""
+        import torch
+
+        kind = torch.float32 if self._dtype == _lib.MFM_DTYPE_F32 else torch.float64
+        for name, t, want in (("indptr", indptr, torch.int64), ("indices", indices, torch.int32),
+                              ("data", data, kind)):
+            if (not t.is_cuda or t.get_device() != self.device or t.dtype != want
+                    or not t.is_contiguous() or t.dim() != 1):
+                raise ValueError(f"{name} must be a contiguous 1-D {want} tensor on "
+                                 f"cuda:{self.device}")
+        if indptr.numel() < 1 or indices.numel() != data.numel():
+            raise ValueError("indptr must have length n_rows + 1 (>= 1), and indices and data "
+                             "the same length")
+        return kind
+
+    def scores_device(self, indptr, indices, data, stream=None):
+        """``predict_device`` into a new tensor: (n_rows,) scores, or (n_rows, n_classes)."""
+        import torch
+
+        kind = self._device_csr(indptr, indices, data)
+        n = indptr.numel() - 1
+        with torch.cuda.stream(stream):
+            out = indptr.new_empty((n,) if self.n_classes == 1 else (n, self.n_classes),
+                                   dtype=kind)
+        return self.predict_device(indptr, indices, data, out, stream)
+
+    def factors_device(self, indptr, indices, data, stream=None):
+        """The rows' factor sums, ``sum of x[b, j] V[j]`` over the entries of row b: a
+        row's place in the latent space (two rows' inner product is their part of
+        the pairwise score), e.g. for nearest-neighbour retrieval. A canonical
+        device CSR as ``predict_device`` takes it; returns a CUDA tensor (n_rows, k),
+        multiclass (n_rows, C, k), FFM (n_rows, F, k) or (n_rows, F, C, k), float32
+        for dtype float32, float64 otherwise (summed in that type)."""
+        import torch
+
+        kind = self._device_csr(indptr, indices, data)
+        n = indptr.numel() - 1
+        shape = (n,) + ((self.n_fields,) if self.kind == "ffm" else ()) + (
+            (self.n_classes,) if self.n_classes > 1 else ()) + (self.k,)
+        s = stream if stream is not None else torch.cuda.current_stream(self.device)
+        with torch.cuda.stream(stream):
+            out = indptr.new_empty(shape, dtype=kind)
+        _check(_lib.lib().mfm_model_factors_device(
+            self._h, indptr.data_ptr(), indices.data_ptr(), data.data_ptr(), n, data.numel(),
+            out.data_ptr(), s.cuda_stream))
+        return out
+
+    def label_logprobs_device(self, indptr, indices, data, labels, bounds=None, stream=None):
+        """Log-probabilities of the rows' labels under the softmax of this model's class
+        scores (``preference.label_logprobs`` of ``scores_device``): the reference of
+        the preference loss (with ``bounds``, the sequences' indptr) and the old
+        log-probabilities of the policy loss."""
+        from .preference import label_logprobs
+
+        if self.n_classes < 2:
+            raise ValueError("label log-probabilities need a model with n_classes >= 2")
+        return label_logprobs(self.scores_device(indptr, indices, data, stream), labels, bounds,
+                              stream)
+
     def close(self):
         if getattr(self, "_h", None):
             _lib.lib().mfm_model_free(self._h)
