@@ -237,6 +237,7 @@ __global__ void __launch_bounds__(kTileChunks)
                        int64_t n_chunks, uint32_t* __restrict__ base,
                        uint32_t* __restrict__ tile_base, unsigned* __restrict__ done,
                        int64_t* __restrict__ count) {
+    after_previous();
     __shared__ uint32_t sm[kTileChunks / 32];
     __shared__ unsigned last;
     const int64_t c = (int64_t)blockIdx.x * kTileChunks + threadIdx.x, e0 = c * kChunk;
@@ -327,12 +328,13 @@ struct GradArgs {
     const uint32_t *keys, *srows;
     const A* scales;
     const int32_t* row_of;  // by position
-    const uint32_t* touched;  // bits of the touched table rows, or NULL: search the keys
+    Fill fill, fill_late;  // the main kernel's part of the untouched rows, the last one's
     const uint32_t *base, *tile_base;
     A *part_head, *part_tail;
     int64_t n_chunks;
     unsigned reduce_blocks, scale_blocks, fill_blocks;  // of the main kernel
     int fill_per;                                       // rows per warp that fills
+    unsigned cross_blocks;
     __device__ __forceinline__ int64_t runs_before(int64_t c) const {
         return (int64_t)tile_base[c / kTileChunks] + base[c];
     }
@@ -429,60 +431,29 @@ __device__ __forceinline__ void reduce_chunk(const GradArgs<G, T, A, O>& a, int6
 // a search among the sorted keys), or the places behind the last touched row.
 // Each row of the result is written once.
 template <class G, class T, class A, class O>
-__device__ __forceinline__ void fill_rest(const GradArgs<G, T, A, O>& a, int per, int64_t warp,
-                                          int64_t n_warps) {
-    const int lane = threadIdx.x & 31;
-    auto clear = [&](O* row) {
-        const int64_t bytes = a.d * (int64_t)sizeof(O);
-        char* p = reinterpret_cast<char*>(row);
-        if (bytes % 16 == 0 && (uintptr_t)p % 16 == 0) {
-            for (int64_t i = lane; i < bytes / 16; i += 32) reinterpret_cast<uint4*>(p)[i] = make_uint4(0, 0, 0, 0);
+__device__ __forceinline__ void fill_rest(const GradArgs<G, T, A, O>& a, unsigned block) {
+    if (a.fill.touched) {
+        fill_untouched(a.fill, block);
+        return;
+    }
+    const int lane = threadIdx.x & 31, per = a.fill_per;
+    const int64_t warp = (int64_t)block * (kMainNT / 32) + threadIdx.x / 32, warps = (int64_t)a.fill_blocks * (kMainNT / 32);
+    const int64_t n = a.in.n, n_rows = a.in.n_rows, bytes = a.d * (int64_t)sizeof(O);
+    char* const base = reinterpret_cast<char*>(a.rows ? a.rows : a.d_table);
+    const bool vec = bytes % 16 == 0 && (uintptr_t)base % 16 == 0;
+    const int64_t first = a.rows ? *a.count : 0, end = a.rows ? (n < n_rows ? n : n_rows) : n_rows;
+    for (int64_t r0 = first + warp * per; r0 < end; r0 += warps * per) {
+        const int rows = (int)(r0 + per < end ? per : end - r0);
+        unsigned touched = 0;
+        if (a.rows) {
+            if (lane < rows) a.keys_out.put(r0 + lane, -1);
         } else {
-            for (int64_t i = lane; i < a.d; i += 32) row[i] = narrow<O>(A(0));
+            int64_t lo, hi;
+            warp_range(a.keys, n, (uint32_t)r0, (uint32_t)(r0 + rows), lo, hi);
+            for (int64_t i = lo + lane; i < hi; i += 32) touched |= 1u << (a.keys[i] - (uint32_t)r0);
+            touched = __reduce_or_sync(0xffffffffu, touched);
         }
-    };
-    if (a.rows) {
-        const int64_t used = *a.count, cap = a.in.n < a.in.n_rows ? a.in.n : a.in.n_rows;
-        for (int64_t r0 = used + warp * per; r0 < cap; r0 += n_warps * per) {
-            const int m = (int)(cap - r0 < per ? cap - r0 : per);
-            if (lane < m) a.keys_out.put(r0 + lane, -1);
-            if (a.d * (int64_t)sizeof(O) >= 512) {
-                for (int i = 0; i < m; ++i) clear(a.rows + (r0 + i) * a.d);
-            } else {  // short rows: together one stretch
-                O* at = a.rows + r0 * a.d;
-                const int64_t total = m * a.d;
-                if (total * sizeof(O) % 16 == 0 && (uintptr_t)at % 16 == 0) {
-                    for (int64_t i = lane; i < total * (int64_t)sizeof(O) / 16; i += 32)
-                        reinterpret_cast<uint4*>(at)[i] = make_uint4(0, 0, 0, 0);
-                } else {
-                    for (int64_t i = lane; i < total; i += 32) at[i] = narrow<O>(A(0));
-                }
-            }
-        }
-    } else {
-        const int64_t n = a.in.n, n_rows = a.in.n_rows, bytes = a.d * (int64_t)sizeof(O);
-        const bool vec = bytes % 16 == 0 && (uintptr_t)a.d_table % 16 == 0;
-        for (int64_t r0 = warp * per; r0 < n_rows; r0 += n_warps * per) {
-            const int rows = (int)(r0 + per < n_rows ? per : n_rows - r0);
-            unsigned touched = 0;
-            if (a.touched) {  // per divides 32
-                touched = a.touched[r0 / 32] >> (r0 & 31);
-            } else {
-                int64_t lo, hi;
-                warp_range(a.keys, n, (uint32_t)r0, (uint32_t)(r0 + rows), lo, hi);
-                for (int64_t i = lo + lane; i < hi; i += 32) touched |= 1u << (a.keys[i] - (uint32_t)r0);
-                touched = __reduce_or_sync(0xffffffffu, touched);
-            }
-            O* at = a.d_table + r0 * a.d;
-            if (vec && bytes <= 1024) {  // the rows' vectors as one stretch
-                const unsigned vr = (unsigned)(bytes / 16), total = (unsigned)rows * vr;
-                for (unsigned i = lane; i < total; i += 32)
-                    if (!(touched >> (i / vr) & 1u)) reinterpret_cast<uint4*>(at)[i] = make_uint4(0, 0, 0, 0);
-            } else {
-                for (unsigned m = ~touched & (rows == 32 ? 0xffffffffu : (1u << rows) - 1u); m; m &= m - 1)
-                    clear(at + (__ffs(m) - 1) * a.d);
-            }
-        }
+        clear_rows(base + r0 * bytes, bytes, rows, touched, vec);
     }
 }
 
@@ -555,6 +526,7 @@ __device__ __forceinline__ void scale_entries(const GradArgs<G, T, A, O>& a, int
 template <class G, class T, class A, class O, int B, int LV>
 __global__ void __launch_bounds__(kMainNT)
     embed_main_kernel(const GradArgs<G, T, A, O> a, int slabs) {
+    after_previous();
     constexpr int N = Lane<G, B>::N, GR = kMainNT / LV;
     const int lane = threadIdx.x % LV, group = threadIdx.x / LV;
     const unsigned work = a.reduce_blocks + a.scale_blocks;
@@ -569,8 +541,7 @@ __global__ void __launch_bounds__(kMainNT)
         fill = work <= a.fill_blocks;
     }
     if (fill) {
-        fill_rest(a, a.fill_per, (int64_t)b * (kMainNT / 32) + threadIdx.x / 32,
-                  (int64_t)a.fill_blocks * (kMainNT / 32));
+        fill_rest(a, b);
     } else if (b < a.reduce_blocks) {
         const int64_t c = (int64_t)(b / slabs) * GR + group;
         const int64_t col = ((int64_t)(b % slabs) * LV + lane) * N;
@@ -587,14 +558,19 @@ constexpr int kLongRun = 16;
 
 template <class G, class T, class A, class O, int B, int LV>
 __global__ void __launch_bounds__(256)
-    embed_cross_kernel(const GradArgs<G, T, A, O> a) {
+    embed_cross_kernel(const GradArgs<G, T, A, O> a, int slabs) {
+    after_previous();
+    if (blockIdx.x >= a.cross_blocks) {
+        fill_untouched(a.fill_late, blockIdx.x - a.cross_blocks);
+        return;
+    }
     constexpr int N = Lane<G, B>::N, GR = 256 / LV;
     __shared__ int64_t run_last[GR];  // last chunk of the run begun in the group's chunk, -1: none
     __shared__ int long_groups[GR], n_long;
     __shared__ A shared_part[256 * N];
     const int lane = threadIdx.x % LV, group = threadIdx.x / LV;
-    const int64_t c0 = (int64_t)blockIdx.x * GR, c = c0 + group, n = a.in.n;
-    const int64_t col = ((int64_t)blockIdx.y * LV + lane) * N;
+    const int64_t c0 = (int64_t)(blockIdx.x / slabs) * GR, c = c0 + group;
+    const int64_t col = ((int64_t)(blockIdx.x % slabs) * LV + lane) * N;
     const uint32_t pad_key = (uint32_t)a.in.n_rows;
     if (threadIdx.x == 0) n_long = 0;
     __syncthreads();
@@ -848,9 +824,33 @@ void grad_launch(int device, GradArgs<G, T, A, O>& a, const GradWs& W, char* ws,
     SortedOut<A> sorted{};
     sorted.scale = a.scale;
     sorted.scales = reinterpret_cast<A*>(ws + W.off_scale);
-    if (a.d_table && n > kSmallSort) sorted.touched = reinterpret_cast<uint32_t*>(ws + W.off_bits);
-    a.touched = sorted.touched;
-    sort_ids(device, W.sort, a.in, row_of, done, words, sorted, s);
+    // a warp fills 32 rows, or fewer where the rows are long
+    const int64_t bytes = a.d * (int64_t)sizeof(O), sm = sm_count(device);
+    a.fill_per = 32;
+    while (a.fill_per > 4 && a.fill_per * bytes > 32768) a.fill_per /= 2;
+    // The untouched rows in parts: the launches behind the first pass take two shares
+    // each, the main one, whose sums take bandwidth too, one (16384 x 2048 tokens into
+    // 32000 rows: 81 us of kernels; 87 us with all of it in the main launch).
+    Fill parts[6] = {};
+    uint32_t* bits = nullptr;
+    const bool late = nc > 1;
+    if (a.d_table && n > kSmallSort) {
+        bits = reinterpret_cast<uint32_t*>(ws + W.off_bits);
+        const int early = W.sort.passes - 1, shares = 2 * early + 1 + (late ? 2 : 0);
+        const int64_t groups = ceil_div(a.in.n_rows, 32);
+        int64_t lo = 0;
+        for (int i = 0, k = 0; i < early + 1 + (late ? 1 : 0); ++i) {
+            k += i == early ? 1 : 2;
+            const int64_t hi = std::min(a.in.n_rows, groups * k / shares * 32);
+            const int64_t warps = ceil_div(hi - lo, (int64_t)a.fill_per);
+            parts[i] = Fill{reinterpret_cast<char*>(a.d_table), bytes, lo, k == shares ? a.in.n_rows : hi, bits, a.fill_per, 0u};
+            parts[i].blocks = (unsigned)std::min<int64_t>(ceil_div(warps, i == early ? kMainNT / 32 : 8), sm * (i == early ? 16 : 4));
+            lo = hi;
+        }
+        a.fill = parts[early];
+        if (late) a.fill_late = parts[early + 1];
+    }
+    sort_ids(device, W.sort, a.in, row_of, done, words, sorted, bits, parts, s);
     a.keys = sorted.keys;
     a.srows = sorted.rows;
     a.scales = a.scale ? sorted.scales : nullptr;
@@ -861,26 +861,24 @@ void grad_launch(int device, GradArgs<G, T, A, O>& a, const GradWs& W, char* ws,
     if (a.rows) {
         uint32_t* base = reinterpret_cast<uint32_t*>(ws + W.off_base);
         uint32_t* tiles = reinterpret_cast<uint32_t*>(ws + W.off_tile);
-        chunk_heads_kernel<<<(unsigned)ceil_div(nc, kTileChunks), kTileChunks, 0, s>>>(
-            a.keys, n, (uint32_t)a.in.n_rows, nc, base, tiles, done, a.count);
+        launch_next(chunk_heads_kernel, (unsigned)ceil_div(nc, kTileChunks), kTileChunks, 0, s,
+                    a.keys, n, (uint32_t)a.in.n_rows, nc, base, tiles, done, a.count);
         a.base = base;
         a.tile_base = tiles;
     }
     with_lanes(dv, [&](auto lv) {
         constexpr int LV = decltype(lv)::value;
-        const int64_t slabs = ceil_div(dv, LV), sm = sm_count(device);
+        const int64_t slabs = ceil_div(dv, LV);
         a.reduce_blocks = (unsigned)(ceil_div(nc, kMainNT / LV) * slabs);
         a.scale_blocks = a.d_scale ? (unsigned)ceil_div(n, kMainNT / LV * kScaleEntries) : 0u;
         const int64_t rest = a.rows ? std::min(n, a.in.n_rows) : a.in.n_rows;
-        // a warp fills 32 rows, or fewer where the rows are long
-        a.fill_per = 32;
-        while (a.fill_per > 4 && a.fill_per * a.d * (int64_t)sizeof(O) > 32768) a.fill_per /= 2;
-        a.fill_blocks = (unsigned)std::min<int64_t>(ceil_div(rest, (int64_t)a.fill_per * (kMainNT / 32)), sm * 16);
-        embed_main_kernel<G, T, A, O, B, LV>
-            <<<a.reduce_blocks + a.scale_blocks + a.fill_blocks, kMainNT, 0, s>>>(a, (int)slabs);
-        if (nc > 1) {
-            const dim3 g((unsigned)ceil_div(nc, 256 / LV), (unsigned)slabs);
-            embed_cross_kernel<G, T, A, O, B, LV><<<g, 256, 0, s>>>(a);
+        a.fill_blocks = bits ? a.fill.blocks
+                             : (unsigned)std::min<int64_t>(ceil_div(rest, (int64_t)a.fill_per * (kMainNT / 32)), sm * 16);
+        launch_next(embed_main_kernel<G, T, A, O, B, LV>, a.reduce_blocks + a.scale_blocks + a.fill_blocks,
+                    kMainNT, 0, s, a, (int)slabs);
+        if (late) {
+            a.cross_blocks = (unsigned)(ceil_div(nc, 256 / LV) * slabs);
+            launch_next(embed_cross_kernel<G, T, A, O, B, LV>, a.cross_blocks + a.fill_late.blocks, 256, 0, s, a, (int)slabs);
         }
     });
     MFM_CHECK_LAUNCH("embedding gradient launch");

@@ -103,6 +103,48 @@ struct Entries {
     }
 };
 
+// Zeros for the rows [lo, hi) of a table of `bytes` a row whose bits in `touched`
+// are clear: the rows of a gradient that no id touches. A warp takes `per` rows
+// (which divides 32) at a time. It only needs the first pass's bits, so its
+// blocks ride along in the launches behind that, which are bound by latency.
+struct Fill {
+    char* base;
+    int64_t bytes, lo, hi;
+    const uint32_t* touched;
+    int per;
+    unsigned blocks;
+};
+
+__device__ __forceinline__ void clear_row(char* p, int64_t bytes, bool vec) {
+    const int lane = threadIdx.x & 31;
+    if (vec) {
+        for (int64_t i = lane; i < bytes / 16; i += 32) reinterpret_cast<uint4*>(p)[i] = make_uint4(0, 0, 0, 0);
+    } else {  // whole elements of at least two bytes
+        for (int64_t i = lane; i < bytes / 2; i += 32) reinterpret_cast<uint16_t*>(p)[i] = 0;
+    }
+}
+
+__device__ __forceinline__ void clear_rows(char* at, int64_t bytes, int rows, unsigned touched, bool vec) {
+    const int lane = threadIdx.x & 31;
+    if (vec && bytes <= 1024) {  // the rows' vectors as one stretch
+        const unsigned vr = (unsigned)(bytes / 16), total = (unsigned)rows * vr;
+        for (unsigned i = lane; i < total; i += 32)
+            if (!(touched >> (i / vr) & 1u)) reinterpret_cast<uint4*>(at)[i] = make_uint4(0, 0, 0, 0);
+    } else {
+        for (unsigned m = ~touched & (rows == 32 ? 0xffffffffu : (1u << rows) - 1u); m; m &= m - 1)
+            clear_row(at + (__ffs(m) - 1) * bytes, bytes, vec);
+    }
+}
+
+__device__ __forceinline__ void fill_untouched(const Fill& f, unsigned block) {
+    const bool vec = f.bytes % 16 == 0 && (uintptr_t)f.base % 16 == 0;
+    const int64_t warps = (int64_t)f.blocks * (blockDim.x / 32);
+    for (int64_t r = f.lo + ((int64_t)block * (blockDim.x / 32) + threadIdx.x / 32) * f.per; r < f.hi; r += warps * f.per) {
+        const int rows = (int)(r + f.per < f.hi ? f.per : f.hi - r);
+        clear_rows(f.base + r * f.bytes, f.bytes, rows, f.touched[r / 32] >> (r & 31), vec);
+    }
+}
+
 // What the last pass writes beside a key: the row and scale of the entry at
 // position p (row_of NULL: the position itself; scale NULL: none).
 template <class A>
@@ -113,7 +155,6 @@ struct SortedOut {
     const int32_t* row_of;
     const A* scale;
     uint32_t pad_key;
-    uint32_t* touched;  // one bit per table row, set for every real key; NULL: not wanted
     __device__ __forceinline__ void load(uint32_t p, uint32_t& row, A& s) const {
         row = row_of ? (uint32_t)row_of[p] : p;
         s = scale ? scale[p] : A(1);
@@ -168,6 +209,7 @@ __global__ void __launch_bounds__(kETileNT)
 __global__ void __launch_bounds__(256)
     id_prefix_kernel(uint32_t* __restrict__ counts, int64_t n_tiles, int digits,
                      uint32_t* __restrict__ totals) {
+    after_previous();
     constexpr int F = 20;  // counts in flight
     __shared__ uint32_t part[8][33];
     const int lane = threadIdx.x & 31, g = threadIdx.x / 32, d = blockIdx.x * 32 + lane;
@@ -271,7 +313,12 @@ __global__ void __launch_bounds__(kETileNT)
                       uint32_t* __restrict__ kout, uint32_t* __restrict__ vout, int64_t n,
                       int64_t n_tiles, int shift, int bits, const uint32_t* __restrict__ counts,
                       const uint32_t* __restrict__ totals, uint32_t* __restrict__ next,
-                      SortedOut<A> out) {
+                      SortedOut<A> out, uint32_t* __restrict__ touched, Fill fill) {
+    after_previous();
+    if (!FIRST && blockIdx.x >= n_tiles) {
+        fill_untouched(fill, blockIdx.x - (unsigned)n_tiles);
+        return;
+    }
     constexpr int NW = kETileNT / 32, D = 1 << BITS, PT = D / kETileNT;  // digits per thread
     extern __shared__ uint4 scatter_mem[];
     uint16_t(*cnt)[D] = reinterpret_cast<uint16_t(*)[D]>(scatter_mem);
@@ -384,6 +431,20 @@ __global__ void __launch_bounds__(kETileNT)
         e[u] = j < m ? skv[j] : make_uint2(0, 0);
         dst[u] = base[(e[u].x >> shift) & mask] + (uint32_t)j;
     }
+    if (FIRST && touched) {
+        // popular ids share their words: the bit is looked at first, so that few
+        // of their entries get as far as the atomic
+        uint32_t seen[kETileItems];
+#pragma unroll
+        for (int u = 0; u < kETileItems; ++u) {
+            const int j = t + u * kETileNT;
+            const bool want = j < m && e[u].x != out.pad_key && (j == 0 || skv[j - 1].x != e[u].x);
+            seen[u] = want ? __ldcg(touched + e[u].x / 32) : 0xffffffffu;
+        }
+#pragma unroll
+        for (int u = 0; u < kETileItems; ++u)
+            if (!(seen[u] >> (e[u].x & 31) & 1u)) atomicOr(touched + e[u].x / 32, 1u << (e[u].x & 31));
+    }
     if (next) {
 #pragma unroll
         for (int u = 0; u < kETileItems; ++u) {
@@ -406,11 +467,7 @@ __global__ void __launch_bounds__(kETileNT)
 #pragma unroll
         for (int u = 0; u < kETileItems; ++u)
             if (t + u * kETileNT < m) {
-                const int j = t + u * kETileNT;
                 out.store(dst[u], e[u].x, row[u], s[u]);
-                // the tile holds equal keys together: one bit operation a run
-                if (out.touched && e[u].x != out.pad_key && (j == 0 || skv[j - 1].x != e[u].x))
-                    atomicOr(out.touched + e[u].x / 32, 1u << (e[u].x & 31));
             }
         if (tile == 0 && t < kSortPad) out.store(n + t, out.pad_key, 0u, A(0));
     }
@@ -515,11 +572,12 @@ struct IdSortPlan {
 };
 
 // Sorts the batch's keys into out.keys with the entries' rows and scales (out's
-// keys and rows are set here, in the workspace); writes row_of (with indptr) and
-// clears *done.
+// keys and rows are set here, in the workspace); writes row_of (with indptr),
+// clears *done and sets the touched rows' bits. The launch of pass p >= 1 fills
+// fills[p - 1].
 template <class A>
 void sort_ids(int device, const IdSortPlan& P, const Entries& in, int32_t* row_of, unsigned* done,
-              uint32_t* ws, SortedOut<A>& out, cudaStream_t s) {
+              uint32_t* ws, SortedOut<A>& out, uint32_t* touched, const Fill* fills, cudaStream_t s) {
     const int64_t n = P.n;
     uint32_t* counts = ws + 4 * P.pitch;
     out.keys = ws;
@@ -550,16 +608,17 @@ void sort_ids(int device, const IdSortPlan& P, const Entries& in, int32_t* row_o
         const bool fused = BITS == 8 && P.n_tiles <= kFuseTiles;
         uint32_t *ki = P.passes % 2 ? k1 : k0, *vi = P.passes % 2 ? v1 : v0;
         uint32_t *ko = P.passes % 2 ? k0 : k1, *vo = P.passes % 2 ? v0 : v1;
-        id_count_kernel<BITS><<<g, kETileNT, 0, s>>>(in, P.passes, (1u << P.bits) - 1u, P.n_tiles, ki, row_of, counts, done, out.touched);
+        id_count_kernel<BITS><<<g, kETileNT, 0, s>>>(in, P.passes, (1u << P.bits) - 1u, P.n_tiles, ki, row_of, counts, done, touched);
         for (int p = 0; p < P.passes; ++p) {
             uint32_t* c = counts + (int64_t)p * P.n_tiles * D;
             uint32_t* next = p + 1 < P.passes ? c + P.n_tiles * D : nullptr;
-            if (!fused) id_prefix_kernel<<<D / 32, 256, 0, s>>>(c, P.n_tiles, D, totals);
+            if (!fused) launch_next(id_prefix_kernel, D / 32, 256, 0, s, c, P.n_tiles, D, totals);
             auto pass = [&](auto first, auto whole) {
                 auto k = id_scatter_kernel<A, BITS, decltype(first)::value, decltype(whole)::value && BITS == 8>;
                 static bool asked[64];
                 if (SM > 48 * 1024) allow_smem(k, device, SM, asked, "id sort shared memory");
-                k<<<g, kETileNT, SM, s>>>(ki, vi, ko, vo, n, P.n_tiles, P.bits * p, P.bits, c, totals, next, out);
+                const Fill fill = p > 0 ? fills[p - 1] : Fill{};
+                launch_next(k, g + fill.blocks, kETileNT, SM, s, ki, vi, ko, vo, n, P.n_tiles, P.bits * p, P.bits, c, totals, next, out, touched, fill);
             };
             if (p == 0 && fused)
                 pass(std::true_type{}, std::true_type{});

@@ -163,6 +163,31 @@ inline bool vec_ok(const void* p, int64_t ld, size_t size, int vec) {
     return ((uintptr_t)p % (size * vec)) == 0 && (ld % vec) == 0;
 }
 
+// Programmatic dependent launch: a kernel launched by launch_next may be scheduled
+// while its predecessor in the stream drains. after_previous, its first
+// statement, waits for the predecessor to be complete and visible, and lets the
+// successor be scheduled in turn. A chain of four to eight short kernels is
+// spent on launch gaps to a tenth.
+__device__ __forceinline__ void after_previous() {
+    asm volatile("griddepcontrol.wait;\ngriddepcontrol.launch_dependents;" ::: "memory");
+}
+
+template <class... KArgs, class... Args>
+void launch_next(void (*kernel)(KArgs...), unsigned grid, unsigned block, size_t smem, cudaStream_t s,
+                 Args&&... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(block);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    MFM_CUDA(cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...), "kernel launch");
+}
+
 template <class F>
 void with_index_type(int ids64, F&& f) {
     if (ids64)
