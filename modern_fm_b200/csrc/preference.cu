@@ -276,6 +276,7 @@ __device__ __forceinline__ double block_sum(double v, double* sm) {
 
 template <class A>
 __device__ __forceinline__ double weight_total(const RowArgs<A>& a) {  // on every lane
+    wait_previous();
     double total = 0.0;
     for (int i = threadIdx.x & 31; i < a.n_wpart; i += 32) total += a.wpart[i];
     return warp_sum(total);
@@ -389,7 +390,7 @@ __global__ void __launch_bounds__(kSmallNT, IsF64<A>::value || CW > 16 ? 4 : kSm
     const int c = (int)a.c, lane = threadIdx.x & 31;
     T* const tiles = reinterpret_cast<T*>(small_smem) + (threadIdx.x / 32) * (2 * kTileRows * c);
     const int first = TURN ? first_column<T>(c) : 0;
-    const double total = M == POLICY ? weight_total(a) : 0.0, inv = inverse(total);
+    if (M == GRAD) wait_previous();
     const double scale = M == GRAD && a.scale ? *a.scale : 1.0;
     double e[3] = {0.0, 0.0, 0.0};
     const int64_t n_tiles = ceil_div(a.n, (int64_t)kTileRows), step = (int64_t)gridDim.x * (kSmallNT / 32);
@@ -416,6 +417,7 @@ __global__ void __launch_bounds__(kSmallNT, IsF64<A>::value || CW > 16 ? 4 : kSm
         inputs(begin(tile));
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
+    const double total = M == POLICY ? weight_total(a) : 0.0, inv = inverse(total);
     for (int buf = 0; tile < n_tiles; tile += step, buf ^= 1) {
         const int64_t t0 = begin(tile), t = t0 + lane;
         const int rows = rows_of(t0), y_now = y;
@@ -567,6 +569,7 @@ __global__ void __launch_bounds__(kNT, cached_blocks<A>(K))
     constexpr int E = (2 * (V - 1) + L - 1) / L;             // edge elements per lane
     __shared__ double sums[kNT / 32];
     const int lane = threadIdx.x % L;
+    if (M == GRAD) wait_previous();
     const double total = M == POLICY ? weight_total(a) : 0.0, inv = inverse(total);
     const double scale = M == GRAD && a.scale ? *a.scale : 1.0;
     double e[3] = {0.0, 0.0, 0.0};
@@ -951,6 +954,7 @@ template <class T, class A, int L>
 __global__ void __launch_bounds__(kNT)
     label_grad_kernel(const T* __restrict__ x, int64_t ld, T* __restrict__ out, int64_t ld_out,
                       RowArgs<A> a) {
+    wait_previous();
     constexpr int V = 16 / sizeof(T), U = 4;
     const int lane = threadIdx.x % L;
     const int64_t t = a.n - 1 - ((int64_t)blockIdx.x * (kNT / L) + threadIdx.x / L);
@@ -1028,6 +1032,7 @@ __global__ void __launch_bounds__(kNT)
                 const A* __restrict__ weight, A* __restrict__ margins, A* __restrict__ sums,
                 double* __restrict__ pair_loss, A* __restrict__ g, unsigned* __restrict__ done,
                 A* __restrict__ loss, double* __restrict__ scale) {
+    after_previous();
     __shared__ double sm[kNT / 32];
     __shared__ unsigned last;
     const int64_t p = (int64_t)blockIdx.x * (kNT / W) + threadIdx.x / W;
@@ -1088,6 +1093,7 @@ template <class A>
 __global__ void __launch_bounds__(kNT)
     weight_kernel(Labels labels, int64_t c, const A* __restrict__ weight, int64_t n,
                   double* __restrict__ part, unsigned* __restrict__ done) {
+    let_next();  // the rows' kernel needs the weights only once it has its first rows
     __shared__ double sm[kNT / 32];
     double a = 0.0;
     constexpr int U = 8;  // tokens in flight per thread
@@ -1137,6 +1143,15 @@ void with_score_types(int dtype, F&& f) {
     }
 }
 
+// A kernel over rows: the statistics start a chain of launches, the others go on in one.
+template <Mode M, class K, class... Args>
+void launch_rows(K kernel, unsigned grid, unsigned block, size_t smem, cudaStream_t s, Args... args) {
+    if (M == STATS)
+        kernel<<<grid, block, smem, s>>>(args...);
+    else
+        launch_next(kernel, grid, block, smem, s, args...);
+}
+
 // Few classes: persistent warps over the tiles, whatever the mode.
 template <class T, class A, Mode M>
 void small_launch(int device, const T* x, int64_t ld, T* out, int64_t ld_out, const RowArgs<A>& a,
@@ -1149,8 +1164,8 @@ void small_launch(int device, const T* x, int64_t ld, T* out, int64_t ld_out, co
         auto k = small_rows_kernel<T, A, decltype(w)::value, decltype(turn)::value, M>;
         static bool asked[64];
         if (bytes > 48 * 1024) allow_smem(k, device, 64 * 1024, asked, "class tile shared memory");
-        k<<<(unsigned)std::min(blocks, most), kSmallNT, bytes, s>>>(
-            x, ld, out, ld_out, a, ld == a.c && (uintptr_t)x % 16 == 0, ld_out == a.c && (uintptr_t)out % 16 == 0);
+        launch_rows<M>(
+            k, (unsigned)std::min(blocks, most), kSmallNT, bytes, s, x, ld, out, ld_out, a, ld == a.c && (uintptr_t)x % 16 == 0, ld_out == a.c && (uintptr_t)out % 16 == 0);
     };
     auto width = [&](auto turn) {
         if (a.c <= 4)
@@ -1180,7 +1195,7 @@ void cached_launch(int device, const T* x, int64_t ld, T* out, int64_t ld_out, c
     auto go = [&](auto l, auto k) {
         constexpr int L = decltype(l)::value, K = decltype(k)::value;
         const int64_t blocks = ceil_div(a.n, (int64_t)kNT / L), most = (int64_t)sm_count(device) * cached_blocks<A>(K);
-        cached_rows_kernel<T, A, L, K, M><<<(unsigned)std::min(blocks, most), kNT, 0, s>>>(x, ld, out, ld_out, a);
+        launch_rows<M>(cached_rows_kernel<T, A, L, K, M>, (unsigned)std::min(blocks, most), kNT, 0, s, x, ld, out, ld_out, a);
     };
     using std::integral_constant;
     if (nv <= 16)
@@ -1209,7 +1224,7 @@ void rows_launch(int device, const T* x, int64_t ld, T* out, int64_t ld_out, con
         static bool asked[64];
         allow_smem(k, device, bytes, asked, "row ring shared memory");
         const int64_t grid = (int64_t)sm_count(device) * ring_blocks(L);
-        k<<<(unsigned)(n < grid ? n : grid), L + 32, bytes, s>>>(x, ld, out, ld_out, a);
+        launch_rows<M>(k, (unsigned)(n < grid ? n : grid), L + 32, bytes, s, x, ld, out, ld_out, a);
     };
     auto scan = [&]() {
         const int64_t warps = (int64_t)sm_count(device) * 32;  // resident at once
@@ -1276,7 +1291,7 @@ void grad_launch(int device, const T* x, int64_t ld, int64_t n, int64_t c, Label
     else if (c / Pack<T>::N <= kCachedVecs)
         cached_launch<T, A, GRAD>(device, x, ld, out, ld_out, a, s);
     else
-        label_grad_kernel<T, A, kNT><<<(unsigned)n, kNT, 0, s>>>(x, ld, out, ld_out, a);
+        launch_rows<GRAD>(label_grad_kernel<T, A, kNT>, (unsigned)n, kNT, 0, s, x, ld, out, ld_out, a);
     MFM_CHECK_LAUNCH("label gradient launch");
 }
 
@@ -1403,7 +1418,7 @@ extern "C" int mfm_preference_loss_device(int dtype, int device, const void* log
             if (n_pairs > 0) {
                 auto pairs = [&](auto w) {
                     constexpr int PW = decltype(w)::value;
-                    pair_kernel<A, PW><<<(unsigned)ceil_div(n_pairs, kNT / PW), kNT, 0, s>>>(
+                    launch_next(pair_kernel<A, PW>, (unsigned)ceil_div(n_pairs, kNT / PW), kNT, 0, s,
                         lp, n_tokens, indptr, n_pairs, (const A*)reference, beta, label_smoothing,
                         (const A*)sample_weight, (A*)margins, (A*)seq_logprobs, pair, coef, done,
                         (A*)loss, scale);

@@ -168,8 +168,11 @@ inline bool vec_ok(const void* p, int64_t ld, size_t size, int vec) {
 // statement, waits for the predecessor to be complete and visible, and lets the
 // successor be scheduled in turn. A chain of four to eight short kernels is
 // spent on launch gaps to a tenth.
+__device__ __forceinline__ void wait_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void let_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void after_previous() {
-    asm volatile("griddepcontrol.wait;\ngriddepcontrol.launch_dependents;" ::: "memory");
+    wait_previous();
+    let_next();
 }
 
 template <class... KArgs, class... Args>
