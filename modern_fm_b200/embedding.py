@@ -18,6 +18,8 @@ from __future__ import annotations
 
 from typing import NamedTuple, Optional
 
+import torch
+
 from . import _lib
 
 
@@ -37,24 +39,13 @@ class EmbeddingRows(NamedTuple):
     scale: Optional[object]
 
 
-_STORAGE = {}
-
-
-def _storage():
-    if not _STORAGE:
-        import torch
-
-        _STORAGE.update({
-            torch.float64: _lib.MFM_DTYPE_F64, torch.float32: _lib.MFM_DTYPE_F32,
-            torch.bfloat16: _lib.MFM_DTYPE_BF16, torch.float16: _lib.MFM_DTYPE_F16})
-    return _STORAGE
+_STORAGE = {torch.float64: _lib.MFM_DTYPE_F64, torch.float32: _lib.MFM_DTYPE_F32,
+            torch.bfloat16: _lib.MFM_DTYPE_BF16, torch.float16: _lib.MFM_DTYPE_F16}
 
 
 def _fail(rc):
-    if rc < 0:
-        raise ValueError(_lib.last_error())
-    if rc != 0:
-        raise RuntimeError(_lib.last_error())
+    if rc:
+        raise (ValueError if rc < 0 else RuntimeError)(_lib.last_error())
 
 
 def _one_device(first, *rest):
@@ -100,8 +91,6 @@ _NOTHING = _Nothing()
 
 def _on(stream, dev):
     """(stream handle, context that allocates on it)."""
-    import torch
-
     if stream is None:
         return torch._C._cuda_getCurrentRawStream(dev), _NOTHING
     if stream.device.index != dev:
@@ -118,9 +107,8 @@ def _hold(stream, *tensors):
 
 
 def _entries(ids, scale, indptr, wide):
-    import torch
-
-    if ids.dtype not in (torch.int32, torch.int64) or not ids.is_contiguous():
+    kind = ids.dtype
+    if not (kind is torch.int64 or kind is torch.int32) or not ids.is_contiguous():
         raise ValueError("ids must be a contiguous int32 or int64 tensor")
     if indptr is not None:
         if ids.dim() != 1:
@@ -133,7 +121,7 @@ def _entries(ids, scale, indptr, wide):
             raise ValueError("scale must be contiguous and have the shape of ids")
         if scale.dtype != wide:
             raise ValueError(f"scale must be {wide}")
-    return 1 if ids.dtype == torch.int64 else 0
+    return 1 if kind is torch.int64 else 0
 
 
 def embedding_lookup(table, ids, scale=None, indptr=None, alpha: float = 1.0, out=None,
@@ -151,10 +139,7 @@ def embedding_lookup(table, ids, scale=None, indptr=None, alpha: float = 1.0, ou
     inputs. Raises ValueError for invalid arguments, RuntimeError for CUDA
     failures.
     """
-    import torch
-
-    storage = _storage()
-    code = storage.get(table.dtype)
+    code = _STORAGE.get(table.dtype)
     if code is None:
         raise ValueError("table must be float64, float32, bfloat16 or float16")
     wide = torch.float64 if table.dtype == torch.float64 else torch.float32
@@ -187,10 +172,7 @@ def embedding_lookup(table, ids, scale=None, indptr=None, alpha: float = 1.0, ou
 
 
 def _grad(grad, ids, n_rows, scale, indptr, alpha, table, dtype, stream, by_rows):
-    import torch
-
-    storage = _storage()
-    code = storage.get(grad.dtype)
+    code = _STORAGE.get(grad.dtype)
     if code is None:
         raise ValueError("grad must be float64, float32, bfloat16 or float16")
     halves = grad.dtype in (torch.bfloat16, torch.float16)
@@ -240,7 +222,7 @@ def _grad(grad, ids, n_rows, scale, indptr, alpha, table, dtype, stream, by_rows
     # empty tensors have no address; the ABI tells its two results apart by theirs
     at = lambda t: None if t is None else (t.data_ptr() or ws.data_ptr())  # noqa: E731
     _fail(L.mfm_embedding_grad_device(
-        code, storage[kind], dev, ids64, ids.data_ptr(), n, _ptr(indptr), n_out, _ptr(scale),
+        code, _STORAGE[kind], dev, ids64, ids.data_ptr(), n, _ptr(indptr), n_out, _ptr(scale),
         float(alpha), gp, ld, tp, ld_table, n_rows, d, at(whole), at(keys), at(rows), at(count),
         _ptr(d_scale), ws.data_ptr(), nbytes, s))
     return whole, keys, rows, count, d_scale

@@ -23,8 +23,10 @@ from __future__ import annotations
 
 from typing import NamedTuple, Optional
 
+import torch
+
 from . import _lib
-from .embedding import _fail, _hold, _matrix, _on, _one_device, _ptr, _storage
+from .embedding import _STORAGE, _fail, _hold, _matrix, _on, _one_device, _ptr
 
 
 class LabelLogprobs(NamedTuple):
@@ -56,9 +58,7 @@ class PolicyLoss(NamedTuple):
 
 def _scores(logits, labels):
     """(dtype code, arithmetic type, pointer, rows, classes, pitch, labels64) of the scores."""
-    import torch
-
-    code = _storage().get(logits.dtype)
+    code = _STORAGE.get(logits.dtype)
     if code is None:
         raise ValueError("logits must be float64, float32, bfloat16 or float16")
     p, n, c, ld = _matrix("logits", logits)
@@ -79,8 +79,6 @@ def _vector(name, t, n, dtype):
 
 def _bounds(indptr):
     """Number of sequences of an indptr."""
-    import torch
-
     if (indptr.dtype != torch.int64 or indptr.dim() != 1 or not indptr.is_contiguous()
             or indptr.numel() < 1):
         raise ValueError("indptr must be a contiguous 1-D int64 tensor (n_sequences + 1)")
@@ -92,8 +90,6 @@ def label_logprobs(logits, labels, indptr=None, stream=None) -> LabelLogprobs:
     ``lse[t] = log sum exp logits[t]`` (also for masked rows). With ``indptr`` (int64,
     n_sequences + 1) the log-probabilities summed over each sequence's rows too,
     as ``preference_loss`` takes its reference."""
-    import torch
-
     code, wide, p, n, c, ld, l64 = _scores(logits, labels)
     n_seq = 0 if indptr is None else _bounds(indptr)
     dev = _one_device(logits, labels, indptr)
@@ -113,8 +109,6 @@ def label_logprobs_grad(grad, logits, labels, lse, stream=None):
     """Gradient of the logits for the gradient ``grad`` of ``label_logprobs``'
     log-probabilities: ``grad[t] * ([c = labels[t]] - exp(logits[t, c] - lse[t]))``, in
     the logits' type. ``lse`` is the forward's."""
-    import torch
-
     code, wide, p, n, c, ld, l64 = _scores(logits, labels)
     _vector("grad", grad, n, wide)
     _vector("lse", lse, n, wide)
@@ -143,8 +137,6 @@ def preference_loss(logits, labels, indptr, reference, beta: float = 0.1,
     e log sigmoid(-z)`` with e = ``label_smoothing``. Pairs of weight 0 are left
     out; weights that sum to 0 give loss and gradient 0.
     """
-    import torch
-
     code, wide, p, n, c, ld, l64 = _scores(logits, labels)
     n_seq = _bounds(indptr)
     if n_seq % 2:
@@ -167,7 +159,8 @@ def preference_loss(logits, labels, indptr, reference, beta: float = 0.1,
         code, dev, p, ld, n, c, l64, labels.data_ptr(), indptr.data_ptr(), n_pairs,
         reference.data_ptr(), float(beta), float(label_smoothing), _ptr(sample_weight), at,
         at + size, at + size * (1 + n_pairs), _ptr(grad), c, ws.data_ptr(), nbytes, s))
-    return PreferenceLoss(out[0], out[1:1 + n_pairs], out[1 + n_pairs:], grad)
+    loss, margins, logprobs = out.split_with_sizes((1, n_pairs, n_seq))
+    return PreferenceLoss(loss.view(()), margins, logprobs, grad)
 
 
 def policy_loss(logits, labels, old_logprobs, advantages, reference=None, clip_low: float = 0.2,
@@ -184,8 +177,6 @@ def policy_loss(logits, labels, old_logprobs, advantages, reference=None, clip_l
     ``sample_weight`` hold one value per row. ``kl`` is the mean of exp(u) - u - 1,
     ``clip_fraction`` the share of rows whose clipped term is the smaller one.
     """
-    import torch
-
     code, wide, p, n, c, ld, l64 = _scores(logits, labels)
     _vector("old_logprobs", old_logprobs, n, wide)
     _vector("advantages", advantages, n, wide)
@@ -208,4 +199,5 @@ def policy_loss(logits, labels, old_logprobs, advantages, reference=None, clip_l
         advantages.data_ptr(), _ptr(reference), float(clip_low), float(clip_high), float(kl_coef),
         _ptr(sample_weight), stats.data_ptr(), lp.data_ptr(), _ptr(grad), c, ws.data_ptr(), nbytes,
         s))
-    return PolicyLoss(stats[0], stats[1], stats[2], lp, grad)
+    loss, kl, clipped = stats.unbind(0)
+    return PolicyLoss(loss, kl, clipped, lp, grad)
