@@ -97,6 +97,17 @@ CASES = [  # n_rows, d, n, table, scale, indptr, ids, hot
     (5, 512, 64, "f16", None, "rows", torch.int32, 0.0),
     (1 << 17, 4, 500_000, "f32", "f32", "rows", torch.int32, 0.4),
     (40, 64, 33, "bf16", "f32", "inside", torch.int32, 0.0),
+    # the sort's paths: one block and tiles (2048 ids), 8-bit digits in one, two and
+    # many tiles' passes, 12-bit digits in two and three; runs over many chunks
+    (200, 4, 2048, "f32", "f32", None, torch.int64, 0.5),
+    (200, 4, 2049, "f32", "f32", None, torch.int64, 0.5),
+    (255, 10, 5000, "f32", "f32", "rows", torch.int32, 0.8),
+    (60000, 2, 450_000, "f32", None, None, torch.int64, 0.05),
+    ((1 << 24) - 1, 1, 30_000, "f32", "f32", None, torch.int32, 0.1),
+    (1 << 25, 1, 20_000, "f16", "f32", "rows", torch.int64, 0.1),
+    (2000, 300, 9000, "f32", "f32", "rows", torch.int32, 0.9),
+    (2000, 6, 40_000, "f64", "f64", None, torch.int64, 0.9),
+    (3, 36, 12_000, "f16", "f32", "rows", torch.int32, 0.4),
 ]
 
 
@@ -304,3 +315,54 @@ def test_gradient_by_differences():
         d[e] = 0.5
         assert loss(table, s + d) - loss(table, s - d) == pytest.approx(float(g.scale[e]),
                                                                         abs=1e-11)
+
+
+def test_offsets_beyond_32_bits():
+    """A table and a gradient of more than 2^32 values: the last rows and the first."""
+    n_rows, d = 66_000, 65_600
+    table = torch.zeros(n_rows, d, device="cuda", dtype=torch.bfloat16)
+    assert table.numel() > 2**32
+    ids = torch.tensor([n_rows - 1, 0, n_rows - 2, n_rows, n_rows - 1], device="cuda")
+    for i in (0, n_rows - 2, n_rows - 1):
+        table[i] = torch.randn(d, device="cuda").bfloat16()
+    out = embedding_lookup(table, ids)
+    assert torch.equal(out[[0, 1, 2, 4]], table[ids[[0, 1, 2, 4]]]) and bool((out[3] == 0).all())
+    two = embedding_lookup(table, ids, None, torch.tensor([0, 3, 5], device="cuda"))
+    # one rounding of a float32 sum of three bfloat16 values
+    want = table[ids[:3]].double().sum(0)
+    assert ((two[0].double() - want).abs() <= want.abs() * 2.0**-8 + 2.0**-20).all()
+    del out, two
+    grad = torch.randn(5, d, device="cuda").bfloat16()
+    g = embedding_grad(grad, ids, n_rows, table=table)
+    assert torch.equal(g.table[0], grad[1]) and torch.equal(g.table[n_rows - 2], grad[2])
+    want = grad[0].double() + grad[4].double()
+    assert ((g.table[n_rows - 1].double() - want).abs() <= want.abs() * 2.0**-8).all()
+    assert int(g.table[1:n_rows - 2].count_nonzero()) == 0
+    assert float(g.scale[3]) == 0.0
+    r = embedding_grad_rows(grad, ids, n_rows)
+    assert r.keys.tolist() == [0, n_rows - 2, n_rows - 1, -1, -1] and int(r.count) == 3
+    assert torch.equal(r.rows[2], g.table[n_rows - 1])
+    # and many ids, through the tiled sort and the touched rows' bits
+    many = torch.randint(n_rows - 40, n_rows, (3000,), device="cuda")
+    g = embedding_grad(torch.ones(3000, d, device="cuda", dtype=torch.bfloat16), many, n_rows)
+    want = torch.bincount(many, minlength=n_rows).bfloat16()
+    assert torch.equal(g.table[:, -1], want) and torch.equal(g.table[:, 0], want)
+    assert int(g.table[:n_rows - 40].count_nonzero()) == 0
+
+
+def test_two_streams_at_once():
+    """Calls in flight on two streams share nothing."""
+    table, ids, s, ip = _make(6, 3000, 24, 40_000, "f32", "f32", "rows", torch.int32, hot=0.3)
+    grad = torch.randn(ip.numel() - 1, 24, device="cuda")
+    want = embedding_grad(grad, ids, 3000, s, ip, table=table)
+    rows = embedding_grad_rows(grad, ids, 3000, s, ip)
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(20):
+        got.append((embedding_grad(grad, ids, 3000, s, ip, table=table, stream=a),
+                    embedding_grad_rows(grad, ids, 3000, s, ip, stream=b)))
+    torch.cuda.synchronize()
+    for x, y in got:
+        assert torch.equal(x.table, want.table) and torch.equal(x.scale, want.scale)
+        assert torch.equal(y.rows, rows.rows) and torch.equal(y.keys, rows.keys)

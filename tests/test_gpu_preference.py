@@ -400,3 +400,50 @@ def test_a_training_step_of_a_linear_policy():
     h = 1e-3
     num = (float(loss(w + h * direction).loss) - float(loss(w - h * direction).loss)) / (2 * h)
     assert num == pytest.approx(norm**0.5, rel=1e-5)
+
+
+def test_offsets_beyond_32_bits():
+    """More than 2^32 scores: a uniform matrix with a few classes raised, in the last row."""
+    n, c = 33_000, 131_072
+    x = torch.zeros(n, c, device="cuda", dtype=torch.bfloat16)
+    assert x.numel() > 2**32
+    x[n - 1, c - 1] = 8.0
+    y = torch.full((n,), c - 1, device="cuda")
+    z = torch.full((n,), -math.log(c), device="cuda")
+    tol = _tol(x[-2:], torch.float32)
+    r = label_logprobs(x, y)
+    last = 8.0 - math.log(c - 1 + math.exp(8.0))
+    assert float((r.logprobs[:-1] + math.log(c)).abs().max()) <= tol
+    assert abs(float(r.logprobs[-1]) - last) <= tol
+    g = label_logprobs_grad(torch.ones(n, device="cuda"), x, y, r.lse)
+    assert float(g[n - 1, c - 1]) == pytest.approx(1 - math.exp(last), rel=2.0**-7)
+    assert float(g[n - 2, 0]) == pytest.approx(-1 / c, rel=2.0**-7)
+    del g
+    q = policy_loss(x, y, z, torch.ones(n, device="cuda"), clip_high=1e9)
+    # every row's ratio is 1 but the last's
+    ratio = math.exp(last + math.log(c))
+    assert float(q.loss) == pytest.approx(-(n - 1 + ratio) / n, rel=1e-5)
+    assert float(q.grad[n - 1, c - 1]) == pytest.approx(-ratio / n * (1 - math.exp(last)), rel=2.0**-6)
+
+
+def test_two_streams_at_once():
+    x, y = _make(10, 3000, 10, "f32")
+    big, yb = _make(11, 40, 30000, "bf16")
+    one = torch.full((3000,), -2.0, device="cuda")
+    adv = torch.randn(3000, device="cuda")
+    ip = torch.arange(0, 41, 10, device="cuda")
+    ref = torch.zeros(4, device="cuda")
+
+    def calls(stream):
+        p = policy_loss(x, y, one, adv, one, kl_coef=0.1, stream=stream)
+        q = policy_loss(big, yb, one[:40], adv[:40], stream=stream)
+        r = preference_loss(big, yb, ip, ref, stream=stream)
+        return (p.loss, p.grad, p.logprobs, q.loss, q.grad, r.loss, r.grad)
+
+    want = calls(None)
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    got = [calls(s) for _ in range(15) for s in (a, b)]
+    torch.cuda.synchronize()
+    for g in got:
+        assert all(torch.equal(u, v) for u, v in zip(g, want))
