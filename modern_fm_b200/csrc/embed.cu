@@ -155,53 +155,61 @@ __device__ __forceinline__ void row_bounds(const int64_t* indptr, int64_t b, int
 // the columns (a vector each; blockIdx.y walks them), EL take every EL-th entry, U
 // entries a lane in flight; their parts are added by shuffles. Bound by the
 // latency of the rows' gathers: 131072 rows of 36 entries, 16 float32 each in
-// float64 arithmetic, 54 us (62 us with a round's ids fetched just before its rows;
-// 67 us with EL = 4, 84 us at five blocks per SM).
+// float64 arithmetic, 51 us at five blocks per SM (55 us at four, 75 us at six, which
+// spill; 62 us with EL = 4; 83 us with eight entries a lane; 54 us with the ids held by
+// every lane, 62 us with those fetched just before their rows).
 template <class T, class A, class O, class I, int B, int LV, int EL>
-__global__ void __launch_bounds__(256, 4)
+__global__ void __launch_bounds__(256, 5)
     embed_sums_kernel(const I* __restrict__ ids, int64_t n, const int64_t* __restrict__ indptr,
                       int64_t n_out, const A* __restrict__ scale, A alpha,
                       const T* __restrict__ table, int64_t n_rows, int64_t d, int64_t ld,
                       O* __restrict__ out, int64_t ld_out) {
     constexpr int U = 4, G = LV * EL, N = Lane<T, B>::N;
-    const int lane = threadIdx.x % LV, el = threadIdx.x % G / LV;
+    constexpr int E = U * EL, K = E > G ? E / G : 1;  // entries a round; ids a lane fetches of them
+    const int lane = threadIdx.x % LV, gl = threadIdx.x % G, el = gl / LV;
     const int64_t b = (int64_t)blockIdx.x * (256 / G) + threadIdx.x / G;
     const int64_t col = ((int64_t)blockIdx.y * LV + lane) * N;
-    const bool in = b < n_out && col < d;
+    const bool in = b < n_out;
     int64_t lo = 0, hi = 0;
     if (in) row_bounds(indptr, b, n, lo, hi);
     A acc[N];
 #pragma unroll
     for (int j = 0; j < N; ++j) acc[j] = A(0);
-    // the next round's ids and scales are on their way while a round's rows are
-    I id[U];
-    A f[U];
+    // a lane fetches the round's entry gl (and every G-th behind it) and hands it
+    // round; the next round's are on their way while a round's rows are
+    int32_t id[K];
+    A f[K];
     auto fetch = [&](int64_t e) {
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            id[u] = -1;
-            f[u] = A(1);
-            if (e + u * EL < hi) {
-                id[u] = ids[e + u * EL];
-                if (scale) f[u] = scale[e + u * EL];
+        for (int k = 0; k < K; ++k) {
+            const int64_t at = e + gl + k * G;
+            id[k] = -1;
+            f[k] = A(1);
+            if (gl + k * G < E && at < hi) {
+                const int64_t i = (int64_t)ids[at];
+                id[k] = i >= 0 && i < n_rows ? (int32_t)i : -1;
+                if (scale) f[k] = scale[at];
             }
         }
     };
-    fetch(lo + el);
-    for (int64_t e = lo + el; e < hi; e += U * EL) {
+    fetch(lo);
+    for (int64_t e = lo; __any_sync(0xffffffffu, e < hi); e += E) {
         Lane<T, B> v[U];
         A w[U];
-        bool live[U];
+        unsigned live = 0;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            live[u] = id[u] >= 0 && id[u] < n_rows;
-            if (live[u]) v[u].load(table + (int64_t)id[u] * ld + col);
-            w[u] = f[u];
+            const int32_t i = __shfl_sync(0xffffffffu, id[u * EL / G], u * EL % G + el, G);
+            w[u] = __shfl_sync(0xffffffffu, f[u * EL / G], u * EL % G + el, G);
+            if (i >= 0 && col < d) {
+                v[u].load(table + (int64_t)i * ld + col);
+                live |= 1u << u;
+            }
         }
-        fetch(e + U * EL);
+        fetch(e + E);
 #pragma unroll
         for (int u = 0; u < U; ++u)
-            if (live[u]) {
+            if (live >> u & 1u) {
                 A p[N];
                 v[u].get(p);
 #pragma unroll
@@ -212,7 +220,7 @@ __global__ void __launch_bounds__(256, 4)
     for (int o = G / 2; o >= LV; o >>= 1)
 #pragma unroll
         for (int j = 0; j < N; ++j) acc[j] += __shfl_xor_sync(0xffffffffu, acc[j], o);
-    if (in && el == 0) {
+    if (in && el == 0 && col < d) {
 #pragma unroll
         for (int j = 0; j < N; ++j) acc[j] *= alpha;
         put(out + b * ld_out + col, acc);
@@ -462,8 +470,8 @@ __device__ __forceinline__ void fill_rest(const GradArgs<G, T, A, O>& a, unsigne
 constexpr int kScaleEntries = 4;
 
 template <class G, class T, class A, class O, int B, int LV>
-__device__ __forceinline__ void scale_entries(const GradArgs<G, T, A, O>& a, int64_t t0, int stride,
-                                              int lane) {
+__device__ __forceinline__ void scale_entries(const GradArgs<G, T, A, O>& a, const int32_t* row_of,
+                                              int64_t t0, int stride, int lane) {
     constexpr int N = Lane<G, B>::N, U = kScaleEntries;
     const T* v[U];
     const G* g[U];
@@ -475,7 +483,7 @@ __device__ __forceinline__ void scale_entries(const GradArgs<G, T, A, O>& a, int
         int64_t id = -1, row = -1;
         if (t < a.in.n) {
             id = a.in.ids[t];
-            row = a.row_of ? (int64_t)a.row_of[t] : t;
+            row = row_of ? (int64_t)row_of[t] : t;
         }
         live[u] = id >= 0 && id < a.in.n_rows && row >= 0;
         v[u] = a.table + (live[u] ? id : 0) * a.ld_table;
@@ -547,7 +555,94 @@ __global__ void __launch_bounds__(kMainNT)
         const int64_t col = ((int64_t)(b % slabs) * LV + lane) * N;
         if (c < a.n_chunks && col < a.d) reduce_chunk<G, T, A, O, B, LV>(a, c, col, col == 0);
     } else {
-        scale_entries<G, T, A, O, B, LV>(a, (int64_t)(b - a.reduce_blocks) * (GR * kScaleEntries) + group, GR, lane);
+        scale_entries<G, T, A, O, B, LV>(a, a.row_of, (int64_t)(b - a.reduce_blocks) * (GR * kScaleEntries) + group, GR, lane);
+    }
+}
+
+// A few ids (at most kFewIds): one launch and no workspace. Every block sorts them
+// for itself (2 us) and then sums runs, takes scales' gradients or fills, a lane
+// group per run and LV vectors of columns. (66 entries into 1003 x 60: a sort, a
+// main and a cross launch take 26 us a call, this one 18 us.)
+template <class G, class T, class A, class O, int B, int LV>
+__global__ void __launch_bounds__(kFewIds)
+    embed_few_kernel(const GradArgs<G, T, A, O> a, int key_bits, int slabs) {
+    constexpr int U = 8, N = Lane<G, B>::N, GR = kFewIds / LV;
+    __shared__ BlockSort<kFewIds, 1> sort;
+    __shared__ int32_t rows[kFewIds];      // by position
+    __shared__ uint32_t key[kFewIds], row[kFewIds], run[kFewIds + 1];
+    __shared__ A scale[kFewIds];
+    const int t = threadIdx.x, lane = t % LV, group = t / LV, n = (int)a.in.n;
+    const uint32_t pad_key = (uint32_t)a.in.n_rows;
+    sort.run(a.in, key_bits, rows);
+    bool live = false, head = false;
+    if (t < n) {
+        const uint2 e = sort.skv[t];
+        live = e.x != pad_key;
+        head = live && (t == 0 || sort.skv[t - 1].x != e.x);
+        key[t] = e.x;
+        row[t] = a.in.indptr ? (uint32_t)rows[e.y] : e.y;
+        scale[t] = a.scale ? a.scale[e.y] : A(1);
+    }
+    uint32_t n_runs;
+    const uint32_t rank = block_exclusive_scan<uint32_t, kFewIds>(head ? 1u : 0u, sort.scan_sm, n_runs);
+    if (head) run[rank] = (uint32_t)t;
+    const int n_live = __syncthreads_count(live);
+    if (t == 0) run[n_runs] = (uint32_t)n_live;
+    __syncthreads();
+    if (blockIdx.x < a.reduce_blocks) {
+        if (a.rows && blockIdx.x == 0 && t == 0) *a.count = n_runs;
+        for (unsigned item = blockIdx.x * GR + group; item < n_runs * (unsigned)slabs; item += a.reduce_blocks * GR) {
+            const unsigned r = item / (unsigned)slabs;
+            const int64_t col = ((int64_t)(item % (unsigned)slabs) * LV + lane) * N;
+            if (col >= a.d) continue;
+            A acc[N];
+#pragma unroll
+            for (int j = 0; j < N; ++j) acc[j] = A(0);
+            const int end = (int)run[r + 1];
+            for (int e = (int)run[r]; e < end; e += U) {
+                Lane<G, B> v[U];
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+                    if (e + u < end) v[u].load(a.grad + (int64_t)row[e + u] * a.ld + col);
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+                    if (e + u < end) {
+                        A w[N];
+                        v[u].get(w);
+#pragma unroll
+                        for (int j = 0; j < N; ++j) acc[j] += scale[e + u] * w[j];
+                    }
+            }
+#pragma unroll
+            for (int j = 0; j < N; ++j) acc[j] *= a.alpha;
+            const uint32_t k = key[run[r]];
+            put((a.rows ? a.rows + (int64_t)r * a.d : a.d_table + (int64_t)k * a.d) + col, acc);
+            if (a.keys_out.p && col == 0) a.keys_out.put(r, k);
+        }
+    } else if (blockIdx.x < a.reduce_blocks + a.scale_blocks) {
+        scale_entries<G, T, A, O, B, LV>(a, a.in.indptr ? rows : nullptr,
+                                         (int64_t)(blockIdx.x - a.reduce_blocks) * (GR * kScaleEntries) + group, GR, lane);
+    } else {  // the rows that nothing touches
+        const int wl = t & 31, per = a.fill_per;
+        const int64_t warp = (int64_t)(blockIdx.x - a.reduce_blocks - a.scale_blocks) * (kFewIds / 32) + t / 32;
+        const int64_t bytes = a.d * (int64_t)sizeof(O), cap = n < a.in.n_rows ? n : a.in.n_rows;
+        char* const base = reinterpret_cast<char*>(a.rows ? a.rows : a.d_table);
+        const bool vec = bytes % 16 == 0 && (uintptr_t)base % 16 == 0;
+        const int64_t first = a.rows ? (int64_t)n_runs : 0, end = a.rows ? cap : a.in.n_rows;
+        for (int64_t r0 = first + warp * per; r0 < end; r0 += (int64_t)a.fill_blocks * (kFewIds / 32) * per) {
+            const int m = (int)(r0 + per < end ? per : end - r0);
+            unsigned touched = 0;
+            if (a.rows) {
+                if (wl < m) a.keys_out.put(r0 + wl, -1);
+            } else {
+                for (int i = wl; i < n; i += 32) {
+                    const int64_t at = (int64_t)key[i] - r0;
+                    if (at >= 0 && at < m) touched |= 1u << at;
+                }
+                touched = __reduce_or_sync(0xffffffffu, touched);
+            }
+            clear_rows(base + r0 * bytes, bytes, m, touched, vec);
+        }
     }
 }
 
@@ -800,6 +895,7 @@ struct GradWs {
     int64_t n_chunks = 0;
     size_t off_row = 0, off_scale = 0, off_base = 0, off_tile = 0, off_head = 0, off_tail = 0, off_bits = 0, bytes = 0;
     GradWs(int dtype, bool by_rows, int64_t n, int64_t n_rows, int64_t d) : sort(n, n_rows) {
+        if (n <= kFewIds) return;  // none
         auto up = [](size_t b) { return (b + 255) / 256 * 256; };
         const size_t a = dtype == MFM_DTYPE_F64 || dtype == MFM_DTYPE_F32_F64 ? 8 : 4;
         n_chunks = ceil_div(n, kChunk);
@@ -815,7 +911,29 @@ struct GradWs {
 };
 
 template <class G, class T, class A, class O, int B>
+void few_launch(int device, GradArgs<G, T, A, O>& a, cudaStream_t s) {
+    const int64_t dv = a.d / Lane<G, B>::N, n = a.in.n, bytes = a.d * (int64_t)sizeof(O), sm = sm_count(device);
+    with_lanes(dv, [&](auto lv) {
+        constexpr int LV = decltype(lv)::value, GR = kFewIds / LV;
+        const int64_t slabs = ceil_div(dv, LV), most = std::min(n, a.in.n_rows);
+        a.reduce_blocks = (unsigned)std::min<int64_t>(ceil_div(most * slabs, GR), sm * 4);
+        a.scale_blocks = a.d_scale ? (unsigned)ceil_div(n, GR * kScaleEntries) : 0u;
+        a.fill_per = 32;
+        while (a.fill_per > 1 && a.fill_per * bytes > 32768) a.fill_per /= 2;
+        a.fill_blocks = (unsigned)std::min<int64_t>(
+            ceil_div(a.rows ? most : a.in.n_rows, (int64_t)a.fill_per * (kFewIds / 32)), sm * 8);
+        embed_few_kernel<G, T, A, O, B, LV><<<a.reduce_blocks + a.scale_blocks + a.fill_blocks, kFewIds, 0, s>>>(
+            a, id_key_bits(a.in.n_rows), (int)slabs);
+    });
+    MFM_CHECK_LAUNCH("embedding gradient launch");
+}
+
+template <class G, class T, class A, class O, int B>
 void grad_launch(int device, GradArgs<G, T, A, O>& a, const GradWs& W, char* ws, cudaStream_t s) {
+    if (a.in.n <= kFewIds) {
+        few_launch<G, T, A, O, B>(device, a, s);
+        return;
+    }
     constexpr int N = Lane<G, B>::N;
     const int64_t n = a.in.n, nc = W.n_chunks, dv = a.d / N;
     uint32_t* words = reinterpret_cast<uint32_t*>(ws);
@@ -888,13 +1006,14 @@ template <class G, class T, class A, class O>
 void grad_entry(int device, GradArgs<G, T, A, O>& a, const GradWs& W, char* ws, cudaStream_t s) {
     const int64_t cap = std::min(a.in.n, a.in.n_rows);
     if (a.in.n == 0 || a.in.n_rows == 0 || a.in.n_out == 0) {  // nothing to add up
-        if (a.d_table) MFM_CUDA(cudaMemsetAsync(a.d_table, 0, (size_t)a.in.n_rows * a.d * sizeof(O), s), "memset");
-        if (a.keys_out.p) {
-            MFM_CUDA(cudaMemsetAsync(a.keys_out.p, 0xff, (size_t)cap * (a.keys_out.is64 ? 8 : 4), s), "memset");
-            MFM_CUDA(cudaMemsetAsync(a.rows, 0, (size_t)cap * a.d * sizeof(O), s), "memset");
-            MFM_CUDA(cudaMemsetAsync(a.count, 0, sizeof(int64_t), s), "memset");
-        }
-        if (a.d_scale) MFM_CUDA(cudaMemsetAsync(a.d_scale, 0, (size_t)a.in.n * sizeof(A), s), "memset");
+        auto set = [&](void* p, int value, size_t bytes) {
+            if (p && bytes) MFM_CUDA(cudaMemsetAsync(p, value, bytes, s), "memset");
+        };
+        set(a.d_table, 0, (size_t)a.in.n_rows * a.d * sizeof(O));
+        set(a.keys_out.p, 0xff, (size_t)cap * (a.keys_out.is64 ? 8 : 4));
+        set(a.rows, 0, (size_t)cap * a.d * sizeof(O));
+        set(a.count, 0, sizeof(int64_t));
+        set(a.d_scale, 0, (size_t)a.in.n * sizeof(A));
         return;
     }
     const O* result = a.d_table ? a.d_table : a.rows;
@@ -976,7 +1095,7 @@ extern "C" int mfm_embedding_grad_device(int dtype, int out_dtype, int device, i
         }
         DeviceGuard g(device);
         const GradWs W(dtype, by_rows, n_entries, n_rows, d);
-        if (n_entries > 0 && (!workspace || workspace_bytes < (int64_t)W.bytes))
+        if (W.bytes > 0 && (!workspace || workspace_bytes < (int64_t)W.bytes))
             fail(MFM_ERR_INVALID, fmt("workspace of %lld bytes, %lld needed", (long long)workspace_bytes,
                                       (long long)W.bytes));
         if ((uintptr_t)workspace % 256) fail(MFM_ERR_INVALID, "workspace must be 256-byte aligned");

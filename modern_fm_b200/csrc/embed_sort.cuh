@@ -15,7 +15,8 @@
 //    by itself (at most 192 KB of L2 reads); else one prefix launch a pass;
 //  * the last pass leaves, beside the sorted keys, each entry's gradient row and
 //    scale instead of its position, so the sums read them in order;
-//  * up to kSmallSort ids one block does every pass in shared memory.
+//  * up to kSmallSort ids one block does every pass in shared memory; up to
+//    kFewIds, every block of the gradient's only launch sorts them for itself.
 #pragma once
 
 #include <type_traits>
@@ -31,6 +32,7 @@ constexpr int kETile = kETileNT * kETileItems;
 constexpr int kFuseTiles = 192;
 constexpr int kWideBits = 12;
 constexpr int64_t kSmallSort = 2048;
+constexpr int kFewIds = 256;
 constexpr int kSortPad = 16;  // places behind the last entry: key n_rows, row 0, scale 0
 
 // The entries of a batch: their ids and, where they are summed by rows, the rows'
@@ -473,75 +475,86 @@ __global__ void __launch_bounds__(kETileNT)
     }
 }
 
-// All passes of up to NT * ITEMS ids in one block.
-template <class A, int NT, int ITEMS>
-__global__ void __launch_bounds__(NT)
-    id_sort_small_kernel(Entries in, int key_bits, int32_t* row_of,
-                         unsigned* __restrict__ done, SortedOut<A> out) {
-    constexpr int NW = NT / 32;
-    __shared__ uint32_t cnt[NW][256];
-    __shared__ uint2 skv[NT * ITEMS];
-    __shared__ uint32_t scan_sm[NW];
-    const int t = threadIdx.x, lane = t & 31, warp = t >> 5, n = (int)in.n;
-    const int q0 = warp * (32 * ITEMS) + lane;
-    uint32_t key[ITEMS], val[ITEMS], digit[ITEMS], rank[ITEMS];
-    int32_t r[ITEMS];
-    in.rows(q0 - lane, r);
-#pragma unroll
-    for (int i = 0; i < ITEMS; ++i) {
-        const int q = q0 + i * 32;
-        key[i] = 0u;
-        val[i] = (uint32_t)q;
-        if (q < n) {
-            if (in.indptr) row_of[q] = r[i];
-            key[i] = in.key(q, r[i]);
-        }
-    }
-    if (t == 0) *done = 0;
-    for (int shift = 0; shift < key_bits; shift += 8) {
-        for (int i = t; i < NW * 256; i += NT) (&cnt[0][0])[i] = 0;
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < ITEMS; ++i)
-            digit[i] = q0 + i * 32 < n ? (key[i] >> shift) & 255u : 0x80000000u + (uint32_t)lane;
-        warp_ranks<ITEMS>(digit, cnt[warp], rank);
-        __syncthreads();
-        uint32_t tot = 0;
-        if (t < 256)
-#pragma unroll
-            for (int w = 0; w < NW; ++w) {
-                const uint32_t c = cnt[w][t];
-                cnt[w][t] = tot;
-                tot += c;
-            }
-        uint32_t all;
-        const uint32_t dstart = block_exclusive_scan<uint32_t, NT>(tot, scan_sm, all);
-        if (t < 256)
-#pragma unroll
-            for (int w = 0; w < NW; ++w) cnt[w][t] += dstart;
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < ITEMS; ++i)
-            if (q0 + i * 32 < n) skv[cnt[warp][digit[i]] + rank[i]] = make_uint2(key[i], val[i]);
-        __syncthreads();
+// All passes of up to NT * ITEMS ids in one block: on return skv holds (key,
+// position) of the sorted entries. rows: where entry q's row goes, or NULL.
+template <int NT, int ITEMS>
+struct BlockSort {
+    static constexpr int NW = NT / 32;
+    uint32_t cnt[NW][256];
+    uint2 skv[NT * ITEMS];
+    uint32_t scan_sm[NW];
+
+    __device__ __forceinline__ void run(const Entries& in, int key_bits, int32_t* rows) {
+        const int t = threadIdx.x, lane = t & 31, warp = t >> 5, n = (int)in.n;
+        const int q0 = warp * (32 * ITEMS) + lane;
+        uint32_t key[ITEMS], val[ITEMS], digit[ITEMS], rank[ITEMS];
+        int32_t r[ITEMS];
+        in.rows(q0 - lane, r);
 #pragma unroll
         for (int i = 0; i < ITEMS; ++i) {
             const int q = q0 + i * 32;
+            key[i] = 0u;
+            val[i] = (uint32_t)q;
             if (q < n) {
-                key[i] = skv[q].x;
-                val[i] = skv[q].y;
+                if (rows) rows[q] = r[i];
+                key[i] = in.key(q, r[i]);
             }
         }
-        __syncthreads();
+        for (int shift = 0; shift < key_bits; shift += 8) {
+            for (int i = t; i < NW * 256; i += NT) (&cnt[0][0])[i] = 0;
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < ITEMS; ++i)
+                digit[i] = q0 + i * 32 < n ? (key[i] >> shift) & 255u : 0x80000000u + (uint32_t)lane;
+            warp_ranks<ITEMS>(digit, cnt[warp], rank);
+            __syncthreads();
+            uint32_t tot = 0;
+            if (t < 256)
+#pragma unroll
+                for (int w = 0; w < NW; ++w) {
+                    const uint32_t c = cnt[w][t];
+                    cnt[w][t] = tot;
+                    tot += c;
+                }
+            uint32_t all;
+            const uint32_t dstart = block_exclusive_scan<uint32_t, NT>(tot, scan_sm, all);
+            if (t < 256)
+#pragma unroll
+                for (int w = 0; w < NW; ++w) cnt[w][t] += dstart;
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < ITEMS; ++i)
+                if (q0 + i * 32 < n) skv[cnt[warp][digit[i]] + rank[i]] = make_uint2(key[i], val[i]);
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < ITEMS; ++i) {
+                const int q = q0 + i * 32;
+                if (q < n) {
+                    key[i] = skv[q].x;
+                    val[i] = skv[q].y;
+                }
+            }
+            __syncthreads();
+        }
     }
+};
+
+template <class A, int NT, int ITEMS>
+__global__ void __launch_bounds__(NT)
+    id_sort_small_kernel(Entries in, int key_bits, int32_t* row_of, unsigned* __restrict__ done,
+                         SortedOut<A> out) {
+    __shared__ BlockSort<NT, ITEMS> sort;
+    const int t = threadIdx.x, n = (int)in.n;
+    if (t == 0) *done = 0;
+    sort.run(in, key_bits, in.indptr ? row_of : nullptr);
     uint32_t row[ITEMS];
     A s[ITEMS];
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i)  // row_of was written by this block, before a barrier
-        if (q0 + i * 32 < n) out.load(val[i], row[i], s[i]);
+        if (t + i * NT < n) out.load(sort.skv[t + i * NT].y, row[i], s[i]);
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i)
-        if (q0 + i * 32 < n) out.store(q0 + i * 32, key[i], row[i], s[i]);
+        if (t + i * NT < n) out.store(t + i * NT, sort.skv[t + i * NT].x, row[i], s[i]);
     if (t < kSortPad) out.store(n + t, out.pad_key, 0u, A(0));
 }
 
@@ -590,9 +603,7 @@ void sort_ids(int device, const IdSortPlan& P, const Entries& in, int32_t* row_o
             constexpr int NT = decltype(nt)::value, IT = decltype(items)::value;
             id_sort_small_kernel<A, NT, IT><<<1, NT, 0, s>>>(in, P.key_bits, row_of, done, out);
         };
-        if (n <= 256)
-            small(integral_constant<int, 256>{}, integral_constant<int, 1>{});
-        else if (n <= 512)
+        if (n <= 512)
             small(integral_constant<int, 512>{}, integral_constant<int, 1>{});
         else
             small(integral_constant<int, 512>{}, integral_constant<int, 4>{});

@@ -209,7 +209,7 @@ def _grad(grad, ids, n_rows, scale, indptr, alpha, table, dtype, stream, by_rows
     _hold(stream, grad, ids, scale, indptr, table)
     keys = rows = count = whole = d_scale = None
     with ctx:
-        ws = grad.new_empty(max(nbytes, 1), dtype=torch.uint8)
+        ws = grad.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
         if by_rows:
             cap = min(n, n_rows)
             keys = ids.new_empty(cap)
@@ -220,11 +220,11 @@ def _grad(grad, ids, n_rows, scale, indptr, alpha, table, dtype, stream, by_rows
         if table is not None:
             d_scale = grad.new_empty(ids.shape, dtype=wide)
     # empty tensors have no address; the ABI tells its two results apart by theirs
-    at = lambda t: None if t is None else (t.data_ptr() or ws.data_ptr())  # noqa: E731
+    at = lambda t: None if t is None else (t.data_ptr() or 256)  # noqa: E731
     _fail(L.mfm_embedding_grad_device(
         code, _STORAGE[kind], dev, ids64, ids.data_ptr(), n, _ptr(indptr), n_out, _ptr(scale),
         float(alpha), gp, ld, tp, ld_table, n_rows, d, at(whole), at(keys), at(rows), at(count),
-        _ptr(d_scale), ws.data_ptr(), nbytes, s))
+        _ptr(d_scale), _ptr(ws), nbytes, s))
     return whole, keys, rows, count, d_scale
 
 

@@ -148,7 +148,9 @@ def test_gradient_host_checks(kw, msg):
 def test_gradient_workspace_sizes():
     f = _lib.lib().mfm_embedding_grad_workspace_bytes
     assert f(1, 0, 0, 10, 4) == 0 and f(1, 1, -1, 10, 4) == 0
-    assert 0 < f(1, 0, 100, 10, 4) <= f(0, 0, 100, 10, 4) <= f(0, 0, 100000, 10, 4)
+    assert f(1, 0, 256, 10, 4) == 0  # a few ids need none
+    assert 0 < f(1, 0, 257, 10, 4) <= f(0, 0, 257, 10, 4) <= f(0, 0, 100000, 10, 4)
+    assert f(1, 1, 100000, 1 << 20, 4) < f(1, 0, 100000, 1 << 20, 4)
 
 
 def test_score_host_checks():

@@ -108,6 +108,12 @@ CASES = [  # n_rows, d, n, table, scale, indptr, ids, hot
     (2000, 300, 9000, "f32", "f32", "rows", torch.int32, 0.9),
     (2000, 6, 40_000, "f64", "f64", None, torch.int64, 0.9),
     (3, 36, 12_000, "f16", "f32", "rows", torch.int32, 0.4),
+    # a few ids: one launch
+    (300, 20, 256, "f32", "f32", "rows", torch.int32, 0.6),
+    (300, 20, 257, "f32", "f32", "rows", torch.int32, 0.6),
+    (1 << 20, 5, 100, "bf16", "f32", "inside", torch.int64, 0.3),
+    (9, 1500, 200, "f32", "f64", "rows", torch.int32, 0.9),
+    (70_000, 64, 3, "f16", None, None, torch.int64, 0.0),
 ]
 
 
