@@ -44,7 +44,7 @@ __device__ __forceinline__ double log_of(double v) { return log(v); }
 __device__ __forceinline__ float quotient(float a, float b) { return __fdividef(a, b); }  // 2 ulp
 __device__ __forceinline__ double quotient(double a, double b) { return a / b; }
 
-// sum + exp(v - off) over N values, and k exp(v - off) for each: two 32-bit lanes an
+// Sums of exp(v - off), and k exp(v - off) for each value: two 32-bit lanes an
 // instruction (the f32x2 forms round each lane as the scalar ones do), since
 // 16-bit scores are otherwise bound by issue slots, not by bytes.
 __device__ __forceinline__ uint64_t pair_of(float a, float b) {
