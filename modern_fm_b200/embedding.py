@@ -186,8 +186,12 @@ def _grad(grad, ids, n_rows, scale, indptr, alpha, table, dtype, stream, by_rows
         raise ValueError("n_rows must be >= 0")
     n = ids.numel()
     n_out = n if indptr is None else indptr.numel() - 1
-    if grad.dim() != 2:
-        grad = grad.reshape(-1, grad.shape[-1]) if grad.dim() > 2 else grad
+    source = grad
+    if grad.dim() > 2:  # a copy where the strides need one, made by the stream that reads it
+        with _NOTHING if stream is None else torch.cuda.stream(stream):
+            grad = grad.flatten(0, -2)
+    elif grad.dim() == 1 and ids.dim() == 0:
+        grad = grad[None]
     gp, given, d, ld = _matrix("grad", grad)
     if d < 1:
         raise ValueError("embedding width must be >= 1")
@@ -206,7 +210,7 @@ def _grad(grad, ids, n_rows, scale, indptr, alpha, table, dtype, stream, by_rows
     L = _lib.lib()
     nbytes = L.mfm_embedding_grad_workspace_bytes(code, 1 if by_rows else 0, n, n_rows, d)
     s, ctx = _on(stream, dev)
-    _hold(stream, grad, ids, scale, indptr, table)
+    _hold(stream, source, grad, ids, scale, indptr, table)
     keys = rows = count = whole = d_scale = None
     with ctx:
         ws = grad.new_empty(nbytes, dtype=torch.uint8) if nbytes else None

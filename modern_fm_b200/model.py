@@ -134,8 +134,11 @@ class DeviceModel:
         """``predict_device`` into a new tensor: (n_rows,) scores, or (n_rows, n_classes)."""
         import torch
 
+        from .embedding import _hold
+
         kind = self._device_csr(indptr, indices, data)
         n = indptr.numel() - 1
+        _hold(stream, indptr, indices, data)
         with torch.cuda.stream(stream):
             out = indptr.new_empty((n,) if self.n_classes == 1 else (n, self.n_classes),
                                    dtype=kind)
@@ -150,11 +153,14 @@ class DeviceModel:
         for dtype float32, float64 otherwise (summed in that type)."""
         import torch
 
+        from .embedding import _hold
+
         kind = self._device_csr(indptr, indices, data)
         n = indptr.numel() - 1
         shape = (n,) + ((self.n_fields,) if self.kind == "ffm" else ()) + (
             (self.n_classes,) if self.n_classes > 1 else ()) + (self.k,)
         s = stream if stream is not None else torch.cuda.current_stream(self.device)
+        _hold(stream, indptr, indices, data)
         with torch.cuda.stream(stream):
             out = indptr.new_empty(shape, dtype=kind)
         _check(_lib.lib().mfm_model_factors_device(

@@ -372,3 +372,25 @@ def test_two_streams_at_once():
     for x, y in got:
         assert torch.equal(x.table, want.table) and torch.equal(x.scale, want.scale)
         assert torch.equal(y.rows, rows.rows) and torch.equal(y.keys, rows.keys)
+
+
+def test_gradient_of_a_view_is_read_by_its_stream():
+    """A gradient that needs a copy is copied by the stream that the call runs on, behind the
+    work that writes it there; one id without an axis takes its result's shape."""
+    ids = torch.randint(0, 50, (64, 32), device="cuda")
+    base = torch.randn(32, 64, 24, device="cuda")
+    want = embedding_grad(base.transpose(0, 1).contiguous(), ids, 50).table
+    late = torch.zeros_like(base)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(20_000_000)
+        late.copy_(base)
+    got = embedding_grad(late.transpose(0, 1), ids, 50, stream=side).table
+    side.synchronize()
+    assert torch.equal(got, want)
+    table, one = torch.randn(9, 5, device="cuda"), torch.tensor(4, device="cuda")
+    row = embedding_lookup(table, one)
+    assert torch.equal(row, table[4])
+    g = embedding_grad(row, one, 9).table
+    assert torch.equal(g[4], row) and int(g.count_nonzero()) == 5

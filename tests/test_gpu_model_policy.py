@@ -113,3 +113,24 @@ def test_losses_of_a_resident_model(dtype, rtol):
             m.label_logprobs_device(*csr, yt)
         with pytest.raises(ValueError, match="n_classes >= 2"):
             preference_eval_device(m, *csr, yt, bt, t(ref))
+
+
+def test_inputs_freed_while_their_stream_still_runs():
+    """Scores and factors of another stream read their inputs before the memory is given away."""
+    X, w0, w, V, R, fid, _ = _case(3, "fm", 3, n=4000)
+    with _model("fm", 3, "float32", X, w0, w, V, R, fid) as m:
+        keep = _csr(X, "float32")
+        want = m.scores_device(*keep), m.factors_device(*keep)
+        side = torch.cuda.Stream()
+        torch.cuda.synchronize()
+        for call, expect in ((m.scores_device, want[0]), (m.factors_device, want[1])):
+            csr = [t.clone() for t in keep]
+            side.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(side):
+                torch.cuda._sleep(20_000_000)
+            got = call(*csr, stream=side)
+            del csr
+            again = [torch.zeros_like(t) for t in keep]  # would take the same places
+            side.synchronize()
+            assert torch.equal(got, expect)
+            del again
