@@ -446,7 +446,8 @@ int mfm_fit_csr_dp(mfm_dp* dp, int dtype, int model, int64_t n_classes, const mf
  * float64 / float32. MFM_DTYPE_F32_F64: float32 table, everything else and the
  * arithmetic float64. Sums have a fixed order: results are bitwise
  * reproducible. n_entries, n_out, n_rows and d < 2^31; their products are not
- * limited. out must not overlap the inputs. */
+ * limited, but rows that are summed by indptr have at most 2097120 values. out
+ * must not overlap the inputs. */
 
 /* out[t] = alpha scale[t] table[ids[t]], or its row sums; out (n_out, d) with
  * row pitch ld_out. */

@@ -1040,6 +1040,8 @@ extern "C" int mfm_embedding_lookup_device(int dtype, int device, int ids64, con
                                            void* stream) {
     return guarded([&] {
         check_embed(dtype, ids, n_entries, indptr, n_out, n_rows, d);
+        if (indptr && d > 65535 * 32)  // a grid's second axis, 32 values or more each
+            fail(MFM_ERR_UNSUPPORTED, fmt("rows of %lld values are too long to be summed", (long long)d));
         if (n_out == 0) return;
         if ((n_rows > 0 && !table) || !out) fail(MFM_ERR_INVALID, "table and out must be provided");
         check_pitch("table", ld_table, d);

@@ -66,7 +66,7 @@ struct Entries {
         const int lane = threadIdx.x & 31;
         int32_t base = 0, len = (int32_t)n_out;  // the first row is in [base, base + len]
         while (len > 0) {
-            const int32_t step = (len + 31) / 32;
+            const int32_t step = len / 32 + (len % 32 != 0);  // len + 31 may pass 2^31
             const int64_t p = (int64_t)(lane + 1) * step;
             const bool ends = p <= len && indptr[base + p] <= q0;
             const int n = __popc(__ballot_sync(0xffffffffu, ends));
@@ -74,7 +74,8 @@ struct Entries {
             const int32_t rest = len - n * step;
             len = rest < step - 1 ? (rest > 0 ? rest : 0) : step - 1;
         }
-        const int64_t end = base + lane < n_out ? indptr[base + lane + 1] : INT64_MAX;
+        const int64_t at = (int64_t)base + lane;
+        const int64_t end = at < n_out ? indptr[at + 1] : INT64_MAX;
 #pragma unroll
         for (int i = 0; i < M; ++i) {
             const int64_t q = q0 + 32 * i + lane;
@@ -451,7 +452,7 @@ __global__ void __launch_bounds__(kETileNT)
 #pragma unroll
         for (int u = 0; u < kETileItems; ++u) {
             const bool valid = t + u * kETileNT < m;
-            // n < 2^31 entries: at most 2^20 tiles of at most 2^12 digits
+            // fewer than 2^20 tiles of 2^12 digits, or 2^20 of 2^8
             const uint32_t bin = valid ? (dst[u] / kETile) * D + ((e[u].x >> (shift + bits)) & mask) : 0xffffffffu;
             if (valid) {
                 kout[dst[u]] = e[u].x;
@@ -574,7 +575,8 @@ struct IdSortPlan {
     IdSortPlan(int64_t n_, int64_t n_rows) : n(n_) {
         key_bits = id_key_bits(n_rows);
         const int narrow = (key_bits + 7) / 8, few = (key_bits + kWideBits - 1) / kWideBits;
-        wide = few < narrow;
+        // with 2^20 tiles of 2^12 digits the last count's index would be the mark of no entry
+        wide = few < narrow && ceil_div(n, kETile) < 1 << 20;
         passes = wide ? few : narrow;
         bits = wide ? (key_bits + passes - 1) / passes : 8;
         n_tiles = ceil_div(n, kETile);

@@ -181,3 +181,32 @@ def test_score_host_checks():
                     (dict(kl=0.1), "kl_coef needs reference"), (dict(old=None), "old_logprobs"),
                     (dict(ws=None), "workspace of")):
         assert policy(**kw) == -1 and msg in _lib.last_error(), msg
+
+
+@pytest.mark.parametrize("f", [embedding.embedding_grad, embedding.embedding_grad_rows])
+@pytest.mark.parametrize("grad,ids,msg", [
+    (_t(3), _t(dtype=I64), "must be a CUDA tensor"),  # one id without an axis: passes the shapes
+    (_t(2, 4, 3).transpose(0, 1), _t(4, 2, dtype=I64), "must be a CUDA tensor"),
+    (_t(2, 4, 0), _t(2, 4, dtype=I64), "width must be >= 1"),
+    (_t(3), _t(1, dtype=I64), "matrix with contiguous rows"),
+    (_t(2, 5, 3), _t(2, 4, dtype=I64), "one row per id"),
+])
+def test_gradient_of_ids_of_any_shape(f, grad, ids, msg):
+    with pytest.raises(ValueError, match=msg):
+        f(grad, ids, 7)
+
+
+def test_rows_too_long_to_be_summed():
+    d = 65536 * 32 + 1  # odd: a value a lane
+    got = _lib.lib().mfm_embedding_lookup_device(1, 0, 1, 16, 4, 16, 4, None, 1.0, 16, 5, d, d, 16, d,
+                                                 None)
+    assert got == -2 and "too long to be summed" in _lib.last_error()
+
+
+def test_workspace_of_the_most_entries():
+    """The sort of the most entries counts digits of 8 bits."""
+    f = _lib.lib().mfm_embedding_grad_workspace_bytes
+    n, rows = 2**31 - 1, 2**23
+    wide, narrow = f(1, 1, n - 2048, rows, 1), f(1, 1, n, rows, 1)
+    # 2 passes of 2^20 tiles' 2^12 digits against 3 passes of their 2^8
+    assert wide - narrow > (2 * 2**12 - 3 * 2**8) * 2**20 * 4 - 2**20
