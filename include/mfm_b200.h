@@ -432,6 +432,8 @@ int mfm_fit_csr_dp(mfm_dp* dp, int dtype, int model, int64_t n_classes, const mf
  * No reference counterpart (its latent rows never leave the kernels that score
  * with them). Every array is DEVICE memory on `device`; calls run on `stream`
  * (a cudaStream_t), allocate nothing, do not synchronise, and may be captured.
+ * Calls that may run at the same time, captured ones among them, need workspaces
+ * of their own.
  *
  * n_entries ids (int32, or int64 with ids64 = 1) select rows of a table
  * (n_rows, d) with row pitch ld_table elements. An id outside [0, n_rows) is
