@@ -184,9 +184,12 @@ struct RowArgs {
     // GRAD
     const A *g, *lse_in;
     const double* scale;  // factor of every g, NULL = 1
-    __device__ __forceinline__ A factor(int64_t t, int y, A l) const {
-        if (y < 0 || l == minus_inf<A>()) return A(0);
-        return scale ? (A)((double)g[t] * *scale) : g[t];
+    // The factor of a token's gradient: 0 for a masked one and for one whose derivative
+    // is 0 (of no sequence, or of a pair of weight 0), whatever the scale: weights that
+    // are NaN, or whose sum is too small to divide by, give one that is not finite.
+    __device__ __forceinline__ A factor(A g, int y, A l, double s) const {
+        if (y < 0 || l == minus_inf<A>() || g == A(0)) return A(0);
+        return scale ? (A)((double)g * s) : g;
     }
 };
 
@@ -365,8 +368,8 @@ __device__ __forceinline__ int first_column(int c) {
 }
 
 // The thread's row of the gradient: k e with e = exp(x - off) in v, and g + k e at the
-// label (its e in ey), rounded once; 0 for a token without one, whatever its scores
-// are. TURN: the thread's first column is not 0.
+// label (its e in ey), rounded once; 0 for a token without one (y < 0, where g is 0),
+// whatever its scores are. TURN: the thread's first column is not 0.
 template <class T, class A, int CW, bool TURN>
 __device__ __forceinline__ void small_grad(T* row, const A (&v)[CW], int c, int first, A g, A k, A ey,
                                            int y) {
@@ -377,7 +380,7 @@ __device__ __forceinline__ void small_grad(T* row, const A (&v)[CW], int c, int 
             row[TURN ? col : j] = narrow<T>(g == A(0) ? A(0) : v[j] * k);
             if (TURN) col = col + 1 == c ? 0 : col + 1;
         }
-    if (g != A(0)) row[y] = narrow<T>(g + k * ey);
+    if (y >= 0 && g != A(0)) row[y] = narrow<T>(g + k * ey);  // there is no row[-1]
 }
 
 // c <= CW classes, a row in a thread's registers.
@@ -467,8 +470,7 @@ __global__ void __launch_bounds__(kSmallNT, IsF64<A>::value || CW > 16 ? 4 : kSm
                     if (out) small_grad<T, A, CW, TURN>(row, v, c, first, g, quotient(-g, s), exp_of(at - off), y_now);
                 }
             } else {
-                A g = y_now >= 0 && off != minus_inf<A>() ? now.w : A(0);
-                if (a.scale) g = (A)((double)g * scale);
+                const A g = a.factor(now.w, y_now, off, scale);
 #pragma unroll
                 for (int j = 0; j < CW; ++j) v[j] = exp_of(v[j] - off);
                 small_grad<T, A, CW, TURN>(row, v, c, first, g, -g, exp_of(at - off), y_now);
@@ -598,8 +600,7 @@ __global__ void __launch_bounds__(kNT, cached_blocks<A>(K))
         A off, g = A(0), k = A(0);
         if (M == GRAD) {
             off = in ? a.lse_in[t] : A(0);
-            g = in && y >= 0 && off != minus_inf<A>() ? a.g[t] : A(0);
-            if (a.scale) g = (A)((double)g * scale);
+            g = a.factor(in ? a.g[t] : A(0), y, off, scale);
             k = -g;
         } else {
             A m = edge[0];
@@ -964,7 +965,7 @@ __global__ void __launch_bounds__(kNT)
     const RowShape<T> sh(row, (int)a.c);
     const bool whole = alike(row, to);
     const int y = a.labels.in(t, a.c);
-    const A l = a.lse_in[t], f = a.factor(t, y, l);
+    const A l = a.lse_in[t], f = a.factor(a.g[t], y, l, a.scale ? *a.scale : 1.0);
     const T xy = row[y >= 0 ? y : 0];
     const bool none = f == A(0);
     if (lane < sh.edges) {
