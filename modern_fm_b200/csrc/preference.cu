@@ -178,9 +178,12 @@ struct RowArgs {
     A clip_lo, clip_hi, kl_coef;  // ratio bounds
     const double* wpart;          // partial sums of the weights
     int n_wpart;
-    double* part;  // three sums per block
+    double* part;  // four sums per block
     A* stats;
-    unsigned* done;  // blocks finished
+    unsigned* done;      // blocks finished
+    unsigned* empties;   // set where a row with a label has no score but -inf
+    double* live_total;  // then: the weights' sum without such rows
+    const unsigned* only_if;  // a second pass: only if this is set, for the gradient alone
     // GRAD
     const A *g, *lse_in;
     const double* scale;  // factor of every g, NULL = 1
@@ -244,11 +247,11 @@ struct Token {
     }
 };
 
-// A token's derivative g, and its weighted loss terms e.
+// A token's derivative g, and its weighted loss terms and weight e.
 template <class A>
 __device__ __forceinline__ A policy_terms(const RowArgs<A>& a, const Token<A>& k, A lp, bool live,
-                                          A inv_total, A (&e)[3]) {
-    e[0] = e[1] = e[2] = A(0);
+                                          A inv_total, A (&e)[4]) {
+    e[0] = e[1] = e[2] = e[3] = A(0);
     // masked, or a token of weight 0: left out, whatever its ratio
     if (!live || k.w == A(0)) return A(0);
     const A ratio = exp_of(lp - k.old);
@@ -263,6 +266,7 @@ __device__ __forceinline__ A policy_terms(const RowArgs<A>& a, const Token<A>& k
     e[0] = k.w * (a.kl_coef * kl - (cut ? bent : ratio) * k.adv);
     e[1] = k.w * kl;
     e[2] = cut ? k.w : A(0);
+    e[3] = k.w;
     return k.w * slope * inv_total;
 }
 
@@ -288,26 +292,44 @@ __device__ __forceinline__ double weight_total(const RowArgs<A>& a) {  // on eve
 // 1 / the sum of the weights; weights that sum to 0 give gradient 0.
 __device__ __forceinline__ double inverse(double total) { return total != 0.0 ? 1.0 / total : 0.0; }
 
-// The block's three sums to `part`; the block that finishes last adds all of
-// them, in block order, into the results.
+// The block's four sums to `part`; the block that finishes last adds all of
+// them, in block order, into the results. `total` is what the labels alone say: where
+// rows turned out empty, the means are over the weights of the others (last sum).
 template <class A>
-__device__ __forceinline__ void policy_finish(const RowArgs<A>& a, const double (&e)[3],
+__device__ __forceinline__ void policy_finish(const RowArgs<A>& a, const double (&e)[4],
                                               double total, double* sm) {
     __shared__ unsigned last;
+    if (a.only_if) return;  // the first pass has done this
     if (threadIdx.x == 0) {
-        for (int i = 0; i < 3; ++i) a.part[3 * (int64_t)blockIdx.x + i] = e[i];
+        for (int i = 0; i < 4; ++i) a.part[4 * (int64_t)blockIdx.x + i] = e[i];
         __threadfence();
         last = atomicAdd(a.done, 1u) == gridDim.x - 1 ? 1u : 0u;
     }
     __syncthreads();
     if (!last) return;
     __threadfence();
-    for (int i = 0; i < 3; ++i) {
+    for (int i = 3; i >= 0; --i) {
+        if (i == 3 && !__ldcg(a.empties)) continue;
         double v = 0.0;
-        for (int64_t b = threadIdx.x; b < gridDim.x; b += blockDim.x) v += __ldcg(a.part + 3 * b + i);
+        for (int64_t b = threadIdx.x; b < gridDim.x; b += blockDim.x) v += __ldcg(a.part + 4 * b + i);
         v = block_sum(v, sm);
-        if (threadIdx.x == 0) a.stats[i] = total != 0.0 ? (A)(v / total) : A(0);
+        if (i == 3)
+            total = v;
+        else if (threadIdx.x == 0)
+            a.stats[i] = total != 0.0 ? (A)(v / total) : A(0);
     }
+    if (threadIdx.x == 0) *a.live_total = total;
+}
+
+// Whether this is a second pass without a row to be done again. The gradient is scaled
+// by the weights' sum, which may have been taken before any row's scores were read; a
+// row of -inf then counts there by its label. So the kernel is launched once more, with
+// the sum that leaves such rows out, and ends here unless there are any.
+template <class A>
+__device__ __forceinline__ bool idle_pass(const RowArgs<A>& a) {
+    if (!a.only_if) return false;
+    wait_previous();
+    return *a.only_if == 0;
 }
 
 // ------------------------------------------------------------ few classes --
@@ -393,9 +415,10 @@ __global__ void __launch_bounds__(kSmallNT, IsF64<A>::value || CW > 16 ? 4 : kSm
     const int c = (int)a.c, lane = threadIdx.x & 31;
     T* const tiles = reinterpret_cast<T*>(small_smem) + (threadIdx.x / 32) * (2 * kTileRows * c);
     const int first = TURN ? first_column<T>(c) : 0;
+    if (M == POLICY && idle_pass(a)) return;
     if (M == GRAD) wait_previous();
     const double scale = M == GRAD && a.scale ? *a.scale : 1.0;
-    double e[3] = {0.0, 0.0, 0.0};
+    double e[4] = {0.0, 0.0, 0.0, 0.0};
     const int64_t n_tiles = ceil_div(a.n, (int64_t)kTileRows), step = (int64_t)gridDim.x * (kSmallNT / 32);
     int64_t tile = (int64_t)blockIdx.x * (kSmallNT / 32) + threadIdx.x / 32;
     // the gradient goes from the last row to the first: the forward that read the
@@ -464,9 +487,10 @@ __global__ void __launch_bounds__(kSmallNT, IsF64<A>::value || CW > 16 ? 4 : kSm
                     if (a.lse) a.lse[t] = empty ? minus_inf<A>() : off + ls;
                     if (a.zero) a.zero[t] = A(0);
                 } else {
-                    A f[3];
+                    A f[4];
                     const A g = policy_terms(a, now, lp, live, (A)inv, f);
-                    for (int i = 0; i < 3; ++i) e[i] += (double)f[i];
+                    for (int i = 0; i < 4; ++i) e[i] += (double)f[i];
+                    if (empty && y_now >= 0) *a.empties = 1;
                     if (out) small_grad<T, A, CW, TURN>(row, v, c, first, g, quotient(-g, s), exp_of(at - off), y_now);
                 }
             } else {
@@ -484,7 +508,7 @@ __global__ void __launch_bounds__(kSmallNT, IsF64<A>::value || CW > 16 ? 4 : kSm
     if (M == STATS) {
         if (a.counter && blockIdx.x == 0 && threadIdx.x == 0) *a.counter = 0;
     } else if (M == POLICY) {
-        for (int i = 0; i < 3; ++i) e[i] = block_sum(e[i], sm);
+        for (int i = 0; i < 4; ++i) e[i] = block_sum(e[i], sm);
         policy_finish(a, e, total, sm);
     }
 }
@@ -537,7 +561,7 @@ __device__ __forceinline__ void store16(T* at, const A (&v)[Pack<T>::N], bool wh
 template <class T, class A, Mode M>
 struct RowResult {
     A g = A(0), k = A(0);
-    A e[3] = {A(0), A(0), A(0)};
+    A e[4] = {A(0), A(0), A(0), A(0)};
     __device__ __forceinline__ RowResult(const RowArgs<A>& a, const Token<A>& tok, int64_t t,
                                          int y, T xy, A m, A s, double inv_total, bool first) {
         const A off = offset_of(m);
@@ -553,6 +577,7 @@ struct RowResult {
         } else {
             g = policy_terms(a, tok, lp, live, (A)inv_total, e);
             k = quotient(-g, s);
+            if (first && empty && y >= 0) *a.empties = 1;
         }
     }
 };
@@ -570,11 +595,15 @@ __global__ void __launch_bounds__(kNT, cached_blocks<A>(K))
     constexpr int V = 16 / sizeof(T), R = 32 / L;            // rows per warp
     constexpr int E = (2 * (V - 1) + L - 1) / L;             // edge elements per lane
     __shared__ double sums[kNT / 32];
-    const int lane = threadIdx.x % L;
+    // a group's terms: in registers they would cost every lane eight (and spill)
+    __shared__ double terms[M == POLICY ? 4 : 1][kNT / L];
+    const int lane = threadIdx.x % L, group = threadIdx.x / L;
+    if (M == POLICY && idle_pass(a)) return;
     if (M == GRAD) wait_previous();
     const double total = M == POLICY ? weight_total(a) : 0.0, inv = inverse(total);
     const double scale = M == GRAD && a.scale ? *a.scale : 1.0;
-    double e[3] = {0.0, 0.0, 0.0};
+    if (M == POLICY && lane == 0)
+        for (int i = 0; i < 4; ++i) terms[i][group] = 0.0;
     const int64_t warps = (int64_t)gridDim.x * (kNT / 32);
     for (int64_t t0 = ((int64_t)blockIdx.x * (kNT / 32) + threadIdx.x / 32) * R; t0 < a.n; t0 += warps * R) {
         // the gradient goes from the last row to the first: the forward that read
@@ -628,7 +657,7 @@ __global__ void __launch_bounds__(kNT, cached_blocks<A>(K))
                 g = r.g;
                 k = r.k;
                 if (M == POLICY && lane == 0)
-                    for (int i = 0; i < 3; ++i) e[i] += (double)r.e[i];
+                    for (int i = 0; i < 4; ++i) terms[i][group] += (double)r.e[i];
             }
         }
         if (M != STATS && out && in) {
@@ -662,7 +691,8 @@ __global__ void __launch_bounds__(kNT, cached_blocks<A>(K))
     if (M == STATS) {
         if (a.counter && blockIdx.x == 0 && threadIdx.x == 0) *a.counter = 0;
     } else if (M == POLICY) {
-        for (int i = 0; i < 3; ++i) e[i] = block_sum(e[i], sums);
+        double e[4];
+        for (int i = 0; i < 4; ++i) e[i] = block_sum(lane == 0 ? terms[i][group] : 0.0, sums);
         policy_finish(a, e, total, sums);
     }
 }
@@ -797,6 +827,7 @@ __global__ void __launch_bounds__(L + 32, ring_blocks(L))
     __shared__ double sums[32];
     __shared__ int stop_flag;
     volatile int* stop = &stop_flag;
+    if (idle_pass(a)) return;
     if (threadIdx.x == 0) {
         stop_flag = 0;
         for (int i = 0; i < S; ++i) {
@@ -807,7 +838,7 @@ __global__ void __launch_bounds__(L + 32, ring_blocks(L))
     }
     __syncthreads();
     const bool grad = out != nullptr;
-    double e[3] = {0.0, 0.0, 0.0}, total = 0.0;
+    double e[4] = {0.0, 0.0, 0.0, 0.0}, total = 0.0;
     if (threadIdx.x >= L) {
         if (threadIdx.x == L) {
             unsigned seq = 0;
@@ -891,7 +922,7 @@ __global__ void __launch_bounds__(L + 32, ring_blocks(L))
             r.s = (lane & 31) < W ? sm_s[it & 1][lane & 31] : A(0);
             across(r, 32);
             const RowResult<T, A, POLICY> res(a, tok, t, y, xy, r.m, r.s, inv, lane == 0);
-            for (int i = 0; i < 3; ++i) e[i] += (double)res.e[i];
+            for (int i = 0; i < 4; ++i) e[i] += (double)res.e[i];
             if (grad) {
                 T* to = out + t * ld_out;
                 const bool whole = alike(row, to), none = res.g == A(0);
@@ -936,7 +967,7 @@ __global__ void __launch_bounds__(L + 32, ring_blocks(L))
             }
             if (*stop && lane == 0) {
                 a.lp[t] = (A)NAN;
-                e[0] = e[1] = e[2] = NAN;
+                e[0] = e[1] = e[2] = e[3] = NAN;
             }
             y = y_next;
         }
@@ -1089,13 +1120,47 @@ __global__ void zero_loss_kernel(A* v, int n) {  // nothing to take a mean of
 
 constexpr int kWeightBlocks = 512;
 
-// Partial sums of the unmasked tokens' weights; also clears the losses' block count.
+// Whether a row has no score but -infinity, by a whole warp.
+template <class T>
+__device__ __forceinline__ bool empty_row(const T* row, int c) {
+    using A = typename Arith<T>::type;
+    constexpr int V = Pack<T>::N, U = 4;
+    const int lane = threadIdx.x & 31;
+    const RowShape<T> sh(row, c);
+    // != also holds for NaN, which is no empty row
+    bool some = lane < sh.edges && widen<A>(row[sh.edge(lane)]) != minus_inf<A>();
+    for (int j0 = 0; j0 < sh.nv && !__any_sync(0xffffffffu, some); j0 += 32 * U) {
+        uint4 v[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int j = j0 + u * 32 + lane;
+            v[u] = j < sh.nv ? load16(row + sh.head + j * V) : Pack<T>::minus_inf();
+        }
+        const uint4 none = Pack<T>::minus_inf();
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            some |= v[u].x != none.x || v[u].y != none.y || v[u].z != none.z || v[u].w != none.w;
+    }
+    return !__any_sync(0xffffffffu, some);
+}
+
+// A block's sum of weights; the first block clears the losses' block count and the mark
+// of empty rows.
+__device__ __forceinline__ void weight_part(double a, double* part, unsigned* done, unsigned* empties) {
+    __shared__ double sm[kNT / 32];
+    a = block_sum(a, sm);
+    if (threadIdx.x == 0) {
+        part[blockIdx.x] = a;
+        if (blockIdx.x == 0) *done = *empties = 0;
+    }
+}
+
+// Partial sums of the weights of the tokens with a label.
 template <class A>
 __global__ void __launch_bounds__(kNT)
     weight_kernel(Labels labels, int64_t c, const A* __restrict__ weight, int64_t n,
-                  double* __restrict__ part, unsigned* __restrict__ done) {
+                  double* __restrict__ part, unsigned* __restrict__ done, unsigned* __restrict__ empties) {
     let_next();  // the rows' kernel needs the weights only once it has its first rows
-    __shared__ double sm[kNT / 32];
     double a = 0.0;
     constexpr int U = 8;  // tokens in flight per thread
     for (int64_t t0 = (int64_t)blockIdx.x * kNT * U + threadIdx.x; t0 < n; t0 += (int64_t)gridDim.x * kNT * U) {
@@ -1111,12 +1176,43 @@ __global__ void __launch_bounds__(kNT)
         for (int u = 0; u < U; ++u)
             if (y[u] >= 0) a += (double)w[u];
     }
-    a = block_sum(a, sm);
-    if (threadIdx.x == 0) {
-        part[blockIdx.x] = a;
-        if (blockIdx.x == 0) *done = 0;
-    }
+    weight_part(a, part, done, empties);
 }
+
+// The same without rows of -infinity: a row is looked at at its label's score, and read,
+// up to the first score that is not -infinity, only where that one is. A warp takes
+// `per` neighbouring tokens.
+template <class T, class A>
+__global__ void __launch_bounds__(kNT)
+    weight_look_kernel(const T* __restrict__ x, int64_t ld, Labels labels, int64_t c,
+                       const A* __restrict__ weight, int64_t n, int per, double* __restrict__ part,
+                       unsigned* __restrict__ done, unsigned* __restrict__ empties) {
+    let_next();
+    double a = 0.0;
+    const int lane = threadIdx.x & 31;
+    const int64_t lo = ((int64_t)blockIdx.x * (kNT / 32) + threadIdx.x / 32) * per;
+    const int64_t hi = lo + per < n ? lo + per : n;
+    for (int64_t t0 = lo; t0 < hi; t0 += 32) {
+        const int64_t t = t0 + lane;
+        const int y = t < hi ? labels.in(t, c) : -1;
+        const A w = weight && t < hi ? weight[t] : A(1);
+        bool live = y >= 0;
+        const bool low = live && widen<A>(x[t * ld + y]) == minus_inf<A>();
+        for (unsigned m = __ballot_sync(0xffffffffu, low); m; m &= m - 1) {
+            const int l = __ffs(m) - 1;
+            if (empty_row(x + (t0 + l) * ld, (int)c) && l == lane) live = false;
+        }
+        if (live) a += (double)w;
+    }
+    weight_part(a, part, done, empties);
+}
+
+// Whether the weights are added up beside a look at the scores, or the rows' kernel is
+// launched a second time in case that rows turn out empty. Small calls are bound by
+// their launches (64 x 1000 bf16: 29 us a call with the look, 32 us with a second
+// launch), large ones would read a sector of every row once more (1000003 x 10 float32:
+// 44.7 us against 43.7 us; 16000 x 5000 float64: 635 us against 612 us).
+inline bool looks_at_scores(int64_t n, int64_t c) { return n <= 65536 && n * c <= 1 << 22; }
 
 // ------------------------------------------------------------- launchers --
 
@@ -1438,11 +1534,11 @@ extern "C" int mfm_preference_loss_device(int dtype, int device, const void* log
 }
 
 namespace {
-struct PolicyWs {  // partial weights and a block count, partial loss terms
+struct PolicyWs {  // partial weights, a block count, the mark and the sum of empty rows, partial loss terms
     size_t part, bytes;
     explicit PolicyWs(int64_t n) {
-        part = up256(kWeightBlocks * 8 + 8);
-        bytes = part + up256((size_t)n * 24);
+        part = up256(kWeightBlocks * 8 + 16);
+        bytes = part + up256((size_t)n * 32);
     }
 };
 }  // namespace
@@ -1476,8 +1572,10 @@ extern "C" int mfm_policy_loss_device(int dtype, int device, const void* logits,
         cudaStream_t s = (cudaStream_t)stream;
         char* ws = (char*)workspace;
         double *wpart = (double*)ws, *part = (double*)(ws + W.part);
-        unsigned* done = (unsigned*)(wpart + kWeightBlocks);
-        const int nw = (int)std::min<int64_t>(kWeightBlocks, ceil_div(n_tokens, 8 * kNT));
+        unsigned *done = (unsigned*)(wpart + kWeightBlocks), *empties = done + 1;
+        const bool look = looks_at_scores(n_tokens, n_classes);
+        // eight tokens a warp that looks, eight a thread otherwise, more beyond the most blocks
+        const int nw = (int)std::min<int64_t>(kWeightBlocks, ceil_div(n_tokens, look ? 8 * (kNT / 32) : 8 * kNT));
         with_score_types(dtype, [&](auto* t) {
             using T = Elem<decltype(t)>;
             using A = typename Arith<T>::type;
@@ -1501,8 +1599,20 @@ extern "C" int mfm_policy_loss_device(int dtype, int device, const void* logits,
                 a.part = part;
                 a.stats = (A*)stats;
                 a.done = done;
-                weight_kernel<A><<<nw, kNT, 0, s>>>(a.labels, n_classes, a.weight, n_tokens, wpart, done);
+                a.empties = empties;
+                a.live_total = wpart + kWeightBlocks + 1;
+                if (look)
+                    weight_look_kernel<T, A><<<nw, kNT, 0, s>>>((const T*)logits, ld, a.labels, n_classes, a.weight, n_tokens,
+                                                                (int)ceil_div(n_tokens, (int64_t)nw * (kNT / 32)), wpart, done, empties);
+                else
+                    weight_kernel<A><<<nw, kNT, 0, s>>>(a.labels, n_classes, a.weight, n_tokens, wpart, done, empties);
                 rows_launch<T, A, POLICY>(device, (const T*)logits, ld, (T*)d_logits, ld_out, a, s);
+                if (d_logits && !look) {
+                    a.wpart = a.live_total;
+                    a.n_wpart = 1;
+                    a.only_if = empties;
+                    rows_launch<T, A, POLICY>(device, (const T*)logits, ld, (T*)d_logits, ld_out, a, s);
+                }
             }
             MFM_CHECK_LAUNCH("policy loss launch");
         });

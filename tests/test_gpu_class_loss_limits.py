@@ -13,9 +13,10 @@ pytestmark = pytest.mark.gpu
 
 torch = pytest.importorskip("torch")
 
-from modern_fm_b200.preference import preference_loss  # noqa: E402
+from modern_fm_b200.preference import policy_loss, preference_loss  # noqa: E402
 
-from test_gpu_preference import TYPES, _make, _wide  # noqa: E402
+from test_gpu_preference import (TYPES, _check_grad, _define, _make, _tol, _u,  # noqa: E402
+                                 _wide)
 
 
 @pytest.mark.parametrize("c", [10, 32, 100, 9001])
@@ -46,3 +47,101 @@ def test_masked_rows_under_a_scale_that_is_not_finite(c, kind):
     w = torch.tensor([0.0, 5e-324 if kind == "f64" else 1e-45], dtype=wide, device="cuda")
     r = preference_loss(x, y, ip, ref, sample_weight=w)
     assert bool((r.grad[~live | ~inside | first] == 0).all())
+
+
+# 2^22 scores or 65536 rows are where the sum of the weights is found in another way
+@pytest.mark.parametrize("n,c", [(1, 3), (40, 10), (40, 32), (300, 100), (3, 2049), (50, 9001),
+                                 (70_001, 3), (140_000, 31), (45_000, 100), (2100, 2049),
+                                 (470, 9001)])
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("weighted", [False, True])
+def test_policy_mean_without_empty_rows(n, c, kind, weighted):
+    """A row whose every score is -infinity is masked as one without a label is: the means
+    and the gradient of the others are those without it, also with a NaN for its weight."""
+    x, y = _make(2, n, c, kind)
+    gen = torch.Generator().manual_seed(3)
+    empty = torch.rand(n, generator=gen) < 0.3
+    some = min(2, n - 1)
+    empty[1:2] = True
+    empty[some] = False
+    empty = empty.cuda()
+    x[empty] = -math.inf
+    y[1:2] = c - 1
+    y[some] = 0
+    wide = _wide(kind)
+    u, e = _u(wide), _tol(x, wide)
+    lp, _, _, live = _define(x, y)
+    assert not bool(live[1:2].any()) and bool(live[some])
+    old = (lp + 0.1).to(wide)  # ratios of exp(-0.1): inside the clip's bounds
+    ref = (lp - 0.3).to(wide)
+    adv = torch.randn(n, generator=gen, dtype=wide).cuda()
+    w = (torch.rand(n, generator=gen, dtype=wide) + 0.5).cuda() if weighted else None
+    if weighted:
+        w[1:2] = math.nan
+    got = policy_loss(x, y, old, adv, ref, kl_coef=0.1, sample_weight=w)
+    a, away = adv.double(), ref.double() - lp
+    ratio = torch.exp(lp - old.double())
+    ww = torch.where(live, w.double() if weighted else torch.ones_like(lp), 0.0)
+    ww = ww / ww.sum()
+    k = torch.expm1(away) - away
+    loss, kl = float((ww * (0.1 * k - ratio * a)).sum()), float((ww * k).sum())
+    # a log-probability's error e moves a term by its slope times e; exp(u) - u - 1 loses
+    # up to 4 u of its terms
+    move = (e + 8 * u) * (ratio * a.abs() + 0.1 * (1 + k) + k)
+    tol = float((ww * move).sum()) + 4 * u
+    assert abs(float(got.loss) - loss) <= tol
+    assert abs(float(got.kl) - kl) <= float((ww * (e + 8 * u)).sum()) + 4 * u
+    assert float(got.clip_fraction) == 0.0
+    assert bool((got.logprobs[~live] == 0).all())
+    g = ww * (-ratio * a - 0.1 * torch.expm1(away))
+    dg = ww * (ratio * a.abs() + 0.1 * torch.exp(away)) * (e + 8 * u) + 4 * u * g.abs()
+    _check_grad(got.grad, x, y, g, dg, wide)
+    only = policy_loss(x, y, old, adv, ref, kl_coef=0.1, sample_weight=w, with_grad=False)
+    assert torch.equal(only.loss, got.loss) and torch.equal(only.kl, got.kl)
+    # the clipped share is of the unmasked rows too
+    far = policy_loss(x, y, old - 5, adv.abs() + 0.1, sample_weight=w, with_grad=False)
+    assert float(far.clip_fraction) == pytest.approx(1.0, abs=4 * u)
+
+
+@pytest.mark.parametrize("n,c", [(30, 10), (30, 100), (30, 9001), (70_000, 10), (45_000, 100),
+                                 (500, 9001)])
+def test_policy_of_empty_rows_alone_and_in_a_graph(n, c):
+    """Nothing but empty rows: 0. A captured call whose rows turn empty, and back."""
+    x, y = _make(4, n, c, "f32", pad=0.0)
+    z = torch.zeros(n, device="cuda")
+    r = policy_loss(torch.full_like(x, -math.inf), y, z, z + 1, z, kl_coef=0.1)
+    assert float(r.loss) == float(r.kl) == float(r.clip_fraction) == 0.0
+    assert bool((r.grad == 0).all())
+    some = x.clone()
+    some[::3] = -math.inf
+    want = [policy_loss(v, y, z - 2, z + 1, z - 2, kl_coef=0.1) for v in (x, some)]
+    graph = torch.cuda.CUDAGraph()
+    at = x.clone()
+    with torch.cuda.graph(graph):
+        got = policy_loss(at, y, z - 2, z + 1, z - 2, kl_coef=0.1)
+    for v, expect in ((x, want[0]), (some, want[1]), (x, want[0])):
+        at.copy_(v)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(got, expect))
+
+
+@pytest.mark.parametrize("n,c", [(40, 10), (40, 100), (40, 9001), (70_000, 10), (45_000, 100),
+                                 (500, 9001)])
+@pytest.mark.parametrize("lo", [0, 1])
+def test_policy_weight_of_a_row_with_any_score(n, c, lo):
+    """A row with a score somewhere is not empty: its weight counts, whichever score that is
+    and whatever its label's score is; also where rows begin off 16 bytes."""
+    x = torch.full((n, c + lo), -math.inf, device="cuda", dtype=torch.bfloat16)[:, lo:]
+    row = torch.arange(n, device="cuda")
+    x[row, row % c] = 1.0
+    x[-1] = -math.inf
+    y = ((row + 1) % c).int()  # a score of -infinity: ratio 0, no loss, no gradient
+    y[::3] = (row % c)[::3].int()  # the only score: log-probability 0
+    y[-2] = int(row[-2]) % c
+    z = torch.zeros(n, device="cuda")
+    r = policy_loss(x, y, z, z + 1)
+    mine = (y == row % c) & (row < n - 1)
+    # ratios of 1 and 0, advantages of 1: minus the share of the first among n - 1 rows
+    assert float(r.loss) == pytest.approx(-int(mine.sum()) / (n - 1), rel=2.0**-22)
+    assert bool((r.logprobs[mine] == 0).all()) and bool((r.grad == 0).all())
