@@ -1260,7 +1260,8 @@ void small_launch(int device, const T* x, int64_t ld, T* out, int64_t ld_out, co
     auto go = [&](auto w, auto turn) {
         auto k = small_rows_kernel<T, A, decltype(w)::value, decltype(turn)::value, M>;
         static bool asked[64];
-        if (bytes > 48 * 1024) allow_smem(k, device, 64 * 1024, asked, "class tile shared memory");
+        // the kernel's own arrays count towards the 48 KB that need no asking
+        if (bytes + 1024 > 48 * 1024) allow_smem(k, device, 64 * 1024, asked, "class tile shared memory");
         launch_rows<M>(
             k, (unsigned)std::min(blocks, most), kSmallNT, bytes, s, x, ld, out, ld_out, a, ld == a.c && (uintptr_t)x % 16 == 0, ld_out == a.c && (uintptr_t)out % 16 == 0);
     };

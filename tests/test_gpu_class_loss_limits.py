@@ -6,6 +6,8 @@ test_gpu_preference.
 """
 
 import math
+import subprocess
+import sys
 
 import pytest
 
@@ -145,3 +147,35 @@ def test_policy_weight_of_a_row_with_any_score(n, c, lo):
     # ratios of 1 and 0, advantages of 1: minus the share of the first among n - 1 rows
     assert float(r.loss) == pytest.approx(-int(mine.sum()) / (n - 1), rel=2.0**-22)
     assert bool((r.logprobs[mine] == 0).all()) and bool((r.grad == 0).all())
+
+
+def _policy_of_classes(c, kind):
+    x, y = _make(6, 70, c, kind)
+    y[0] = 0
+    wide = _wide(kind)
+    u, e = _u(wide), _tol(x, wide)
+    lp, _, _, live = _define(x, y)
+    old = (lp + 0.1).to(wide)  # inside the clip's bounds
+    adv = torch.randn(70, generator=torch.Generator().manual_seed(7), dtype=wide).cuda()
+    got = policy_loss(x, y, old, adv)
+    ratio, share = torch.exp(lp - old.double()), live.double() / live.sum()
+    want = float(-(share * ratio * adv.double()).sum())
+    move = (share * ratio * adv.double().abs()) * (e + 8 * u)
+    assert abs(float(got.loss) - want) <= float(move.sum()) + 4 * u
+    _check_grad(got.grad, x, y, -share * ratio * adv.double(), move, wide)
+
+
+@pytest.mark.parametrize("c", range(1, 35))
+@pytest.mark.parametrize("kind", list(TYPES))
+def test_policy_of_every_small_number_of_classes(c, kind):
+    _policy_of_classes(c, kind)
+
+
+def test_the_first_call_of_a_process_has_24_float64_classes():
+    """Its tiles fill the shared memory that needs no asking, its own arrays go beyond; no call
+    before it has asked for more."""
+    code = ("import test_gpu_class_loss_limits as t\n"
+            "for c in (24, 23, 25, 32): t._policy_of_classes(c, 'f64')\n")
+    r = subprocess.run([sys.executable, "-c", "import sys; sys.path[:0] = " + repr(sys.path) + "\n" + code],
+                       capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]
