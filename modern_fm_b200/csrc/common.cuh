@@ -29,12 +29,16 @@ std::string fmt(const char* f, ...);
 [[noreturn]] void fail(int code, const std::string& msg);
 void set_last_error(const std::string& msg);
 
+// The runtime keeps a failure for the next cudaGetLastError: it is taken out here, or
+// the next call's launch check would report it once more.
 #define MFM_CUDA(call, what)                                                        \
     do {                                                                            \
         cudaError_t e_ = (call);                                                    \
-        if (e_ != cudaSuccess)                                                      \
+        if (e_ != cudaSuccess) {                                                    \
+            cudaGetLastError();                                                     \
             ::mfm::fail(MFM_ERR_CUDA, ::mfm::fmt("CUDA %s failed: %s", (what),      \
                                                  cudaGetErrorString(e_)));          \
+        }                                                                           \
     } while (0)
 
 #define MFM_CHECK_LAUNCH(what) MFM_CUDA(cudaGetLastError(), what)
