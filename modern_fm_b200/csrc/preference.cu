@@ -1088,7 +1088,10 @@ __global__ void __launch_bounds__(kNT)
             sums[p] = (A)s[0];
             sums[n_pairs + p] = (A)s[1];
             const double soft = log1p(exp(-fabs(z)));
-            pair_loss[p] = w == 0.0 ? 0.0 : w * (soft + (1.0 - eps) * fmax(-z, 0.0) + eps * fmax(z, 0.0));
+            // a margin may be infinite (a label whose score is -infinity): a side without a
+            // factor is left out, not multiplied by 0
+            const double wrong = eps < 1.0 ? (1.0 - eps) * fmax(-z, 0.0) : 0.0, right = eps > 0.0 ? eps * fmax(z, 0.0) : 0.0;
+            pair_loss[p] = w == 0.0 ? 0.0 : w * (soft + wrong + right);
         }
         if (g)
             for (int i = 0; i < 2; ++i)

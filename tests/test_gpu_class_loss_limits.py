@@ -179,3 +179,25 @@ def test_the_first_call_of_a_process_has_24_float64_classes():
     r = subprocess.run([sys.executable, "-c", "import sys; sys.path[:0] = " + repr(sys.path) + "\n" + code],
                        capture_output=True, text=True, timeout=300)
     assert r.returncode == 0, r.stderr[-2000:]
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("eps,first", [(0.0, 1), (1.0, 0)])
+def test_preference_of_an_infinite_margin(kind, eps, first):
+    """A label that cannot be drawn on the side that should lose: the pair's loss is 0 as the
+    limit says, and the mean is the other pair's; on the other side the loss is infinite."""
+    x, y = _make(8, 8, 10, kind, pad=0.0)
+    y[:] = 3
+    x[4 * first, 3] = -math.inf  # of pair 0's second sequence, or of its first one
+    ip = torch.tensor([0, 2, 4, 6, 8], device="cuda")
+    ref = torch.zeros(4, dtype=_wide(kind), device="cuda")
+    r = preference_loss(x, y, ip, ref, 0.5, eps)
+    assert float(r.margins[0]) == (math.inf if first else -math.inf)
+    s = _define(x, y)[0].reshape(4, 2).sum(1)
+    z = 0.5 * float(s[1] - s[3])
+    e = 0.5 * 4 * _tol(torch.where(torch.isinf(x), 0.0, x), _wide(kind))
+    want = math.log1p(math.exp(z if eps else -z)) / 2
+    assert float(r.loss) == pytest.approx(want, abs=e + 4 * _u(_wide(kind)))
+    assert bool((r.grad[[0, 1, 4, 5]] == 0).all()) and torch.isfinite(r.grad.double()).all()
+    half = preference_loss(x, y, ip, ref, 0.5, 0.5)
+    assert float(half.loss) == math.inf and torch.isfinite(half.grad.double()).all()
