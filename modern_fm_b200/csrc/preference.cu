@@ -212,12 +212,12 @@ __device__ __forceinline__ void kl_terms(float u, float& em1, float& kl) {
         em1 = u + kl;
     } else {
         em1 = exp_of(u) - 1.0f;
-        kl = em1 - u;
+        kl = u == INFINITY ? u : em1 - u;
     }
 }
 __device__ __forceinline__ void kl_terms(double u, double& em1, double& kl) {
     em1 = expm1(u);
-    kl = em1 - u;
+    kl = u == INFINITY ? u : em1 - u;
     if (fabs(u) < 0.125) {
         double r = 1.0 / 6227020800.0;
         r = r * u + 1.0 / 479001600.0;

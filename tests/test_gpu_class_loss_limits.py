@@ -201,3 +201,26 @@ def test_preference_of_an_infinite_margin(kind, eps, first):
     assert bool((r.grad[[0, 1, 4, 5]] == 0).all()) and torch.isfinite(r.grad.double()).all()
     half = preference_loss(x, y, ip, ref, 0.5, 0.5)
     assert float(half.loss) == math.inf and torch.isfinite(half.grad.double()).all()
+
+
+@pytest.mark.parametrize("c", [10, 100, 9001])
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("side", ["model", "reference"])
+def test_policy_kl_term_without_end(c, kind, side):
+    """A label that the model or the reference cannot draw: exp(u) - u - 1 is infinite on both
+    sides, and so are the mean and a loss that has the term in it."""
+    x, y = _make(9, 20, c, kind, pad=0.0)
+    y[:] = 2
+    one = torch.ones(20, dtype=_wide(kind), device="cuda")
+    ref = -one
+    if side == "model":
+        x[3, 2] = -math.inf
+    else:
+        ref[3] = -math.inf
+    r = policy_loss(x, y, -2 * one, one, ref, kl_coef=0.1)
+    assert float(r.kl) == float(r.loss) == math.inf
+    rest = torch.arange(20, device="cuda") != 3
+    # a slope of 0.1 exp(u) / 20 beyond float16's 65504 (u > 16.4, lp < -17.4) is infinite there
+    assert not torch.isnan(r.grad[rest]).any()
+    if side == "reference":  # the term's slope is 1 there
+        assert not torch.isnan(r.grad).any()
