@@ -257,13 +257,16 @@ __device__ __forceinline__ A policy_terms(const RowArgs<A>& a, const Token<A>& k
     const A ratio = exp_of(lp - k.old);
     const A bent = fmin(fmax(ratio, a.clip_lo), a.clip_hi);
     const bool cut = ratio * k.adv > bent * k.adv;
-    A slope = cut ? A(0) : -ratio * k.adv, kl = A(0);
+    A slope = cut ? A(0) : -ratio * k.adv, kl = A(0), part = A(0);
     if (a.ref) {
         A em1;
         kl_terms(k.ref - lp, em1, kl);
-        slope -= a.kl_coef * em1;
+        if (a.kl_coef != A(0)) {  // without one the term may be infinite, and is not the loss's
+            slope -= a.kl_coef * em1;
+            part = a.kl_coef * kl;
+        }
     }
-    e[0] = k.w * (a.kl_coef * kl - (cut ? bent : ratio) * k.adv);
+    e[0] = k.w * (part - (cut ? bent : ratio) * k.adv);
     e[1] = k.w * kl;
     e[2] = cut ? k.w : A(0);
     e[3] = k.w;

@@ -224,3 +224,20 @@ def test_policy_kl_term_without_end(c, kind, side):
     assert not torch.isnan(r.grad[rest]).any()
     if side == "reference":  # the term's slope is 1 there
         assert not torch.isnan(r.grad).any()
+
+
+@pytest.mark.parametrize("c", [10, 100, 9001])
+@pytest.mark.parametrize("kind", list(TYPES))
+def test_policy_kl_without_a_coefficient(c, kind):
+    """With kl_coef 0 the reference only gives the statistic, also where that is infinite: loss
+    and gradient are those without a reference."""
+    x, y = _make(9, 20, c, kind, pad=0.0)
+    y[:] = 2
+    x[3, 2] = -math.inf  # log-probability -infinity: an infinite term
+    x[4, 2] = -2000.0  # exp(reference - lp) overflows in 64 bits
+    one = torch.ones(20, dtype=_wide(kind), device="cuda")
+    a = policy_loss(x, y, -2 * one, one, -one)
+    b = policy_loss(x, y, -2 * one, one)
+    assert float(a.kl) == math.inf and math.isfinite(float(b.loss))
+    assert torch.equal(a.loss, b.loss) and torch.equal(a.clip_fraction, b.clip_fraction)
+    assert torch.equal(a.grad, b.grad) and torch.isfinite(a.grad.double()).all()
