@@ -256,8 +256,10 @@ __device__ __forceinline__ A policy_terms(const RowArgs<A>& a, const Token<A>& k
     if (!live || k.w == A(0)) return A(0);
     const A ratio = exp_of(lp - k.old);
     const A bent = fmin(fmax(ratio, a.clip_lo), a.clip_hi);
-    const bool cut = ratio * k.adv > bent * k.adv;
-    A slope = cut ? A(0) : -ratio * k.adv, kl = A(0), part = A(0);
+    // no advantage, no term, also where the ratio is beyond the type's range
+    const A plain = k.adv == A(0) && ratio == ratio ? A(0) : ratio * k.adv;
+    const bool cut = plain > bent * k.adv;
+    A slope = cut ? A(0) : -plain, kl = A(0), part = A(0);
     if (a.ref) {
         A em1;
         kl_terms(k.ref - lp, em1, kl);
@@ -266,7 +268,7 @@ __device__ __forceinline__ A policy_terms(const RowArgs<A>& a, const Token<A>& k
             part = a.kl_coef * kl;
         }
     }
-    e[0] = k.w * (part - (cut ? bent : ratio) * k.adv);
+    e[0] = k.w * (part - (cut ? bent * k.adv : plain));
     e[1] = k.w * kl;
     e[2] = cut ? k.w : A(0);
     e[3] = k.w;

@@ -241,3 +241,18 @@ def test_policy_kl_without_a_coefficient(c, kind):
     assert float(a.kl) == math.inf and math.isfinite(float(b.loss))
     assert torch.equal(a.loss, b.loss) and torch.equal(a.clip_fraction, b.clip_fraction)
     assert torch.equal(a.grad, b.grad) and torch.isfinite(a.grad.double()).all()
+
+
+@pytest.mark.parametrize("c", [10, 100, 9001])
+@pytest.mark.parametrize("kind", list(TYPES))
+def test_policy_ratio_beyond_the_range_without_an_advantage(c, kind):
+    """A token without an advantage has no term, however far its ratio is out (exp overflows)."""
+    x, y = _make(10, 20, c, kind, pad=0.0)
+    one = torch.ones(20, dtype=_wide(kind), device="cuda")
+    old, adv = -2 * one, one.clone()
+    old[3], adv[3] = -2000.0, 0.0
+    r = policy_loss(x, y, old, adv, clip_high=math.inf)
+    keep = torch.arange(20, device="cuda") != 3
+    want = policy_loss(x[keep], y[keep], old[keep], adv[keep], clip_high=math.inf)
+    assert float(r.loss) == pytest.approx(0.95 * float(want.loss), rel=8 * _u(_wide(kind)))
+    assert bool((r.grad[3] == 0).all()) and torch.isfinite(r.grad.double()).all()
