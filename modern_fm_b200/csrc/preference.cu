@@ -250,7 +250,7 @@ struct Token {
 // A token's derivative g, and its weighted loss terms and weight e.
 template <class A>
 __device__ __forceinline__ A policy_terms(const RowArgs<A>& a, const Token<A>& k, A lp, bool live,
-                                          A inv_total, A (&e)[4]) {
+                                          double inv_total, A (&e)[4]) {
     e[0] = e[1] = e[2] = e[3] = A(0);
     // masked, or a token of weight 0: left out, whatever its ratio
     if (!live || k.w == A(0)) return A(0);
@@ -272,7 +272,8 @@ __device__ __forceinline__ A policy_terms(const RowArgs<A>& a, const Token<A>& k
     e[1] = k.w * kl;
     e[2] = cut ? k.w : A(0);
     e[3] = k.w;
-    return k.w * slope * inv_total;
+    // in 64 bits: the inverse of very small or very large weights' sum leaves 32 bits
+    return (A)((double)(k.w * slope) * inv_total);
 }
 
 // Sum over the block in a fixed order, on every thread.
@@ -493,7 +494,7 @@ __global__ void __launch_bounds__(kSmallNT, IsF64<A>::value || CW > 16 ? 4 : kSm
                     if (a.zero) a.zero[t] = A(0);
                 } else {
                     A f[4];
-                    const A g = policy_terms(a, now, lp, live, (A)inv, f);
+                    const A g = policy_terms(a, now, lp, live, inv, f);
                     for (int i = 0; i < 4; ++i) e[i] += (double)f[i];
                     if (empty && y_now >= 0) *a.empties = 1;
                     if (out) small_grad<T, A, CW, TURN>(row, v, c, first, g, quotient(-g, s), exp_of(at - off), y_now);
@@ -580,7 +581,7 @@ struct RowResult {
             if (first && a.lse) a.lse[t] = empty ? minus_inf<A>() : off + ls;
             if (first && a.zero) a.zero[t] = A(0);
         } else {
-            g = policy_terms(a, tok, lp, live, (A)inv_total, e);
+            g = policy_terms(a, tok, lp, live, inv_total, e);
             k = quotient(-g, s);
             if (first && empty && y >= 0) *a.empties = 1;
         }

@@ -256,3 +256,24 @@ def test_policy_ratio_beyond_the_range_without_an_advantage(c, kind):
     want = policy_loss(x[keep], y[keep], old[keep], adv[keep], clip_high=math.inf)
     assert float(r.loss) == pytest.approx(0.95 * float(want.loss), rel=8 * _u(_wide(kind)))
     assert bool((r.grad[3] == 0).all()) and torch.isfinite(r.grad.double()).all()
+
+
+@pytest.mark.parametrize("c", [10, 100, 9001])
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("n,weight", [(3, 2.0**-129), (3, 2.0**-131), (1000, 2.0**120)])
+def test_policy_weights_of_any_size(n, c, kind, weight):
+    """All weights alike give the loss and the gradient of none at all, also where the inverse of
+    their sum is beyond float32 or below its normal range. A product of a weight of 2^-129 and
+    a slope is below it too: off by half of 2^-149, which is 2^-21 of the weight."""
+    x, y = _make(11, n, c, kind, pad=0.0)
+    lp = _define(x, y)[0].float()
+    adv = torch.randn(n, generator=torch.Generator().manual_seed(1)).cuda()
+    args = (x, y, lp + 0.1, adv, lp - 0.2)
+    a = policy_loss(*args, kl_coef=0.1)
+    b = policy_loss(*args, kl_coef=0.1, sample_weight=torch.full_like(adv, weight))
+    lost = 2.0**-150 / weight if weight < 1 else 0.0
+    assert abs(float(b.loss) - float(a.loss)) <= 1e-6 * abs(float(a.loss)) + 4 * lost
+    # the row's factor moves by that, and by three roundings; the result is rounded in both
+    off = (a.grad.double() - b.grad.double()).abs()
+    tol = a.grad.double().abs() * (6 * 2.0**-24 + torch.finfo(x.dtype).eps) + lost / n + 1e-37
+    assert bool((off <= tol).all())
