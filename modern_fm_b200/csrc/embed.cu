@@ -241,10 +241,8 @@ constexpr int kMainNT = 128;
 // of kHeadTile entries; tile_base[t] = how many before tile t, by the block that
 // finishes last, and *count = all of them.
 __global__ void __launch_bounds__(kTileChunks)
-    chunk_heads_kernel(const uint32_t* __restrict__ keys, int64_t n, uint32_t pad_key,
-                       int64_t n_chunks, uint32_t* __restrict__ base,
-                       uint32_t* __restrict__ tile_base, unsigned* __restrict__ done,
-                       int64_t* __restrict__ count) {
+    chunk_heads_kernel(const uint32_t* keys, int64_t n, uint32_t pad_key, int64_t n_chunks,
+                       uint32_t* base, uint32_t* tile_base, unsigned* done, int64_t* count) {
     after_previous();
     __shared__ uint32_t sm[kTileChunks / 32];
     __shared__ unsigned last;

@@ -210,8 +210,7 @@ __global__ void __launch_bounds__(kETileNT)
 // Turns each digit's counts into their prefix over the tiles, in place, and writes
 // its total: a block takes 32 digits, 8 threads each a stretch of the tiles.
 __global__ void __launch_bounds__(256)
-    id_prefix_kernel(uint32_t* __restrict__ counts, int64_t n_tiles, int digits,
-                     uint32_t* __restrict__ totals) {
+    id_prefix_kernel(uint32_t* counts, int64_t n_tiles, int digits, uint32_t* totals) {
     after_previous();
     constexpr int F = 20;  // counts in flight
     __shared__ uint32_t part[8][33];
@@ -312,11 +311,10 @@ constexpr int scatter_smem() {  // counts per warp (16 bits), offsets, the tile
 // pass's counts; NULL: the last pass, which writes through `out`.
 template <class A, int BITS, bool FIRST, bool FUSED>
 __global__ void __launch_bounds__(kETileNT)
-    id_scatter_kernel(const uint32_t* __restrict__ kin, const uint32_t* __restrict__ vin,
-                      uint32_t* __restrict__ kout, uint32_t* __restrict__ vout, int64_t n,
-                      int64_t n_tiles, int shift, int bits, const uint32_t* __restrict__ counts,
-                      const uint32_t* __restrict__ totals, uint32_t* __restrict__ next,
-                      SortedOut<A> out, uint32_t* __restrict__ touched, Fill fill) {
+    id_scatter_kernel(const uint32_t* kin, const uint32_t* vin, uint32_t* kout, uint32_t* vout,
+                      int64_t n, int64_t n_tiles, int shift, int bits, const uint32_t* counts,
+                      const uint32_t* totals, uint32_t* next, SortedOut<A> out, uint32_t* touched,
+                      Fill fill) {
     after_previous();
     if (!FIRST && blockIdx.x >= n_tiles) {
         fill_untouched(fill, blockIdx.x - (unsigned)n_tiles);

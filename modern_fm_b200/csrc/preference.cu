@@ -1065,11 +1065,11 @@ __global__ void __launch_bounds__(kNT)
 // that finishes last adds the losses and the weights, in a fixed order.
 template <class A, int W>
 __global__ void __launch_bounds__(kNT)
-    pair_kernel(const double* __restrict__ lp, int64_t n, const int64_t* __restrict__ indptr,
-                int64_t n_pairs, const A* __restrict__ reference, double beta, double eps,
+    pair_kernel(const double* lp, int64_t n, const int64_t* __restrict__ indptr, int64_t n_pairs,
+                const A* __restrict__ reference, double beta, double eps,
                 const A* __restrict__ weight, A* __restrict__ margins, A* __restrict__ sums,
-                double* __restrict__ pair_loss, A* __restrict__ g, unsigned* __restrict__ done,
-                A* __restrict__ loss, double* __restrict__ scale) {
+                double* __restrict__ pair_loss, A* g, unsigned* done, A* __restrict__ loss,
+                double* __restrict__ scale) {
     after_previous();
     __shared__ double sm[kNT / 32];
     __shared__ unsigned last;

@@ -167,7 +167,9 @@ inline bool vec_ok(const void* p, int64_t ld, size_t size, int vec) {
 // while its predecessor in the stream drains. after_previous, its first
 // statement, waits for the predecessor to be complete and visible, and lets the
 // successor be scheduled in turn. A chain of four to eight short kernels is
-// spent on launch gaps to a tenth.
+// spent on launch gaps to a tenth. What the chain writes is no __restrict__ argument of a
+// kernel that reads it: such a load may be issued as one of memory that is constant
+// while the kernel runs, and the kernel runs before the wait.
 __device__ __forceinline__ void wait_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void let_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void after_previous() {
