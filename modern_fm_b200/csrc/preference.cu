@@ -41,8 +41,9 @@ __device__ __noinline__ double exp_call(double d) { return exp(d); }
 __device__ __forceinline__ double exp_of(double d) { return exp_call(d); }
 __device__ __forceinline__ float log_of(float v) { return logf(v); }
 __device__ __forceinline__ double log_of(double v) { return log(v); }
-__device__ __forceinline__ float quotient(float a, float b) { return __fdividef(a, b); }  // 2 ulp
-__device__ __forceinline__ double quotient(double a, double b) { return a / b; }
+// once a row: to the last bit or two
+__device__ __forceinline__ float ratio_of(float d) { return expf(d); }
+__device__ __forceinline__ double ratio_of(double d) { return exp_call(d); }
 
 // Sums of exp(v - off), and k exp(v - off) for each value: two 32-bit lanes an
 // instruction (the f32x2 forms round each lane as the scalar ones do), since
@@ -196,30 +197,37 @@ struct RowArgs {
     }
 };
 
-// em1 = exp(u) - 1 and kl = exp(u) - u - 1. Near 0 both by the series of kl, where the
-// differences would lose what is left: to u^8 / 8! below 1/4 in 32 bits (what is cut
-// off is 2^-33 of kl), to u^13 / 13! below 1/8 in 64 bits (2^-66).
+// em1 = exp(u) - 1 and kl = exp(u) - u - 1. Below 1 both by the series of kl, where the
+// differences would lose what is left: to u^11 / 11! in 32 bits (what is cut off is 2^-27
+// of kl), to u^18 / 18! in 64 bits (2^-55).
 __device__ __forceinline__ void kl_terms(float u, float& em1, float& kl) {
-    if (fabsf(u) < 0.25f) {
-        float r = 1.0f / 40320;
-        r = r * u + 1.0f / 5040;
-        r = r * u + 1.0f / 720;
-        r = r * u + 1.0f / 120;
-        r = r * u + 1.0f / 24;
-        r = r * u + 1.0f / 6;
+    if (fabsf(u) < 1.0f) {
+        float r = 1.0f / 39916800.0f;
+        r = r * u + 1.0f / 3628800.0f;
+        r = r * u + 1.0f / 362880.0f;
+        r = r * u + 1.0f / 40320.0f;
+        r = r * u + 1.0f / 5040.0f;
+        r = r * u + 1.0f / 720.0f;
+        r = r * u + 1.0f / 120.0f;
+        r = r * u + 1.0f / 24.0f;
+        r = r * u + 1.0f / 6.0f;
         r = r * u + 0.5f;
         kl = r * u * u;
         em1 = u + kl;
     } else {
-        em1 = exp_of(u) - 1.0f;
+        em1 = expf(u) - 1.0f;
         kl = u == INFINITY ? u : em1 - u;
     }
 }
 __device__ __forceinline__ void kl_terms(double u, double& em1, double& kl) {
     em1 = expm1(u);
-    kl = u == INFINITY ? u : em1 - u;
-    if (fabs(u) < 0.125) {
-        double r = 1.0 / 6227020800.0;
+    if (fabs(u) < 1.0) {
+        double r = 1.0 / 6402373705728000.0;
+        r = r * u + 1.0 / 355687428096000.0;
+        r = r * u + 1.0 / 20922789888000.0;
+        r = r * u + 1.0 / 1307674368000.0;
+        r = r * u + 1.0 / 87178291200.0;
+        r = r * u + 1.0 / 6227020800.0;
         r = r * u + 1.0 / 479001600.0;
         r = r * u + 1.0 / 39916800.0;
         r = r * u + 1.0 / 3628800.0;
@@ -232,6 +240,8 @@ __device__ __forceinline__ void kl_terms(double u, double& em1, double& kl) {
         r = r * u + 1.0 / 6.0;
         r = r * u + 0.5;
         kl = r * u * u;
+    } else {
+        kl = u == INFINITY ? u : em1 - u;
     }
 }
 
@@ -254,7 +264,7 @@ __device__ __forceinline__ A policy_terms(const RowArgs<A>& a, const Token<A>& k
     e[0] = e[1] = e[2] = e[3] = A(0);
     // masked, or a token of weight 0: left out, whatever its ratio
     if (!live || k.w == A(0)) return A(0);
-    const A ratio = exp_of(lp - k.old);
+    const A ratio = ratio_of(lp - k.old);
     const A bent = fmin(fmax(ratio, a.clip_lo), a.clip_hi);
     // no advantage, no term, also where the ratio is beyond the type's range
     const A plain = k.adv == A(0) && ratio == ratio ? A(0) : ratio * k.adv;
@@ -497,7 +507,7 @@ __global__ void __launch_bounds__(kSmallNT, IsF64<A>::value || CW > 16 ? 4 : kSm
                     const A g = policy_terms(a, now, lp, live, inv, f);
                     for (int i = 0; i < 4; ++i) e[i] += (double)f[i];
                     if (empty && y_now >= 0) *a.empties = 1;
-                    if (out) small_grad<T, A, CW, TURN>(row, v, c, first, g, quotient(-g, s), exp_of(at - off), y_now);
+                    if (out) small_grad<T, A, CW, TURN>(row, v, c, first, g, -g / s, exp_of(at - off), y_now);
                 }
             } else {
                 const A g = a.factor(now.w, y_now, off, scale);
@@ -582,7 +592,7 @@ struct RowResult {
             if (first && a.zero) a.zero[t] = A(0);
         } else {
             g = policy_terms(a, tok, lp, live, inv_total, e);
-            k = quotient(-g, s);
+            k = -g / s;
             if (first && empty && y >= 0) *a.empties = 1;
         }
     }

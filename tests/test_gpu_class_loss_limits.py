@@ -15,7 +15,8 @@ pytestmark = pytest.mark.gpu
 
 torch = pytest.importorskip("torch")
 
-from modern_fm_b200.preference import policy_loss, preference_loss  # noqa: E402
+from modern_fm_b200.preference import (label_logprobs, policy_loss,  # noqa: E402
+                                       preference_loss)
 
 from test_gpu_preference import (TYPES, _check_grad, _define, _make, _tol, _u,  # noqa: E402
                                  _wide)
@@ -277,3 +278,33 @@ def test_policy_weights_of_any_size(n, c, kind, weight):
     off = (a.grad.double() - b.grad.double()).abs()
     tol = a.grad.double().abs() * (6 * 2.0**-24 + torch.finfo(x.dtype).eps) + lost / n + 1e-37
     assert bool((off <= tol).all())
+
+
+@pytest.mark.parametrize("c", [10, 100, 9001])
+@pytest.mark.parametrize("kind", ["f64", "f32"])
+def test_policy_terms_of_one_token_to_the_last_bits(c, kind):
+    """One token's ratio and KL term from its own log-probability, so that the differences are
+    the only roundings before them. Both inputs of the KL term's u are near, so that u is
+    exact; the term by its series (ten or 17 steps, each less than a rounding of the whole) or
+    by exp to 2 u and two differences, of at most 1.72 times what is left; the ratio by exp
+    of a difference rounded to u |d|."""
+    wide = _wide(kind)
+    u = _u(wide)
+    x = torch.zeros(1, c, dtype=wide, device="cuda")
+    y = torch.tensor([1], device="cuda")
+    lp = label_logprobs(x, y).logprobs
+    one = torch.ones(1, dtype=wide, device="cuda")
+    for i in range(-40, 41):
+        away = 0.043 * i  # |u| < |lp| / 2 for c = 10 up to 1.15: exact there
+        ref = lp + away
+        if kind == "f32" and abs(away) * 2 > abs(float(lp)):
+            continue
+        old = lp + 5 * away
+        r = policy_loss(x, y, old, one, ref, clip_high=math.inf, with_grad=False)
+        d, a = float(lp) - float(old), float(ref) - float(lp)
+        if abs(a) > 1e-6:
+            want = math.expm1(a) - a if abs(a) > 0.4 else sum(
+                a**k / math.factorial(k) for k in range(2, 24))
+            rel = 8 * u + (16 * 2.0**-53 if abs(a) > 0.4 else 0)
+            assert float(r.kl) == pytest.approx(want, rel=rel, abs=0), a
+        assert float(r.loss) == pytest.approx(-math.exp(d), rel=(4 + abs(d)) * u, abs=0), d
