@@ -1259,9 +1259,14 @@ void with_score_types(int dtype, F&& f) {
     }
 }
 
+// The most blocks of a policy kernel, each with its sums in the workspace (one wave is
+// eight an SM at most).
+constexpr unsigned kPolicyBlocks = 2048;
+
 // A kernel over rows: the statistics start a chain of launches, the others go on in one.
 template <Mode M, class K, class... Args>
 void launch_rows(K kernel, unsigned grid, unsigned block, size_t smem, cudaStream_t s, Args... args) {
+    if (M == POLICY) grid = std::min(grid, kPolicyBlocks);
     if (M == STATS)
         kernel<<<grid, block, smem, s>>>(args...);
     else
@@ -1558,7 +1563,7 @@ struct PolicyWs {  // partial weights, a block count, the mark and the sum of em
     size_t part, bytes;
     explicit PolicyWs(int64_t n) {
         part = up256(kWeightBlocks * 8 + 16);
-        bytes = part + up256((size_t)n * 32);
+        bytes = part + up256((size_t)std::min<int64_t>(n, kPolicyBlocks) * 32);
     }
 };
 }  // namespace
