@@ -15,8 +15,8 @@ pytestmark = pytest.mark.gpu
 
 torch = pytest.importorskip("torch")
 
-from modern_fm_b200.preference import (label_logprobs, policy_loss,  # noqa: E402
-                                       preference_loss)
+from modern_fm_b200.preference import (label_logprobs, label_logprobs_grad,  # noqa: E402
+                                       policy_loss, preference_loss)
 
 from test_gpu_preference import (TYPES, _check_grad, _define, _make, _tol, _u,  # noqa: E402
                                  _wide)
@@ -308,3 +308,44 @@ def test_policy_terms_of_one_token_to_the_last_bits(c, kind):
             rel = 8 * u + (16 * 2.0**-53 if abs(a) > 0.4 else 0)
             assert float(r.kl) == pytest.approx(want, rel=rel, abs=0), a
         assert float(r.loss) == pytest.approx(-math.exp(d), rel=(4 + abs(d)) * u, abs=0), d
+
+
+@pytest.mark.parametrize("n,c", [(40, 10), (40, 100), (60, 4097), (30, 9001), (600, 9000)])
+@pytest.mark.parametrize("lo", [0, 1, 2, 8])
+@pytest.mark.parametrize("kind", list(TYPES))
+def test_losses_of_pitched_scores(n, c, lo, kind):
+    """Scores inside a wider matrix: their rows and the gradient's begin at other places within
+    16 bytes, in every kernel that writes a gradient."""
+    big, y = _make(12, n, c + 9 - c % 2, kind)
+    x = big[:, lo:lo + c]
+    y = torch.where(y >= c, -1, y)
+    y[0], y[1], y[2] = 0, c - 1, c // 2
+    wide = _wide(kind)
+    u, e = _u(wide), _tol(x, wide)
+    lp, lse, _, live = _define(x, y)
+    zero = torch.zeros(n, dtype=torch.float64, device="cuda")
+    r = label_logprobs(x, y)
+    assert (r.lse.double() - lse).abs().max() <= e and (r.logprobs.double() - lp).abs().max() <= e
+    g = torch.randn(n, generator=torch.Generator().manual_seed(1), dtype=wide).cuda()
+    _check_grad(label_logprobs_grad(g, x, y, r.lse), x, y, g.double(), zero, wide)
+    # the policy loss, all ratios exp(-0.1), inside the clip's bounds
+    old = (lp + 0.1).to(wide)
+    ratio, share = torch.exp(lp - old.double()), live.double() / live.sum()
+    got = policy_loss(x, y, old, g)
+    move = share * ratio * g.double().abs() * (e + 8 * u)
+    assert abs(float(got.loss) + float((share * ratio * g.double()).sum())) <= float(move.sum()) + 4 * u
+    _check_grad(got.grad, x, y, -share * ratio * g.double(), move, wide)
+    # the preference loss of two pairs
+    ip = torch.tensor([0, 8, 15, 22, n - 1], device="cuda")
+    seq = torch.searchsorted(ip, torch.arange(n, device="cuda"), right=True) - 1
+    s = torch.zeros(5, dtype=torch.float64, device="cuda").index_add_(0, seq, lp)[:4]
+    ref = s.to(wide)
+    q = s - ref.double()
+    z = 0.3 * (q[:2] - q[2:])
+    got = preference_loss(x, y, ip, ref, 0.3)
+    assert float(got.loss) == pytest.approx(float(-torch.nn.functional.logsigmoid(z).mean()),
+                                            abs=0.3 * n * e + 8 * u)
+    slope = -0.15 * torch.sigmoid(-z)
+    d = torch.cat([slope, -slope, torch.zeros(1, device="cuda", dtype=torch.float64)])[seq]
+    moved = torch.where(d != 0, 0.15 * 0.3 * n * e / 4, 0.0)  # sigmoid's slope is at most 1 / 4
+    _check_grad(got.grad, x, y, d, moved + 4 * u * d.abs(), wide)
