@@ -146,16 +146,6 @@ struct Pack<__half> {
     static __device__ __forceinline__ uint4 minus_inf() { return make_uint4(0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u); }
 };
 
-// Bytes per element of an MFM_DTYPE_* storage type.
-inline size_t dtype_size(int dtype) {
-    switch (dtype) {
-        case MFM_DTYPE_F64: return 8;
-        case MFM_DTYPE_BF16:
-        case MFM_DTYPE_F16: return 2;
-        default: return 4;
-    }
-}
-
 // The largest vector, in elements, that divides every row start: VEC * size
 // bytes at most 16, the base addresses and the row pitches (in elements)
 // multiples of it.
