@@ -984,6 +984,7 @@ __global__ void __launch_bounds__(L + 32, ring_blocks(L))
             if (*stop && lane == 0) {
                 a.lp[t] = (A)NAN;
                 e[0] = e[1] = e[2] = e[3] = NAN;
+                if (a.only_if) a.stats[0] = (A)NAN;  // the first pass has written it
             }
             y = y_next;
         }
