@@ -449,7 +449,8 @@ int mfm_fit_csr_dp(mfm_dp* dp, int dtype, int model, int64_t n_classes, const mf
  * arithmetic float64. Sums have a fixed order: results are bitwise
  * reproducible. n_entries, n_out, n_rows and d < 2^31; their products are not
  * limited, but rows that are summed by indptr have at most 2097120 values. out
- * must not overlap the inputs. */
+ * must not overlap the inputs. A row summed by indptr is the work of at most 32
+ * lanes: a single row of 10^6 entries takes tens of milliseconds. */
 
 /* out[t] = alpha scale[t] table[ids[t]], or its row sums; out (n_out, d) with
  * row pitch ld_out. */
@@ -494,12 +495,13 @@ int mfm_embedding_grad_device(int dtype, int out_dtype, int device, int ids64, c
  * labels64 = 1; a label outside [0, n_classes) masks its token
  * (log-probability 0, gradient 0), and so does a row whose every score is
  * -infinity. Everything else is in the arithmetic type: float64 for F64, else
- * float32. Sums over tokens and pairs run in float64 in a fixed order. */
+ * float32. Sums over tokens and pairs run in float64 in a fixed order. A row with a
+ * NaN or +infinity among its scores gives NaN, unless its label masks it. */
 
 /* logprobs[t] = logits[t, labels[t]] - lse[t], lse[t] = log sum exp logits[t]
  * (written for masked tokens too). sums (n_seq; NULL = not wanted): the sum of
  * logprobs over tokens [indptr[s], indptr[s+1]) (int64, n_seq + 1, limited to
- * [0, n_tokens]). */
+ * [0, n_tokens]), of the values as written to logprobs. */
 int mfm_label_logprobs_device(int dtype, int device, const void* logits, int64_t ld,
                               int64_t n_tokens, int64_t n_classes, int labels64,
                               const void* labels, const int64_t* indptr, int64_t n_seq,
@@ -518,9 +520,11 @@ int mfm_label_logprobs_grad_device(int dtype, int device, const void* logits, in
  *   z[p] = beta ((S[p] - R[p]) - (S[n_pairs + p] - R[n_pairs + p]))
  *   loss = sum w[p] (-(1 - e) log sigmoid(z[p]) - e log sigmoid(-z[p])) / sum w[p]
  * with e = label_smoothing and w = sample_weight (NULL = 1). Pairs of weight 0
- * are left out; weights that sum to 0 give loss and gradient 0. Writes loss (1), margins z (n_pairs), seq_logprobs
- * S (2 n_pairs) and, unless NULL, d_logits (as above; tokens of no sequence get
- * 0). workspace: mfm_preference_workspace_bytes(...) bytes, 256-byte aligned. */
+ * are left out; weights that sum to 0 give loss and gradient 0. An infinite margin (a
+ * label whose score is -infinity) is taken in the limit. Writes loss (1), margins z
+ * (n_pairs), seq_logprobs S (2 n_pairs) and, unless NULL, d_logits (as above; tokens
+ * of no sequence get 0). workspace: mfm_preference_workspace_bytes(...) bytes,
+ * 256-byte aligned. */
 int64_t mfm_preference_workspace_bytes(int dtype, int64_t n_tokens, int64_t n_pairs);
 int mfm_preference_loss_device(int dtype, int device, const void* logits, int64_t ld,
                                int64_t n_tokens, int64_t n_classes, int labels64,
@@ -533,9 +537,10 @@ int mfm_preference_loss_device(int dtype, int device, const void* logits, int64_
 /* Clipped policy loss with a KL term. Per token, with lp its log-probability,
  * r = exp(lp - old_logprobs) and u = reference - lp:
  *   l = -min(r A, clamp(r, 1 - clip_low, 1 + clip_high) A) + kl_coef (exp(u) - u - 1)
- * with A = advantages (reference NULL: no KL term). loss = sum w l / sum w over the
- * unmasked tokens, w = sample_weight (NULL = 1); tokens of weight 0 are left out,
- * and weights that sum to 0 give 0.
+ * with A = advantages (reference NULL: no KL term; kl_coef 0: it is only reported). loss
+ * = sum w l / sum w over the unmasked tokens (neither sum has those whose every score
+ * is -infinity), w = sample_weight (NULL = 1); tokens of weight 0 are left out, and
+ * weights that sum to 0 give 0.
  * stats (3): the loss, the mean of exp(u) - u - 1, and the share of tokens whose
  * clipped term is the smaller one. Writes logprobs (n_tokens) and, unless NULL,
  * d_logits. workspace: mfm_policy_workspace_bytes(...) bytes, 256-byte aligned. */

@@ -30,7 +30,12 @@ constexpr int kSmallC = 32;
 constexpr int kSmallNT = 128;
 constexpr int kSmallPerSm = 8;  // blocks of 64 registers a thread
 
-// exp(d): the 32-bit form is one multiply and ex2 (2^-22 of the value), exact at 0.
+// exp(d). The 32-bit form, one multiply and ex2, is exact at 0 and off by at most
+// (4 + 2 |d|) 2^-24 of the value (ex2.approx 2^-22; the product's and the constant's
+// roundings), 0 below 2^-126. It is taken for the values of a row, where d <= 0: a value
+// e^d of a sum of 1 or more is off by less than 2^-22 of 1, whatever d is. expf there
+// takes 123 us instead of 100 us (log-probabilities, 8195 x 32000 bf16), 313 us instead
+// of 229 us (policy, 4096 x 65536 bf16), 96 us instead of 84 us (400000 x 100 bf16).
 __device__ __forceinline__ float exp_of(float d) {
     float r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d * 1.4426950408889634f));
@@ -136,8 +141,8 @@ struct Labels {
 template <class A>
 __device__ __forceinline__ A offset_of(A m) { return m == minus_inf<A>() ? A(0) : m; }
 
-// x - off - log s with nothing rounded to 32 bits: a sequence adds up hundreds of
-// them, and a margin is the difference of two such sums.
+// x - off - log s with nothing rounded to 32 bits but the sum s itself: a sequence adds
+// up hundreds of them, and a margin is the difference of two such sums.
 template <class T, class A>
 __device__ __noinline__ double exact_logprob(T x, A off, A s) {
     return (widen<double>(x) - (double)off) - log((double)s);
@@ -715,9 +720,12 @@ __global__ void __launch_bounds__(kNT, cached_blocks<A>(K))
 
 // ------------------------------------------- long rows, statistics alone --
 
-// Rows read once with a running maximum: L lanes a row, U vectors a lane in
-// flight. The fewest lanes that still fill the GPU: what a row costs besides its
-// values (reductions, log) is paid once a warp.
+// Rows read once with a running maximum: L lanes a row, U vectors a lane in flight.
+// What a row costs besides its values (reductions, log) is paid once a warp, so short
+// rows take few lanes, long ones as many as keep their loads in flight, and few rows a
+// whole block each. 32, 64, 128, 256 lanes a row, bf16: 60000 x 4096 92, 111, 178,
+// 354 us; 100000 x 5000 184, 264, 291, 581; 8195 x 32000 108, 104, 98, 100; 2000 x 65536
+// 66, 61, 63, 59; 50 x 65536 41, 27, 18, 12. (The rule takes 64 for the first two.)
 template <class T, class A, int L>
 __global__ void __launch_bounds__(kNT, IsF64<A>::value ? 2 : 4)
     scan_rows_kernel(const T* __restrict__ x, int64_t ld, RowArgs<A> a) {
@@ -1308,7 +1316,12 @@ void small_launch(int device, const T* x, int64_t ld, T* out, int64_t ld_out, co
         width(std::false_type{});
 }
 
-// Rows of up to kCachedVecs vectors: the fewest lanes that hold one.
+// Rows of up to kCachedVecs vectors: the fewest lanes that hold one. Sixteen vectors a
+// lane of a warp are the most that registers hold, and beat the ring and the elementwise
+// gradient (60000 x 4096 bf16: policy 199 us against 268 us, gradient 159 us against
+// 207 us; 100000 x 2049: 215 us against 303 us). The statistics alone stop at half of
+// it: float32 rows of 2000 take 88 us by the scan, 96 us held (60000 rows), bf16 rows of
+// 4096 the other way round 111 us and 100 us.
 constexpr int64_t kCachedVecs = 512;
 
 template <class T, class A, Mode M>
@@ -1396,7 +1409,8 @@ void stats_launch(int device, const T* x, int64_t ld, int64_t n, int64_t c, Labe
     MFM_CHECK_LAUNCH("label log-probabilities launch");
 }
 
-// The gradient for given g and lse: elementwise.
+// The gradient for given g and lse: elementwise. lse comes in the arithmetic type, as the
+// forward returns it: in 32 bits a probability is off by |lse| 2^-24 of itself by that.
 template <class T, class A>
 void grad_launch(int device, const T* x, int64_t ld, int64_t n, int64_t c, Labels labels,
                  const A* g, const double* scale, const A* lse, T* out, int64_t ld_out,

@@ -11,7 +11,9 @@ All calls take CUDA tensors on one device, run on ``stream`` (a
 torch.cuda.Stream, default the current one of that device) and neither
 synchronise nor copy to the host, so they can be captured into a CUDA graph.
 Ids outside ``[0, n_rows)`` are padding: a zero row, no gradient. Every sum has a
-fixed order: results are bitwise reproducible.
+fixed order: results are bitwise reproducible. The calls are not part of torch's
+autograd: results carry no graph, whether or not an input requires a gradient, and
+a backward pass is a call of its own (``embedding_grad``).
 """
 
 from __future__ import annotations
@@ -136,7 +138,8 @@ def embedding_lookup(table, ids, scale=None, indptr=None, alpha: float = 1.0, ou
     float64 result (the engine's default arithmetic). Returns ids.shape + (d,) or
     (n_out, d) in the table's type, sums rounded once; ``out`` (2-D for a 1-D
     ids) takes the result instead of a new tensor and must not overlap the
-    inputs. Raises ValueError for invalid arguments, RuntimeError for CUDA
+    inputs. A CSR row is summed by one group of lanes: rows of up to some thousand
+    entries, or many of them, are what it is made for. Raises ValueError for invalid arguments, RuntimeError for CUDA
     failures.
     """
     code = _STORAGE.get(table.dtype)

@@ -146,8 +146,10 @@ class DeviceModel:
 
     def factors_device(self, indptr, indices, data, stream=None):
         """The rows' factor sums, ``sum of x[b, j] V[j]`` over the entries of row b: a
-        row's place in the latent space (two rows' inner product is their part of
-        the pairwise score), e.g. for nearest-neighbour retrieval. A canonical
+        row's place in the latent space, e.g. for nearest-neighbour retrieval. In an FM
+        two rows' inner product is their part of the pairwise score; in an FwFM the
+        pairs carry ``r`` besides, in an FFM each pair takes the factors of the other
+        one's field, so there it is not. A canonical
         device CSR as ``predict_device`` takes it; returns a CUDA tensor (n_rows, k),
         multiclass (n_rows, C, k), FFM (n_rows, F, k) or (n_rows, F, C, k), float32
         for dtype float32, float64 otherwise (summed in that type)."""

@@ -16,7 +16,10 @@ synchronise nor copy to the host, so they can be captured into a CUDA graph.
 pitch; labels int32 or int64, a label outside ``[0, n_classes)`` masks its row
 (log-probability 0, gradient 0), as does a row whose every score is -infinity.
 Everything else is in the arithmetic type: float64 for float64 logits, else
-float32; sums over rows run in float64 in a fixed order.
+float32; sums over rows run in float64 in a fixed order. A row with a NaN or
++infinity among its scores gives NaN, unless its label masks it. The calls are not
+part of torch's autograd: results carry no graph, and the gradients are what they
+return.
 """
 
 from __future__ import annotations
@@ -89,7 +92,8 @@ def label_logprobs(logits, labels, indptr=None, stream=None) -> LabelLogprobs:
     """Log-probability of each row's label, ``logits[t, labels[t]] - lse[t]``, and
     ``lse[t] = log sum exp logits[t]`` (also for masked rows). With ``indptr`` (int64,
     n_sequences + 1) the log-probabilities summed over each sequence's rows too,
-    as ``preference_loss`` takes its reference."""
+    as ``preference_loss`` takes its reference: added in float64 as they are returned
+    and rounded to the arithmetic type (in float32 a sum near -8000 has steps of 5e-4)."""
     code, wide, p, n, c, ld, l64 = _scores(logits, labels)
     n_seq = 0 if indptr is None else _bounds(indptr)
     dev = _one_device(logits, labels, indptr)
@@ -135,7 +139,10 @@ def preference_loss(logits, labels, indptr, reference, beta: float = 0.1,
     ``z = beta * ((S[p] - R[p]) - (S[n_pairs + p] - R[n_pairs + p]))`` and the loss the
     mean, weighted by ``sample_weight`` (n_pairs), of ``-(1 - e) log sigmoid(z) -
     e log sigmoid(-z)`` with e = ``label_smoothing``. Pairs of weight 0 are left
-    out; weights that sum to 0 give loss and gradient 0.
+    out; weights that sum to 0 give loss and gradient 0. S is summed from unrounded
+    log-probabilities, ``reference`` is in the arithmetic type: against itself a model's
+    margins are 0 up to its rounding. An infinite margin (a label whose score is
+    -infinity) is taken in the limit: loss 0 on the right side without smoothing.
     """
     code, wide, p, n, c, ld, l64 = _scores(logits, labels)
     n_seq = _bounds(indptr)
@@ -174,8 +181,10 @@ def policy_loss(logits, labels, old_logprobs, advantages, reference=None, clip_l
     their mean weighted by ``sample_weight`` (rows of weight 0 are left out;
     weights that sum to 0 give 0). ``old_logprobs`` (the policy the labels were
     drawn from), ``advantages``, ``reference`` (None: no KL term) and
-    ``sample_weight`` hold one value per row. ``kl`` is the mean of exp(u) - u - 1,
-    ``clip_fraction`` the share of rows whose clipped term is the smaller one.
+    ``sample_weight`` hold one value per row. ``kl`` is the mean of exp(u) - u - 1
+    (also with ``kl_coef`` 0, where it is only reported), ``clip_fraction`` the share of
+    rows whose clipped term is the smaller one. All means are over the unmasked rows'
+    weights, so rows whose every score is -infinity are in none of them.
     """
     code, wide, p, n, c, ld, l64 = _scores(logits, labels)
     _vector("old_logprobs", old_logprobs, n, wide)

@@ -349,3 +349,35 @@ def test_losses_of_pitched_scores(n, c, lo, kind):
     d = torch.cat([slope, -slope, torch.zeros(1, device="cuda", dtype=torch.float64)])[seq]
     moved = torch.where(d != 0, 0.15 * 0.3 * n * e / 4, 0.0)  # sigmoid's slope is at most 1 / 4
     _check_grad(got.grad, x, y, d, moved + 4 * u * d.abs(), wide)
+
+
+@pytest.mark.parametrize("n,c", [(40, 10), (40, 32), (40, 100), (40, 4097), (20, 9001), (600, 9001)])
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+def test_scores_that_are_no_numbers_stay_in_their_rows(n, c, kind, bad):
+    """A NaN or +infinity anywhere in a row makes the row NaN, masked rows keep their zeros, and
+    no other row changes."""
+    x, y = _make(13, n, c, kind, pad=0.0)
+    rows = torch.arange(0, n, 3, device="cuda")
+    x2, y2 = x.clone(), y.clone()
+    x2[rows, (rows * 7919) % c] = bad
+    y2[::6] = -1
+    y[::6] = -1
+    hit = torch.zeros(n, dtype=torch.bool, device="cuda")
+    hit[rows] = True
+    masked = y2 < 0
+    one = torch.ones(n, dtype=_wide(kind), device="cuda")
+    a, b = label_logprobs(x, y), label_logprobs(x2, y2)
+    assert torch.equal(a.logprobs[~hit], b.logprobs[~hit]) and torch.equal(a.lse[~hit], b.lse[~hit])
+    assert torch.isnan(b.lse[hit]).all() and torch.isnan(b.logprobs[hit & ~masked]).all()
+    assert bool((b.logprobs[masked] == 0).all())
+    g = label_logprobs_grad(one, x2, y2, b.lse)
+    assert torch.isnan(g[hit & ~masked].double()).all() and bool((g[masked] == 0).all())
+    assert torch.equal(g[~hit], label_logprobs_grad(one, x, y, a.lse)[~hit])
+    w = (~hit).to(one.dtype)  # rows of weight 0 are left out, whatever is in them
+    p, q = (policy_loss(v, l, -2 * one, one, -one, kl_coef=0.1, sample_weight=w)
+            for v, l in ((x, y), (x2, y2)))
+    assert torch.equal(p.loss, q.loss) and torch.equal(p.grad, q.grad)
+    q = policy_loss(x2, y2, -2 * one, one)
+    assert math.isnan(float(q.loss)) and bool((q.grad[masked] == 0).all())
+    assert torch.equal(q.grad[~hit], policy_loss(x, y, -2 * one, one).grad[~hit])
