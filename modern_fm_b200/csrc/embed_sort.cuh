@@ -12,13 +12,14 @@
 //  * a pass's scatter counts the next pass's digits while it writes (integer
 //    adds, grouped per warp), so only the first pass has a counting launch;
 //  * 8-bit digits of up to kFuseTiles tiles: each tile sums the counts before it
-//    by itself (at most 192 KB of L2 reads); else one prefix launch a pass (whole
-//    gradients by the first and the second: 4000 ids 37 and 39 us, 60000 41 and 43,
-//    130000 43 and 45, 260000 51 and 49, 390000 65 and 61, 800000 112 and 80);
+//    by itself (at most 192 KB of L2 reads); else one prefix launch a pass (a call for
+//    the touched rows of 60000 x 4 by the first and the second: 4000 ids 37 and 39 us,
+//    60000 41 and 43, 130000 43 and 45, 260000 51 and 49, 390000 65 and 61, 800000 112
+//    and 80);
 //  * the last pass leaves, beside the sorted keys, each entry's gradient row and
 //    scale instead of its position, so the sums read them in order;
-//  * up to kSmallSort ids one block does every pass in shared memory (whole
-//    gradients of 600 ids 22 us, 31 us by tiles; of 2048 ids 27 us and 37 us); up to
+//  * up to kSmallSort ids one block does every pass in shared memory (touched rows of
+//    60000 x 16: 600 ids 22 us, 31 us by tiles; 2048 ids 27 us and 37 us); up to
 //    kFewIds, every block of the gradient's only launch sorts them for itself.
 #pragma once
 
