@@ -218,8 +218,9 @@ def _prepare_rows(case, g):
     st = dict(case=case, param=_normal(g, (n, d), kind, 0.3), keys=keys, rows=rows,
               count=torch.tensor(used, device="cuda"), used=used, step=torch.tensor(case["steps"], device="cuda"),
               row_steps=torch.randint(0, case["steps"] + 1, (n,), generator=g, device="cuda", dtype=torch.int32))
-    live = (torch.arange(pitch, device="cuda") < d).repeat(n) & (st["row_steps"] > 0).repeat_interleave(pitch)
-    _moments(st, g, n * pitch, wide, live)
+    live = torch.zeros(_padded(n * pitch), device="cuda", dtype=torch.bool)
+    live[:n * pitch] = (torch.arange(pitch, device="cuda") < d).repeat(n) & (st["row_steps"] > 0).repeat_interleave(pitch)
+    _moments(st, g, live.numel(), wide, live)
     return st
 
 
@@ -424,7 +425,7 @@ def _plain_rows(st):
             st[k].view(n, -1)[keys] = x.view(used, -1)
         m, v = (_decode(st[k], st[k + "_exp"], k == "m").bfloat16() for k in ("m", "v"))
     else:
-        m, v = st["m"].view(n, d), st["v"].view(n, d)
+        m, v = st["m"][:n * d].view(n, d), st["v"][:n * d].view(n, d)
         p, m[keys], v[keys] = _step(case, p, g, m[keys], v[keys], t1, t2)
         m, v = st["m"], st["v"]
     st["param"][keys] = p.to(st["param"].dtype)
@@ -520,7 +521,8 @@ def _exact_step(case, st):
     for k in ("m", "v"):
         whole[k] = _decode(st[k], st[k + "_exp"], k == "m").double() if eight else st[k].double().clone()
     if rows:
-        m, v = (whole[k].view(case["n"], -1)[keys, :d] for k in ("m", "v"))
+        pitch = _padded(d) if eight else d
+        m, v = (whole[k][:case["n"] * pitch].view(-1, pitch)[keys, :d] for k in ("m", "v"))
         t = (st["row_steps"][keys] + 1).double()[:, None]
     else:
         m, v, t = whole["m"], whole["v"], (st["step"] + 1).double()
@@ -534,7 +536,7 @@ def _exact_step(case, st):
         m, v = _exact_code(m, None, True), _exact_code(v, _random_bits(st, st["step"] + 1), False)
     if rows:
         for k, x in (("m", m), ("v", v)):
-            whole[k].view(case["n"], -1)[keys] = x.reshape(used, -1)
+            whole[k][:case["n"] * pitch].view(-1, pitch)[keys] = x.reshape(used, pitch)
         table = st["param"].double()
         table[keys] = p
         out = {"param": table, "m": whole["m"], "v": whole["v"], "row_steps": None}
