@@ -553,6 +553,71 @@ int mfm_policy_loss_device(int dtype, int device, const void* logits, int64_t ld
                            void* stats, void* logprobs, void* d_logits, int64_t ld_out,
                            void* workspace, int64_t workspace_bytes, void* stream);
 
+/* ---- AdamW over many tensors ------------------------------------------------
+ * The engine's own optimizers step its models inside fit (rust/src/optimizer.rs:68-85
+ * is the lazy Adam that the by-row form resembles); this one steps a caller's
+ * parameters by given gradients. Every array is DEVICE memory on `device`; calls run
+ * on `stream`, allocate nothing, do not synchronise, and may be captured.
+ *
+ * Per value, with t = *step + 1 and s = grad_scale min(1, max_norm / norm):
+ *   g = s grad, m = b1 m + (1 - b1) g, v = b2 v + (1 - b2) g^2
+ *   p -= lr weight_decay p + lr (m / (1 - b1^t)) / (sqrt(v / (1 - b2^t)) + epsilon)
+ * in float64 for MFM_DTYPE_F64 parameters, else in float32, each result rounded once.
+ *
+ * A dense tensor has n_rows = 1, d contiguous values, keys NULL. A table with keys
+ * (int32, or int64 with keys64 = 1; rows of pitch ld) is stepped by touched rows, as
+ * mfm_embedding_grad_device returns them: grad (n_keys, d) contiguous, of which the
+ * first *count rows belong to the ascending ids in keys; a key outside [0, n_rows), or
+ * not above the one before it, is left out. t is then the row's own count, row_steps
+ * (n_rows). The arrays of two tensors must not overlap.
+ *
+ * m, v: state_bits 32: float64 for F64 parameters, else float32, (n_rows, d)
+ * contiguous. state_bits 8: one byte a value, rows (of a dense tensor: the whole) padded
+ * to multiples of 32, and one byte in m_exp / v_exp for each 32 values: with shared
+ * exponent X, code k > 0 of a magnitude stands for the float32 whose upper 11 bits below
+ * the sign are 8 X + k, code 0 for 0; m has its sign in the code's highest bit. m is rounded
+ * to nearest, v up or down by random bits of seed, the tensor's place in the list, the
+ * step and the value's place (a value above 0 stays above 0).
+ * master (NULL, or float32 laid out as m; 16-bit parameters only): the parameters in
+ * 32 bits; param is then written only, rounded from them. */
+typedef struct {
+    void* param;
+    const void* grad; /* NULL: the tensor stays as it is */
+    void *m, *v;
+    uint8_t *m_exp, *v_exp;
+    float* master;
+    const void* keys;
+    const int64_t* count;
+    int32_t* row_steps;
+    int64_t n_rows, d, ld, n_keys;
+    double weight_decay;
+    int dtype, grad_dtype, keys64; /* grad_dtype: dtype, or MFM_DTYPE_F32 for 16 bits */
+} mfm_adamw_tensor;
+
+typedef struct {
+    double learning_rate, beta_1, beta_2, epsilon, grad_scale;
+    double max_norm;                /* < 0: no norm is taken */
+    const double* learning_rate_at; /* device; NULL = the numbers above */
+    const double* grad_scale_at;
+    uint32_t seed;
+    int state_bits;
+} mfm_adamw;
+
+/* One step; *step goes up by one. With max_norm >= 0 the norm |grad_scale| sqrt(sum of
+ * squares of all gradients) goes to norm (float64 if any tensor is F64, else float32);
+ * where it is not finite nothing else is written. workspace: 256-byte aligned,
+ * mfm_adamw_workspace_bytes() bytes, zero before the first step, kept from step to step;
+ * two steps that may run at the same time need two. */
+int64_t mfm_adamw_workspace_bytes(void);
+int mfm_adamw_step_device(int device, const mfm_adamw_tensor* tensors, int64_t n_tensors,
+                          const mfm_adamw* hyper, int64_t* step, void* norm, void* workspace,
+                          int64_t workspace_bytes, void* stream);
+
+/* 8-bit moments as the values that they stand for, exact in bfloat16: n codes (a
+ * multiple of 32, or the last block's beginning), is_signed 1 for m. */
+int mfm_adamw_moments_device(int device, int is_signed, const uint8_t* code,
+                             const uint8_t* exponent, int64_t n, void* out, void* stream);
+
 /* Device time (seconds, CUDA events) of the calling thread's last fit, by
  * phase: out[0] uploads and setup, out[1] the epochs' plans (sorts), out[2]
  * the epochs' batches, out[3] the download of parameters and state. No

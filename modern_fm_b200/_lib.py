@@ -51,6 +51,21 @@ class Group(ct.Structure):
     _fields_ = [(n, f64p) for n in ("param", "acc", "m", "s", "t", "z", "n")]
 
 
+class AdamW(ct.Structure):
+    _fields_ = [(n, ct.c_double) for n in ("learning_rate", "beta_1", "beta_2", "epsilon",
+                                           "grad_scale", "max_norm")] + [
+        ("learning_rate_at", ct.c_void_p), ("grad_scale_at", ct.c_void_p), ("seed", ct.c_uint32),
+        ("state_bits", ct.c_int)]
+
+
+# mfm_adamw_tensor as an array's element type
+ADAMW_TENSOR = np.dtype(
+    [(n, np.uint64) for n in ("param", "grad", "m", "v", "m_exp", "v_exp", "master", "keys",
+                              "count", "row_steps")]
+    + [(n, np.int64) for n in ("n_rows", "d", "ld", "n_keys")] + [("weight_decay", np.float64)]
+    + [(n, np.int32) for n in ("dtype", "grad_dtype", "keys64")], align=True)
+
+
 class DevGroup(ct.Structure):
     """mfm_dev_group: device pointers (integers) in the compute dtype."""
     _fields_ = [(n, ct.c_void_p) for n in ("param", "acc", "m", "s", "t", "z", "n")]
@@ -157,6 +172,12 @@ _SIGNATURES = {
         ct.c_int, ct.c_int, ct.c_void_p, ct.c_int64, ct.c_int64, ct.c_int64, ct.c_int, ct.c_void_p,
         ct.c_void_p, ct.c_void_p, ct.c_void_p, ct.c_double, ct.c_double, ct.c_double, ct.c_void_p,
         ct.c_void_p, ct.c_void_p, ct.c_void_p, ct.c_int64, ct.c_void_p, ct.c_int64, ct.c_void_p]),
+    "mfm_adamw_workspace_bytes": (ct.c_int64, []),
+    "mfm_adamw_step_device": (ct.c_int, [
+        ct.c_int, ct.c_void_p, ct.c_int64, ct.POINTER(AdamW), ct.c_void_p, ct.c_void_p, ct.c_void_p,
+        ct.c_int64, ct.c_void_p]),
+    "mfm_adamw_moments_device": (ct.c_int, [ct.c_int, ct.c_int, ct.c_void_p, ct.c_void_p,
+                                            ct.c_int64, ct.c_void_p, ct.c_void_p]),
     "mfm_fm_predict_device": (ct.c_int, [ct.c_int, ct.c_int, ct.c_void_p, ct.c_void_p,
                                          ct.c_void_p, ct.c_int64, ct.c_double, ct.c_void_p,
                                          ct.c_void_p, ct.c_int64, ct.c_void_p, ct.c_void_p]),

@@ -1,0 +1,681 @@
+// adamw.cu — the AdamW step over many tensors at once: moments in 32 or 64 bits or in
+// 8, master weights, a clip of the gradients' norm, and tables stepped by touched rows.
+//
+//   g = s grad,  m = b1 m + (1 - b1) g,  v = b2 v + (1 - b2) g^2
+//   p -= lr wd p + lr (m / (1 - b1^t)) / (sqrt(v / (1 - b2^t)) + eps)
+// with s = grad_scale min(1, max_norm / norm). t is the device's own count, so that a
+// captured step goes on; a table's rows have one each (the engine's lazy Adam).
+//
+// One pass over p, g, m, v: bound by HBM (28 bytes a value with float32 everything, 10
+// with 16-bit values and 8-bit moments). All tensors of one kind of types are one
+// launch: their descriptions travel in the kernel's parameters, and persistent blocks
+// walk chunks of kChunk values across them. A norm is one launch more, whose last block
+// leaves the factor s.
+#include "vecio.cuh"
+
+#include <algorithm>
+#include <cmath>
+
+namespace mfm {
+namespace {
+
+constexpr int kNT = 256;
+constexpr int kPer = 8;                     // values a thread and chunk
+constexpr int64_t kChunk = kNT * kPer;      // values a block takes at once
+constexpr int kFew = 40, kMany = 400;       // descriptions a launch carries (4 or 32 KB of parameters)
+constexpr int kNormFew = 100, kNormMany = 800;
+constexpr unsigned kNormBlocks = 1024;      // the most, each with its sum in the workspace
+
+// ------------------------------------------------------------ 8-bit moments --
+
+// Blocks of 32 neighbouring values share an exponent byte X. Code k > 0 stands for the
+// float32 whose upper 11 bits (exponent and 3 bits of mantissa) are the number 8 X + k.
+// m has a sign and 7 bits (15 octaves), v 8 bits (31 octaves: it holds squares). Scales
+// are powers of two, so a value that stays is encoded as itself whatever its block's
+// largest does.
+constexpr unsigned kHalfStep = (1u << 19) + 64;  // see m_code
+template <bool SIGNED>
+struct Code {
+    static constexpr unsigned kMost = SIGNED ? 127 : 255, kReach = SIGNED ? 15 : 31;
+    static __device__ __forceinline__ float value(unsigned code, unsigned x) {
+        const unsigned k = code & kMost, bits = k ? (8 * x + k) << 20 : 0;
+        return __uint_as_float(SIGNED ? bits | (code & 128) << 24 : bits);
+    }
+    // The number of a magnitude's bits after `add` below it; finite values stay finite,
+    // infinity and NaN stay what they are (whose bits could wrap).
+    static __device__ __forceinline__ unsigned number(unsigned bits, unsigned add) {
+        return bits < 0x7f800000u ? min((bits + add) >> 20, 0x7f7u) : bits == 0x7f800000u ? 0x7f8u : 0x7fcu;
+    }
+    // The shared exponent by the block's largest magnitude, as it rounds (v: as it may).
+    static __device__ __forceinline__ unsigned shared(unsigned largest) {
+        const unsigned top = number(largest, SIGNED ? kHalfStep : (1u << 20) - 1) >> 3;
+        return top > kReach ? top - kReach : 0;
+    }
+    // `add`: for m half a step and 64 units of the last place, so that ties, which 0.9 m +
+    // 0.1 g of values of few bits often is, go up whatever the sum's last bits are; for v 20
+    // random bits: b2 = 0.999 moves v by a thousandth of itself, and rounded to nearest it
+    // would stand still until g^2 is some 50 times v. What is above 0 stays above 0 in v,
+    // where 0 would leave m / eps.
+    static __device__ __forceinline__ unsigned code(float v, unsigned add, unsigned x) {
+        const unsigned bits = __float_as_uint(v) & 0x7fffffffu, n = number(bits, add), base = 8 * x;
+        if (bits == 0) return 0;
+        const unsigned k = n > base ? min(n - base, kMost) : SIGNED ? 0u : 1u;
+        return SIGNED && k ? k | (__float_as_uint(v) >> 31) << 7 : k;
+    }
+};
+using MCode = Code<true>;
+using VCode = Code<false>;
+
+// 32 bits that depend on each bit of x: two rounds of shift, xor and product (the
+// finaliser of MurmurHash3, A. Appleby).
+__host__ __device__ __forceinline__ uint32_t mix(uint32_t x) {
+    x = (x ^ (x >> 16)) * 0x85ebca6bu;
+    x = (x ^ (x >> 13)) * 0xc2b2ae35u;
+    return x ^ (x >> 16);
+}
+// The rounding of value e of a tensor, 20 bits; key: of seed, tensor and step.
+__device__ __forceinline__ uint32_t round_bits(uint32_t key, int64_t e) {
+    return mix((uint32_t)e ^ (key + 0x9e3779b9u * (uint32_t)(e >> 32))) >> 12;
+}
+
+// ------------------------------------------------------------------- norm --
+
+struct Summand {
+    const void* p;
+    int64_t n;             // values, or with `count`: rows at most
+    const int64_t* count;  // rows in use, NULL = a dense tensor
+    int first, d, dtype;   // its first chunk, row width
+};
+template <int N>
+struct Summands {
+    Summand of[N];
+};
+
+struct Hyper {
+    double lr, b1, b2, eps, ln_b1, ln_b2, grad_scale, max_norm;
+    const double *lr_at, *grad_scale_at;  // on the device, NULL = the numbers above
+    int64_t* step;
+    uint32_t seed;
+};
+
+// What a call keeps on the device between its launches, and the count of finished blocks, which is
+// 0 between launches.
+struct Work {
+    unsigned done;
+    double factor;  // of every gradient
+    double part[kNormBlocks];
+};
+
+__device__ __forceinline__ double block_sum(double v, double* sm) {
+    v = warp_sum(v);
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) sm[threadIdx.x / 32] = v;
+    __syncthreads();
+    double t = 0.0;
+    for (int w = 0; w < (int)blockDim.x / 32; ++w) t += sm[w];
+    return t;
+}
+
+// The block that finishes last: on every thread whether this is it; the count is left at 0.
+__device__ __forceinline__ bool last_block(unsigned* done) {
+    __shared__ unsigned last;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        __threadfence();
+        last = atomicAdd(done, 1u) == gridDim.x - 1 ? 1u : 0u;
+        if (last) *done = 0;
+    }
+    __syncthreads();
+    if (!last) return false;
+    __threadfence();
+    return true;
+}
+
+// Squares are added in 32 bits over a thread's values of a chunk, and in 64 bits from
+// there; values whose squares leave the 32-bit range are squared in 64.
+template <class G>
+__device__ __forceinline__ double square_sum(const G* g, int64_t n, int64_t base) {
+    using A = typename Arith<G>::type;
+    A v[kPer], s = A(0), big = A(0);
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+        const int64_t e = base + j * kNT;
+        v[j] = e < n ? widen<A>(g[e]) : A(0);
+    }
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+        s += v[j] * v[j];
+        big = fmax(big, fabs(v[j]));
+    }
+    if (!IsF64<A>::value && (!(s < A(1e37)) || (s < A(1e-25) && big > A(0)))) {
+        double w = 0.0;
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) w += (double)v[j] * (double)v[j];
+        return w;
+    }
+    return (double)s;
+}
+
+// Sums of squares by block; the last block of the last launch (`finish`) adds them, in
+// block order, to the norm and the gradients' factor. A norm that is not finite leaves
+// NaN there, and the step does nothing.
+template <int N>
+__global__ void __launch_bounds__(kNT)
+    norm_kernel(const __grid_constant__ Summands<N> list, int n_of, int64_t chunks, Work* work,
+                int part_at, bool finish, const __grid_constant__ Hyper h, int norm64, void* norm) {
+    __shared__ double sm[kNT / 32];
+    after_previous();
+    double a = 0.0;
+    int i = 0;
+    for (int64_t c = blockIdx.x; c < chunks; c += gridDim.x) {
+        while (i + 1 < n_of && c >= list.of[i + 1].first) ++i;
+        const Summand& s = list.of[i];
+        int64_t n = s.n;
+        if (s.count) {
+            const int64_t used = *s.count;
+            n = (used < 0 ? 0 : used > n ? n : used) * s.d;
+        }
+        const int64_t base = (c - s.first) * kChunk + threadIdx.x;
+        if (base >= n) continue;
+        if (s.dtype == MFM_DTYPE_F64)
+            a += square_sum((const double*)s.p, n, base);
+        else if (s.dtype == MFM_DTYPE_F32)
+            a += square_sum((const float*)s.p, n, base);
+        else if (s.dtype == MFM_DTYPE_BF16)
+            a += square_sum((const __nv_bfloat16*)s.p, n, base);
+        else
+            a += square_sum((const __half*)s.p, n, base);
+    }
+    a = block_sum(a, sm);
+    if (threadIdx.x == 0) work->part[part_at + blockIdx.x] = a;
+    if (!last_block(&work->done) || !finish) return;
+    double t = 0.0;
+    for (int b = threadIdx.x; b < part_at + (int)gridDim.x; b += kNT) t += __ldcg(work->part + b);
+    t = block_sum(t, sm);
+    if (threadIdx.x != 0) return;
+    const double scale = h.grad_scale_at ? *h.grad_scale_at : h.grad_scale;
+    const double whole = sqrt(t) * fabs(scale);
+    if (norm64)
+        *(double*)norm = whole;
+    else
+        *(float*)norm = (float)whole;
+    // whole = 0: nothing to scale
+    work->factor = !isfinite(whole) ? (double)NAN : whole > h.max_norm ? scale * (h.max_norm / whole) : scale;
+}
+
+// ------------------------------------------------------------------- step --
+
+// What every value of a launch shares.
+template <class A>
+struct Shared {
+    A lr, b1, c1, b2, c2, eps, scale, i1, i2;  // c = 1 - b, i = 1 / (1 - b^t)
+};
+
+template <class A>
+__device__ __forceinline__ A step_one(const Shared<A>& k, A p, A g, A& m, A& v, A decay) {
+    g *= k.scale;
+    m = k.b1 * m + k.c1 * g;
+    v = k.b2 * v + k.c2 * (g * g);
+    const A move = m * k.i1 / (sqrt(v * k.i2) + k.eps);
+    // lr wd p by itself: 1 - lr wd would lose most of its digits
+    return (p - decay * p) - k.lr * move;
+}
+
+__device__ __forceinline__ float count_left(float t_ln_b) { return -expm1f(t_ln_b); }
+__device__ __forceinline__ double count_left(double t_ln_b) { return -expm1(t_ln_b); }
+
+template <class A>
+__device__ __forceinline__ Shared<A> shared_of(const Hyper& h, const Work* work, bool clipped, double& lr) {
+    Shared<A> k;
+    lr = h.lr_at ? *h.lr_at : h.lr;
+    k.lr = (A)lr;
+    k.b1 = (A)h.b1;
+    k.c1 = (A)(1.0 - h.b1);
+    k.b2 = (A)h.b2;
+    k.c2 = (A)(1.0 - h.b2);
+    k.eps = (A)h.eps;
+    k.scale = (A)(clipped ? work->factor : h.grad_scale_at ? *h.grad_scale_at : h.grad_scale);
+    k.i1 = k.i2 = A(1);
+    return k;
+}
+
+struct Tensor {
+    void* param;
+    const void* grad;
+    void *m, *v;
+    uint8_t *m_exp, *v_exp;
+    float* master;
+    int64_t n;  // values
+    double decay;
+    int first, number;  // its first chunk, its place in the caller's list
+};
+template <int N>
+struct Tensors {
+    Tensor of[N];
+};
+
+// One value of the arrays of a tensor or a table row. e: in the moments; ep: in p.
+template <class P, class G, class A, bool MASTER, int BITS>
+struct Values {
+    A p, g, m, v;
+    __device__ __forceinline__ void load(const P* param, const G* grad, const void* ms, const void* vs,
+                                         const float* master, int64_t ep, int64_t eg, int64_t e) {
+        p = MASTER ? (A)master[e] : widen<A>(param[ep]);
+        g = widen<A>(grad[eg]);
+        if constexpr (BITS != 8) {
+            m = ((const A*)ms)[e];
+            v = ((const A*)vs)[e];
+        }
+    }
+    __device__ __forceinline__ void store(P* param, void* ms, void* vs, float* master, int64_t ep, int64_t e) const {
+        if (MASTER) master[e] = (float)p;
+        param[ep] = narrow<P>(p);
+        if constexpr (BITS != 8) {
+            ((A*)ms)[e] = m;
+            ((A*)vs)[e] = v;
+        }
+    }
+};
+
+// Lane `lane` of 32 neighbouring values: moments read from codes and written to them, the
+// whole warp at once (a lane without a value takes part with 0).
+__device__ __forceinline__ void moments_of(const uint8_t* m, const uint8_t* v, unsigned xm, unsigned xv, int64_t e,
+                                           bool in, float& fm, float& fv) {
+    fm = in ? MCode::value(m[e], xm) : 0.0f;
+    fv = in ? VCode::value(v[e], xv) : 0.0f;
+}
+__device__ __forceinline__ void moments_to(uint8_t* m, uint8_t* v, uint8_t* m_exp, uint8_t* v_exp, int64_t block,
+                                           int64_t e, bool in, float fm, float fv, uint32_t random) {
+    const unsigned xm = MCode::shared(__reduce_max_sync(0xffffffffu, __float_as_uint(fm) & 0x7fffffffu));
+    const unsigned xv = VCode::shared(__reduce_max_sync(0xffffffffu, __float_as_uint(fv) & 0x7fffffffu));
+    if (in) {
+        m[e] = (uint8_t)MCode::code(fm, kHalfStep, xm);
+        v[e] = (uint8_t)VCode::code(fv, random, xv);
+    }
+    if ((threadIdx.x & 31) == 0) {
+        m_exp[block] = (uint8_t)xm;
+        v_exp[block] = (uint8_t)xv;
+    }
+}
+
+// Dense tensors of one kind. A warp's 32 lanes take 32 neighbouring values kPer times.
+// Chunks are walked from the last to the first: the norm's pass left the last gradients
+// in L2.
+template <class P, class G, bool MASTER, int BITS, int N>
+__global__ void __launch_bounds__(kNT)
+    adamw_kernel(const __grid_constant__ Tensors<N> list, int n_of, int64_t chunks, Work* work, bool clipped,
+                 bool count, const __grid_constant__ Hyper h) {
+    using A = typename Arith<P>::type;
+    __shared__ double left[2];
+    after_previous();
+    const int64_t t = *h.step + 1;
+    if (threadIdx.x == 0) left[0] = -1.0 / expm1((double)t * h.ln_b1);
+    if (threadIdx.x == 32) left[1] = -1.0 / expm1((double)t * h.ln_b2);
+    __syncthreads();
+    double lr;
+    Shared<A> k = shared_of<A>(h, work, clipped, lr);
+    k.i1 = (A)left[0];
+    k.i2 = (A)left[1];
+    if (clipped && isnan(work->factor)) {
+        last_block(&work->done);
+        return;
+    }
+    int i = n_of - 1;
+    for (int64_t c = chunks - 1 - blockIdx.x; c >= 0; c -= gridDim.x) {
+        while (c < list.of[i].first) --i;
+        const Tensor& s = list.of[i];
+        P* param = (P*)s.param;
+        const G* grad = (const G*)s.grad;
+        const A decay = (A)(lr * s.decay);
+        const int64_t base = (c - s.first) * kChunk + threadIdx.x;
+        Values<P, G, A, MASTER, BITS> v[kPer];
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) {
+            const int64_t e = base + j * kNT;
+            if (e < s.n) v[j].load(param, grad, s.m, s.v, s.master, e, e, e);
+        }
+        const uint32_t key = mix(mix(mix(h.seed) + (uint32_t)s.number) + (uint32_t)t);
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) {
+            const int64_t e = base + j * kNT, block = e / 32;
+            const bool in = e < s.n;
+            if constexpr (BITS == 8) {
+                if (block * 32 < s.n) {  // uniform over the warp
+                    float fm, fv;
+                    moments_of((const uint8_t*)s.m, (const uint8_t*)s.v, s.m_exp[block], s.v_exp[block], e, in, fm, fv);
+                    if (in) v[j].p = step_one(k, v[j].p, v[j].g, fm, fv, decay);
+                    moments_to((uint8_t*)s.m, (uint8_t*)s.v, s.m_exp, s.v_exp, block, e, in, fm, fv, round_bits(key, e));
+                    if (in) v[j].store(param, s.m, s.v, s.master, e, e);
+                }
+            } else if (in) {
+                v[j].p = step_one(k, v[j].p, v[j].g, v[j].m, v[j].v, decay);
+                v[j].store(param, s.m, s.v, s.master, e, e);
+            }
+        }
+    }
+    // every block has read the step count when the last one finishes
+    if (last_block(&work->done) && count && threadIdx.x == 0) *h.step = t;
+}
+
+// A table by touched rows.
+struct Table {
+    void* param;
+    const void* grad;
+    void *m, *v;
+    uint8_t *m_exp, *v_exp;
+    float* master;
+    const void* keys;
+    const int64_t* count;
+    int32_t* row_steps;
+    int64_t n_rows, d, ld, pitch, n_keys;
+    double decay;
+    int number;
+};
+
+// L lanes a row. A key outside the table, or not above the one before it, is left out.
+template <class P, class G, bool MASTER, int BITS, class K, int L>
+__global__ void __launch_bounds__(kNT)
+    adamw_rows_kernel(const __grid_constant__ Table s, Work* work, bool clipped, bool count,
+                      const __grid_constant__ Hyper h) {
+    using A = typename Arith<P>::type;
+    after_previous();
+    const int64_t t_all = *h.step + 1;
+    double lr;
+    Shared<A> k = shared_of<A>(h, work, clipped, lr);
+    if (clipped && isnan(work->factor)) {
+        last_block(&work->done);
+        return;
+    }
+    P* param = (P*)s.param;
+    const G* grad = (const G*)s.grad;
+    const K* keys = (const K*)s.keys;
+    const A decay = (A)(lr * s.decay);
+    const uint32_t key32 = mix(mix(mix(h.seed) + (uint32_t)s.number) + (uint32_t)t_all);
+    const int lane = threadIdx.x % L;
+    int64_t used = *s.count;
+    used = used < 0 ? 0 : used > s.n_keys ? s.n_keys : used;
+    const int64_t groups = (int64_t)gridDim.x * (kNT / L);
+    // uniform over the warp, whose rows go round together
+    for (int64_t at = ((int64_t)blockIdx.x * kNT + threadIdx.x) / 32 * (32 / L); at < used; at += groups) {
+        const int64_t slot = at + threadIdx.x % 32 / L;
+        int64_t r = -1;
+        if (slot < used) {
+            r = (int64_t)keys[slot];
+            if (r >= s.n_rows || (slot > 0 && (int64_t)keys[slot - 1] >= r)) r = -1;
+        }
+        if (r < 0) r = -1;
+        int t = 0;
+        if (r >= 0 && lane == 0) {
+            t = s.row_steps[r] + 1;
+            s.row_steps[r] = t;
+        }
+        t = __shfl_sync(0xffffffffu, t, 0, L);
+        k.i1 = A(1) / count_left((A)t * (A)h.ln_b1);
+        k.i2 = A(1) / count_left((A)t * (A)h.ln_b2);
+        for (int64_t c0 = 0; c0 < s.d; c0 += L) {
+            const int64_t c = c0 + lane, e = r * s.pitch + c;
+            const bool in = r >= 0 && c < s.d;
+            Values<P, G, A, MASTER, BITS> v;
+            if (in) v.load(param, grad, s.m, s.v, s.master, r * s.ld + c, slot * s.d + c, e);
+            if constexpr (BITS == 8) {
+                if (r < 0) break;  // L = 32: uniform over the warp
+                const int64_t block = (r * s.pitch + c0) / 32;
+                float fm, fv;
+                moments_of((const uint8_t*)s.m, (const uint8_t*)s.v, s.m_exp[block], s.v_exp[block], e, in, fm, fv);
+                if (in) v.p = step_one(k, v.p, v.g, fm, fv, decay);
+                moments_to((uint8_t*)s.m, (uint8_t*)s.v, s.m_exp, s.v_exp, block, e, in, fm, fv,
+                           round_bits(key32, r * s.d + c));
+                if (in) v.store(param, s.m, s.v, s.master, r * s.ld + c, e);
+            } else if (in) {
+                v.p = step_one(k, v.p, v.g, v.m, v.v, decay);
+                v.store(param, s.m, s.v, s.master, r * s.ld + c, e);
+            }
+        }
+    }
+    if (last_block(&work->done) && count && threadIdx.x == 0) *h.step = t_all;
+}
+
+// A step without a gradient still counts.
+__global__ void count_kernel(Work* work, bool clipped, const __grid_constant__ Hyper h) {
+    after_previous();
+    if (threadIdx.x == 0 && (!clipped || !isnan(work->factor))) *h.step += 1;
+}
+
+// Codes as the values that they stand for, exact in bfloat16.
+template <bool SIGNED>
+__global__ void __launch_bounds__(kNT)
+    moments_kernel(const uint8_t* __restrict__ code, const uint8_t* __restrict__ shared, int64_t n,
+                   __nv_bfloat16* __restrict__ out) {
+    for (int64_t e = (int64_t)blockIdx.x * kNT + threadIdx.x; e < n; e += (int64_t)gridDim.x * kNT)
+        out[e] = __float2bfloat16_rn(Code<SIGNED>::value(code[e], shared[e / 32]));
+}
+
+// ------------------------------------------------------------- launchers --
+
+size_t size_of(int dtype) { return dtype == MFM_DTYPE_F64 ? 8 : dtype == MFM_DTYPE_F32 ? 4 : 2; }
+
+void check_tensor(const mfm_adamw_tensor& t, int64_t i, int bits) {
+    auto bad = [&](const char* what) { fail(MFM_ERR_INVALID, fmt("tensor %lld: %s", (long long)i, what)); };
+    if (t.dtype != MFM_DTYPE_F64 && t.dtype != MFM_DTYPE_F32 && t.dtype != MFM_DTYPE_BF16 && t.dtype != MFM_DTYPE_F16)
+        fail(MFM_ERR_INVALID, fmt("tensor %lld: unknown dtype %d", (long long)i, t.dtype));
+    const bool half = t.dtype == MFM_DTYPE_BF16 || t.dtype == MFM_DTYPE_F16;
+    if (t.grad_dtype != t.dtype && !(half && t.grad_dtype == MFM_DTYPE_F32))
+        bad("grad_dtype must be dtype, or MFM_DTYPE_F32 for 16-bit parameters");
+    if (t.n_rows < 0 || t.d < 0) bad("n_rows and d must be >= 0");
+    if (t.master && !half) bad("master weights are for 16-bit parameters");
+    if (bits == 8 && t.dtype == MFM_DTYPE_F64) bad("8-bit moments are for parameters of at most 32 bits");
+    const bool rows = t.keys != nullptr;
+    if (!rows && t.n_rows != 1) bad("a tensor without keys has n_rows = 1");
+    if (rows && (!t.count || !t.row_steps)) bad("keys need count and row_steps");
+    if (rows && (t.n_keys < 0 || t.n_rows > INT32_MAX || t.n_keys > INT32_MAX || t.d > INT32_MAX))
+        bad("n_rows, n_keys and d of a table must be in [0, 2^31)");
+    if (rows && t.ld < t.d) bad("row pitch below d");
+    if (t.d > 0 && t.n_rows > 0 && (!t.param || !t.m || !t.v || (bits == 8 && (!t.m_exp || !t.v_exp))))
+        bad("param, m and v (and their exponents in 8 bits) must be provided");
+    const size_t s = size_of(t.dtype), wide = bits == 8 ? 1 : t.dtype == MFM_DTYPE_F64 ? 8 : 4;
+    if ((uintptr_t)t.param % s || (uintptr_t)t.grad % size_of(t.grad_dtype) || (uintptr_t)t.m % wide ||
+        (uintptr_t)t.v % wide || (uintptr_t)t.master % 4 || (uintptr_t)t.keys % (t.keys64 ? 8 : 4))
+        bad("an array does not begin at a multiple of its element's size");
+}
+
+template <class F>
+void with_kind(const mfm_adamw_tensor& t, int bits, F&& f) {
+    using std::integral_constant;
+    auto state = [&](auto* p, auto* g, auto master) {
+        if (bits == 8)
+            f(p, g, master, integral_constant<int, 8>{});
+        else
+            f(p, g, master, integral_constant<int, 32>{});
+    };
+    auto half = [&](auto* p) {
+        auto grad = [&](auto* g) {
+            if (t.master)
+                state(p, g, std::true_type{});
+            else
+                state(p, g, std::false_type{});
+        };
+        if (t.grad_dtype == MFM_DTYPE_F32)
+            grad((float*)nullptr);
+        else
+            grad(p);
+    };
+    switch (t.dtype) {
+        case MFM_DTYPE_F64: f((double*)nullptr, (double*)nullptr, std::false_type{}, integral_constant<int, 32>{}); break;
+        case MFM_DTYPE_F32: state((float*)nullptr, (float*)nullptr, std::false_type{}); break;
+        case MFM_DTYPE_BF16: half((__nv_bfloat16*)nullptr); break;
+        default: half((__half*)nullptr); break;
+    }
+}
+
+int kind_of(const mfm_adamw_tensor& t) { return (t.dtype * 8 + t.grad_dtype) * 2 + (t.master ? 1 : 0); }
+
+template <class X>
+using Bare = std::remove_pointer_t<X>;
+
+// Blocks of a persistent kernel: one wave.
+template <auto Kernel>
+unsigned wave(int device, int64_t most) {
+    static int per_sm[64];  // of this kernel: the answer stays
+    int per = per_sm[device & 63];
+    if (per == 0) {
+        MFM_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, Kernel, kNT, 0), "occupancy");
+        per_sm[device & 63] = per = std::max(per, 1);
+    }
+    return (unsigned)std::max<int64_t>(1, std::min<int64_t>(most, (int64_t)sm_count(device) * per));
+}
+
+}  // namespace
+}  // namespace mfm
+
+using namespace mfm;
+
+extern "C" int64_t mfm_adamw_workspace_bytes(void) { return (int64_t)sizeof(Work); }
+
+extern "C" int mfm_adamw_step_device(int device, const mfm_adamw_tensor* tensors, int64_t n_tensors,
+                                     const mfm_adamw* hyper, int64_t* step, void* norm, void* workspace,
+                                     int64_t workspace_bytes, void* stream) {
+    return guarded([&] {
+        if (!hyper || !step || n_tensors < 0 || (n_tensors > 0 && !tensors))
+            fail(MFM_ERR_INVALID, "tensors, hyper and step must be provided");
+        const mfm_adamw& o = *hyper;
+        if (!(o.beta_1 >= 0.0 && o.beta_1 < 1.0 && o.beta_2 >= 0.0 && o.beta_2 < 1.0))
+            fail(MFM_ERR_INVALID, "beta_1 and beta_2 must be in [0, 1)");
+        if (!(o.epsilon >= 1.2e-38)) fail(MFM_ERR_INVALID, "epsilon must be at least 2^-126");
+        if (o.state_bits != 32 && o.state_bits != 8) fail(MFM_ERR_INVALID, "state_bits must be 32 or 8");
+        const bool clipped = o.max_norm >= 0.0;
+        if (std::isnan(o.max_norm)) fail(MFM_ERR_INVALID, "max_norm must be a number");
+        if (clipped && !norm) fail(MFM_ERR_INVALID, "max_norm needs norm");
+        if (!workspace || workspace_bytes < (int64_t)sizeof(Work))
+            fail(MFM_ERR_INVALID, fmt("workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)sizeof(Work)));
+        if ((uintptr_t)workspace % 256) fail(MFM_ERR_INVALID, "workspace must be 256-byte aligned");
+        bool wide = false;
+        for (int64_t i = 0; i < n_tensors; ++i) {
+            if (tensors[i].grad) check_tensor(tensors[i], i, o.state_bits);
+            wide |= tensors[i].dtype == MFM_DTYPE_F64;
+        }
+        DeviceGuard guard(device);
+        cudaStream_t s = (cudaStream_t)stream;
+        Work* work = (Work*)workspace;
+        Hyper h{o.learning_rate, o.beta_1, o.beta_2, o.epsilon, std::log(o.beta_1), std::log(o.beta_2),
+                o.grad_scale, o.max_norm, o.learning_rate_at, o.grad_scale_at, step, o.seed};
+        // the tensors with a gradient, tables apart, and the dense ones by kind
+        std::vector<int64_t> dense, tables;
+        for (int64_t i = 0; i < n_tensors; ++i) {
+            const mfm_adamw_tensor& t = tensors[i];
+            if (!t.grad || t.d == 0 || t.n_rows == 0 || (t.keys && t.n_keys == 0)) continue;
+            (t.keys ? tables : dense).push_back(i);
+        }
+        std::stable_sort(dense.begin(), dense.end(),
+                         [&](int64_t a, int64_t b) { return kind_of(tensors[a]) < kind_of(tensors[b]); });
+        bool begun = false;  // the first launch of a call waits for all before it, the others go on in a chain
+        auto launch = [&](auto kernel, unsigned grid, auto&&... args) {
+            if (begun)
+                launch_next(kernel, grid, kNT, 0, s, args...);
+            else
+                kernel<<<grid, kNT, 0, s>>>(args...);
+            begun = true;
+        };
+        auto chunk = [](int64_t at) {
+            if (at > INT32_MAX) fail(MFM_ERR_UNSUPPORTED, "tensors of one kind exceed the engine's 2^42 values");
+            return (int)at;
+        };
+        if (clipped) {
+            std::vector<int64_t> all = dense;
+            all.insert(all.end(), tables.begin(), tables.end());
+            const size_t launches = std::max<size_t>(1, (size_t)ceil_div((int64_t)all.size(), kNormMany));
+            const unsigned share = kNormBlocks / (unsigned)std::min<size_t>(launches, kNormBlocks);
+            if (launches > kNormBlocks) fail(MFM_ERR_UNSUPPORTED, "more tensors than a norm is taken of");
+            int part = 0;
+            for (size_t l = 0; l < launches; ++l) {
+                const size_t lo = l * kNormMany, hi = std::min(all.size(), lo + kNormMany);
+                auto go = [&](auto most) {
+                    constexpr int N = decltype(most)::value;
+                    static thread_local Summands<N> list;
+                    int64_t chunks = 0;
+                    for (size_t q = lo; q < hi; ++q) {
+                        const mfm_adamw_tensor& t = tensors[all[q]];
+                        const int64_t rows = t.keys ? t.n_keys : 1;
+                        list.of[q - lo] = Summand{t.grad, t.keys ? t.n_keys : t.d, t.keys ? t.count : nullptr,
+                                                  chunk(chunks), t.keys ? (int)t.d : 1, t.grad_dtype};
+                        chunks += ceil_div(rows * t.d, kChunk);
+                    }
+                    const unsigned grid = (unsigned)std::max<int64_t>(1, std::min<int64_t>({chunks, (int64_t)share, (int64_t)sm_count(device) * 6}));
+                    launch(norm_kernel<N>, grid, list, (int)(hi - lo), chunks, work, part, l + 1 == launches, h, wide ? 1 : 0, norm);
+                    part += (int)grid;
+                };
+                if (hi - lo <= kNormFew)
+                    go(std::integral_constant<int, kNormFew>{});
+                else
+                    go(std::integral_constant<int, kNormMany>{});
+            }
+        }
+        // dense tensors: as many of one kind as a launch carries
+        for (size_t lo = 0; lo < dense.size();) {
+            size_t hi = lo;
+            while (hi < dense.size() && hi - lo < kMany && kind_of(tensors[dense[hi]]) == kind_of(tensors[dense[lo]])) ++hi;
+            const bool last = hi == dense.size() && tables.empty();
+            with_kind(tensors[dense[lo]], o.state_bits, [&](auto* p, auto* g, auto master, auto bits) {
+                using P = Bare<decltype(p)>;
+                using G = Bare<decltype(g)>;
+                auto go = [&](auto most) {
+                    constexpr int N = decltype(most)::value;
+                    static thread_local Tensors<N> list;
+                    int64_t chunks = 0;
+                    for (size_t q = lo; q < hi; ++q) {
+                        const mfm_adamw_tensor& t = tensors[dense[q]];
+                        list.of[q - lo] = Tensor{t.param, t.grad, t.m, t.v, t.m_exp, t.v_exp, t.master, t.d,
+                                                 t.weight_decay, chunk(chunks), (int)dense[q]};
+                        chunks += ceil_div(t.d, kChunk);
+                    }
+                    constexpr auto kernel = adamw_kernel<P, G, decltype(master)::value, decltype(bits)::value, N>;
+                    launch(kernel, wave<kernel>(device, chunks), list, (int)(hi - lo), chunks, work, clipped, last, h);
+                };
+                if (hi - lo <= kFew)
+                    go(std::integral_constant<int, kFew>{});
+                else
+                    go(std::integral_constant<int, kMany>{});
+            });
+            lo = hi;
+        }
+        for (size_t q = 0; q < tables.size(); ++q) {
+            const mfm_adamw_tensor& t = tensors[tables[q]];
+            with_kind(t, o.state_bits, [&](auto* p, auto* g, auto master, auto bits) {
+                using P = Bare<decltype(p)>;
+                using G = Bare<decltype(g)>;
+                constexpr int B = decltype(bits)::value;
+                const int64_t pitch = B == 8 ? ceil_div(t.d, 32) * 32 : t.d;
+                const Table table{t.param, t.grad, t.m, t.v, t.m_exp, t.v_exp, t.master, t.keys, t.count, t.row_steps,
+                                  t.n_rows, t.d, t.ld, pitch, t.n_keys, t.weight_decay, (int)tables[q]};
+                with_index_type(t.keys64, [&](auto* kp) {
+                    using K = std::remove_const_t<Bare<decltype(kp)>>;
+                    auto go = [&](auto lanes) {
+                        constexpr int L = decltype(lanes)::value;
+                        constexpr auto kernel = adamw_rows_kernel<P, G, decltype(master)::value, B, K, L>;
+                        launch(kernel, wave<kernel>(device, ceil_div(t.n_keys, kNT / L)), table, work, clipped,
+                               q + 1 == tables.size(), h);
+                    };
+                    if constexpr (B != 8) {
+                        if (t.d <= 16) return go(std::integral_constant<int, 16>{});
+                    }
+                    go(std::integral_constant<int, 32>{});
+                });
+            });
+        }
+        if (dense.empty() && tables.empty()) launch(count_kernel, 1, work, clipped, h);
+        MFM_CHECK_LAUNCH("AdamW step launch");
+    });
+}
+
+extern "C" int mfm_adamw_moments_device(int device, int is_signed, const uint8_t* code, const uint8_t* exponent,
+                                        int64_t n, void* out, void* stream) {
+    return guarded([&] {
+        if (n < 0) fail(MFM_ERR_INVALID, "n must be >= 0");
+        if (n == 0) return;
+        if (!code || !exponent || !out) fail(MFM_ERR_INVALID, "code, exponent and out must be provided");
+        DeviceGuard guard(device);
+        auto kernel = is_signed ? moments_kernel<true> : moments_kernel<false>;
+        const int64_t grid = std::min<int64_t>(ceil_div(n, kNT), (int64_t)sm_count(device) * 8);
+        kernel<<<(unsigned)grid, kNT, 0, (cudaStream_t)stream>>>(code, exponent, n, (__nv_bfloat16*)out);
+        MFM_CHECK_LAUNCH("moments launch");
+    });
+}
