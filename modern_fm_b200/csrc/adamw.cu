@@ -106,16 +106,6 @@ struct Work {
     double part[kNormBlocks];
 };
 
-__device__ __forceinline__ double block_sum(double v, double* sm) {
-    v = warp_sum(v);
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) sm[threadIdx.x / 32] = v;
-    __syncthreads();
-    double t = 0.0;
-    for (int w = 0; w < (int)blockDim.x / 32; ++w) t += sm[w];
-    return t;
-}
-
 // The block that finishes last: on every thread whether this is it; the count is left at 0.
 __device__ __forceinline__ bool last_block(unsigned* done) {
     __shared__ unsigned last;

@@ -183,6 +183,17 @@ void launch_next(void (*kernel)(KArgs...), unsigned grid, unsigned block, size_t
     MFM_CUDA(cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...), "kernel launch");
 }
 
+// Sum over the block in a fixed order, on every thread.
+__device__ __forceinline__ double block_sum(double v, double* sm) {
+    v = warp_sum(v);
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) sm[threadIdx.x / 32] = v;
+    __syncthreads();
+    double t = 0.0;
+    for (int w = 0; w < (int)blockDim.x / 32; ++w) t += sm[w];
+    return t;
+}
+
 template <class F>
 void with_index_type(int ids64, F&& f) {
     if (ids64)
