@@ -553,6 +553,33 @@ int mfm_policy_loss_device(int dtype, int device, const void* logits, int64_t ld
                            void* stats, void* logprobs, void* d_logits, int64_t ld_out,
                            void* workspace, int64_t workspace_bytes, void* stream);
 
+/* What else a row of class scores says. With labels (NULL: none): logprobs as above and
+ * ranks, the label's place among the classes in order of falling score, ties by index
+ * (0: the best). lse as above, entropy = -sum p log p, and the first `top` classes of that order
+ * (top <= 32, n_classes): top_ids and top_logprobs, (n_tokens, top). ranks and top_ids
+ * have the labels' type (labels64, also without labels). A class of score -infinity
+ * has probability 0 and a place in the order. A row that its label masks, or whose every
+ * score is -infinity, has log-probabilities and entropy 0, rank and ids -1, and lse 0
+ * (-infinity for the latter); a row with a NaN or +infinity has NaN and -1. */
+int mfm_label_alternatives_device(int dtype, int device, const void* logits, int64_t ld,
+                                  int64_t n_tokens, int64_t n_classes, int labels64,
+                                  const void* labels, int top, void* logprobs, void* lse,
+                                  void* entropy, void* ranks, void* top_ids, void* top_logprobs,
+                                  void* stream);
+
+/* The scores' gradient for the gradients of logprobs, entropy and top_logprobs (each may
+ * be NULL or, with top = 0, absent; lse, entropy and top_ids are the forward's):
+ *   d_logits[t, c] = sum of the gradients of log-probabilities of class c
+ *                    - p (their sum over the row + grad_entropy (log p + entropy))
+ * 0 for masked rows. Places of top_ids outside [0, n_classes) have no part in it; a
+ * class that several places name has the sum of theirs. Must not overlap logits. */
+int mfm_label_alternatives_grad_device(int dtype, int device, const void* logits, int64_t ld,
+                                       int64_t n_tokens, int64_t n_classes, int labels64,
+                                       const void* labels, const void* lse, const void* entropy,
+                                       const void* grad_logprobs, const void* grad_entropy,
+                                       int top, const void* top_ids, const void* grad_top,
+                                       void* d_logits, int64_t ld_out, void* stream);
+
 /* ---- AdamW over many tensors ------------------------------------------------
  * The engine's own optimizers step its models inside fit (rust/src/optimizer.rs:68-85
  * is the lazy Adam that the by-row form resembles); this one steps a caller's

@@ -172,6 +172,13 @@ _SIGNATURES = {
         ct.c_int, ct.c_int, ct.c_void_p, ct.c_int64, ct.c_int64, ct.c_int64, ct.c_int, ct.c_void_p,
         ct.c_void_p, ct.c_void_p, ct.c_void_p, ct.c_double, ct.c_double, ct.c_double, ct.c_void_p,
         ct.c_void_p, ct.c_void_p, ct.c_void_p, ct.c_int64, ct.c_void_p, ct.c_int64, ct.c_void_p]),
+    "mfm_label_alternatives_device": (ct.c_int, [
+        ct.c_int, ct.c_int, ct.c_void_p, ct.c_int64, ct.c_int64, ct.c_int64, ct.c_int, ct.c_void_p,
+        ct.c_int] + [ct.c_void_p] * 7),
+    "mfm_label_alternatives_grad_device": (ct.c_int, [
+        ct.c_int, ct.c_int, ct.c_void_p, ct.c_int64, ct.c_int64, ct.c_int64, ct.c_int]
+        + [ct.c_void_p] * 5 + [ct.c_int, ct.c_void_p, ct.c_void_p, ct.c_void_p, ct.c_int64,
+                               ct.c_void_p]),
     "mfm_adamw_workspace_bytes": (ct.c_int64, []),
     "mfm_adamw_step_device": (ct.c_int, [
         ct.c_int, ct.c_void_p, ct.c_int64, ct.POINTER(AdamW), ct.c_void_p, ct.c_void_p, ct.c_void_p,

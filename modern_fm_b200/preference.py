@@ -59,18 +59,31 @@ class PolicyLoss(NamedTuple):
     grad: Optional[object]
 
 
+class LabelAlternatives(NamedTuple):
+    """``logprobs`` and ``ranks`` of the labels (None without labels), ``lse`` and
+    ``entropy`` per row; ``top_ids`` and ``top_logprobs`` (n_rows, top), or None."""
+    logprobs: Optional[object]
+    lse: object
+    entropy: object
+    ranks: Optional[object]
+    top_ids: Optional[object]
+    top_logprobs: Optional[object]
+
+
 def _scores(logits, labels):
-    """(dtype code, arithmetic type, pointer, rows, classes, pitch, labels64) of the scores."""
+    """(dtype code, arithmetic type, pointer, rows, classes, pitch, labels64) of the scores;
+    labels None: none, with 64-bit ids."""
     code = _STORAGE.get(logits.dtype)
     if code is None:
         raise ValueError("logits must be float64, float32, bfloat16 or float16")
     p, n, c, ld = _matrix("logits", logits)
     if c < 1:
         raise ValueError("logits must have at least one class")
-    kind = labels.dtype
+    kind = torch.int64 if labels is None else labels.dtype
     if kind is not torch.int64 and kind is not torch.int32:
         raise ValueError("labels must be int32 or int64")
-    _vector("labels", labels, n, kind)
+    if labels is not None:
+        _vector("labels", labels, n, kind)
     wide = torch.float64 if code == _lib.MFM_DTYPE_F64 else torch.float32
     return code, wide, p, n, c, ld, 1 if kind is torch.int64 else 0
 
@@ -123,6 +136,85 @@ def label_logprobs_grad(grad, logits, labels, lse, stream=None):
         out = logits.new_empty((n, c))
     _fail(_lib.lib().mfm_label_logprobs_grad_device(
         code, dev, p, ld, n, c, l64, labels.data_ptr(), grad.data_ptr(), lse.data_ptr(),
+        out.data_ptr(), c, s))
+    return out
+
+
+def label_alternatives(logits, labels=None, top: int = 0, stream=None) -> LabelAlternatives:
+    """What a row of class scores says besides its label's log-probability.
+
+    ``logprobs`` and ``lse`` as ``label_logprobs`` has them, the ``entropy``
+    ``-sum p log p``, the label's ``rank`` in the order of falling score (0: the best;
+    classes of one score by index), and the first ``top`` classes of that order with
+    their log-probabilities, ``top`` at most 32 and the number of classes. ``ranks`` and
+    ``top_ids`` have the labels' type (int64 without labels). A class of score
+    -infinity has probability 0 and its place in the order. Masked rows have
+    log-probabilities and entropy 0, rank and ids -1, and lse 0 (rows whose every score is
+    -infinity: lse -infinity); rows with a NaN or +infinity have NaN and -1.
+    """
+    code, wide, p, n, c, ld, l64 = _scores(logits, labels)
+    top = int(top)
+    if not 0 <= top <= min(32, c):
+        raise ValueError("top must be between 0 and 32, and at most the number of classes")
+    dev = _one_device(logits, labels)
+    s, ctx = _on(stream, dev)
+    _hold(stream, logits, labels)
+    kind = torch.int64 if l64 else torch.int32
+    ids = lps = lp = ranks = None
+    with ctx:
+        lse = logits.new_empty(n, dtype=wide)
+        entropy = logits.new_empty(n, dtype=wide)
+        if labels is not None:
+            lp = logits.new_empty(n, dtype=wide)
+            ranks = logits.new_empty(n, dtype=kind)
+        if top:
+            ids = logits.new_empty((n, top), dtype=kind)
+            lps = logits.new_empty((n, top), dtype=wide)
+    _fail(_lib.lib().mfm_label_alternatives_device(
+        code, dev, p, ld, n, c, l64, _ptr(labels), top, _ptr(lp), lse.data_ptr(),
+        entropy.data_ptr(), _ptr(ranks), _ptr(ids), _ptr(lps), s))
+    return LabelAlternatives(lp, lse, entropy, ranks, ids, lps)
+
+
+def label_alternatives_grad(logits, lse, entropy=None, labels=None, grad_logprobs=None,
+                            grad_entropy=None, top_ids=None, grad_top=None, stream=None):
+    """Gradient of the logits, in their type, for the gradients of ``label_alternatives``'
+    log-probabilities, entropy and best classes' log-probabilities, each of which may be
+    None: ``[sum of the log-probabilities' gradients at class c] - p[c] (their sum over
+    the row + grad_entropy (log p[c] + entropy))``. ``lse``, ``entropy`` and ``top_ids`` are
+    the forward's; ids outside the classes have no part in it, a class named twice has the
+    sum."""
+    code, wide, p, n, c, ld, l64 = _scores(logits, labels)
+    _vector("lse", lse, n, wide)
+    if grad_logprobs is not None:
+        if labels is None:
+            raise ValueError("grad_logprobs needs labels")
+        _vector("grad_logprobs", grad_logprobs, n, wide)
+    if grad_entropy is not None:
+        if entropy is None:
+            raise ValueError("grad_entropy needs entropy")
+        _vector("entropy", entropy, n, wide)
+        _vector("grad_entropy", grad_entropy, n, wide)
+    top = 0
+    if (top_ids is None) != (grad_top is None):
+        raise ValueError("top_ids and grad_top go together")
+    if top_ids is not None:
+        kind = torch.int64 if l64 else torch.int32
+        top = top_ids.shape[-1] if top_ids.dim() == 2 else -1
+        if not 0 <= top <= 32 or top_ids.dtype != kind or tuple(top_ids.shape) != (n, top) \
+                or not top_ids.is_contiguous():
+            raise ValueError(f"top_ids must be a contiguous {kind} matrix of one row per row of "
+                             "logits and at most 32 columns")
+        if grad_top.dtype != wide or grad_top.shape != top_ids.shape or not grad_top.is_contiguous():
+            raise ValueError(f"grad_top must be contiguous, {wide} and have the shape of top_ids")
+    dev = _one_device(logits, lse, entropy, labels, grad_logprobs, grad_entropy, top_ids, grad_top)
+    s, ctx = _on(stream, dev)
+    _hold(stream, logits, lse, entropy, labels, grad_logprobs, grad_entropy, top_ids, grad_top)
+    with ctx:
+        out = logits.new_empty((n, c))
+    _fail(_lib.lib().mfm_label_alternatives_grad_device(
+        code, dev, p, ld, n, c, l64, _ptr(labels), lse.data_ptr(), _ptr(entropy),
+        _ptr(grad_logprobs), _ptr(grad_entropy), top, _ptr(top_ids), _ptr(grad_top),
         out.data_ptr(), c, s))
     return out
 
