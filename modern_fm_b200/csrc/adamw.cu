@@ -56,6 +56,13 @@ struct Code {
     // random bits: b2 = 0.999 moves v by a thousandth of itself, and rounded to nearest it
     // would stand still until g^2 is some 50 times v. What is above 0 stays above 0 in v,
     // where 0 would leave m / eps.
+    // of magnitudes whose number stays finite
+    static __device__ __forceinline__ unsigned plain_code(float v, unsigned add, unsigned x) {
+        const unsigned bits = __float_as_uint(v) & 0x7fffffffu;
+        const int k = min(max((int)((bits + add) >> 20) - (int)(8 * x), SIGNED ? 0 : 1), (int)kMost);
+        if (SIGNED) return (unsigned)k | (k ? (__float_as_uint(v) >> 31) << 7 : 0u);
+        return bits ? (unsigned)k : 0u;
+    }
     static __device__ __forceinline__ unsigned code(float v, unsigned add, unsigned x) {
         const unsigned bits = __float_as_uint(v) & 0x7fffffffu, n = number(bits, add), base = 8 * x;
         if (bits == 0) return 0;
@@ -201,18 +208,29 @@ struct Shared {
     A lr, b1, c1, b2, c2, eps, scale, i1, i2;  // c = 1 - b, i = 1 / (1 - b^t)
 };
 
+// a / (sqrt(b) + eps), in 32 bits off by at most 7 units of 2^-24 of itself (root 2, sum 1,
+// quotient 4: the approximate forms of one instruction; the denominator is below 2^126,
+// where the quotient's holds).
+__device__ __forceinline__ float over_root(float a, float b, float eps) {
+    float r;
+    asm("sqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(b));
+    return __fdividef(a, r + eps);
+}
+__device__ __forceinline__ double over_root(double a, double b, double eps) { return a / (sqrt(b) + eps); }
+
 template <class A>
 __device__ __forceinline__ A step_one(const Shared<A>& k, A p, A g, A& m, A& v, A decay) {
     g *= k.scale;
     m = k.b1 * m + k.c1 * g;
     v = k.b2 * v + k.c2 * (g * g);
-    const A move = m * k.i1 / (sqrt(v * k.i2) + k.eps);
+    const A move = over_root(m * k.i1, v * k.i2, k.eps);
     // lr wd p by itself: 1 - lr wd would lose most of its digits
     return (p - decay * p) - k.lr * move;
 }
 
-__device__ __forceinline__ float count_left(float t_ln_b) { return -expm1f(t_ln_b); }
-__device__ __forceinline__ double count_left(double t_ln_b) { return -expm1(t_ln_b); }
+// 1 / (1 - b^t) by t log b
+__device__ __forceinline__ float inverse_left(double t_ln_b, float) { return 1.0f / -expm1f((float)t_ln_b); }
+__device__ __forceinline__ double inverse_left(double t_ln_b, double) { return 1.0 / -expm1(t_ln_b); }
 
 template <class A>
 __device__ __forceinline__ Shared<A> shared_of(const Hyper& h, const Work* work, bool clipped, double& lr) {
@@ -288,11 +306,147 @@ __device__ __forceinline__ void moments_to(uint8_t* m, uint8_t* v, uint8_t* m_ex
     }
 }
 
-// Dense tensors of one kind. A warp's 32 lanes take 32 neighbouring values kPer times.
-// Chunks are walked from the last to the first: the norm's pass left the last gradients
-// in L2.
-template <class P, class G, bool MASTER, int BITS, int N>
-__global__ void __launch_bounds__(kNT)
+// Eight neighbouring values as one access of 16 or 32 bytes.
+template <class T>
+struct Eight;
+template <>
+struct Eight<float> {
+    float v[8];
+    __device__ __forceinline__ void load(const float* p) {
+        asm volatile("ld.global.v8.f32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                     : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7])
+                     : "l"(p)
+                     : "memory");
+    }
+    __device__ __forceinline__ float get(int i) const { return v[i]; }
+    static __device__ __forceinline__ void store(float* p, const float (&o)[8]) {
+        asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "f"(o[0]), "f"(o[1]), "f"(o[2]),
+                     "f"(o[3]), "f"(o[4]), "f"(o[5]), "f"(o[6]), "f"(o[7])
+                     : "memory");
+    }
+};
+template <class H>
+struct EightHalves {
+    uint4 r;
+    __device__ __forceinline__ void load(const H* p) { r = *reinterpret_cast<const uint4*>(p); }
+    __device__ __forceinline__ float get(int i) const {
+        const unsigned w = i < 2 ? r.x : i < 4 ? r.y : i < 6 ? r.z : r.w;
+        const unsigned h = i & 1 ? w >> 16 : w & 0xffffu;
+        const unsigned short b = (unsigned short)h;
+        return widen<float>(*reinterpret_cast<const H*>(&b));
+    }
+    static __device__ __forceinline__ void store(H* p, const float (&o)[8]) {
+        *reinterpret_cast<uint4*>(p) = Pack<H>::pack(o);
+    }
+};
+template <>
+struct Eight<__nv_bfloat16> : EightHalves<__nv_bfloat16> {};
+template <>
+struct Eight<__half> : EightHalves<__half> {};
+
+__device__ __forceinline__ unsigned byte_of(const uint2& w, int i) { return (i < 4 ? w.x : w.y) >> (8 * (i & 3)) & 255u; }
+
+// Eight neighbouring values: at `ep` in p, `eg` in the gradient, `e` in moments and master
+// weights, number `at` of the tensor for their random bits. Whole warps call it: four
+// lanes share a block of 8-bit moments; a lane without values takes part with zeros.
+template <class P, class G, bool MASTER, int BITS>
+__device__ __forceinline__ void step_eight(const Shared<float>& k, float decay, P* param, const G* grad, void* ms,
+                                           void* vs, uint8_t* m_exp, uint8_t* v_exp, float* master, int64_t ep,
+                                           int64_t eg, int64_t e, int64_t at, uint32_t key, bool in) {
+    Eight<P> p;
+    Eight<G> g;
+    Eight<float> w, fm, fv;
+    uint2 cm, cv;
+    unsigned xm, xv;
+    if (!in) ep = eg = e = 0;  // there are eight values there
+    if (MASTER)
+        w.load(master + e);
+    else
+        p.load(param + ep);
+    g.load(grad + eg);
+    if (BITS == 8) {
+        cm = *reinterpret_cast<const uint2*>((const uint8_t*)ms + e);
+        cv = *reinterpret_cast<const uint2*>((const uint8_t*)vs + e);
+        xm = m_exp[e / 32];
+        xv = v_exp[e / 32];
+    } else {
+        fm.load((const float*)ms + e);
+        fv.load((const float*)vs + e);
+    }
+    float out[8], m[8], v[8];
+    unsigned top_m = 0, top_v = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        m[i] = BITS == 8 ? MCode::value(byte_of(cm, i), xm) : fm.get(i);
+        v[i] = BITS == 8 ? VCode::value(byte_of(cv, i), xv) : fv.get(i);
+        out[i] = step_one(k, MASTER ? w.get(i) : p.get(i), g.get(i), m[i], v[i], decay);
+        if (BITS == 8) {
+            top_m = max(top_m, __float_as_uint(m[i]) & 0x7fffffffu);
+            top_v = max(top_v, __float_as_uint(v[i]));
+        }
+    }
+    if (BITS == 8) {
+        if (!in) top_m = top_v = 0;
+#pragma unroll
+        for (int o = 1; o < 4; o *= 2) {
+            top_m = max(top_m, __shfl_xor_sync(0xffffffffu, top_m, o));
+            top_v = max(top_v, __shfl_xor_sync(0xffffffffu, top_v & 0x7fffffffu, o));
+        }
+        xm = MCode::shared(top_m);
+        xv = VCode::shared(top_v & 0x7fffffffu);
+        const bool plain = top_m < 0x7f700000u && (top_v & 0x7fffffffu) < 0x7f700000u;
+        unsigned bm[8], bv[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            bm[i] = plain ? MCode::plain_code(m[i], kHalfStep, xm) : MCode::code(m[i], kHalfStep, xm);
+            const uint32_t random = round_bits(key, at + i);
+            bv[i] = plain ? VCode::plain_code(v[i], random, xv) : VCode::code(v[i], random, xv);
+        }
+        cm = make_uint2(bm[0] | bm[1] << 8 | bm[2] << 16 | bm[3] << 24, bm[4] | bm[5] << 8 | bm[6] << 16 | bm[7] << 24);
+        cv = make_uint2(bv[0] | bv[1] << 8 | bv[2] << 16 | bv[3] << 24, bv[4] | bv[5] << 8 | bv[6] << 16 | bv[7] << 24);
+    }
+    if (!in) return;
+    if (MASTER) Eight<float>::store(master + e, out);
+    Eight<P>::store(param + ep, out);
+    if (BITS == 8) {
+        *reinterpret_cast<uint2*>((uint8_t*)ms + e) = cm;
+        *reinterpret_cast<uint2*>((uint8_t*)vs + e) = cv;
+        if (e % 32 == 0) {
+            m_exp[e / 32] = (uint8_t)xm;
+            v_exp[e / 32] = (uint8_t)xv;
+        }
+    } else {
+        Eight<float>::store((float*)ms + e, m);
+        Eight<float>::store((float*)vs + e, v);
+    }
+}
+
+// One value: of p at `ep`, of the gradient at `eg`, else at `e`. Whole warps call it: 32
+// lanes share a block of 8-bit moments.
+template <class P, class G, class A, bool MASTER, int BITS>
+__device__ __forceinline__ void step_value(const Shared<A>& k, A decay, P* param, const G* grad, void* ms, void* vs,
+                                           uint8_t* m_exp, uint8_t* v_exp, float* master, int64_t ep, int64_t eg,
+                                           int64_t e, int64_t at, uint32_t key, bool in) {
+    Values<P, G, A, MASTER, BITS> v;
+    if (in) v.load(param, grad, ms, vs, master, ep, eg, e);
+    if constexpr (BITS == 8) {
+        const int64_t block = (e - (threadIdx.x & 31)) / 32;
+        float fm, fv;
+        moments_of((const uint8_t*)ms, (const uint8_t*)vs, m_exp[block], v_exp[block], e, in, fm, fv);
+        if (in) v.p = step_one(k, v.p, v.g, fm, fv, decay);
+        moments_to((uint8_t*)ms, (uint8_t*)vs, m_exp, v_exp, block, e, in, fm, fv, round_bits(key, at));
+    } else if (in) {
+        v.p = step_one(k, v.p, v.g, v.m, v.v, decay);
+    }
+    if (in) v.store(param, ms, vs, master, ep, e);
+}
+
+// Dense tensors of one kind. EIGHTS: they begin at whole vectors, and a thread takes eight
+// neighbouring values, up to the last whole block of 32; elsewhere a warp's 32 lanes
+// take 32 neighbouring values kPer times. Chunks are walked from the last to the first: the
+// norm's pass left the last gradients in L2.
+template <class P, class G, bool MASTER, int BITS, bool EIGHTS, int N>
+__global__ void __launch_bounds__(kNT, IsF64<typename Arith<P>::type>::value ? 2 : 3)
     adamw_kernel(const __grid_constant__ Tensors<N> list, int n_of, int64_t chunks, Work* work, bool clipped,
                  bool count, const __grid_constant__ Hyper h) {
     using A = typename Arith<P>::type;
@@ -317,30 +471,34 @@ __global__ void __launch_bounds__(kNT)
         P* param = (P*)s.param;
         const G* grad = (const G*)s.grad;
         const A decay = (A)(lr * s.decay);
-        const int64_t base = (c - s.first) * kChunk + threadIdx.x;
-        Values<P, G, A, MASTER, BITS> v[kPer];
-#pragma unroll
-        for (int j = 0; j < kPer; ++j) {
-            const int64_t e = base + j * kNT;
-            if (e < s.n) v[j].load(param, grad, s.m, s.v, s.master, e, e, e);
-        }
         const uint32_t key = mix(mix(mix(h.seed) + (uint32_t)s.number) + (uint32_t)t);
-#pragma unroll
-        for (int j = 0; j < kPer; ++j) {
-            const int64_t e = base + j * kNT, block = e / 32;
-            const bool in = e < s.n;
-            if constexpr (BITS == 8) {
-                if (block * 32 < s.n) {  // uniform over the warp
-                    float fm, fv;
-                    moments_of((const uint8_t*)s.m, (const uint8_t*)s.v, s.m_exp[block], s.v_exp[block], e, in, fm, fv);
-                    if (in) v[j].p = step_one(k, v[j].p, v[j].g, fm, fv, decay);
-                    moments_to((uint8_t*)s.m, (uint8_t*)s.v, s.m_exp, s.v_exp, block, e, in, fm, fv, round_bits(key, e));
-                    if (in) v[j].store(param, s.m, s.v, s.master, e, e);
-                }
-            } else if (in) {
-                v[j].p = step_one(k, v[j].p, v[j].g, v[j].m, v[j].v, decay);
-                v[j].store(param, s.m, s.v, s.master, e, e);
+        const int64_t base = (c - s.first) * kChunk;
+        if constexpr (EIGHTS) {
+            const int64_t e = base + threadIdx.x * kPer, end = s.n / 32 * 32;
+            if (base < end)
+                step_eight<P, G, MASTER, BITS>(k, decay, param, grad, s.m, s.v, s.m_exp, s.v_exp, s.master, e, e, e, e, key, e < end);
+            if (base + kChunk > s.n && end < s.n && threadIdx.x < 32) {  // the tensor's last values
+                const int64_t q = end + threadIdx.x;
+                step_value<P, G, A, MASTER, BITS>(k, decay, param, grad, s.m, s.v, s.m_exp, s.v_exp, s.master, q, q, q, q, key, q < s.n);
             }
+        } else if constexpr (BITS == 8) {
+            for (int j = 0; j < kPer; ++j) {
+                const int64_t e = base + threadIdx.x + j * kNT;
+                if (e - (threadIdx.x & 31) < s.n)  // uniform over the warp
+                    step_value<P, G, A, MASTER, BITS>(k, decay, param, grad, s.m, s.v, s.m_exp, s.v_exp, s.master, e, e, e, e, key, e < s.n);
+            }
+        } else {
+            Values<P, G, A, MASTER, BITS> v[kPer];
+            const int64_t e = base + threadIdx.x;
+#pragma unroll
+            for (int j = 0; j < kPer; ++j)
+                if (e + j * kNT < s.n) v[j].load(param + e, grad + e, (A*)s.m + e, (A*)s.v + e, s.master + e, j * kNT, j * kNT, j * kNT);
+#pragma unroll
+            for (int j = 0; j < kPer; ++j)
+                if (e + j * kNT < s.n) {
+                    v[j].p = step_one(k, v[j].p, v[j].g, v[j].m, v[j].v, decay);
+                    v[j].store(param + e, (A*)s.m + e, (A*)s.v + e, s.master + e, j * kNT, j * kNT);
+                }
         }
     }
     // every block has read the step count when the last one finishes
@@ -362,9 +520,19 @@ struct Table {
     int number;
 };
 
-// L lanes a row. A key outside the table, or not above the one before it, is left out.
-template <class P, class G, bool MASTER, int BITS, class K, int L>
-__global__ void __launch_bounds__(kNT)
+// The row of slot `slot`, -1 for one that is left out: a key outside the table, or not above
+// the one before it.
+template <class K>
+__device__ __forceinline__ int64_t row_of(const Table& s, int64_t slot, int64_t used) {
+    if (slot >= used) return -1;
+    const K* keys = (const K*)s.keys;
+    const int64_t r = (int64_t)keys[slot], before = slot > 0 ? (int64_t)keys[slot - 1] : -1;
+    return r < s.n_rows && r > before && r >= 0 ? r : -1;
+}
+
+// L lanes a row, a value a lane or (EIGHTS) eight neighbouring ones. A key outside the table, or not above the one before it, is left out.
+template <class P, class G, bool MASTER, int BITS, class K, bool EIGHTS, int L>
+__global__ void __launch_bounds__(kNT, EIGHTS ? 3 : 4)
     adamw_rows_kernel(const __grid_constant__ Table s, Work* work, bool clipped, bool count,
                       const __grid_constant__ Hyper h) {
     using A = typename Arith<P>::type;
@@ -378,7 +546,6 @@ __global__ void __launch_bounds__(kNT)
     }
     P* param = (P*)s.param;
     const G* grad = (const G*)s.grad;
-    const K* keys = (const K*)s.keys;
     const A decay = (A)(lr * s.decay);
     const uint32_t key32 = mix(mix(mix(h.seed) + (uint32_t)s.number) + (uint32_t)t_all);
     const int lane = threadIdx.x % L;
@@ -388,37 +555,27 @@ __global__ void __launch_bounds__(kNT)
     // uniform over the warp, whose rows go round together
     for (int64_t at = ((int64_t)blockIdx.x * kNT + threadIdx.x) / 32 * (32 / L); at < used; at += groups) {
         const int64_t slot = at + threadIdx.x % 32 / L;
-        int64_t r = -1;
-        if (slot < used) {
-            r = (int64_t)keys[slot];
-            if (r >= s.n_rows || (slot > 0 && (int64_t)keys[slot - 1] >= r)) r = -1;
-        }
-        if (r < 0) r = -1;
+        const int64_t r = row_of<K>(s, slot, used);
         int t = 0;
         if (r >= 0 && lane == 0) {
             t = s.row_steps[r] + 1;
             s.row_steps[r] = t;
         }
         t = __shfl_sync(0xffffffffu, t, 0, L);
-        k.i1 = A(1) / count_left((A)t * (A)h.ln_b1);
-        k.i2 = A(1) / count_left((A)t * (A)h.ln_b2);
-        for (int64_t c0 = 0; c0 < s.d; c0 += L) {
-            const int64_t c = c0 + lane, e = r * s.pitch + c;
-            const bool in = r >= 0 && c < s.d;
-            Values<P, G, A, MASTER, BITS> v;
-            if (in) v.load(param, grad, s.m, s.v, s.master, r * s.ld + c, slot * s.d + c, e);
-            if constexpr (BITS == 8) {
-                if (r < 0) break;  // L = 32: uniform over the warp
-                const int64_t block = (r * s.pitch + c0) / 32;
-                float fm, fv;
-                moments_of((const uint8_t*)s.m, (const uint8_t*)s.v, s.m_exp[block], s.v_exp[block], e, in, fm, fv);
-                if (in) v.p = step_one(k, v.p, v.g, fm, fv, decay);
-                moments_to((uint8_t*)s.m, (uint8_t*)s.v, s.m_exp, s.v_exp, block, e, in, fm, fv,
-                           round_bits(key32, r * s.d + c));
-                if (in) v.store(param, s.m, s.v, s.master, r * s.ld + c, e);
-            } else if (in) {
-                v.p = step_one(k, v.p, v.g, v.m, v.v, decay);
-                v.store(param, s.m, s.v, s.master, r * s.ld + c, e);
+        k.i1 = inverse_left((double)t * h.ln_b1, A(0));
+        k.i2 = inverse_left((double)t * h.ln_b2, A(0));
+        if constexpr (EIGHTS) {
+            for (int64_t c0 = 0; c0 < s.pitch; c0 += L * 8) {
+                const int64_t c = c0 + lane * 8;
+                step_eight<P, G, MASTER, BITS>(k, decay, param, grad, s.m, s.v, s.m_exp, s.v_exp, s.master, r * s.ld + c,
+                                               slot * s.d + c, r * s.pitch + c, r * s.d + c, key32, r >= 0 && c < s.d);
+            }
+        } else {
+            for (int64_t c0 = 0; c0 < s.d; c0 += L) {
+                const int64_t c = c0 + lane;
+                if (BITS == 8 && r < 0) break;  // L = 32: uniform over the warp
+                step_value<P, G, A, MASTER, BITS>(k, decay, param, grad, s.m, s.v, s.m_exp, s.v_exp, s.master, r * s.ld + c,
+                                                  slot * s.d + c, r * s.pitch + c, r * s.d + c, key32, r >= 0 && c < s.d);
             }
         }
     }
@@ -431,13 +588,29 @@ __global__ void count_kernel(Work* work, bool clipped, const __grid_constant__ H
     if (threadIdx.x == 0 && (!clipped || !isnan(work->factor))) *h.step += 1;
 }
 
-// Codes as the values that they stand for, exact in bfloat16.
+// Codes as the values that they stand for, exact in bfloat16: a number's bits are the float32's
+// upper ones, so a code becomes a bfloat16 by a sum and a shift.
+template <bool SIGNED>
+__device__ __forceinline__ unsigned short half_of(unsigned code, unsigned x) {
+    const unsigned k = code & Code<SIGNED>::kMost, bits = k ? (8 * x + k) << 4 : 0;
+    return (unsigned short)(SIGNED ? bits | (code & 128) << 8 : bits);
+}
 template <bool SIGNED>
 __global__ void __launch_bounds__(kNT)
     moments_kernel(const uint8_t* __restrict__ code, const uint8_t* __restrict__ shared, int64_t n,
-                   __nv_bfloat16* __restrict__ out) {
-    for (int64_t e = (int64_t)blockIdx.x * kNT + threadIdx.x; e < n; e += (int64_t)gridDim.x * kNT)
-        out[e] = __float2bfloat16_rn(Code<SIGNED>::value(code[e], shared[e / 32]));
+                   unsigned short* __restrict__ out, bool whole) {
+    const int64_t step = (int64_t)gridDim.x * kNT, first = (int64_t)blockIdx.x * kNT + threadIdx.x;
+    const int64_t eights = whole ? n / 8 : 0;
+    for (int64_t i = first; i < eights; i += step) {
+        const uint2 c = *reinterpret_cast<const uint2*>(code + 8 * i);
+        const unsigned x = shared[i / 4];
+        unsigned w[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+            w[q] = half_of<SIGNED>(byte_of(c, 2 * q), x) | (unsigned)half_of<SIGNED>(byte_of(c, 2 * q + 1), x) << 16;
+        *reinterpret_cast<uint4*>(out + 8 * i) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    for (int64_t e = eights * 8 + first; e < n; e += step) out[e] = half_of<SIGNED>(code[e], shared[e / 32]);
 }
 
 // ------------------------------------------------------------- launchers --
@@ -466,6 +639,15 @@ void check_tensor(const mfm_adamw_tensor& t, int64_t i, int bits) {
     if ((uintptr_t)t.param % s || (uintptr_t)t.grad % size_of(t.grad_dtype) || (uintptr_t)t.m % wide ||
         (uintptr_t)t.v % wide || (uintptr_t)t.master % 4 || (uintptr_t)t.keys % (t.keys64 ? 8 : 4))
         bad("an array does not begin at a multiple of its element's size");
+}
+
+// Whether eight neighbouring values are whole vectors in every array: they begin at them, and
+// rows at multiples of `row` values (0: no rows).
+bool eights(const mfm_adamw_tensor& t, int bits, int64_t row) {
+    if (t.dtype == MFM_DTYPE_F64 || row % 8) return false;
+    const uintptr_t p = t.dtype == MFM_DTYPE_F32 ? 32 : 16, g = t.grad_dtype == MFM_DTYPE_F32 ? 32 : 16;
+    return (uintptr_t)t.param % p == 0 && (uintptr_t)t.grad % g == 0 && ((uintptr_t)t.m | (uintptr_t)t.v) % (bits == 8 ? 8 : 32) == 0 &&
+           (uintptr_t)t.master % 32 == 0;
 }
 
 template <class F>
@@ -497,7 +679,9 @@ void with_kind(const mfm_adamw_tensor& t, int bits, F&& f) {
     }
 }
 
-int kind_of(const mfm_adamw_tensor& t) { return (t.dtype * 8 + t.grad_dtype) * 2 + (t.master ? 1 : 0); }
+int kind_of(const mfm_adamw_tensor& t, int bits) {
+    return ((t.dtype * 8 + t.grad_dtype) * 2 + (t.master ? 1 : 0)) * 2 + (eights(t, bits, 0) ? 1 : 0);
+}
 
 template <class X>
 using Bare = std::remove_pointer_t<X>;
@@ -556,7 +740,7 @@ extern "C" int mfm_adamw_step_device(int device, const mfm_adamw_tensor* tensors
             (t.keys ? tables : dense).push_back(i);
         }
         std::stable_sort(dense.begin(), dense.end(),
-                         [&](int64_t a, int64_t b) { return kind_of(tensors[a]) < kind_of(tensors[b]); });
+                         [&](int64_t a, int64_t b) { return kind_of(tensors[a], o.state_bits) < kind_of(tensors[b], o.state_bits); });
         bool begun = false;  // the first launch of a call waits for all before it, the others go on in a chain
         auto launch = [&](auto kernel, unsigned grid, auto&&... args) {
             if (begun)
@@ -602,12 +786,13 @@ extern "C" int mfm_adamw_step_device(int device, const mfm_adamw_tensor* tensors
         // dense tensors: as many of one kind as a launch carries
         for (size_t lo = 0; lo < dense.size();) {
             size_t hi = lo;
-            while (hi < dense.size() && hi - lo < kMany && kind_of(tensors[dense[hi]]) == kind_of(tensors[dense[lo]])) ++hi;
+            const int kind = kind_of(tensors[dense[lo]], o.state_bits);
+            while (hi < dense.size() && hi - lo < kMany && kind_of(tensors[dense[hi]], o.state_bits) == kind) ++hi;
             const bool last = hi == dense.size() && tables.empty();
             with_kind(tensors[dense[lo]], o.state_bits, [&](auto* p, auto* g, auto master, auto bits) {
                 using P = Bare<decltype(p)>;
                 using G = Bare<decltype(g)>;
-                auto go = [&](auto most) {
+                auto go = [&](auto most, auto aligned) {
                     constexpr int N = decltype(most)::value;
                     static thread_local Tensors<N> list;
                     int64_t chunks = 0;
@@ -617,13 +802,19 @@ extern "C" int mfm_adamw_step_device(int device, const mfm_adamw_tensor* tensors
                                                  t.weight_decay, chunk(chunks), (int)dense[q]};
                         chunks += ceil_div(t.d, kChunk);
                     }
-                    constexpr auto kernel = adamw_kernel<P, G, decltype(master)::value, decltype(bits)::value, N>;
+                    constexpr auto kernel = adamw_kernel<P, G, decltype(master)::value, decltype(bits)::value, decltype(aligned)::value, N>;
                     launch(kernel, wave<kernel>(device, chunks), list, (int)(hi - lo), chunks, work, clipped, last, h);
                 };
-                if (hi - lo <= kFew)
-                    go(std::integral_constant<int, kFew>{});
-                else
-                    go(std::integral_constant<int, kMany>{});
+                auto size = [&](auto aligned) {
+                    if (hi - lo <= kFew)
+                        go(std::integral_constant<int, kFew>{}, aligned);
+                    else
+                        go(std::integral_constant<int, kMany>{}, aligned);
+                };
+                if constexpr (!IsF64<P>::value) {
+                    if (kind & 1) return size(std::true_type{});
+                }
+                size(std::false_type{});
             });
             lo = hi;
         }
@@ -638,16 +829,26 @@ extern "C" int mfm_adamw_step_device(int device, const mfm_adamw_tensor* tensors
                                   t.n_rows, t.d, t.ld, pitch, t.n_keys, t.weight_decay, (int)tables[q]};
                 with_index_type(t.keys64, [&](auto* kp) {
                     using K = std::remove_const_t<Bare<decltype(kp)>>;
-                    auto go = [&](auto lanes) {
+                    auto go = [&](auto lanes, auto aligned) {
                         constexpr int L = decltype(lanes)::value;
-                        constexpr auto kernel = adamw_rows_kernel<P, G, decltype(master)::value, B, K, L>;
+                        constexpr auto kernel = adamw_rows_kernel<P, G, decltype(master)::value, B, K, decltype(aligned)::value, L>;
                         launch(kernel, wave<kernel>(device, ceil_div(t.n_keys, kNT / L)), table, work, clipped,
                                q + 1 == tables.size(), h);
                     };
-                    if constexpr (B != 8) {
-                        if (t.d <= 16) return go(std::integral_constant<int, 16>{});
+                    using std::integral_constant;
+                    if constexpr (!IsF64<P>::value) {
+                        // in 8 bits every block of 32 has its four lanes, also where a row ends in it
+                        if (eights(t, o.state_bits, t.d | t.ld)) {
+                            if (B != 8 && t.d <= 16) return go(integral_constant<int, B == 8 ? 4 : 2>{}, std::true_type{});
+                            if (t.d <= 32) return go(integral_constant<int, 4>{}, std::true_type{});
+                            if (t.d <= 128) return go(integral_constant<int, 16>{}, std::true_type{});
+                            return go(integral_constant<int, 32>{}, std::true_type{});
+                        }
                     }
-                    go(std::integral_constant<int, 32>{});
+                    if constexpr (B != 8) {
+                        if (t.d <= 16) return go(integral_constant<int, 16>{}, std::false_type{});
+                    }
+                    go(integral_constant<int, 32>{}, std::false_type{});
                 });
             });
         }
@@ -664,8 +865,9 @@ extern "C" int mfm_adamw_moments_device(int device, int is_signed, const uint8_t
         if (!code || !exponent || !out) fail(MFM_ERR_INVALID, "code, exponent and out must be provided");
         DeviceGuard guard(device);
         auto kernel = is_signed ? moments_kernel<true> : moments_kernel<false>;
-        const int64_t grid = std::min<int64_t>(ceil_div(n, kNT), (int64_t)sm_count(device) * 8);
-        kernel<<<(unsigned)grid, kNT, 0, (cudaStream_t)stream>>>(code, exponent, n, (__nv_bfloat16*)out);
+        const int64_t grid = std::min<int64_t>(ceil_div(n, 8 * kNT), (int64_t)sm_count(device) * 8);
+        kernel<<<(unsigned)grid, kNT, 0, (cudaStream_t)stream>>>(code, exponent, n, (unsigned short*)out,
+                                                                 (uintptr_t)code % 8 == 0 && (uintptr_t)out % 16 == 0);
         MFM_CHECK_LAUNCH("moments launch");
     });
 }

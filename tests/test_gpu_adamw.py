@@ -304,7 +304,8 @@ def test_codes_of_extreme_values():
 
 
 @pytest.mark.parametrize("kind,grad", [("f64", "f64"), ("f32", "f32"), ("bf16", "f32"), ("f16", "f16")])
-@pytest.mark.parametrize("n,d,pitch", [(7, 1, 1), (40, 16, 16), (40, 17, 20), (100, 33, 33), (300, 8, 8), (50, 300, 304)])
+@pytest.mark.parametrize("n,d,pitch", [(7, 1, 1), (40, 16, 16), (40, 17, 20), (100, 33, 33), (300, 8, 8), (50, 300, 304), (60, 24, 24), (30, 40, 48),
+                                       (20, 256, 256), (9, 1000, 1000), (30, 104, 104)])
 @pytest.mark.parametrize("bits", [32, 8])
 @pytest.mark.parametrize("ids", [torch.int32, torch.int64])
 def test_rows(kind, grad, n, d, pitch, bits, ids):
