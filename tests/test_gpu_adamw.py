@@ -273,6 +273,26 @@ def test_rounding_of_v_keeps_its_average():
     assert torch.equal(others[0].state.v, others[1].state.v) and not torch.equal(others[0].state.v, others[2].state.v)
 
 
+@pytest.mark.parametrize("off", [0, 1])
+@pytest.mark.parametrize("scale", [1e-36, 1e-30, 1e-3, 1.0, 3.0, 1000.0, 3e4, 7e4, 1e10, 1e17])
+def test_codes_at_every_scale(scale, off):
+    """b1 = b2 = 0: m is the gradient to 1 / 16 of itself (half a step; 2^-13 more for where
+    ties go), v its square to 1 / 8, if they are within the codes' reach of 15 and 31 octaves.
+    Below 2^-126 float32 values, and codes, have steps of one size: 2^-129 with 3 bits, of which half
+    (and 2^-13) is lost, and all of a value below half."""
+    g = torch.Generator().manual_seed(1)
+    size = torch.exp2(-12 * torch.rand(4096 + off, generator=g)) * torch.where(torch.rand(4096 + off, generator=g) < 0.5, -1, 1)
+    x = (size * scale).cuda()[off:]
+    opt = AdamW([torch.zeros(4096 + off, device="cuda")[off:]], state_bits=8, betas=(0.0, 0.0), lr=0.0)
+    opt.step([x])
+    m, v = (t.double() for t in opt.moments())
+    x = x.double()
+    assert bool(((m - x).abs() <= x.abs() * (1 / 16 + 2.0**-13) + 2.0**-130 * (1 + 2.0**-12)).all())
+    if 1e-18 < scale:
+        assert bool(((v - x * x).abs() <= x * x * (1 / 8 + 2.0**-20)).all())
+    assert bool((torch.sign(m) == torch.sign(x))[x.abs() >= 2.0**-129].all())
+
+
 def test_codes_of_extreme_values():
     """Zero, infinity and NaN, and magnitudes from the smallest to the largest float32."""
     x = torch.tensor([0.0, -0.0, 1.0, -1.0, 1.9999999, 3.4028235e38, -3.4028235e38, 1e-38, 1e-45, 1.17e-38] + [0.0] * 22,
