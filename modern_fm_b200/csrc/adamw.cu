@@ -226,35 +226,35 @@ __global__ void __launch_bounds__(kNT)
 // What every value of a launch shares.
 template <class A>
 struct Shared {
-    A lr, b1, c1, b2, c2, eps, scale, i1, i2;  // c = 1 - b, i = 1 / (1 - b^t)
-    A root_scale, unscale;                     // i2 comes times the first, the root times the second
+    A lr, b1, c1, b2, c2, eps, scale;  // c = 1 - b
+    A i1, i2;                          // lr / (1 - b1^t), 1 / (1 - b2^t)
+    A root_scale, unscale;             // i2 comes times the first, the root times the second
     __device__ __forceinline__ void corrections(A one, A two) {
-        i1 = one;
+        i1 = lr * one;
         i2 = two * root_scale;
     }
 };
 
-// a / (sqrt(b) + eps), in 32 bits off by at most 7 units of 2^-24 of itself (root 2, sum 1,
-// reciprocal 2, product 1: the approximate forms of one instruction; the denominator is
-// at least eps, a normal number).
-// A root flushes what is below 2^-126 to 0, which an eps of 1e-11 or more does not notice; beside a
-// smaller one b comes 2^24 times as large (then a move is 0 from b = 2^104 on).
-__device__ __forceinline__ float over_root(float a, float b, float eps, float unscale) {
+// 1 / (sqrt(b) + eps), in 32 bits off by at most 5 units of 2^-24 of itself (root 2, sum 1,
+// reciprocal 2: the approximate forms of one instruction; the denominator is at least eps, a
+// normal number). A root flushes what is below 2^-126 to 0, which an eps of 1e-11 or more
+// does not notice; beside a smaller one b comes 2^24 times as large (then a move is 0 from
+// b = 2^104 on).
+__device__ __forceinline__ float over_root(float b, float eps, float unscale) {
     float r;
     asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(b));
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(r * unscale + eps));
-    return a * r;
+    return r;
 }
-__device__ __forceinline__ double over_root(double a, double b, double eps, double) { return a / (sqrt(b) + eps); }
+__device__ __forceinline__ double over_root(double b, double eps, double) { return 1.0 / (sqrt(b) + eps); }
 
 template <class A>
 __device__ __forceinline__ A step_one(const Shared<A>& k, A p, A g, A& m, A& v, A decay) {
     g *= k.scale;
     m = k.b1 * m + k.c1 * g;
     v = k.b2 * v + k.c2 * (g * g);
-    const A move = over_root(m * k.i1, v * k.i2, k.eps, k.unscale);
     // lr wd p by itself: 1 - lr wd would lose most of its digits
-    return (p - decay * p) - k.lr * move;
+    return (p - decay * p) - (m * k.i1) * over_root(v * k.i2, k.eps, k.unscale);
 }
 
 // 1 / (1 - b^t) by t log b
@@ -374,8 +374,24 @@ struct Eight<__nv_bfloat16> : EightHalves<__nv_bfloat16> {};
 template <>
 struct Eight<__half> : EightHalves<__half> {};
 
-// Eight neighbouring values: at `ep` in p, `eg` in the gradient, `e` in moments and master
-// weights, number `at` of the tensor for their random bits.
+// Where eight neighbouring values lie. Bases that a block shares and offsets of 32 bits make
+// addresses of one instruction.
+template <class P, class G>
+struct At {
+    P* param;
+    const G* grad;
+    char *m, *v;  // float32, or codes
+    uint8_t *m_exp, *v_exp;
+    float* master;
+    // of the tensor's or row's value `e`, a multiple of 32 for a dense tensor; p: of the parameter
+    template <int BITS, class S>
+    static __device__ __forceinline__ At of(const S& s, int64_t ep, int64_t eg, int64_t e) {
+        constexpr int size = BITS == 8 ? 1 : 4;
+        return At{(P*)s.param + ep, (const G*)s.grad + eg, (char*)s.m + e * size, (char*)s.v + e * size,
+                  s.m_exp + e / 32, s.v_exp + e / 32, s.master + e};
+    }
+};
+
 template <class P, class G, bool MASTER, int BITS>
 struct Step8 {
     Eight<P> p;
@@ -384,28 +400,26 @@ struct Step8 {
     uint2 cm, cv;
     uint8_t xm, xv;
     // Whole warps take a step: four lanes share a block of 8-bit moments. A lane without
-    // values (`in` false) takes part with the first ones there are, and stores nothing.
-    __device__ __forceinline__ void load(const P* param, const G* grad, const void* ms, const void* vs,
-                                         const uint8_t* m_exp, const uint8_t* v_exp, const float* master, int64_t ep,
-                                         int64_t eg, int64_t e, bool in) {
-        if (!in) ep = eg = e = 0;
+    // values (`in` false) takes part with those at offset 0, and stores nothing.
+    __device__ __forceinline__ void load(const At<P, G>& at, unsigned off) {
         if (MASTER)
-            w.load(master + e);
+            w.load(at.master + off);
         else
-            p.load(param + ep);
-        g.load(grad + eg);
+            p.load(at.param + off);
+        g.load(at.grad + off);
         if (BITS == 8) {
-            cm = *reinterpret_cast<const uint2*>((const uint8_t*)ms + e);
-            cv = *reinterpret_cast<const uint2*>((const uint8_t*)vs + e);
-            xm = m_exp[e / 32];
-            xv = v_exp[e / 32];
+            cm = *reinterpret_cast<const uint2*>(at.m + off);
+            cv = *reinterpret_cast<const uint2*>(at.v + off);
+            xm = at.m_exp[off / 32];
+            xv = at.v_exp[off / 32];
         } else {
-            fm.load((const float*)ms + e);
-            fv.load((const float*)vs + e);
+            fm.load((const float*)at.m + off);
+            fv.load((const float*)at.v + off);
         }
     }
-    __device__ __forceinline__ void step(const Shared<float>& k, float decay, P* param, void* ms, void* vs, uint8_t* m_exp,
-                                         uint8_t* v_exp, float* master, int64_t ep, int64_t e, int64_t at, uint32_t key, bool in) {
+    // e: the first value's place in the tensor, which its random bits go by
+    __device__ __forceinline__ void step(const Shared<float>& k, float decay, const At<P, G>& at, unsigned off, int64_t e,
+                                         uint32_t key, bool in) {
         float out[8], m[8], v[8];
         if (BITS == 8) {
             const unsigned was_m = (unsigned)xm * 0x00800080u, was_v = (unsigned)xv * 0x00800080u;
@@ -444,7 +458,7 @@ struct Step8 {
             x_v = VCode::shared(top_v);
             // up to 61440 in m: twice a number's distance from the base then fits in 31 bits
             if (top_m < 0x47700000u && top_v < 0x7f700000u) {
-                const uint32_t from = round_from(at, key), folded = from ^ (from >> 16);
+                const uint32_t from = round_from(e, key), folded = from ^ (from >> 16);
                 // No number is more than its code's most above the base, which the largest one gave;
                 // m: 0 for what is below it, v: 1, but 0 stays 0 (other values are no less than 1).
                 const unsigned add_m = 2 * (kHalfStep - (x_m << 23)), less_v = x_v << 23;
@@ -468,24 +482,24 @@ struct Step8 {
                     cms[w] = cvs[w] = 0;
                     for (int i = 0; i < 4; ++i) {
                         cms[w] |= MCode::code(m[4 * w + i], kHalfStep, x_m) << (8 * i);
-                        cvs[w] |= VCode::code(v[4 * w + i], round_bits(key, at + 4 * w + i), x_v) << (8 * i);
+                        cvs[w] |= VCode::code(v[4 * w + i], round_bits(key, e + 4 * w + i), x_v) << (8 * i);
                     }
                 }
             }
         }
         if (!in) return;
-        if (MASTER) Eight<float>::store(master + e, out);
-        Eight<P>::store(param + ep, out);
+        if (MASTER) Eight<float>::store(at.master + off, out);
+        Eight<P>::store(at.param + off, out);
         if (BITS == 8) {
-            *reinterpret_cast<uint2*>((uint8_t*)ms + e) = make_uint2(cms[0], cms[1]);
-            *reinterpret_cast<uint2*>((uint8_t*)vs + e) = make_uint2(cvs[0], cvs[1]);
-            if (e % 32 == 0) {
-                m_exp[e / 32] = (uint8_t)x_m;
-                v_exp[e / 32] = (uint8_t)x_v;
+            *reinterpret_cast<uint2*>(at.m + off) = make_uint2(cms[0], cms[1]);
+            *reinterpret_cast<uint2*>(at.v + off) = make_uint2(cvs[0], cvs[1]);
+            if (off % 32 == 0) {
+                at.m_exp[off / 32] = (uint8_t)x_m;
+                at.v_exp[off / 32] = (uint8_t)x_v;
             }
         } else {
-            Eight<float>::store((float*)ms + e, m);
-            Eight<float>::store((float*)vs + e, v);
+            Eight<float>::store((float*)at.m + off, m);
+            Eight<float>::store((float*)at.v + off, v);
         }
     }
 };
@@ -516,7 +530,7 @@ __device__ __forceinline__ void step_value(const Shared<A>& k, A decay, P* param
 // norm's pass left the last gradients in L2.
 template <class P, class G, bool MASTER, int BITS, bool EIGHTS, int N>
 __global__ void __launch_bounds__(kNT, IsF64<typename Arith<P>::type>::value ? 2 : 3)
-    adamw_kernel(const __grid_constant__ Tensors<N> list, int n_of, int64_t chunks, Work* work, bool clipped,
+    adamw_kernel(const __grid_constant__ Tensors<N> list, int n_of, int64_t chunks, int rounds, Work* work, bool clipped,
                  bool count, const __grid_constant__ Hyper h) {
     using A = typename Arith<P>::type;
     __shared__ double left[2];
@@ -534,43 +548,36 @@ __global__ void __launch_bounds__(kNT, IsF64<typename Arith<P>::type>::value ? 2
     }
     int i = n_of - 1;
     if constexpr (EIGHTS) {
-        // 8-bit moments are bound by instructions: a chunk's loads are under way while the one
-        // before it is worked on (184 M values: PRE us without that). The others wait for
-        // memory whatever they do, and need the registers for blocks.
+        // A thread's eights of a chunk, kChunk apart. 8-bit moments are bound by instructions:
+        // there the loads of one are under way while the one before it is worked on. The
+        // others wait for memory whatever they do, and need the registers for blocks.
         constexpr bool AHEAD = BITS == 8;
-        using Step = Step8<P, G, MASTER, BITS>;
-        Step now, next;
-        int64_t c = chunks - 1 - blockIdx.x;
-        auto find = [&](int64_t at, int from) {
-            while (at < list.of[from].first) --from;
-            return from;
-        };
-        auto fetch = [&](Step& to, int64_t at, const Tensor& s) {
-            const int64_t e = (at - s.first) * kChunk + threadIdx.x * kPer, end = s.n / 32 * 32;
-            if ((at - s.first) * kChunk < end)
-                to.load((const P*)s.param, (const G*)s.grad, s.m, s.v, s.m_exp, s.v_exp, s.master, e, e, e, e < end);
-        };
-        if (AHEAD && c >= 0) fetch(now, c, list.of[i = find(c, i)]);
-        for (; c >= 0; c -= gridDim.x) {
-            const int64_t c_next = c - gridDim.x;
-            int i_next = i;
-            if (!AHEAD)
-                fetch(now, c, list.of[i = find(c, i)]);
-            else if (c_next >= 0)
-                fetch(next, c_next, list.of[i_next = find(c_next, i)]);
+        const int64_t size = kChunk * rounds;
+        for (int64_t c = chunks - 1 - blockIdx.x; c >= 0; c -= gridDim.x) {
+            while (c < list.of[i].first) --i;
             const Tensor& s = list.of[i];
-            P* param = (P*)s.param;
             const A decay = (A)(lr * s.decay);
             const uint32_t key = mix(mix(mix(h.seed) + (uint32_t)s.number) + (uint32_t)t);
-            const int64_t base = (c - s.first) * kChunk, e = base + threadIdx.x * kPer, end = s.n / 32 * 32;
-            if (base < end) now.step(k, decay, param, s.m, s.v, s.m_exp, s.v_exp, s.master, e, e, e, key, e < end);
-            if (base + kChunk > s.n && end < s.n && threadIdx.x < 32) {  // the tensor's last values
-                const int64_t q = end + threadIdx.x;
-                step_value<P, G, A, MASTER, BITS>(k, decay, param, (const G*)s.grad, s.m, s.v, s.m_exp, s.v_exp, s.master, q, q, q, q, key, q < s.n);
+            const int64_t base = (c - s.first) * size, whole = s.n / 32 * 32 - base;
+            // values of the chunk that vectors take: whole blocks of 32
+            const unsigned n = (unsigned)(whole < 0 ? 0 : whole > size ? size : whole);
+            const At<P, G> at = At<P, G>::template of<BITS>(s, base, base, base);
+            unsigned off = threadIdx.x * kPer;
+            Step8<P, G, MASTER, BITS> now, next;
+            if (AHEAD && n) now.load(at, off < n ? off : 0);
+#pragma unroll 1
+            for (unsigned done = 0; done < n; done += kChunk, off += kChunk) {
+                const unsigned coming = off + kChunk;
+                if (!AHEAD)
+                    now.load(at, off < n ? off : 0);
+                else if (done + kChunk < n)
+                    next.load(at, coming < n ? coming : 0);
+                now.step(k, decay, at, off, base + off, key, off < n);
+                if (AHEAD) now = next;
             }
-            if (AHEAD) {
-                now = next;
-                i = i_next;
+            if (base + size > s.n && s.n % 32 && threadIdx.x < 32) {  // the tensor's last values
+                const int64_t q = s.n / 32 * 32 + threadIdx.x;
+                step_value<P, G, A, MASTER, BITS>(k, decay, (P*)s.param, (const G*)s.grad, s.m, s.v, s.m_exp, s.v_exp, s.master, q, q, q, q, key, q < s.n);
             }
         }
     } else {
@@ -666,11 +673,13 @@ __global__ void __launch_bounds__(kNT, EIGHTS ? 3 : 4)
         k.corrections(inverse_left((double)t * h.ln_b1, A(0)), inverse_left((double)t * h.ln_b2, A(0)));
         if constexpr (EIGHTS) {
             for (int64_t c0 = 0; c0 < s.pitch; c0 += L * 8) {
-                const int64_t c = c0 + lane * 8;
+                const unsigned c = (unsigned)c0 + lane * 8;
                 const bool in = r >= 0 && c < s.d;
                 Step8<P, G, MASTER, BITS> now;
-                now.load(param, grad, s.m, s.v, s.m_exp, s.v_exp, s.master, r * s.ld + c, slot * s.d + c, r * s.pitch + c, in);
-                now.step(k, decay, param, s.m, s.v, s.m_exp, s.v_exp, s.master, r * s.ld + c, r * s.pitch + c, r * s.d + c, key32, in);
+                const At<P, G> at = r < 0 ? At<P, G>::template of<BITS>(s, 0, 0, 0)
+                                          : At<P, G>::template of<BITS>(s, r * s.ld, slot * s.d, r * s.pitch);
+                now.load(at, in ? c : 0);
+                now.step(k, decay, at, c, r * s.d + c, key32, in);
             }
         } else {
             for (int64_t c0 = 0; c0 < s.d; c0 += L) {
@@ -901,15 +910,20 @@ extern "C" int mfm_adamw_step_device(int device, const mfm_adamw_tensor* tensors
                 auto go = [&](auto most, auto aligned) {
                     constexpr int N = decltype(most)::value;
                     static thread_local Tensors<N> list;
-                    int64_t chunks = 0;
+                    // chunks of 8-bit moments are larger where there are enough of them: what a chunk
+                    // costs a thread is shared by more values (184 M values: 495 us with single
+                    // rounds, POST us with four)
+                    int64_t chunks = 0, values = 0;
+                    for (size_t q = lo; q < hi; ++q) values += tensors[dense[q]].d;
+                    const int rounds = decltype(bits)::value == 8 && decltype(aligned)::value && values >= 32 * kChunk * sm_count(device) ? 4 : 1;
                     for (size_t q = lo; q < hi; ++q) {
                         const mfm_adamw_tensor& t = tensors[dense[q]];
                         list.of[q - lo] = Tensor{t.param, t.grad, t.m, t.v, t.m_exp, t.v_exp, t.master, t.d,
                                                  t.weight_decay, chunk(chunks), (int)dense[q]};
-                        chunks += ceil_div(t.d, kChunk);
+                        chunks += ceil_div(t.d, kChunk * rounds);
                     }
                     constexpr auto kernel = adamw_kernel<P, G, decltype(master)::value, decltype(bits)::value, decltype(aligned)::value, N>;
-                    launch(kernel, wave<kernel>(device, chunks), list, (int)(hi - lo), chunks, work, clipped, last, h);
+                    launch(kernel, wave<kernel>(device, chunks), list, (int)(hi - lo), chunks, rounds, work, clipped, last, h);
                 };
                 auto size = [&](auto aligned) {
                     if (hi - lo <= kFew)
