@@ -911,11 +911,13 @@ extern "C" int mfm_adamw_step_device(int device, const mfm_adamw_tensor* tensors
                     constexpr int N = decltype(most)::value;
                     static thread_local Tensors<N> list;
                     // chunks of 8-bit moments are larger where there are enough of them: what a chunk
-                    // costs a thread is shared by more values (184 M values: 495 us with single
-                    // rounds, POST us with four)
+                    // costs a thread is shared by more values (184 M values: 495 us with one round,
+                    // 459 with four, 444 with eight)
                     int64_t chunks = 0, values = 0;
                     for (size_t q = lo; q < hi; ++q) values += tensors[dense[q]].d;
-                    const int rounds = decltype(bits)::value == 8 && decltype(aligned)::value && values >= 32 * kChunk * sm_count(device) ? 4 : 1;
+                    const int rounds = decltype(bits)::value == 8 && decltype(aligned)::value
+                                           ? (int)std::clamp<int64_t>(values / (kChunk * 12 * sm_count(device)), 1, 8)
+                                           : 1;
                     for (size_t q = lo; q < hi; ++q) {
                         const mfm_adamw_tensor& t = tensors[dense[q]];
                         list.of[q - lo] = Tensor{t.param, t.grad, t.m, t.v, t.m_exp, t.v_exp, t.master, t.d,

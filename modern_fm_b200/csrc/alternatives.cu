@@ -12,6 +12,8 @@
 // exponential a value.
 #include "score_rows.cuh"
 
+#include <cooperative_groups.h>
+
 #include <algorithm>
 
 namespace mfm {
@@ -165,9 +167,9 @@ __global__ void __launch_bounds__(kSmallNT)
     }
 }
 
-// --------------------------------------------------------------- any rows --
+// ------------------------------------------------------------ longer rows --
 
-// A row's group of L threads within a block.
+// A row's, or a part of a row's, group of L threads within a block.
 template <int L>
 __device__ __forceinline__ void group_sync() {
     if (L == 32)
@@ -178,25 +180,128 @@ __device__ __forceinline__ void group_sync() {
         asm volatile("bar.sync %0, %1;" ::"r"(1 + threadIdx.x / L), "n"(L) : "memory");
 }
 
-// exp and exp times its argument over N values.
-template <int N>
-__device__ __forceinline__ void add_terms(const float (&v)[N], float off, float& s, float& d) {
+// Sums of e = exp(v - off) and of e (v - off). In 32 bits as powers of two, two values an
+// instruction, the second sum in units of log 2: 16-bit scores are otherwise bound by issue slots.
+template <class A>
+struct Terms {
+    uint64_t s = 0, d = 0, minus_off;
+    __device__ __forceinline__ explicit Terms(float off) : minus_off(pair_of(-off, -off)) {}
+    template <int N>
+    __device__ __forceinline__ void add(const float (&v)[N]) {
 #pragma unroll
-    for (int q = 0; q < N; ++q) {
-        const float z = v[q] - off, e = exp_of(z);
-        s += e;
-        d += e * floor_of(z);
+        for (int q = 0; q < N; q += 2) {
+            float a, b, ea, eb;
+            pair_to(pair_mul(pair_add(pair_of(v[q], v[q + 1]), minus_off), pair_of(1.4426950408889634f, 1.4426950408889634f)), a, b);
+            asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(ea) : "f"(a));
+            asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(eb) : "f"(b));
+            const uint64_t e = pair_of(ea, eb);
+            s = pair_add(s, e);
+            // an exponential of 0 times -infinity would be NaN; NaN is in e already
+            asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(d) : "l"(e), "l"(pair_of(fmaxf(a, -200.0f), fmaxf(b, -200.0f))));
+        }
     }
-}
-template <int N>
-__device__ __forceinline__ void add_terms(const double (&v)[N], double off, double& s, double& d) {
+    __device__ __forceinline__ void to(float& sum, float& moved) const {
+        float a, b;
+        pair_to(s, a, b);
+        sum += a + b;
+        pair_to(d, a, b);
+        moved += (a + b) * 0.6931471805599453f;
+    }
+};
+template <>
+struct Terms<double> {
+    double s = 0.0, d = 0.0, off;
+    __device__ __forceinline__ explicit Terms(double o) : off(o) {}
+    template <int N>
+    __device__ __forceinline__ void add(const double (&v)[N]) {
 #pragma unroll
-    for (int q = 0; q < N; ++q) {
-        const double z = v[q] - off, e = exp_of(z);
-        s += e;
-        d += e * floor_of(z);
+        for (int q = 0; q < N; ++q) {
+            const double z = v[q] - off, e = exp_of(z);
+            s += e;
+            d += e * floor_of(z);
+        }
     }
-}
+    __device__ __forceinline__ void to(double& sum, double& moved) const {
+        sum += s;
+        moved += d;
+    }
+};
+
+// How many of a row's values come before its label's: those above it, and of the ones
+// equal to it those before its index, which are above the next lower value of the type. The
+// vector that the label is in counts as one behind it; `fix` adds what that leaves out.
+template <class T>
+struct Before {
+    T own, lower;  // lower: NaN below -infinity, where everything counts
+    int y;         // may lie outside the values that are looked at
+    __device__ __forceinline__ Before(T xy, int label) : own(xy), lower(below(xy)), y(label) {}
+    static __device__ __forceinline__ float below(float v) {
+        const int b = __float_as_int(v);
+        return v == 0.0f ? __int_as_float((int)0x80000001) : v == minus_inf<float>() ? NAN : __int_as_float(v > 0.0f ? b - 1 : b + 1);
+    }
+    static __device__ __forceinline__ double below(double v) {
+        const long long b = __double_as_longlong(v);
+        return v == 0.0 ? __longlong_as_double((long long)0x8000000000000001ull)
+                        : v == minus_inf<double>() ? (double)NAN : __longlong_as_double(v > 0.0 ? b - 1 : b + 1);
+    }
+    static __device__ __forceinline__ __nv_bfloat16 below(__nv_bfloat16 v) {
+        const unsigned short b = __bfloat16_as_ushort(v);
+        return __ushort_as_bfloat16((b & 0x7fff) == 0 ? 0x8001 : b == 0xff80 ? 0x7fff : b & 0x8000 ? b + 1 : b - 1);
+    }
+    static __device__ __forceinline__ __half below(__half v) {
+        const unsigned short b = __half_as_ushort(v);
+        return __ushort_as_half((b & 0x7fff) == 0 ? 0x8001 : b == 0xfc00 ? 0x7fff : b & 0x8000 ? b + 1 : b - 1);
+    }
+    template <class A>
+    static __device__ __forceinline__ bool above(A v, A bound) { return !(v <= bound); }  // NaN: everything
+    __device__ __forceinline__ int one(T v, int i) const {
+        using A = typename Arith<T>::type;
+        return above<A>(widen<A>(v), widen<A>(i < y ? lower : own)) ? 1 : 0;
+    }
+    // of the vector's values before the label that are equal to it
+    __device__ __forceinline__ int fix(const T* row, int first) const {
+        using A = typename Arith<T>::type;
+        int n = 0;
+        for (int i = first; i < y; ++i) n += widen<A>(row[i]) == widen<A>(own) ? 1 : 0;
+        return n;
+    }
+};
+// Counts over a few vectors; total() at most once each 64 of them (16-bit counters hold 256).
+template <class T>
+struct Count {
+    int n = 0;
+    template <class A, int N>
+    __device__ __forceinline__ void add(const uint4&, const A (&v)[N], T bound) {
+        const A b = widen<A>(bound);
+#pragma unroll
+        for (int q = 0; q < N; ++q)
+            if (!(v[q] <= b)) ++n;
+    }
+    __device__ __forceinline__ int total() const { return n; }
+};
+template <class P, class T>
+struct PairCount {
+    P n;
+    __device__ __forceinline__ void four(const uint4& r, P bound) {
+        n = __hadd2(n, __hgtu2(as_pair<P>(r.x), bound));
+        n = __hadd2(n, __hgtu2(as_pair<P>(r.y), bound));
+        n = __hadd2(n, __hgtu2(as_pair<P>(r.z), bound));
+        n = __hadd2(n, __hgtu2(as_pair<P>(r.w), bound));
+    }
+    __device__ __forceinline__ int total() const { return (int)(__low2float(n) + __high2float(n)); }
+};
+template <>
+struct Count<__nv_bfloat16> : PairCount<__nv_bfloat162, __nv_bfloat16> {
+    __device__ __forceinline__ Count() { n = __float2bfloat162_rn(0.0f); }
+    template <int N>
+    __device__ __forceinline__ void add(const uint4& r, const float (&)[N], __nv_bfloat16 bound) { four(r, __bfloat162bfloat162(bound)); }
+};
+template <>
+struct Count<__half> : PairCount<__half2, __half> {
+    __device__ __forceinline__ Count() { n = __float2half2_rn(0.0f); }
+    template <int N>
+    __device__ __forceinline__ void add(const uint4& r, const float (&)[N], __half bound) { four(r, __half2half2(bound)); }
+};
 
 template <class A>
 struct Candidate {
@@ -207,15 +312,16 @@ struct Candidate {
 
 constexpr int kSegments = 16;  // of a thread's vectors, each with its largest value
 
-// What a group shares.
-template <class A, int L>
+// What a group shares: MOST of each of a scanning thread's segments.
+template <class A, int L, bool SCAN>
 struct Shared {
     A m[L / 32], s[L / 32], d[L / 32];
+    A one[L / 32], every[L / 32];
     int rank[L / 32];
-    A sorted[L / 32][32];  // each warp's threads' largest values in falling order
-    A most[kSegments][L];
+    int count, listed;
+    Candidate<A> best[kTop];  // the answer
     Candidate<A> cand[kCand];
-    int count;
+    A most[SCAN ? kSegments : 1][SCAN ? L : 1];
 };
 
 // The 32 lanes' values in falling order.
@@ -233,27 +339,30 @@ __device__ __forceinline__ A sorted_lanes(A v) {
     return v;
 }
 
-// Walks the values of a row that thread `lane` of L has, by segments whose largest is at
-// least `bound`: f(value, index).
-template <class T, class A, int L, class F>
-__device__ __forceinline__ void walk(const T* row, const RowShape<T>& sh, int lane, const Shared<A, L>& g, A mine,
-                                     A bound, A edge, F&& f) {
-    constexpr int V = 16 / sizeof(T), U = 8;
-    if (!(mine >= bound)) return;
-    if (lane < sh.edges && edge >= bound) f(edge, sh.edge(lane));
-    const int batches = (sh.nv + L * U - 1) / (L * U), per = (batches + kSegments - 1) / kSegments;
-    for (int b = 0; b < batches; ++b) {
-        if (!(g.most[b / per][lane] >= bound)) continue;
-        for (int u = 0; u < U; ++u) {
-            const int j = (b * U + u) * L + lane;
-            if (j >= sh.nv) break;
-            A p[V];
-            Pack<T>::unpack(load16(row + sh.head + (int64_t)j * V), p);
-#pragma unroll
-            for (int q = 0; q < V; ++q)
-                if (p[q] >= bound) f(p[q], sh.head + j * V + q);
+// Values that at least a and b of the 32 lanes' values reach (b <= a): the a-th and b-th
+// largest, or below. Few of them by so many maxima of the warp (of distinct values: what is
+// found may be lower), more by sorting.
+__device__ __forceinline__ void reached(float v, int a, int b, float& at_a, float& at_b) {
+    if (a <= 8) {
+        const int bits = __float_as_int(v);
+        unsigned u = (unsigned)(bits ^ (bits >> 31 | (int)0x80000000));
+        for (int i = 1;; ++i) {
+            const unsigned top = __reduce_max_sync(0xffffffffu, u);
+            const int back = (int)top < 0 ? (int)(top & 0x7fffffffu) : (int)~top;
+            at_a = top ? __int_as_float(back) : minus_inf<float>();  // 0: every lane has been passed
+            if (i == b) at_b = at_a;
+            if (i == a) return;
+            if (u == top) u = 0;
         }
     }
+    v = sorted_lanes(v);
+    at_a = __shfl_sync(0xffffffffu, v, a - 1);
+    at_b = __shfl_sync(0xffffffffu, v, b - 1);
+}
+__device__ __forceinline__ void reached(double v, int a, int b, double& at_a, double& at_b) {
+    v = sorted_lanes(v);
+    at_a = __shfl_sync(0xffffffffu, v, a - 1);
+    at_b = __shfl_sync(0xffffffffu, v, b - 1);
 }
 
 // The first `want` values of the row that equal v, in index order, by one warp:
@@ -287,16 +396,104 @@ __device__ __noinline__ void first_equal(const T* row, int c, A v, int want, F&&
     }
 }
 
-template <class T, class A, int L>
-__global__ void __launch_bounds__(kNT)
-    rows_kernel(const T* __restrict__ x, int64_t ld, Args<A> a) {
-    constexpr int V = 16 / sizeof(T), U = 8, W = L / 32;
-    extern __shared__ uint4 rows_smem[];
-    Shared<A, L>& g = reinterpret_cast<Shared<A, L>*>(rows_smem)[threadIdx.x / L];
-    const int lane = threadIdx.x % L, warp = lane / 32;
-    const int64_t t = (int64_t)blockIdx.x * (kNT / L) + threadIdx.x / L;
-    if (t >= a.n) return;  // the whole group
-    const int y = a.label(t), top = a.top;
+// The first `top` of a row's c values (fewer, if it has fewer) in their order to g.best, by the
+// group. `bound`: what at least `top` of them reach. `walk(f)` calls f(value, index) for
+// every value that reaches it.
+template <class T, class A, int L, bool SCAN, class W>
+__device__ __forceinline__ void choose(Shared<A, L, SCAN>& g, const T* row, int c, int top, A bound, W&& walk) {
+    const int lane = threadIdx.x % L;
+    auto take = [&](A v, int i) {
+        const int at = atomicAdd(&g.count, 1);
+        if (at < kCand) g.cand[at] = Candidate<A>{v, i};
+    };
+    // the places of the candidates among each other
+    auto places = [&](int count) {
+        for (int q = lane; q < count; q += L) {
+            const Candidate<A> me = g.cand[q];
+            int place = 0;
+            for (int o = 0; o < count; ++o) place += g.cand[o].before(me) ? 1 : 0;
+            if (place < top) g.best[place] = me;
+        }
+    };
+    walk(take);
+    group_sync<L>();
+    int count = g.count;
+    if (count <= kCand) {
+        places(count);
+        return;
+    }
+    // Too many reach it: mostly ties, as of masked classes. Those above it, and the first
+    // of those that are equal.
+    group_sync<L>();
+    if (lane == 0) g.count = 0;
+    group_sync<L>();
+    walk([&](A v, int i) {
+        if (v > bound) take(v, i);
+    });
+    group_sync<L>();
+    count = g.count;
+    if (count <= kCand) {
+        places(count);
+        if (count < top && lane < 32)
+            first_equal<T, A>(row, c, bound, top - count, [&](int place, int i) { g.best[count + place] = Candidate<A>{bound, i}; });
+        return;
+    }
+    // Too many above it (a few threads hold most of the large values): one at a time, each
+    // the first behind the one before.
+    Candidate<A> last{(A)INFINITY, -1};
+    for (int place = 0; place < top; ++place) {
+        Candidate<A> best{minus_inf<A>(), INT32_MAX};
+        for (int64_t j = lane; j < c; j += L) {
+            const Candidate<A> o{widen<A>(row[j]), (int)j};
+            if (last.before(o) && o.before(best)) best = o;
+        }
+#pragma unroll
+        for (int s = 16; s > 0; s >>= 1) {
+            const Candidate<A> o{__shfl_xor_sync(0xffffffffu, best.v, s), __shfl_xor_sync(0xffffffffu, best.i, s)};
+            if (o.before(best)) best = o;
+        }
+        if (L > 32) {
+            group_sync<L>();
+            if ((lane & 31) == 0) g.cand[lane / 32] = best;
+            group_sync<L>();
+            for (int w = 0; w < L / 32; ++w)
+                if (g.cand[w].before(best)) best = g.cand[w];
+        }
+        last = best;
+        if (lane == 0) g.best[place] = best;
+    }
+}
+
+// What a row's finished statistics say, by one thread; false where there is no more to say.
+template <class A>
+__device__ __forceinline__ bool finish(const Args<A>& a, int64_t t, A xy, const Stats<A>& r, int rank, A& off, A& ls, bool write) {
+    off = offset_of(r.m);
+    ls = log_of(r.s);
+    const bool empty = r.m == minus_inf<A>() && r.s == A(0);
+    if (empty || r.s != r.s) {
+        if (write) a.nothing(t, empty ? minus_inf<A>() : r.s, empty ? A(0) : r.s);
+        return false;
+    }
+    if (write) {
+        if (a.lp) a.lp[t] = (xy - off) - ls;
+        a.lse[t] = off + ls;
+        a.entropy[t] = entropy_of(ls, r.s, r.d);
+        if (a.ranks) a.id(a.ranks, t, rank);
+    }
+    return true;
+}
+
+// Rows of up to 32 K vectors: a warp each, the row in its registers.
+template <class T, class A, int K>
+__global__ void __launch_bounds__(kNT, IsF64<A>::value || K > 4 ? 2 : 4)
+    held_kernel(const T* __restrict__ x, int64_t ld, Args<A> a) {
+    constexpr int V = 16 / sizeof(T);
+    __shared__ Shared<A, 32, false> shared[kNT / 32];
+    Shared<A, 32, false>& g = shared[threadIdx.x / 32];
+    const int lane = threadIdx.x & 31, top = a.top;
+    const int64_t t = (int64_t)blockIdx.x * (kNT / 32) + threadIdx.x / 32;
+    if (t >= a.n) return;
+    const int y = a.label(t);
     if (y < 0) {
         if (lane == 0) a.nothing(t, A(0), A(0));
         if (lane < top) a.no_class(t, lane, A(0));
@@ -304,53 +501,155 @@ __global__ void __launch_bounds__(kNT)
     }
     const T* row = x + t * ld;
     const RowShape<T> sh(row, (int)a.c);
-    const A xy = widen<A>(row[y]);
-    const A edge = lane < sh.edges ? widen<A>(row[sh.edge(lane)]) : minus_inf<A>();
-    const int batches = (sh.nv + L * U - 1) / (L * U), per = (batches + kSegments - 1) / kSegments;
-    int rank = lane < sh.edges && (edge > xy || (edge == xy && sh.edge(lane) < y)) ? 1 : 0;
+    uint4 v[K];
+#pragma unroll
+    for (int i = 0; i < K; ++i) v[i] = lane + i * 32 < sh.nv ? load16(row + sh.head + (lane + i * 32) * V) : Pack<T>::minus_inf();
+    const T low = narrow<T>(minus_inf<A>()), last = lane < sh.edges ? row[sh.edge(lane)] : low;
+    const A edge = widen<A>(last);
+    const Before<T> before(row[y], y);
+    A mine = edge;
+#pragma unroll
+    for (int i = 0; i < K; ++i) mine = fmax(mine, Pack<T>::top(v[i]));
+    Stats<A> r{mine, A(0), A(0)};
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) r.m = fmax(r.m, __shfl_xor_sync(0xffffffffu, r.m, o));
+    A off = offset_of(r.m), ls;
+    Terms<A> terms(off);
+    Count<T> counted;
+    int rank = lane < sh.edges ? before.one(last, sh.edge(lane)) : 0;
+#pragma unroll
+    for (int i = 0; i < K; ++i) {
+        A p[V];
+        Pack<T>::unpack(v[i], p);
+        terms.add(p);
+        const int i0 = sh.head + (lane + i * 32) * V;
+        if (lane + i * 32 < sh.nv) {
+            counted.add(v[i], p, i0 + V <= y ? before.lower : before.own);
+            if (i0 < y && y < i0 + V) rank += before.fix(row, i0);
+        }
+    }
+    terms.to(r.s, r.d);
+    const A e = exp_of(edge - off);
+    r.s += e;
+    r.d += e * floor_of(edge - off);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        r.s += __shfl_xor_sync(0xffffffffu, r.s, o);
+        r.d += __shfl_xor_sync(0xffffffffu, r.d, o);
+    }
+    rank = __reduce_add_sync(0xffffffffu, rank + counted.total());
+    if (!finish(a, t, widen<A>(before.own), r, rank, off, ls, lane == 0)) {
+        if (lane < top) a.no_class(t, lane, r.s != r.s ? r.s : A(0));
+        return;
+    }
+    if (top == 0) return;
+    if (lane == 0) g.count = 0;
+    A bound, same;
+    reached(mine, top, top, bound, same);
+    __syncwarp();
+    choose<T, A, 32, false>(g, row, (int)a.c, top, bound, [&](auto&& f) {
+        if (lane < sh.edges && edge >= bound) f(edge, sh.edge(lane));
+#pragma unroll
+        for (int i = 0; i < K; ++i)
+            if (lane + i * 32 < sh.nv && Pack<T>::top(v[i]) >= bound) {
+                A p[V];
+                Pack<T>::unpack(v[i], p);
+#pragma unroll
+                for (int q = 0; q < V; ++q)
+                    if (p[q] >= bound) f(p[q], sh.head + (lane + i * 32) * V + q);
+            }
+    });
+    __syncwarp();
+    if (lane < top) {
+        a.id(a.top_ids, t * top + lane, g.best[lane].i);
+        a.top_lp[t * top + lane] = (g.best[lane].v - off) - ls;
+    }
+}
+
+// Longer rows, read once with a running maximum: L threads a row, or a cluster of CL blocks
+// of L threads where rows are few, each block on a part of the row and the first one on
+// what the others found, in distributed shared memory.
+template <class T, class A, int L, int CL>
+__global__ void __launch_bounds__(kNT, IsF64<A>::value ? 2 : 4)
+    scan_kernel(const T* __restrict__ x, int64_t ld, Args<A> a) {
+    constexpr int V = 16 / sizeof(T), U = 8, W = L / 32;
+    using G = Shared<A, L, true>;
+    extern __shared__ uint4 rows_smem[];
+    G& g = reinterpret_cast<G*>(rows_smem)[threadIdx.x / L];
+    const int lane = threadIdx.x % L, warp = lane / 32, top = a.top;
+    const int64_t t = CL > 1 ? blockIdx.x / CL : (int64_t)blockIdx.x * (kNT / L) + threadIdx.x / L;
+    if (t >= a.n) return;  // the whole group, the whole cluster
+    const int y_row = a.label(t);
+    if (y_row < 0) {
+        const bool first = CL == 1 || blockIdx.x % CL == 0;
+        if (first && lane == 0) a.nothing(t, A(0), A(0));
+        if (first && lane < top) a.no_class(t, lane, A(0));
+        return;
+    }
+    // this block's part of the row: columns [begin, begin + c)
+    int begin = 0, c = (int)a.c;
+    if (CL > 1) {
+        const int64_t share = ceil_div(a.c, (int64_t)CL * 64) * 64, part = blockIdx.x % CL;
+        begin = (int)min(part * share, a.c);
+        c = (int)(min((part + 1) * share, a.c) - begin);
+    }
+    const T* row = x + t * ld + begin;
+    const RowShape<T> sh(row, c);
+    const T xy = x[t * ld + y_row];
+    const Before<T> before(xy, y_row - begin);
+    const T last = lane < sh.edges ? row[sh.edge(lane)] : narrow<T>(minus_inf<A>());
+    const A edge = widen<A>(last);
+    const int per = (sh.nv + L * U * kSegments - 1) / (L * U * kSegments);  // batches a segment
+    int rank = lane < sh.edges ? before.one(last, sh.edge(lane)) : 0;
     Stats<A> r{edge, A(0), A(0)};
     r.s = exp_of(edge - offset_of(edge));  // 1, 0 for -infinity, NaN
-    A part = minus_inf<A>();
-    for (int b = 0; b < batches; ++b) {
+    A part_most = minus_inf<A>();
+    int in_part = 0, segment = 0;
+    for (int j0 = lane; j0 - lane < sh.nv; j0 += L * U) {
         uint4 v[U];
         A best = minus_inf<A>();
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int j = (b * U + u) * L + lane;
-            v[u] = j < sh.nv ? load16(row + sh.head + (int64_t)j * V) : Pack<T>::minus_inf();
-        }
+        for (int u = 0; u < U; ++u) v[u] = j0 + u * L < sh.nv ? load16(row + sh.head + (int64_t)(j0 + u * L) * V) : Pack<T>::minus_inf();
 #pragma unroll
         for (int u = 0; u < U; ++u) best = fmax(best, Pack<T>::top(v[u]));
-        part = b % per == 0 ? best : fmax(part, best);
-        g.most[b / per][lane] = part;
+        if (top) {
+            part_most = fmax(part_most, best);
+            if (++in_part == per || j0 - lane + L * U >= sh.nv) {
+                g.most[segment++][lane] = part_most;
+                part_most = minus_inf<A>();
+                in_part = 0;
+            }
+        }
         if (best > r.m) r.raise(best);
-        const A off = offset_of(r.m);
+        Terms<A> terms(offset_of(r.m));
+        Count<T> counted;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             A p[V];
             Pack<T>::unpack(v[u], p);
-            add_terms(p, off, r.s, r.d);
-            const int i0 = sh.head + ((b * U + u) * L + lane) * V;
-#pragma unroll
-            for (int q = 0; q < V; ++q) rank += p[q] > xy || (p[q] == xy && i0 + q < y) ? 1 : 0;
+            terms.add(p);
+            const int j = j0 + u * L;
+            if (j < sh.nv) {
+                const int behind = before.y - sh.head - j * V;  // of the label behind the vector's first value
+                counted.add(v[u], p, behind >= V ? before.lower : before.own);
+                if (behind > 0 && behind < V) rank += before.fix(row, sh.head + j * V);
+            }
         }
-    }
-    // -infinity behind the row's end counts as a tie of a label of -infinity
-    if (xy == minus_inf<A>()) {
-        rank = lane < sh.edges && (edge > xy || sh.edge(lane) < y) ? 1 : 0;
-        for (int j = lane; j < sh.nv; j += L) {
-            A p[V];
-            Pack<T>::unpack(load16(row + sh.head + (int64_t)j * V), p);
-#pragma unroll
-            for (int q = 0; q < V; ++q) rank += p[q] > xy || sh.head + j * V + q < y ? 1 : 0;
-        }
+        terms.to(r.s, r.d);
+        rank += counted.total();
     }
     const A mine = r.m;
     join(r, 32);
     rank = __reduce_add_sync(0xffffffffu, rank);
     if (top) {
-        const A in_order = sorted_lanes(mine);
-        g.sorted[warp][lane & 31] = in_order;
+        // what ceil(top / W) threads of every warp reach, top values of the row do; and what
+        // top threads of one warp do
+        A one, every;
+        reached(mine, top, (top + W - 1) / W, one, every);
+        if ((lane & 31) == 0) {
+            g.one[warp] = one;
+            g.every[warp] = every;
+        }
     }
     if ((lane & 31) == 0) {
         g.m[warp] = r.m;
@@ -359,6 +658,7 @@ __global__ void __launch_bounds__(kNT)
         g.rank[warp] = rank;
     }
     if (lane == 0) g.count = 0;
+    if (CL > 1 && lane < kTop) g.best[lane] = Candidate<A>{minus_inf<A>(), INT32_MAX};
     group_sync<L>();
     if (W > 1) {
         const int w = lane & 31;
@@ -369,93 +669,83 @@ __global__ void __launch_bounds__(kNT)
         join(r, 32);
         rank = __reduce_add_sync(0xffffffffu, rank);
     }
-    const A off = offset_of(r.m), ls = log_of(r.s);
-    const bool empty = r.m == minus_inf<A>() && r.s == A(0);
-    if (empty || r.s != r.s) {
-        const A v0 = empty ? A(0) : r.s;
-        if (lane == 0) a.nothing(t, empty ? minus_inf<A>() : r.s, v0);
-        if (lane < top) a.no_class(t, lane, v0);
+    A off, ls;
+    if (CL == 1 && !finish(a, t, widen<A>(xy), r, rank, off, ls, lane == 0)) {
+        if (lane < top) a.no_class(t, lane, r.s != r.s ? r.s : A(0));
         return;
     }
-    if (lane == 0) {
-        if (a.lp) a.lp[t] = (xy - off) - ls;
-        a.lse[t] = off + ls;
-        a.entropy[t] = entropy_of(ls, r.s, r.d);
-        if (a.ranks) a.id(a.ranks, t, rank);
-    }
-    if (top == 0) return;
-    // A value that at least `top` values of the row reach: the top-th of one warp's threads'
-    // largest, or what ceil(top / W) threads of every warp reach.
-    A one = minus_inf<A>(), every = (A)INFINITY;
+    // a part with a NaN or without a value has no order, and none is asked for
+    if (top && r.s == r.s && c > 0) {
+        A one = g.one[0], every = g.every[0];
 #pragma unroll
-    for (int w = 0; w < W; ++w) {
-        one = fmax(one, g.sorted[w][top - 1]);
-        every = fmin(every, g.sorted[w][(top + W - 1) / W - 1]);
-    }
-    const A bound = fmax(one, every);
-    auto take = [&](A v, int i) {
-        const int at = atomicAdd(&g.count, 1);
-        if (at < kCand) g.cand[at] = Candidate<A>{v, i};
-    };
-    auto put = [&](int place, A v, int i) {
-        a.id(a.top_ids, t * top + place, i);
-        a.top_lp[t * top + place] = (v - off) - ls;
-    };
-    // the places of the candidates among each other: those below `top` are the answer
-    auto choose = [&](int count) {
-        for (int q = lane; q < count; q += L) {
-            const Candidate<A> me = g.cand[q];
-            int place = 0;
-            for (int o = 0; o < count; ++o) place += g.cand[o].before(me) ? 1 : 0;
-            if (place < top) put(place, me.v, me.i);
+        for (int w = 1; w < W; ++w) {
+            one = fmax(one, g.one[w]);
+            every = fmin(every, g.every[w]);
         }
-    };
-    walk<T, A, L>(row, sh, lane, g, mine, bound, edge, take);
-    group_sync<L>();
-    int count = g.count;
-    if (count <= kCand) {
-        choose(count);
-        return;
-    }
-    // Too many reach it: mostly ties, as of masked classes. Those above it, and the first
-    // of those that are equal.
-    group_sync<L>();
-    if (lane == 0) g.count = 0;
-    group_sync<L>();
-    walk<T, A, L>(row, sh, lane, g, mine, bound, edge, [&](A v, int i) {
-        if (v > bound) take(v, i);
-    });
-    group_sync<L>();
-    count = g.count;
-    if (count <= kCand) {
-        choose(count);
-        if (count < top && warp == 0)
-            first_equal<T, A>(row, (int)a.c, bound, top - count, [&](int place, int i) { put(count + place, bound, i); });
-        return;
-    }
-    // Too many above it (a few threads hold most of the large values): one at a time, each
-    // the first behind the one before.
-    Candidate<A> last{(A)INFINITY, -1};
-    for (int place = 0; place < top; ++place) {
-        Candidate<A> best{minus_inf<A>(), INT32_MAX};
-        for (int64_t j = lane; j < a.c; j += L) {
-            const Candidate<A> o{widen<A>(row[j]), (int)j};
-            if (last.before(o) && o.before(best)) best = o;
-        }
+        const A bound = fmax(one, every);
+        const int wanted = CL > 1 && c < top ? c : top;
+        choose<T, A, L, true>(g, row, c, wanted, bound, [&](auto&& f) {
+            if (!(mine >= bound)) return;
+            if (lane < sh.edges && edge >= bound) f(edge, sh.edge(lane));
+            for (int s = 0; s * per * L * U < sh.nv; ++s) {
+                if (!(g.most[s][lane] >= bound)) continue;
+                for (int j = s * per * L * U + lane; j < sh.nv && j < (s + 1) * per * L * U; j += L) {
+                    A p[V];
+                    Pack<T>::unpack(load16(row + sh.head + (int64_t)j * V), p);
 #pragma unroll
-        for (int s = 16; s > 0; s >>= 1) {
-            const Candidate<A> o{__shfl_xor_sync(0xffffffffu, best.v, s), __shfl_xor_sync(0xffffffffu, best.i, s)};
-            if (o.before(best)) best = o;
+                    for (int q = 0; q < V; ++q)
+                        if (p[q] >= bound) f(p[q], sh.head + j * V + q);
+                }
+            }
+        });
+        group_sync<L>();
+    }
+    if constexpr (CL > 1) {
+        namespace cg = cooperative_groups;
+        auto cluster = cg::this_cluster();
+        if (lane == 0) {
+            g.m[0] = r.m;
+            g.s[0] = r.s;
+            g.d[0] = r.d;
+            g.rank[0] = rank;
+            g.listed = begin;
         }
-        if (W > 1) {
-            group_sync<L>();
-            if ((lane & 31) == 0) g.cand[warp] = best;
-            group_sync<L>();
-            for (int w = 0; w < W; ++w)
-                if (g.cand[w].before(best)) best = g.cand[w];
+        cluster.sync();
+        if (cluster.block_rank() == 0) {
+            // the parts' statistics, one a lane of each warp, and their candidates
+            G* other = cluster.map_shared_rank(&g, (lane & 31) % CL);
+            const bool in = (lane & 31) < CL;
+            r.m = in ? other->m[0] : minus_inf<A>();
+            r.s = in ? other->s[0] : A(0);
+            r.d = in ? other->d[0] : A(0);
+            rank = __reduce_add_sync(0xffffffffu, in ? other->rank[0] : 0);
+            join(r, 32);
+            const bool go = finish(a, t, widen<A>(xy), r, rank, off, ls, lane == 0);
+            if (!go && lane < top) a.no_class(t, lane, r.s != r.s ? r.s : A(0));
+            if (go && top) {
+                const int count = top * CL;
+                for (int q = lane; q < count; q += L) {
+                    const G* o = cluster.map_shared_rank(&g, q / top);
+                    Candidate<A> k = o->best[q % top];
+                    if (k.i != INT32_MAX) k.i += o->listed;
+                    g.cand[q] = k;
+                }
+                group_sync<L>();
+                for (int q = lane; q < count; q += L) {
+                    const Candidate<A> me = g.cand[q];
+                    int place = 0;
+                    for (int o = 0; o < count; ++o) place += g.cand[o].before(me) ? 1 : 0;
+                    if (place < top && me.i != INT32_MAX) {
+                        a.id(a.top_ids, t * top + place, me.i);
+                        a.top_lp[t * top + place] = (me.v - off) - ls;
+                    }
+                }
+            }
         }
-        last = best;
-        if (lane == 0) put(place, best.v, best.i);
+        cluster.sync();  // the others' shared memory is read until here
+    } else if (lane < top) {
+        a.id(a.top_ids, t * top + lane, g.best[lane].i);
+        a.top_lp[t * top + lane] = (g.best[lane].v - off) - ls;
     }
 }
 
@@ -565,20 +855,50 @@ void rows_launch(int device, const T* x, int64_t ld, const Args<A>& a, cudaStrea
             go(std::integral_constant<int, 32>{});
         return;
     }
-    auto go = [&](auto l) {
-        constexpr int L = decltype(l)::value, bytes = (int)sizeof(Shared<A, L>) * (kNT / L);
-        auto k = rows_kernel<T, A, L>;
+    const int64_t nv = a.c / Pack<T>::N, sms = sm_count(device);
+    using std::integral_constant;
+    auto held = [&](auto k) {
+        held_kernel<T, A, decltype(k)::value><<<(unsigned)ceil_div(a.n, kNT / 32), kNT, 0, s>>>(x, ld, a);
+    };
+    auto scan = [&](auto l) {
+        constexpr int L = decltype(l)::value, bytes = (int)sizeof(Shared<A, L, true>) * (kNT / L);
+        auto k = scan_kernel<T, A, L, 1>;
         static bool asked[64];
         allow_smem(k, device, bytes, asked, "row shared memory");
         k<<<(unsigned)ceil_div(a.n, kNT / L), kNT, bytes, s>>>(x, ld, a);
     };
-    const int64_t nv = a.c / Pack<T>::N, warps = (int64_t)sm_count(device) * 32;
-    if (nv >= 1024 && a.n * 4 < warps)
-        go(std::integral_constant<int, kNT>{});
+    if (nv <= 32)
+        held(integral_constant<int, 1>{});
+    else if (nv <= 64)
+        held(integral_constant<int, 2>{});
+    else if (nv <= 128)
+        held(integral_constant<int, 4>{});
+    else if (nv <= 256)
+        held(integral_constant<int, 8>{});
+    else if (nv >= 1024 && a.n <= sms / 2) {
+        // so few rows that a cluster of eight blocks each fits at once
+        constexpr int bytes = (int)sizeof(Shared<A, kNT, true>);
+        auto k = scan_kernel<T, A, kNT, 8>;
+        static bool asked[64];
+        allow_smem(k, device, bytes, asked, "row shared memory");
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3((unsigned)a.n * 8);
+        cfg.blockDim = dim3(kNT);
+        cfg.dynamicSmemBytes = bytes;
+        cfg.stream = s;
+        cudaLaunchAttribute at[1];
+        at[0].id = cudaLaunchAttributeClusterDimension;
+        at[0].val.clusterDim.x = 8;
+        at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+        cfg.attrs = at;
+        cfg.numAttrs = 1;
+        MFM_CUDA(cudaLaunchKernelEx(&cfg, k, x, ld, a), "kernel launch");
+    } else if (nv >= 1024 && a.n * 4 < sms * 32)
+        scan(integral_constant<int, kNT>{});
     else if (nv >= 512)
-        go(std::integral_constant<int, 128>{});
+        scan(integral_constant<int, 128>{});
     else
-        go(std::integral_constant<int, 32>{});
+        scan(integral_constant<int, 32>{});
 }
 
 template <class T, class A>
