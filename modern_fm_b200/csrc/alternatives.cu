@@ -96,24 +96,51 @@ __device__ __forceinline__ A entropy_of(A ls, A s, A d) {
 
 // ------------------------------------------------------------ few classes --
 
-// A thread per row over tiles of 32 rows copied through shared memory. Every class's
-// place is counted against every other: c (c - 1) / 2 comparisons.
+// A thread per row over tiles of 32 rows, of which the next is copied through shared memory
+// while one is worked on. Every class's place is counted against every other, c (c - 1) / 2
+// comparisons; the places name the classes in shared memory, from where the warp
+// writes the tile's lists as they lie.
 template <class T, class A, int CW>
-__global__ void __launch_bounds__(kSmallNT)
-    small_kernel(const T* __restrict__ x, int64_t ld, Args<A> a, bool whole) {
+struct SmallWarp {  // behind it: the warp's two tiles
+    A off[kTileRows], ls[kTileRows];
+    uint8_t order[kTileRows][CW];  // the classes in their order, kNone in a row without
+};
+constexpr unsigned kNone = 255;
+
+template <class T, class A, int CW>
+__host__ __device__ constexpr size_t small_bytes(int c) {
+    return (sizeof(SmallWarp<T, A, CW>) + 15) / 16 * 16 + 2 * kTileRows * c * sizeof(T);
+}
+
+template <class T, class A, int CW>
+__global__ void __launch_bounds__(kSmallNT, IsF64<A>::value || CW > 16 ? 4 : 8)
+    small_kernel(const T* __restrict__ x, int64_t ld, Args<A> a, bool whole, unsigned by_top) {
     extern __shared__ uint4 small_smem[];
-    const int c = (int)a.c, lane = threadIdx.x & 31;
-    T* const tile = reinterpret_cast<T*>(small_smem) + (threadIdx.x / 32) * (kTileRows * c);
-    const int64_t tiles = ceil_div(a.n, (int64_t)kTileRows);
-    for (int64_t i = (int64_t)blockIdx.x * (kSmallNT / 32) + threadIdx.x / 32; i < tiles; i += (int64_t)gridDim.x * (kSmallNT / 32)) {
-        const int64_t t0 = i * kTileRows, t = t0 + lane;
-        const int rows = (int)(a.n - t0 < kTileRows ? a.n - t0 : kTileRows);
-        tile_fetch(x, ld, t0, rows, c, whole, tile);
-        asm volatile("cp.async.commit_group;\ncp.async.wait_group 0;" ::: "memory");
+    const int c = (int)a.c, lane = threadIdx.x & 31, top = a.top;
+    char* const mine = reinterpret_cast<char*>(small_smem) + (threadIdx.x / 32) * small_bytes<T, A, CW>(c);
+    SmallWarp<T, A, CW>& w = *reinterpret_cast<SmallWarp<T, A, CW>*>(mine);
+    T* const tiles = reinterpret_cast<T*>(mine + (sizeof(SmallWarp<T, A, CW>) + 15) / 16 * 16);
+    const int64_t n_tiles = ceil_div(a.n, (int64_t)kTileRows), step = (int64_t)gridDim.x * (kSmallNT / 32);
+    auto rows_of = [&](int64_t t0) { return (int)(a.n - t0 < kTileRows ? a.n - t0 : kTileRows); };
+    int64_t i = (int64_t)blockIdx.x * (kSmallNT / 32) + threadIdx.x / 32;
+    int y = -1;
+    if (i < n_tiles) {
+        tile_fetch(x, ld, i * kTileRows, rows_of(i * kTileRows), c, whole, tiles);
+        if (lane < rows_of(i * kTileRows)) y = a.label(i * kTileRows + lane);
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    for (int buf = 0; i < n_tiles; i += step, buf ^= 1) {
+        const int64_t t0 = i * kTileRows, t = t0 + lane, next = (i + step) * kTileRows;
+        const int rows = rows_of(t0), y_now = y;
+        const T* const tile = tiles + buf * (kTileRows * c);
+        if (i + step < n_tiles) {
+            tile_fetch(x, ld, next, rows_of(next), c, whole, tiles + (buf ^ 1) * (kTileRows * c));
+            if (lane < rows_of(next)) y = a.label(next + lane);
+        }
+        asm volatile("cp.async.commit_group;\ncp.async.wait_group 1;" ::: "memory");
         __syncwarp();
         if (lane < rows) {
             const T* row = tile + lane * c;
-            const int y = a.label(t);
             A v[CW], m = minus_inf<A>();
 #pragma unroll
             for (int j = 0; j < CW; ++j) {
@@ -124,47 +151,58 @@ __global__ void __launch_bounds__(kSmallNT)
             A s = A(0), d = A(0);
 #pragma unroll
             for (int j = 0; j < CW; ++j) {
-                const A e = exp_of(v[j] - off);
+                const A z = v[j] - off, e = exp_of(z);
                 s += e;
-                d += e * floor_of(v[j] - off);
+                d += e * floor_of(z);
             }
+            const A xy = widen<A>(row[y_now < 0 ? 0 : y_now]);
+            int rank = 0;
+#pragma unroll
+            for (int j = 0; j < CW; ++j) rank += j < c && (j < y_now ? v[j] >= xy : v[j] > xy) ? 1 : 0;
             const bool empty = m == minus_inf<A>() && s == A(0);
-            if (y < 0 || empty || s != s) {
-                const A v0 = y >= 0 && !empty ? s : A(0);
-                a.nothing(t, y < 0 ? A(0) : empty ? minus_inf<A>() : s, v0);
-                for (int j = 0; j < a.top; ++j) a.no_class(t, j, v0);
+            const A ls = log_of(s);
+            if (y_now < 0 || empty || s != s) {
+                const A v0 = y_now >= 0 && !empty ? s : A(0);
+                a.nothing(t, y_now < 0 ? A(0) : empty ? minus_inf<A>() : s, v0);
+                w.off[lane] = v0;
+                for (int j = 0; j < top; ++j) w.order[lane][j] = kNone;
             } else {
-                const A ls = log_of(s), xy = widen<A>(row[y]);
                 a.lse[t] = off + ls;
                 a.entropy[t] = entropy_of(ls, s, d);
                 if (a.lp) a.lp[t] = (xy - off) - ls;
-                int rank = 0, place[CW];
-#pragma unroll
-                for (int j = 0; j < CW; ++j) {
-                    rank += j < c && (v[j] > xy || (v[j] == xy && j < y)) ? 1 : 0;
-                    place[j] = 0;
-                }
                 if (a.ranks) a.id(a.ranks, t, rank);
-                if (a.top) {
+                w.off[lane] = off;
+                w.ls[lane] = ls;
+                if (top) {
+                    int place[CW];
+#pragma unroll
+                    for (int j = 0; j < CW; ++j) place[j] = 0;
 #pragma unroll
                     for (int j = 1; j < CW; ++j)
 #pragma unroll
-                        for (int q = 0; q < j; ++q)
-                            if (v[j] > v[q])
-                                ++place[q];
-                            else
-                                ++place[j];
-#pragma unroll
-                    for (int j = 0; j < CW; ++j)
-                        if (j < c && place[j] < a.top) {
-                            a.id(a.top_ids, t * a.top + place[j], j);
-                            a.top_lp[t * a.top + place[j]] = (v[j] - off) - ls;
+                        for (int q = 0; q < j; ++q) {
+                            const int up = v[j] > v[q] ? 1 : 0;
+                            place[q] += up;
+                            place[j] += 1 - up;
                         }
+#pragma unroll
+                    for (int j = 0; j < CW; ++j) w.order[lane][place[j]] = (uint8_t)j;  // padding comes last: below -infinity's ties
                 }
             }
         }
-        __syncwarp();  // the tile is filled again
+        __syncwarp();
+        for (int e = lane; e < rows * top; e += 32) {
+            const int r = (int)(e * by_top >> 16), j = w.order[r][e - r * top];
+            const int64_t to = t0 * top + e;
+            if (a.ids64)
+                static_cast<int64_t*>(a.top_ids)[to] = j == kNone ? -1 : j;
+            else
+                static_cast<int32_t*>(a.top_ids)[to] = j == kNone ? -1 : j;
+            a.top_lp[to] = j == kNone ? w.off[r] : (widen<A>(tile[r * c + j]) - w.off[r]) - w.ls[r];
+        }
+        __syncwarp();  // the tile and the order are filled again
     }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
 
 // ------------------------------------------------------------ longer rows --
@@ -232,9 +270,12 @@ struct Terms<double> {
 // vector that the label is in counts as one behind it; `fix` adds what that leaves out.
 template <class T>
 struct Before {
-    T own, lower;  // lower: NaN below -infinity, where everything counts
-    int y;         // may lie outside the values that are looked at
-    __device__ __forceinline__ Before(T xy, int label) : own(xy), lower(below(xy)), y(label) {}
+    T own, lower;     // lower: NaN below -infinity, where everything counts
+    int y, vector;    // the label, which may lie outside the values that are looked at, and its vector;
+                      // vectors from the last one on, which are -infinity, are behind it
+    __device__ __forceinline__ Before(T xy, int label, const RowShape<T>& sh)
+        : own(xy), lower(below(xy)), y(label), vector(label < sh.head ? -1 : min((label - sh.head) / RowShape<T>::V, sh.nv)) {}
+    __device__ __forceinline__ T bound(int j) const { return j < vector ? lower : own; }
     static __device__ __forceinline__ float below(float v) {
         const int b = __float_as_int(v);
         return v == 0.0f ? __int_as_float((int)0x80000001) : v == minus_inf<float>() ? NAN : __int_as_float(v > 0.0f ? b - 1 : b + 1);
@@ -258,11 +299,12 @@ struct Before {
         using A = typename Arith<T>::type;
         return above<A>(widen<A>(v), widen<A>(i < y ? lower : own)) ? 1 : 0;
     }
-    // of the vector's values before the label that are equal to it
-    __device__ __forceinline__ int fix(const T* row, int first) const {
+    // of the label's vector's values before the label that are equal to it, by one thread
+    __device__ __forceinline__ int fix(const T* row, const RowShape<T>& sh) const {
         using A = typename Arith<T>::type;
         int n = 0;
-        for (int i = first; i < y; ++i) n += widen<A>(row[i]) == widen<A>(own) ? 1 : 0;
+        if (vector >= 0 && vector < sh.nv)
+            for (int i = sh.head + vector * RowShape<T>::V; i < y; ++i) n += widen<A>(row[i]) == widen<A>(own) ? 1 : 0;
         return n;
     }
 };
@@ -303,12 +345,92 @@ struct Count<__half> : PairCount<__half2, __half> {
     __device__ __forceinline__ void add(const uint4& r, const float (&)[N], __half bound) { four(r, __half2half2(bound)); }
 };
 
+// The largest of a few vectors' values: in 16 bits two at a time up to the last step.
+template <class T, class A, int U>
+__device__ __forceinline__ A top_of(const uint4 (&v)[U]) {
+    A best = Pack<T>::top(v[0]);
+#pragma unroll
+    for (int u = 1; u < U; ++u) best = fmax(best, Pack<T>::top(v[u]));
+    return best;
+}
+template <class P, int U>
+__device__ __forceinline__ float top_of_pairs(const uint4 (&v)[U]) {
+    P m = as_pair<P>(v[0].x);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+        m = __hmax2(__hmax2(__hmax2(m, as_pair<P>(v[u].x)), __hmax2(as_pair<P>(v[u].y), as_pair<P>(v[u].z))), as_pair<P>(v[u].w));
+    return fmaxf(__low2float(m), __high2float(m));
+}
+template <>
+__device__ __forceinline__ float top_of<__nv_bfloat16, float, 8>(const uint4 (&v)[8]) { return top_of_pairs<__nv_bfloat162>(v); }
+template <>
+__device__ __forceinline__ float top_of<__half, float, 8>(const uint4 (&v)[8]) { return top_of_pairs<__half2>(v); }
+
+// A value with its index, as a number that grows in the order of the classes. In 32 bits one word: the
+// value's bits in the order of values above the complement of the index.
 template <class A>
-struct Candidate {
-    A v;
-    int i;
-    __device__ __forceinline__ bool before(const Candidate& o) const { return v > o.v || (v == o.v && i < o.i); }
+struct Key;
+template <>
+struct Key<float> {
+    uint64_t k;
+    Key() = default;
+    __device__ __forceinline__ Key(float v, int i) {
+        const int b = __float_as_int(v + 0.0f);  // -0 is 0
+        k = (uint64_t)(unsigned)(b ^ (b >> 31 | (int)0x80000000)) << 32 | (unsigned)~i;
+    }
+    static __device__ __forceinline__ Key none() {
+        Key r;
+        r.k = 0;
+        return r;
+    }
+    __device__ __forceinline__ bool before(const Key& o) const { return k > o.k; }
+    __device__ __forceinline__ bool is_none() const { return k == 0; }
+    __device__ __forceinline__ float value() const {
+        const int b = (int)(k >> 32);
+        return __int_as_float(b ^ (~(b >> 31) | (int)0x80000000));
+    }
+    __device__ __forceinline__ int index() const { return (int)~(unsigned)k; }
+    __device__ __forceinline__ void move(int by) { k -= by; }  // the index goes up
+    __device__ __forceinline__ Key across(int lanes) const {
+        Key r;
+        r.k = __shfl_xor_sync(0xffffffffu, k, lanes);
+        return r;
+    }
 };
+template <>
+struct Key<double> {
+    double v;
+    int64_t i;
+    Key() = default;
+    __device__ __forceinline__ Key(double value, int index) : v(value), i(index) {}
+    static __device__ __forceinline__ Key none() {
+        Key r;
+        r.v = minus_inf<double>();
+        r.i = INT64_MAX;
+        return r;
+    }
+    __device__ __forceinline__ bool before(const Key& o) const { return v > o.v || (v == o.v && i < o.i); }
+    __device__ __forceinline__ bool is_none() const { return i == INT64_MAX; }
+    __device__ __forceinline__ double value() const { return v; }
+    __device__ __forceinline__ int index() const { return (int)i; }
+    __device__ __forceinline__ void move(int by) {
+        if (!is_none()) i += by;
+    }
+    __device__ __forceinline__ Key across(int lanes) const {
+        Key r;
+        r.v = __shfl_xor_sync(0xffffffffu, v, lanes);
+        r.i = __shfl_xor_sync(0xffffffffu, i, lanes);
+        return r;
+    }
+};
+// How many of n keys come before `me`.
+template <class A>
+__device__ __forceinline__ int place_of(const Key<A>* keys, int n, const Key<A>& me) {
+    int place = 0;
+#pragma unroll 4
+    for (int o = 0; o < n; ++o) place += keys[o].before(me) ? 1 : 0;
+    return place;
+}
 
 constexpr int kSegments = 16;  // of a thread's vectors, each with its largest value
 
@@ -319,8 +441,8 @@ struct Shared {
     A one[L / 32], every[L / 32];
     int rank[L / 32];
     int count, listed;
-    Candidate<A> best[kTop];  // the answer
-    Candidate<A> cand[kCand];
+    Key<A> best[kTop];  // the answer
+    Key<A> cand[kCand];
     A most[SCAN ? kSegments : 1][SCAN ? L : 1];
 };
 
@@ -365,10 +487,9 @@ __device__ __forceinline__ void reached(double v, int a, int b, double& at_a, do
     at_b = __shfl_sync(0xffffffffu, v, b - 1);
 }
 
-// The first `want` values of the row that equal v, in index order, by one warp:
-// f(place, index).
-template <class T, class A, class F>
-__device__ __noinline__ void first_equal(const T* row, int c, A v, int want, F&& f) {
+// The first `want` values of the row that equal v, in index order, by one warp.
+template <class T, class A>
+__device__ __noinline__ void first_equal(const T* row, int c, A v, int want, Key<A>* to) {
     const int lane = threadIdx.x & 31;
     int found = 0;
     for (int64_t j0 = 0; j0 < c && found < want; j0 += 32 * 8) {
@@ -389,29 +510,56 @@ __device__ __noinline__ void first_equal(const T* row, int c, A v, int want, F&&
         before += found - mine;
         for (int q = 0; q < 8; ++q)
             if (bits >> q & 1) {
-                if (before < want) f(before, (int)(j0 + lane * 8 + q));
+                if (before < want) to[before] = Key<A>(v, (int)(j0 + lane * 8 + q));
                 ++before;
             }
         found += all;
     }
 }
 
-// The first `top` of a row's c values (fewer, if it has fewer) in their order to g.best, by the
-// group. `bound`: what at least `top` of them reach. `walk(f)` calls f(value, index) for
-// every value that reaches it.
+// The first `top` values one at a time, each the first behind the one before, by a group: for
+// rows of which a few threads hold most of the large values.
+template <class T, class A, int L>
+__device__ __noinline__ void one_by_one(const T* row, int c, int top, Key<A>* parts, Key<A>* to) {
+    const int lane = threadIdx.x % L;
+    Key<A> last;
+    for (int place = 0; place < top; ++place) {
+        Key<A> best = Key<A>::none();
+        for (int64_t j = lane; j < c; j += L) {
+            const Key<A> o(widen<A>(row[j]), (int)j);
+            if ((place == 0 || last.before(o)) && o.before(best)) best = o;
+        }
+#pragma unroll
+        for (int s = 16; s > 0; s >>= 1) {
+            const Key<A> o = best.across(s);
+            if (o.before(best)) best = o;
+        }
+        if (L > 32) {
+            group_sync<L>();
+            if ((lane & 31) == 0) parts[lane / 32] = best;
+            group_sync<L>();
+            for (int w = 0; w < L / 32; ++w)
+                if (parts[w].before(best)) best = parts[w];
+        }
+        last = best;
+        if (lane == 0) to[place] = best;
+    }
+}
+
+// The first `top` of a row's c values in their order to g.best, by the group. `bound`: what at
+// least `top` of them reach. `walk(f)` calls f(value, index) for every value that reaches it.
 template <class T, class A, int L, bool SCAN, class W>
 __device__ __forceinline__ void choose(Shared<A, L, SCAN>& g, const T* row, int c, int top, A bound, W&& walk) {
     const int lane = threadIdx.x % L;
     auto take = [&](A v, int i) {
         const int at = atomicAdd(&g.count, 1);
-        if (at < kCand) g.cand[at] = Candidate<A>{v, i};
+        if (at < kCand) g.cand[at] = Key<A>(v, i);
     };
     // the places of the candidates among each other
     auto places = [&](int count) {
         for (int q = lane; q < count; q += L) {
-            const Candidate<A> me = g.cand[q];
-            int place = 0;
-            for (int o = 0; o < count; ++o) place += g.cand[o].before(me) ? 1 : 0;
+            const Key<A> me = g.cand[q];
+            const int place = place_of(g.cand, count, me);
             if (place < top) g.best[place] = me;
         }
     };
@@ -434,34 +582,10 @@ __device__ __forceinline__ void choose(Shared<A, L, SCAN>& g, const T* row, int 
     count = g.count;
     if (count <= kCand) {
         places(count);
-        if (count < top && lane < 32)
-            first_equal<T, A>(row, c, bound, top - count, [&](int place, int i) { g.best[count + place] = Candidate<A>{bound, i}; });
+        if (count < top && lane < 32) first_equal(row, c, bound, top - count, g.best + count);
         return;
     }
-    // Too many above it (a few threads hold most of the large values): one at a time, each
-    // the first behind the one before.
-    Candidate<A> last{(A)INFINITY, -1};
-    for (int place = 0; place < top; ++place) {
-        Candidate<A> best{minus_inf<A>(), INT32_MAX};
-        for (int64_t j = lane; j < c; j += L) {
-            const Candidate<A> o{widen<A>(row[j]), (int)j};
-            if (last.before(o) && o.before(best)) best = o;
-        }
-#pragma unroll
-        for (int s = 16; s > 0; s >>= 1) {
-            const Candidate<A> o{__shfl_xor_sync(0xffffffffu, best.v, s), __shfl_xor_sync(0xffffffffu, best.i, s)};
-            if (o.before(best)) best = o;
-        }
-        if (L > 32) {
-            group_sync<L>();
-            if ((lane & 31) == 0) g.cand[lane / 32] = best;
-            group_sync<L>();
-            for (int w = 0; w < L / 32; ++w)
-                if (g.cand[w].before(best)) best = g.cand[w];
-        }
-        last = best;
-        if (lane == 0) g.best[place] = best;
-    }
+    one_by_one<T, A, L>(row, c, top, g.cand, g.best);
 }
 
 // What a row's finished statistics say, by one thread; false where there is no more to say.
@@ -506,7 +630,7 @@ __global__ void __launch_bounds__(kNT, IsF64<A>::value || K > 4 ? 2 : 4)
     for (int i = 0; i < K; ++i) v[i] = lane + i * 32 < sh.nv ? load16(row + sh.head + (lane + i * 32) * V) : Pack<T>::minus_inf();
     const T low = narrow<T>(minus_inf<A>()), last = lane < sh.edges ? row[sh.edge(lane)] : low;
     const A edge = widen<A>(last);
-    const Before<T> before(row[y], y);
+    const Before<T> before(row[y], y, sh);
     A mine = edge;
 #pragma unroll
     for (int i = 0; i < K; ++i) mine = fmax(mine, Pack<T>::top(v[i]));
@@ -517,16 +641,13 @@ __global__ void __launch_bounds__(kNT, IsF64<A>::value || K > 4 ? 2 : 4)
     Terms<A> terms(off);
     Count<T> counted;
     int rank = lane < sh.edges ? before.one(last, sh.edge(lane)) : 0;
+    if (lane == 0) rank += before.fix(row, sh);
 #pragma unroll
     for (int i = 0; i < K; ++i) {
         A p[V];
         Pack<T>::unpack(v[i], p);
         terms.add(p);
-        const int i0 = sh.head + (lane + i * 32) * V;
-        if (lane + i * 32 < sh.nv) {
-            counted.add(v[i], p, i0 + V <= y ? before.lower : before.own);
-            if (i0 < y && y < i0 + V) rank += before.fix(row, i0);
-        }
+        counted.add(v[i], p, before.bound(lane + i * 32));
     }
     terms.to(r.s, r.d);
     const A e = exp_of(edge - off);
@@ -561,8 +682,8 @@ __global__ void __launch_bounds__(kNT, IsF64<A>::value || K > 4 ? 2 : 4)
     });
     __syncwarp();
     if (lane < top) {
-        a.id(a.top_ids, t * top + lane, g.best[lane].i);
-        a.top_lp[t * top + lane] = (g.best[lane].v - off) - ls;
+        a.id(a.top_ids, t * top + lane, g.best[lane].index());
+        a.top_lp[t * top + lane] = (g.best[lane].value() - off) - ls;
     }
 }
 
@@ -596,22 +717,23 @@ __global__ void __launch_bounds__(kNT, IsF64<A>::value ? 2 : 4)
     const T* row = x + t * ld + begin;
     const RowShape<T> sh(row, c);
     const T xy = x[t * ld + y_row];
-    const Before<T> before(xy, y_row - begin);
+    const Before<T> before(xy, y_row - begin, sh);
     const T last = lane < sh.edges ? row[sh.edge(lane)] : narrow<T>(minus_inf<A>());
     const A edge = widen<A>(last);
     const int per = (sh.nv + L * U * kSegments - 1) / (L * U * kSegments);  // batches a segment
     int rank = lane < sh.edges ? before.one(last, sh.edge(lane)) : 0;
+    if (lane == 0) rank += before.fix(row, sh);
     Stats<A> r{edge, A(0), A(0)};
     r.s = exp_of(edge - offset_of(edge));  // 1, 0 for -infinity, NaN
     A part_most = minus_inf<A>();
     int in_part = 0, segment = 0;
-    for (int j0 = lane; j0 - lane < sh.nv; j0 += L * U) {
+    // U vectors a thread; `full`: there are as many
+    auto batch = [&](int j0, auto full) {
         uint4 v[U];
-        A best = minus_inf<A>();
 #pragma unroll
-        for (int u = 0; u < U; ++u) v[u] = j0 + u * L < sh.nv ? load16(row + sh.head + (int64_t)(j0 + u * L) * V) : Pack<T>::minus_inf();
-#pragma unroll
-        for (int u = 0; u < U; ++u) best = fmax(best, Pack<T>::top(v[u]));
+        for (int u = 0; u < U; ++u)
+            v[u] = decltype(full)::value || j0 + u * L < sh.nv ? load16(row + sh.head + (int64_t)(j0 + u * L) * V) : Pack<T>::minus_inf();
+        const A best = top_of<T, A>(v);
         if (top) {
             part_most = fmax(part_most, best);
             if (++in_part == per || j0 - lane + L * U >= sh.nv) {
@@ -628,16 +750,14 @@ __global__ void __launch_bounds__(kNT, IsF64<A>::value ? 2 : 4)
             A p[V];
             Pack<T>::unpack(v[u], p);
             terms.add(p);
-            const int j = j0 + u * L;
-            if (j < sh.nv) {
-                const int behind = before.y - sh.head - j * V;  // of the label behind the vector's first value
-                counted.add(v[u], p, behind >= V ? before.lower : before.own);
-                if (behind > 0 && behind < V) rank += before.fix(row, sh.head + j * V);
-            }
+            counted.add(v[u], p, before.bound(j0 + u * L));
         }
         terms.to(r.s, r.d);
         rank += counted.total();
-    }
+    };
+    int j0 = lane;
+    for (; j0 - lane + L * U <= sh.nv; j0 += L * U) batch(j0, std::true_type{});
+    if (j0 - lane < sh.nv) batch(j0, std::false_type{});
     const A mine = r.m;
     join(r, 32);
     rank = __reduce_add_sync(0xffffffffu, rank);
@@ -658,7 +778,7 @@ __global__ void __launch_bounds__(kNT, IsF64<A>::value ? 2 : 4)
         g.rank[warp] = rank;
     }
     if (lane == 0) g.count = 0;
-    if (CL > 1 && lane < kTop) g.best[lane] = Candidate<A>{minus_inf<A>(), INT32_MAX};
+    if (CL > 1 && lane < kTop) g.best[lane] = Key<A>::none();
     group_sync<L>();
     if (W > 1) {
         const int w = lane & 31;
@@ -684,17 +804,31 @@ __global__ void __launch_bounds__(kNT, IsF64<A>::value ? 2 : 4)
         }
         const A bound = fmax(one, every);
         const int wanted = CL > 1 && c < top ? c : top;
+        // A segment of a thread's whose largest reaches the bound is read again by eight lanes,
+        // a vector each, four of them at a time.
         choose<T, A, L, true>(g, row, c, wanted, bound, [&](auto&& f) {
-            if (!(mine >= bound)) return;
             if (lane < sh.edges && edge >= bound) f(edge, sh.edge(lane));
+            if (!__any_sync(0xffffffffu, mine >= bound)) return;
             for (int s = 0; s * per * L * U < sh.nv; ++s) {
-                if (!(g.most[s][lane] >= bound)) continue;
-                for (int j = s * per * L * U + lane; j < sh.nv && j < (s + 1) * per * L * U; j += L) {
-                    A p[V];
-                    Pack<T>::unpack(load16(row + sh.head + (int64_t)j * V), p);
+                unsigned hits = __ballot_sync(0xffffffffu, g.most[s][lane] >= bound);
+                while (hits) {
+                    int owner = -1;
 #pragma unroll
-                    for (int q = 0; q < V; ++q)
-                        if (p[q] >= bound) f(p[q], sh.head + j * V + q);
+                    for (int q = 0; q < 4; ++q) {
+                        if ((lane & 31) / 8 == q && hits) owner = __ffs(hits) - 1;
+                        hits &= hits - 1;
+                    }
+                    for (int b = s * per; b < (s + 1) * per; ++b) {
+                        const int j = (b * U + (lane & 7)) * L + warp * 32 + owner;
+                        if (owner < 0 || j >= sh.nv) continue;
+                        const uint4 v = load16(row + sh.head + (int64_t)j * V);
+                        if (!(Pack<T>::top(v) >= bound)) continue;
+                        A p[V];
+                        Pack<T>::unpack(v, p);
+#pragma unroll
+                        for (int q = 0; q < V; ++q)
+                            if (p[q] >= bound) f(p[q], sh.head + j * V + q);
+                    }
                 }
             }
         });
@@ -726,26 +860,25 @@ __global__ void __launch_bounds__(kNT, IsF64<A>::value ? 2 : 4)
                 const int count = top * CL;
                 for (int q = lane; q < count; q += L) {
                     const G* o = cluster.map_shared_rank(&g, q / top);
-                    Candidate<A> k = o->best[q % top];
-                    if (k.i != INT32_MAX) k.i += o->listed;
+                    Key<A> k = o->best[q % top];
+                    if (!k.is_none()) k.move(o->listed);
                     g.cand[q] = k;
                 }
                 group_sync<L>();
                 for (int q = lane; q < count; q += L) {
-                    const Candidate<A> me = g.cand[q];
-                    int place = 0;
-                    for (int o = 0; o < count; ++o) place += g.cand[o].before(me) ? 1 : 0;
-                    if (place < top && me.i != INT32_MAX) {
-                        a.id(a.top_ids, t * top + place, me.i);
-                        a.top_lp[t * top + place] = (me.v - off) - ls;
+                    const Key<A> me = g.cand[q];
+                    const int place = place_of(g.cand, count, me);
+                    if (place < top && !me.is_none()) {
+                        a.id(a.top_ids, t * top + place, me.index());
+                        a.top_lp[t * top + place] = (me.value() - off) - ls;
                     }
                 }
             }
         }
         cluster.sync();  // the others' shared memory is read until here
     } else if (lane < top) {
-        a.id(a.top_ids, t * top + lane, g.best[lane].i);
-        a.top_lp[t * top + lane] = (g.best[lane].v - off) - ls;
+        a.id(a.top_ids, t * top + lane, g.best[lane].index());
+        a.top_lp[t * top + lane] = (g.best[lane].value() - off) - ls;
     }
 }
 
@@ -763,10 +896,120 @@ struct GradArgs {
     }
 };
 
+// A row's gradient by p alone: -p (sum + gh (x - lse + h)).
+template <class A>
+struct Slope {
+    A l, whole, gh;  // whole = sum + gh h
+    __device__ __forceinline__ A of(A v) const {
+        const A z = v - l;
+        return -exp_of(z) * (whole + gh * floor_of(z));
+    }
+    template <int N>
+    __device__ __forceinline__ void all(double (&v)[N]) const {
+#pragma unroll
+        for (int q = 0; q < N; ++q) v[q] = of(v[q]);
+    }
+    // two at a time, the difference in units of log 2
+    template <int N>
+    __device__ __forceinline__ void all(float (&v)[N]) const {
+        const uint64_t ml = pair_of(-l, -l), w = pair_of(-whole, -whole), k = pair_of(gh * -0.6931471805599453f, gh * -0.6931471805599453f);
+#pragma unroll
+        for (int q = 0; q < N; q += 2) {
+            float a, b, ea, eb;
+            pair_to(pair_mul(pair_add(pair_of(v[q], v[q + 1]), ml), pair_of(1.4426950408889634f, 1.4426950408889634f)), a, b);
+            asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(ea) : "f"(a));
+            asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(eb) : "f"(b));
+            uint64_t t;
+            asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(t) : "l"(pair_of(fmaxf(a, -200.0f), fmaxf(b, -200.0f))), "l"(k), "l"(w));
+            pair_to(pair_mul(pair_of(ea, eb), t), v[q], v[q + 1]);
+        }
+    }
+};
+
+// Few classes: a thread per row as in small_kernel, the gradient written in its row's place.
+template <class T, class A, int CW>
+__global__ void __launch_bounds__(kSmallNT, IsF64<A>::value || CW > 16 ? 4 : 8)
+    small_grad_kernel(const T* __restrict__ x, int64_t ld, T* __restrict__ out, int64_t ld_out, GradArgs<A> a,
+                      bool whole_in, bool whole_out) {
+    extern __shared__ uint4 small_smem[];
+    const int c = (int)a.c, lane = threadIdx.x & 31;
+    T* const tiles = reinterpret_cast<T*>(small_smem) + (threadIdx.x / 32) * (2 * kTileRows * c);
+    const int64_t n_tiles = ceil_div(a.n, (int64_t)kTileRows), step = (int64_t)gridDim.x * (kSmallNT / 32);
+    // from the last row to the first: the forward left the last ones in L2
+    auto begin = [&](int64_t i) { return (n_tiles - 1 - i) * kTileRows; };
+    auto rows_of = [&](int64_t t0) { return (int)(a.n - t0 < kTileRows ? a.n - t0 : kTileRows); };
+    int64_t i = (int64_t)blockIdx.x * (kSmallNT / 32) + threadIdx.x / 32;
+    int y = -1;
+    A l = A(0), g_lp = A(0), g_h = A(0), h = A(0);
+    auto inputs = [&](int64_t t0) {
+        const int64_t t = t0 + lane;
+        if (lane >= rows_of(t0)) return;
+        y = a.labels.p ? a.labels.in(t, a.c) : 0;
+        l = a.lse[t];
+        g_lp = a.g_lp ? a.g_lp[t] : A(0);
+        g_h = a.g_entropy ? a.g_entropy[t] : A(0);
+        h = a.g_entropy ? a.entropy[t] : A(0);
+    };
+    if (i < n_tiles) {
+        tile_fetch(x, ld, begin(i), rows_of(begin(i)), c, whole_in, tiles);
+        inputs(begin(i));
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    for (int buf = 0; i < n_tiles; i += step, buf ^= 1) {
+        const int64_t t0 = begin(i), t = t0 + lane;
+        const int rows = rows_of(t0), y_now = y;
+        const A l_now = l, lp_now = g_lp, h_now = h;
+        A gh = g_h;
+        T* const tile = tiles + buf * (kTileRows * c);
+        if (i + step < n_tiles) {
+            const int64_t next = begin(i + step);
+            tile_fetch(x, ld, next, rows_of(next), c, whole_in, tiles + (buf ^ 1) * (kTileRows * c));
+            inputs(next);
+        }
+        asm volatile("cp.async.commit_group;\ncp.async.wait_group 1;" ::: "memory");
+        __syncwarp();
+        if (lane < rows) {
+            T* row = tile + lane * c;
+            const bool dead = y_now < 0 || l_now == minus_inf<A>();
+            A sum = A(0), v[CW];
+            if (!dead) {
+                for (int j = 0; j < a.top; ++j) {
+                    const int64_t id = a.id(t * a.top + j);
+                    if (id >= 0 && id < a.c) sum += a.g_top[t * a.top + j];
+                }
+                sum += lp_now;
+            } else {
+                gh = A(0);
+            }
+            const bool none = sum == A(0) && gh == A(0);
+            const Slope<A> slope{l_now, gh == A(0) ? sum : sum + gh * h_now, gh};
+#pragma unroll
+            for (int j = 0; j < CW; ++j)
+                if (j < c) v[j] = none ? A(0) : slope.of(widen<A>(row[j]));
+            if (!dead) {
+                auto name = [&](int64_t id, A g) {
+#pragma unroll
+                    for (int j = 0; j < CW; ++j)
+                        if (j == id) v[j] += g;
+                };
+                if (a.g_lp) name(y_now, lp_now);
+                for (int j = 0; j < a.top; ++j) name(a.id(t * a.top + j), a.g_top[t * a.top + j]);
+            }
+#pragma unroll
+            for (int j = 0; j < CW; ++j)
+                if (j < c) row[j] = narrow<T>(v[j]);
+        }
+        __syncwarp();
+        tile_put(out, ld_out, t0, rows, c, whole_out, tile);
+        __syncwarp();  // the tile's buffer is filled again
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+}
+
 // L threads a row: every value by p alone, then again those of the label and the best
 // classes with their gradients, summed over all places that name the class.
 template <class T, class A, int L>
-__global__ void __launch_bounds__(kNT)
+__global__ void __launch_bounds__(kNT, IsF64<A>::value ? 2 : 4)
     grad_kernel(const T* __restrict__ x, int64_t ld, T* __restrict__ out, int64_t ld_out, GradArgs<A> a) {
     constexpr int V = 16 / sizeof(T), U = 4;
     __shared__ A own[kNT / L][kTop + 1];
@@ -779,29 +1022,34 @@ __global__ void __launch_bounds__(kNT)
     const RowShape<T> sh(row, (int)a.c);
     const bool whole = alike(row, to);
     const int y = a.labels.p ? a.labels.in(t, a.c) : 0;
-    const A l = a.lse[t];
+    const A l = a.lse[t], g_lp = a.g_lp ? a.g_lp[t] : A(0);
+    A gh = a.g_entropy ? a.g_entropy[t] : A(0), h = a.g_entropy ? a.entropy[t] : A(0);
     const bool dead = y < 0 || l == minus_inf<A>();
-    const int places = dead ? 0 : a.top + 1;  // the last one is the label's
+    const int top = dead ? 0 : a.top, named = dead ? 0 : a.top + (a.g_lp ? 1 : 0);
     // places are at most 33, threads at least 32
-    for (int j = lane; j < places; j += L) {
-        const int64_t i = j < a.top ? a.id(t * a.top + j) : (int64_t)y;
-        const bool in = i >= 0 && i < a.c && (j < a.top || a.g_lp);
-        at[group][j] = in ? (int)i : -1;
-        own[group][j] = in ? (j < a.top ? a.g_top[t * a.top + j] : a.g_lp[t]) : A(0);
-    }
-    group_sync<L>();
     A sum = A(0);
-    for (int j = 0; j < places; ++j) sum += own[group][j];
-    const A gh = dead || !a.g_entropy ? A(0) : a.g_entropy[t];
-    const A h = gh == A(0) ? A(0) : a.entropy[t];
+    if (top) {
+        for (int j = lane; j < named; j += L) {
+            const int64_t i = j < top ? a.id(t * top + j) : (int64_t)y;
+            const bool in = i >= 0 && i < a.c;
+            at[group][j] = in ? (int)i : -1;
+            own[group][j] = in ? (j < top ? a.g_top[t * top + j] : g_lp) : A(0);
+        }
+        group_sync<L>();
+        const int w = threadIdx.x & 31;
+        sum = w < named ? own[group][w] : A(0);
+        if (w == 0 && named > 32) sum += own[group][32];
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    } else if (!dead) {
+        sum = g_lp;
+    }
+    if (dead) gh = A(0);
     const bool none = sum == A(0) && gh == A(0);
-    auto slope = [&](A v) {
-        const A z = v - l;
-        return -exp_of(z) * (sum + gh * (floor_of(z) + h));
-    };
+    const Slope<A> slope{l, gh == A(0) ? sum : sum + gh * h, gh};
     if (lane < sh.edges) {
         const int j = sh.edge(lane);
-        to[j] = narrow<T>(none ? A(0) : slope(widen<A>(row[j])));
+        to[j] = narrow<T>(none ? A(0) : slope.of(widen<A>(row[j])));
     }
     for (int j0 = lane; j0 < sh.nv; j0 += L * U) {
         uint4 v[U];
@@ -819,40 +1067,73 @@ __global__ void __launch_bounds__(kNT)
                     for (int q = 0; q < V; ++q) p[q] = A(0);
                 } else {
                     Pack<T>::unpack(v[u], p);
-#pragma unroll
-                    for (int q = 0; q < V; ++q) p[q] = slope(p[q]);
+                    slope.all(p);
                 }
                 store16<T, A>(to + sh.head + (int64_t)(j0 + u * L) * V, p, whole);
             }
     }
+    if (named == 0) return;
     group_sync<L>();  // the places' values come after all others
-    for (int j = lane; j < places; j += L) {
+    if (top == 0) {
+        if (lane == 0) to[y] = narrow<T>(g_lp + (none ? A(0) : slope.of(widen<A>(row[y]))));
+        return;
+    }
+    for (int j = lane; j < named; j += L) {
         const int i = at[group][j];
         if (i < 0) continue;
+        const T v = row[i];
         A mine = A(0);
-        for (int o = 0; o < places; ++o)
-            if (at[group][o] == i) mine += own[group][o];
-        to[i] = narrow<T>(mine + (none ? A(0) : slope(widen<A>(row[i]))));
+#pragma unroll 4
+        for (int o = 0; o < named; ++o) mine += at[group][o] == i ? own[group][o] : A(0);
+        to[i] = narrow<T>(mine + (none ? A(0) : slope.of(widen<A>(v))));
     }
 }
 
 // ------------------------------------------------------------- launchers --
 
+// The width of the registers that hold c classes.
+template <class F>
+void small_widths(int c, F&& f) {
+    using std::integral_constant;
+    if (c <= 4)
+        f(integral_constant<int, 4>{});
+    else if (c <= 8)
+        f(integral_constant<int, 8>{});
+    else if (c <= 12)
+        f(integral_constant<int, 12>{});
+    else if (c <= 16)
+        f(integral_constant<int, 16>{});
+    else if (c <= 24)
+        f(integral_constant<int, 24>{});
+    else
+        f(integral_constant<int, 32>{});
+}
+
+// One wave of blocks of a kernel over tiles, with the shared memory it asks for.
+template <auto Kernel>
+unsigned small_grid(int device, int64_t n, int c, size_t bytes) {
+    static bool asked[64];
+    allow_smem(Kernel, device, 128 * 1024, asked, "class tile shared memory");
+    static int per_sm[64][kSmallC + 1];  // the answer stays
+    int per = per_sm[device & 63][c];
+    if (per == 0) {
+        MFM_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, Kernel, kSmallNT, bytes), "occupancy");
+        per_sm[device & 63][c] = per = std::max(per, 1);
+    }
+    return (unsigned)std::min(ceil_div(n, kTileRows * (kSmallNT / 32)), (int64_t)sm_count(device) * per);
+}
+
 template <class T, class A>
 void rows_launch(int device, const T* x, int64_t ld, const Args<A>& a, cudaStream_t s) {
     if (a.c <= kSmallC) {
-        const size_t bytes = (size_t)(kSmallNT / 32) * kTileRows * a.c * sizeof(T);
-        const int64_t blocks = std::min(ceil_div(a.n, kTileRows * (kSmallNT / 32)), (int64_t)sm_count(device) * 16);
         const bool whole = ld == a.c && (uintptr_t)x % 16 == 0;
-        auto go = [&](auto w) {
-            small_kernel<T, A, decltype(w)::value><<<(unsigned)blocks, kSmallNT, bytes, s>>>(x, ld, a, whole);
-        };
-        if (a.c <= 8)
-            go(std::integral_constant<int, 8>{});
-        else if (a.c <= 16)
-            go(std::integral_constant<int, 16>{});
-        else
-            go(std::integral_constant<int, 32>{});
+        small_widths((int)a.c, [&](auto w) {
+            constexpr int CW = decltype(w)::value;
+            constexpr auto k = small_kernel<T, A, CW>;
+            const size_t bytes = (kSmallNT / 32) * small_bytes<T, A, CW>((int)a.c);
+            // e / top for e < 32 top as a product: exact, since 1024 / 65536 < 1 / 32
+            k<<<small_grid<k>(device, a.n, (int)a.c, bytes), kSmallNT, bytes, s>>>(x, ld, a, whole, a.top ? 65536u / a.top + 1 : 0);
+        });
         return;
     }
     const int64_t nv = a.c / Pack<T>::N, sms = sm_count(device);
@@ -902,7 +1183,16 @@ void rows_launch(int device, const T* x, int64_t ld, const Args<A>& a, cudaStrea
 }
 
 template <class T, class A>
-void grad_launch(const T* x, int64_t ld, T* out, int64_t ld_out, const GradArgs<A>& a, cudaStream_t s) {
+void grad_launch(int device, const T* x, int64_t ld, T* out, int64_t ld_out, const GradArgs<A>& a, cudaStream_t s) {
+    if (a.c <= kSmallC) {
+        small_widths((int)a.c, [&](auto w) {
+            constexpr auto k = small_grad_kernel<T, A, decltype(w)::value>;
+            const size_t bytes = (size_t)(kSmallNT / 32) * 2 * kTileRows * a.c * sizeof(T);
+            k<<<small_grid<k>(device, a.n, (int)a.c, bytes), kSmallNT, bytes, s>>>(
+                x, ld, out, ld_out, a, ld == a.c && (uintptr_t)x % 16 == 0, ld_out == a.c && (uintptr_t)out % 16 == 0);
+        });
+        return;
+    }
     auto go = [&](auto l) {
         constexpr int L = decltype(l)::value;
         grad_kernel<T, A, L><<<(unsigned)ceil_div(a.n, kNT / L), kNT, 0, s>>>(x, ld, out, ld_out, a);
@@ -965,7 +1255,7 @@ extern "C" int mfm_label_alternatives_grad_device(int dtype, int device, const v
             const GradArgs<A> a{Labels{labels, labels64}, n_tokens, n_classes, top, labels64, (const A*)lse,
                                 (const A*)entropy, (const A*)grad_logprobs, (const A*)grad_entropy,
                                 (const A*)grad_top, top_ids};
-            grad_launch<T, A>((const T*)logits, ld, (T*)d_logits, ld_out, a, (cudaStream_t)stream);
+            grad_launch<T, A>(device, (const T*)logits, ld, (T*)d_logits, ld_out, a, (cudaStream_t)stream);
         });
         MFM_CHECK_LAUNCH("label alternatives gradient launch");
     });
