@@ -210,7 +210,7 @@ __global__ void __launch_bounds__(kSmallNT, IsF64<A>::value || CW > 16 ? 4 : 8)
 // A row's, or a part of a row's, group of L threads within a block.
 template <int L>
 __device__ __forceinline__ void group_sync() {
-    if (L == 32)
+    if (L <= 32)
         __syncwarp();
     else if (L == kNT)
         __syncthreads();
@@ -434,16 +434,56 @@ __device__ __forceinline__ int place_of(const Key<A>* keys, int n, const Key<A>&
 
 constexpr int kSegments = 16;  // of a thread's vectors, each with its largest value
 
-// What a group shares: MOST of each of a scanning thread's segments.
-template <class A, int L, bool SCAN>
-struct Shared {
+// What a group shares.
+template <class A, int CAP>
+struct Lists {
+    int count, listed;
+    Key<A> best[kTop];  // the answer
+    Key<A> cand[CAP];
+};
+template <class A, int L>
+struct Shared : Lists<A, kCand> {
     A m[L / 32], s[L / 32], d[L / 32];
     A one[L / 32], every[L / 32];
     int rank[L / 32];
-    int count, listed;
-    Key<A> best[kTop];  // the answer
-    Key<A> cand[kCand];
-    A most[SCAN ? kSegments : 1][SCAN ? L : 1];
+    A most[kSegments][L];  // of each of a thread's segments
+};
+
+// Which of a vector's values are above `bound`, or (!STRICT) reach it: a bit each.
+template <class T, bool STRICT>
+struct Bits {
+    template <class A>
+    static __device__ __forceinline__ unsigned of(const uint4& r, A bound) {
+        A p[Pack<T>::N];
+        Pack<T>::unpack(r, p);
+        unsigned bits = 0;
+#pragma unroll
+        for (int q = 0; q < Pack<T>::N; ++q) bits |= (STRICT ? p[q] > bound : p[q] >= bound) ? 1u << q : 0u;
+        return bits;
+    }
+};
+template <class P, bool STRICT>
+__device__ __forceinline__ unsigned pair_bits(const uint4& r, P bound) {
+    const unsigned w[4] = {r.x, r.y, r.z, r.w};
+    unsigned bits = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const unsigned m = STRICT ? __hgt2_mask(as_pair<P>(w[i]), bound) : __hge2_mask(as_pair<P>(w[i]), bound);
+        bits |= m & (0x00020001u << (2 * i));
+    }
+    return (bits | bits >> 16) & 0xffu;
+}
+template <bool STRICT>
+struct Bits<__nv_bfloat16, STRICT> {  // the bound is one of the values: exact in their type
+    static __device__ __forceinline__ unsigned of(const uint4& r, float bound) {
+        return pair_bits<__nv_bfloat162, STRICT>(r, __float2bfloat162_rn(bound));
+    }
+};
+template <bool STRICT>
+struct Bits<__half, STRICT> {
+    static __device__ __forceinline__ unsigned of(const uint4& r, float bound) {
+        return pair_bits<__half2, STRICT>(r, __float2half2_rn(bound));
+    }
 };
 
 // The 32 lanes' values in falling order.
@@ -485,6 +525,22 @@ __device__ __forceinline__ void reached(double v, int a, int b, double& at_a, do
     v = sorted_lanes(v);
     at_a = __shfl_sync(0xffffffffu, v, a - 1);
     at_b = __shfl_sync(0xffffffffu, v, b - 1);
+}
+// The same of each group of L lanes, by maxima.
+template <class A, int L>
+__device__ __forceinline__ A reached_in_group(A v, int a) {
+    A at = minus_inf<A>();
+    if constexpr (L == 32) {
+        reached(v, a, a, at, at);
+    } else {
+        for (int i = 0; i < a; ++i) {
+            at = v;
+#pragma unroll
+            for (int o = L / 2; o > 0; o >>= 1) at = fmax(at, __shfl_xor_sync(0xffffffffu, at, o));
+            if (v == at) v = minus_inf<A>();
+        }
+    }
+    return at;
 }
 
 // The first `want` values of the row that equal v, in index order, by one warp.
@@ -546,43 +602,34 @@ __device__ __noinline__ void one_by_one(const T* row, int c, int top, Key<A>* pa
     }
 }
 
+// The places of a group's candidates among each other: the first `top` to g.best.
+template <class A, int L, int CAP>
+__device__ __forceinline__ void places(Lists<A, CAP>& g, int count, int top) {
+    for (int q = threadIdx.x % L; q < count; q += L) {
+        const Key<A> me = g.cand[q];
+        const int place = place_of(g.cand, count, me);
+        if (place < top) g.best[place] = me;
+    }
+}
+
 // The first `top` of a row's c values in their order to g.best, by the group. `bound`: what at
-// least `top` of them reach. `walk(f)` calls f(value, index) for every value that reaches it.
-template <class T, class A, int L, bool SCAN, class W>
-__device__ __forceinline__ void choose(Shared<A, L, SCAN>& g, const T* row, int c, int top, A bound, W&& walk) {
-    const int lane = threadIdx.x % L;
-    auto take = [&](A v, int i) {
-        const int at = atomicAdd(&g.count, 1);
-        if (at < kCand) g.cand[at] = Key<A>(v, i);
-    };
-    // the places of the candidates among each other
-    auto places = [&](int count) {
-        for (int q = lane; q < count; q += L) {
-            const Key<A> me = g.cand[q];
-            const int place = place_of(g.cand, count, me);
-            if (place < top) g.best[place] = me;
+// least `top` of them reach. `walk(strict)` lists the values that reach it (strict: that are above it) as
+// candidates and says how many there are, or, where that is more than fit, that it is.
+template <class T, class A, int L, class W>
+__device__ __forceinline__ void choose(Lists<A, kCand>& g, const T* row, int c, int top, A bound, W&& walk) {
+    if (bound != minus_inf<A>()) {
+        const int count = walk(std::false_type{});
+        if (count <= kCand) {
+            places<A, L>(g, count, top);
+            return;
         }
-    };
-    walk(take);
-    group_sync<L>();
-    int count = g.count;
-    if (count <= kCand) {
-        places(count);
-        return;
     }
     // Too many reach it: mostly ties, as of masked classes. Those above it, and the first
     // of those that are equal.
-    group_sync<L>();
-    if (lane == 0) g.count = 0;
-    group_sync<L>();
-    walk([&](A v, int i) {
-        if (v > bound) take(v, i);
-    });
-    group_sync<L>();
-    count = g.count;
+    const int count = walk(std::true_type{});
     if (count <= kCand) {
-        places(count);
-        if (count < top && lane < 32) first_equal(row, c, bound, top - count, g.best + count);
+        places<A, L>(g, count, top);
+        if (count < top && threadIdx.x % L < 32) first_equal(row, c, bound, top - count, g.best + count);
         return;
     }
     one_by_one<T, A, L>(row, c, top, g.cand, g.best);
@@ -607,94 +654,137 @@ __device__ __forceinline__ bool finish(const Args<A>& a, int64_t t, A xy, const 
     return true;
 }
 
-// Rows of up to 32 K vectors: a warp each, the row in its registers.
-template <class T, class A, int K>
-__global__ void __launch_bounds__(kNT, IsF64<A>::value || K > 4 ? 2 : 4)
+// Rows of up to L K vectors: L lanes each, the row in their registers.
+template <class A, int V, int L, int K>
+constexpr int held_cand() { return L * K * V + 2 * (V - 1) < kCand ? L * K * V + 2 * (V - 1) : kCand; }
+
+template <class T, class A, int L, int K>
+__global__ void __launch_bounds__(kNT, IsF64<A>::value ? 2 : K > 4 ? 3 : 4)
     held_kernel(const T* __restrict__ x, int64_t ld, Args<A> a) {
-    constexpr int V = 16 / sizeof(T);
-    __shared__ Shared<A, 32, false> shared[kNT / 32];
-    Shared<A, 32, false>& g = shared[threadIdx.x / 32];
-    const int lane = threadIdx.x & 31, top = a.top;
-    const int64_t t = (int64_t)blockIdx.x * (kNT / 32) + threadIdx.x / 32;
-    if (t >= a.n) return;
-    const int y = a.label(t);
-    if (y < 0) {
+    constexpr int V = 16 / sizeof(T), E = (2 * (V - 1) + L - 1) / L, CAP = held_cand<A, V, L, K>();
+    __shared__ Lists<A, CAP> shared[kNT / L];
+    Lists<A, CAP>& g = shared[threadIdx.x / L];
+    const int lane = threadIdx.x % L, top = a.top;
+    const int64_t t = (int64_t)blockIdx.x * (kNT / L) + threadIdx.x / L;
+    const int y = t < a.n ? a.label(t) : -1;
+    if (t < a.n && y < 0) {
         if (lane == 0) a.nothing(t, A(0), A(0));
-        if (lane < top) a.no_class(t, lane, A(0));
-        return;
+        for (int j = lane; j < top; j += L) a.no_class(t, j, A(0));
     }
-    const T* row = x + t * ld;
-    const RowShape<T> sh(row, (int)a.c);
+    if (L == 32 ? y < 0 : __all_sync(0xffffffffu, y < 0)) return;  // the whole warp
+    const bool in = y >= 0;
+    const T* row = x + (in ? t : 0) * ld;
+    const RowShape<T> sh(row, in ? (int)a.c : 0);
     uint4 v[K];
 #pragma unroll
-    for (int i = 0; i < K; ++i) v[i] = lane + i * 32 < sh.nv ? load16(row + sh.head + (lane + i * 32) * V) : Pack<T>::minus_inf();
-    const T low = narrow<T>(minus_inf<A>()), last = lane < sh.edges ? row[sh.edge(lane)] : low;
-    const A edge = widen<A>(last);
-    const Before<T> before(row[y], y, sh);
-    A mine = edge;
+    for (int i = 0; i < K; ++i) v[i] = lane + i * L < sh.nv ? load16(row + sh.head + (lane + i * L) * V) : Pack<T>::minus_inf();
+    const T low = narrow<T>(minus_inf<A>());
+    T last[E];
+    A mine = minus_inf<A>();
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+        last[i] = lane + i * L < sh.edges ? row[sh.edge(lane + i * L)] : low;
+        mine = fmax(mine, widen<A>(last[i]));
+    }
+    const Before<T> before(row[in ? y : 0], y, sh);
 #pragma unroll
     for (int i = 0; i < K; ++i) mine = fmax(mine, Pack<T>::top(v[i]));
     Stats<A> r{mine, A(0), A(0)};
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) r.m = fmax(r.m, __shfl_xor_sync(0xffffffffu, r.m, o));
+    for (int o = L / 2; o > 0; o >>= 1) r.m = fmax(r.m, __shfl_xor_sync(0xffffffffu, r.m, o));
     A off = offset_of(r.m), ls;
     Terms<A> terms(off);
     Count<T> counted;
-    int rank = lane < sh.edges ? before.one(last, sh.edge(lane)) : 0;
-    if (lane == 0) rank += before.fix(row, sh);
+    int rank = lane == 0 ? before.fix(row, sh) : 0;
 #pragma unroll
     for (int i = 0; i < K; ++i) {
         A p[V];
         Pack<T>::unpack(v[i], p);
         terms.add(p);
-        counted.add(v[i], p, before.bound(lane + i * 32));
+        counted.add(v[i], p, before.bound(lane + i * L));
     }
     terms.to(r.s, r.d);
-    const A e = exp_of(edge - off);
-    r.s += e;
-    r.d += e * floor_of(edge - off);
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
+    for (int i = 0; i < E; ++i) {
+        const A z = widen<A>(last[i]) - off, e = exp_of(z);
+        r.s += e;
+        r.d += e * floor_of(z);
+        if (lane + i * L < sh.edges) rank += before.one(last[i], sh.edge(lane + i * L));
+    }
+    rank += counted.total();
+#pragma unroll
+    for (int o = L / 2; o > 0; o >>= 1) {
         r.s += __shfl_xor_sync(0xffffffffu, r.s, o);
         r.d += __shfl_xor_sync(0xffffffffu, r.d, o);
+        rank += __shfl_xor_sync(0xffffffffu, rank, o);
     }
-    rank = __reduce_add_sync(0xffffffffu, rank + counted.total());
-    if (!finish(a, t, widen<A>(before.own), r, rank, off, ls, lane == 0)) {
-        if (lane < top) a.no_class(t, lane, r.s != r.s ? r.s : A(0));
-        return;
-    }
-    if (top == 0) return;
-    if (lane == 0) g.count = 0;
-    A bound, same;
-    reached(mine, top, top, bound, same);
-    __syncwarp();
-    choose<T, A, 32, false>(g, row, (int)a.c, top, bound, [&](auto&& f) {
-        if (lane < sh.edges && edge >= bound) f(edge, sh.edge(lane));
+    const bool go = in && finish(a, t, widen<A>(before.own), r, rank, off, ls, lane == 0);
+    if (in && !go)
+        for (int j = lane; j < top; j += L) a.no_class(t, j, r.s != r.s ? r.s : A(0));
+    if (top == 0 || (L == 32 ? !go : __all_sync(0xffffffffu, !go))) return;
+    const A bound = reached_in_group<A, L>(mine, top);
+    // A bit for each value that is listed; then they are taken one a lane at a time.
+    auto walk = [&](auto strict) {
+        constexpr bool S = decltype(strict)::value;
+        const unsigned group = L == 32 ? 0xffffffffu : ((1u << (L & 31)) - 1) << (threadIdx.x & 31 & ~(L - 1));
+        const unsigned before_me = group & ((1u << (threadIdx.x & 31)) - 1);
+        uint64_t bits = 0;
 #pragma unroll
-        for (int i = 0; i < K; ++i)
-            if (lane + i * 32 < sh.nv && Pack<T>::top(v[i]) >= bound) {
-                A p[V];
-                Pack<T>::unpack(v[i], p);
+        for (int i = 0; i < K; ++i) bits |= (uint64_t)Bits<T, S>::of(v[i], bound) << (i * V);
+        int count = 0;
+        // the -infinity behind the row's end reaches a bound of -infinity
+        if (!go)
+            bits = 0;
+        else if (!S && bound == minus_inf<A>())
 #pragma unroll
-                for (int q = 0; q < V; ++q)
-                    if (p[q] >= bound) f(p[q], sh.head + (lane + i * 32) * V + q);
+            for (int i = 0; i < K; ++i)
+                if (lane + i * L >= sh.nv) bits &= ~(((1ull << V) - 1) << (i * V));
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+            const A e = widen<A>(last[i]);
+            const bool hit = go && lane + i * L < sh.edges && (S ? e > bound : e >= bound);
+            const unsigned hits = __ballot_sync(0xffffffffu, hit) & group;
+            if (hit) g.cand[count + __popc(hits & before_me)] = Key<A>(e, sh.edge(lane + i * L));
+            count += __popc(hits);
+        }
+        for (;;) {
+            const unsigned all = __ballot_sync(0xffffffffu, bits != 0 && count <= CAP), hits = all & group;
+            if (all == 0) break;
+            if (hits >> (threadIdx.x & 31) & 1) {
+                const int q = __ffsll((long long)bits) - 1, i = sh.head + (lane + q / V * L) * V + q % V;
+                const int to = count + __popc(hits & before_me);
+                if (to < CAP) g.cand[to] = Key<A>(widen<A>(row[i]), i);
+                bits &= bits - 1;
             }
-    });
+            count += __popc(hits);
+        }
+        __syncwarp();
+        return count;
+    };
+    if constexpr (CAP < kCand || L < 32)
+        places<A, L>(g, walk(std::false_type{}), top);  // every value fits
+    else
+        choose<T, A, L>(g, row, (int)a.c, top, bound, walk);
     __syncwarp();
-    if (lane < top) {
-        a.id(a.top_ids, t * top + lane, g.best[lane].index());
-        a.top_lp[t * top + lane] = (g.best[lane].value() - off) - ls;
-    }
+    if (go)
+        for (int j = lane; j < top; j += L) {
+            a.id(a.top_ids, t * top + j, g.best[j].index());
+            a.top_lp[t * top + j] = (g.best[j].value() - off) - ls;
+        }
 }
 
 // Longer rows, read once with a running maximum: L threads a row, or a cluster of CL blocks
 // of L threads where rows are few, each block on a part of the row and the first one on
-// what the others found, in distributed shared memory.
+// what the others found, in distributed shared memory. A row's own work (reductions, the
+// bound, the candidates) costs each of its warps several hundred instructions, so short rows
+// take few lanes. 32, 64, 128, 256 lanes a row, the five best of bf16 rows: 30000 x 5000 92, 131,
+// 172, 329 us; 8195 x 32000 119, 116, 121, 142; 4096 x 65536 117, 115, 112, 117; 300 x 65536
+// 45, 27, 23, 23.
 template <class T, class A, int L, int CL>
 __global__ void __launch_bounds__(kNT, IsF64<A>::value ? 2 : 4)
     scan_kernel(const T* __restrict__ x, int64_t ld, Args<A> a) {
     constexpr int V = 16 / sizeof(T), U = 8, W = L / 32;
-    using G = Shared<A, L, true>;
+    using G = Shared<A, L>;
     extern __shared__ uint4 rows_smem[];
     G& g = reinterpret_cast<G*>(rows_smem)[threadIdx.x / L];
     const int lane = threadIdx.x % L, warp = lane / 32, top = a.top;
@@ -806,12 +896,17 @@ __global__ void __launch_bounds__(kNT, IsF64<A>::value ? 2 : 4)
         const int wanted = CL > 1 && c < top ? c : top;
         // A segment of a thread's whose largest reaches the bound is read again by eight lanes,
         // a vector each, four of them at a time.
-        choose<T, A, L, true>(g, row, c, wanted, bound, [&](auto&& f) {
-            if (lane < sh.edges && edge >= bound) f(edge, sh.edge(lane));
-            if (!__any_sync(0xffffffffu, mine >= bound)) return;
-            for (int s = 0; s * per * L * U < sh.nv; ++s) {
-                unsigned hits = __ballot_sync(0xffffffffu, g.most[s][lane] >= bound);
-                while (hits) {
+        choose<T, A, L>(g, row, c, wanted, bound, [&](auto strict) {
+            constexpr bool S = decltype(strict)::value;
+            auto reaches = [&](A v) { return S ? v > bound : v >= bound; };
+            auto take = [&](A v, int i) {
+                const int at = atomicAdd(&g.count, 1);
+                if (at < kCand) g.cand[at] = Key<A>(v, i);
+            };
+            if (lane < sh.edges && reaches(edge)) take(edge, sh.edge(lane));
+            for (int s = 0; __any_sync(0xffffffffu, reaches(mine)) && s * per * L * U < sh.nv; ++s) {
+                unsigned hits = __ballot_sync(0xffffffffu, reaches(g.most[s][lane]));
+                while (hits && __all_sync(0xffffffffu, *(volatile int*)&g.count <= kCand)) {
                     int owner = -1;
 #pragma unroll
                     for (int q = 0; q < 4; ++q) {
@@ -821,16 +916,19 @@ __global__ void __launch_bounds__(kNT, IsF64<A>::value ? 2 : 4)
                     for (int b = s * per; b < (s + 1) * per; ++b) {
                         const int j = (b * U + (lane & 7)) * L + warp * 32 + owner;
                         if (owner < 0 || j >= sh.nv) continue;
-                        const uint4 v = load16(row + sh.head + (int64_t)j * V);
-                        if (!(Pack<T>::top(v) >= bound)) continue;
-                        A p[V];
-                        Pack<T>::unpack(v, p);
-#pragma unroll
-                        for (int q = 0; q < V; ++q)
-                            if (p[q] >= bound) f(p[q], sh.head + j * V + q);
+                        for (unsigned bits = Bits<T, S>::of(load16(row + sh.head + (int64_t)j * V), bound); bits; bits &= bits - 1) {
+                            const int i = sh.head + j * V + __ffs((int)bits) - 1;
+                            take(widen<A>(row[i]), i);
+                        }
                     }
                 }
             }
+            group_sync<L>();
+            const int count = g.count;
+            group_sync<L>();
+            if (lane == 0) g.count = 0;  // for a second walk, which begins behind the next barrier
+            if (!S) group_sync<L>();
+            return count;
         });
         group_sync<L>();
     }
@@ -1138,27 +1236,33 @@ void rows_launch(int device, const T* x, int64_t ld, const Args<A>& a, cudaStrea
     }
     const int64_t nv = a.c / Pack<T>::N, sms = sm_count(device);
     using std::integral_constant;
-    auto held = [&](auto k) {
-        held_kernel<T, A, decltype(k)::value><<<(unsigned)ceil_div(a.n, kNT / 32), kNT, 0, s>>>(x, ld, a);
+    auto held = [&](auto l, auto k) {
+        constexpr int L = decltype(l)::value;
+        held_kernel<T, A, L, decltype(k)::value><<<(unsigned)ceil_div(a.n, kNT / L), kNT, 0, s>>>(x, ld, a);
     };
     auto scan = [&](auto l) {
-        constexpr int L = decltype(l)::value, bytes = (int)sizeof(Shared<A, L, true>) * (kNT / L);
+        constexpr int L = decltype(l)::value, bytes = (int)sizeof(Shared<A, L>) * (kNT / L);
         auto k = scan_kernel<T, A, L, 1>;
         static bool asked[64];
         allow_smem(k, device, bytes, asked, "row shared memory");
         k<<<(unsigned)ceil_div(a.n, kNT / L), kNT, bytes, s>>>(x, ld, a);
     };
-    if (nv <= 32)
-        held(integral_constant<int, 1>{});
+    // several rows a warp where that leaves enough lanes for the bound
+    if (nv <= 16 && a.top <= 5)
+        held(integral_constant<int, 8>{}, integral_constant<int, 2>{});
+    else if (nv <= 32 && a.top <= 8)
+        held(integral_constant<int, 16>{}, integral_constant<int, 2>{});
+    else if (nv <= 32)
+        held(integral_constant<int, 32>{}, integral_constant<int, 1>{});
     else if (nv <= 64)
-        held(integral_constant<int, 2>{});
+        held(integral_constant<int, 32>{}, integral_constant<int, 2>{});
     else if (nv <= 128)
-        held(integral_constant<int, 4>{});
+        held(integral_constant<int, 32>{}, integral_constant<int, 4>{});
     else if (nv <= 256)
-        held(integral_constant<int, 8>{});
+        held(integral_constant<int, 32>{}, integral_constant<int, 8>{});
     else if (nv >= 1024 && a.n <= sms / 2) {
         // so few rows that a cluster of eight blocks each fits at once
-        constexpr int bytes = (int)sizeof(Shared<A, kNT, true>);
+        constexpr int bytes = (int)sizeof(Shared<A, kNT>);
         auto k = scan_kernel<T, A, kNT, 8>;
         static bool asked[64];
         allow_smem(k, device, bytes, asked, "row shared memory");
@@ -1174,10 +1278,12 @@ void rows_launch(int device, const T* x, int64_t ld, const Args<A>& a, cudaStrea
         cfg.attrs = at;
         cfg.numAttrs = 1;
         MFM_CUDA(cudaLaunchKernelEx(&cfg, k, x, ld, a), "kernel launch");
-    } else if (nv >= 1024 && a.n * 4 < sms * 32)
+    } else if (nv >= 1024 && a.n <= 2 * sms)
         scan(integral_constant<int, kNT>{});
-    else if (nv >= 512)
+    else if (nv >= 6144)
         scan(integral_constant<int, 128>{});
+    else if (nv >= 1024)
+        scan(integral_constant<int, 64>{});
     else
         scan(integral_constant<int, 32>{});
 }
