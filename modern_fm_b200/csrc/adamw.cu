@@ -854,8 +854,20 @@ extern "C" int mfm_adamw_step_device(int device, const mfm_adamw_tensor* tensors
             if (!t.grad || t.d == 0 || t.n_rows == 0 || (t.keys && t.n_keys == 0)) continue;
             (t.keys ? tables : dense).push_back(i);
         }
-        std::stable_sort(dense.begin(), dense.end(),
-                         [&](int64_t a, int64_t b) { return kind_of(tensors[a], o.state_bits) < kind_of(tensors[b], o.state_bits); });
+        // Tensors that begin at whole vectors make launches of their own where they hold enough
+        // values for one; fewer go with those of their types that do not (300 tensors of
+        // 21.7 M float32 values behind each other, 37 of them aligned: PRE us in two launches,
+        // POST in one).
+        int64_t kinds[256][2] = {};
+        for (int64_t i : dense) {
+            const int kind = kind_of(tensors[i], o.state_bits);
+            kinds[kind / 2][kind & 1] += tensors[i].d;
+        }
+        auto kind = [&](int64_t i) {
+            const int k = kind_of(tensors[i], o.state_bits);
+            return (k & 1) && kinds[k / 2][0] > 0 && kinds[k / 2][1] < 1 << 23 ? k & ~1 : k;
+        };
+        std::stable_sort(dense.begin(), dense.end(), [&](int64_t a, int64_t b) { return kind(a) < kind(b); });
         bool begun = false;  // the first launch of a call waits for all before it, the others go on in a chain
         auto launch = [&](auto kernel, unsigned grid, auto&&... args) {
             if (begun)
@@ -901,8 +913,8 @@ extern "C" int mfm_adamw_step_device(int device, const mfm_adamw_tensor* tensors
         // dense tensors: as many of one kind as a launch carries
         for (size_t lo = 0; lo < dense.size();) {
             size_t hi = lo;
-            const int kind = kind_of(tensors[dense[lo]], o.state_bits);
-            while (hi < dense.size() && hi - lo < kMany && kind_of(tensors[dense[hi]], o.state_bits) == kind) ++hi;
+            const int one = kind(dense[lo]);
+            while (hi < dense.size() && hi - lo < kMany && kind(dense[hi]) == one) ++hi;
             const bool last = hi == dense.size() && tables.empty();
             with_kind(tensors[dense[lo]], o.state_bits, [&](auto* p, auto* g, auto master, auto bits) {
                 using P = Bare<decltype(p)>;
@@ -934,7 +946,7 @@ extern "C" int mfm_adamw_step_device(int device, const mfm_adamw_tensor* tensors
                         go(std::integral_constant<int, kMany>{}, aligned);
                 };
                 if constexpr (!IsF64<P>::value) {
-                    if (kind & 1) return size(std::true_type{});
+                    if (one & 1) return size(std::true_type{});
                 }
                 size(std::false_type{});
             });

@@ -265,6 +265,43 @@ struct Terms<double> {
     }
 };
 
+// Which of a vector's values are above `bound`, or (!STRICT) reach it: a bit each.
+template <class T, bool STRICT>
+struct Bits {
+    template <class A>
+    static __device__ __forceinline__ unsigned of(const uint4& r, A bound) {
+        A p[Pack<T>::N];
+        Pack<T>::unpack(r, p);
+        unsigned bits = 0;
+#pragma unroll
+        for (int q = 0; q < Pack<T>::N; ++q) bits |= (STRICT ? p[q] > bound : p[q] >= bound) ? 1u << q : 0u;
+        return bits;
+    }
+};
+template <class P, bool STRICT>
+__device__ __forceinline__ unsigned pair_bits(const uint4& r, P bound) {
+    const unsigned w[4] = {r.x, r.y, r.z, r.w};
+    unsigned bits = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const unsigned m = STRICT ? __hgt2_mask(as_pair<P>(w[i]), bound) : __hge2_mask(as_pair<P>(w[i]), bound);
+        bits |= m & (0x00020001u << (2 * i));
+    }
+    return (bits | bits >> 16) & 0xffu;
+}
+template <bool STRICT>
+struct Bits<__nv_bfloat16, STRICT> {  // the bound is one of the values: exact in their type
+    static __device__ __forceinline__ unsigned of(const uint4& r, float bound) {
+        return pair_bits<__nv_bfloat162, STRICT>(r, __float2bfloat162_rn(bound));
+    }
+};
+template <bool STRICT>
+struct Bits<__half, STRICT> {
+    static __device__ __forceinline__ unsigned of(const uint4& r, float bound) {
+        return pair_bits<__half2, STRICT>(r, __float2half2_rn(bound));
+    }
+};
+
 // How many of a row's values come before its label's: those above it, and of the ones
 // equal to it those before its index, which are above the next lower value of the type. The
 // vector that the label is in counts as one behind it; `fix` adds what that leaves out.
@@ -302,10 +339,12 @@ struct Before {
     // of the label's vector's values before the label that are equal to it, by one thread
     __device__ __forceinline__ int fix(const T* row, const RowShape<T>& sh) const {
         using A = typename Arith<T>::type;
-        int n = 0;
-        if (vector >= 0 && vector < sh.nv)
-            for (int i = sh.head + vector * RowShape<T>::V; i < y; ++i) n += widen<A>(row[i]) == widen<A>(own) ? 1 : 0;
-        return n;
+        if (vector < 0 || vector >= sh.nv) return 0;
+        const int first = sh.head + vector * RowShape<T>::V;
+        const uint4 v = load16(row + first);
+        const A own_wide = widen<A>(own);
+        const unsigned equal = Bits<T, false>::of(v, own_wide) & ~Bits<T, true>::of(v, own_wide);
+        return __popc(equal & ((1u << (y - first)) - 1));
     }
 };
 // Counts over a few vectors; total() at most once each 64 of them (16-bit counters hold 256).
@@ -449,43 +488,6 @@ struct Shared : Lists<A, kCand> {
     A most[kSegments][L];  // of each of a thread's segments
 };
 
-// Which of a vector's values are above `bound`, or (!STRICT) reach it: a bit each.
-template <class T, bool STRICT>
-struct Bits {
-    template <class A>
-    static __device__ __forceinline__ unsigned of(const uint4& r, A bound) {
-        A p[Pack<T>::N];
-        Pack<T>::unpack(r, p);
-        unsigned bits = 0;
-#pragma unroll
-        for (int q = 0; q < Pack<T>::N; ++q) bits |= (STRICT ? p[q] > bound : p[q] >= bound) ? 1u << q : 0u;
-        return bits;
-    }
-};
-template <class P, bool STRICT>
-__device__ __forceinline__ unsigned pair_bits(const uint4& r, P bound) {
-    const unsigned w[4] = {r.x, r.y, r.z, r.w};
-    unsigned bits = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const unsigned m = STRICT ? __hgt2_mask(as_pair<P>(w[i]), bound) : __hge2_mask(as_pair<P>(w[i]), bound);
-        bits |= m & (0x00020001u << (2 * i));
-    }
-    return (bits | bits >> 16) & 0xffu;
-}
-template <bool STRICT>
-struct Bits<__nv_bfloat16, STRICT> {  // the bound is one of the values: exact in their type
-    static __device__ __forceinline__ unsigned of(const uint4& r, float bound) {
-        return pair_bits<__nv_bfloat162, STRICT>(r, __float2bfloat162_rn(bound));
-    }
-};
-template <bool STRICT>
-struct Bits<__half, STRICT> {
-    static __device__ __forceinline__ unsigned of(const uint4& r, float bound) {
-        return pair_bits<__half2, STRICT>(r, __float2half2_rn(bound));
-    }
-};
-
 // The 32 lanes' values in falling order.
 template <class A>
 __device__ __forceinline__ A sorted_lanes(A v) {
@@ -541,6 +543,25 @@ __device__ __forceinline__ A reached_in_group(A v, int a) {
         }
     }
     return at;
+}
+
+// The k-th largest of a warp's values, N and one more a lane, by its bits from the highest on:
+// for rows of fewer vectors than the places that are asked for, where the lanes' largest say
+// nothing. BITS: the upper bits in which the values differ.
+template <int BITS, int N>
+__device__ __forceinline__ float kth_of_warp(const float (&v)[N], float one, int k) {
+    unsigned u = 0;
+    for (int b = 31; b > 31 - BITS; --b) {
+        const unsigned with = u | 1u << b;
+        const float f = __int_as_float((int)with < 0 ? (int)(with & 0x7fffffffu) : (int)~with);  // NaN: reached by none
+        int count = one >= f ? 1 : 0;
+#pragma unroll
+        for (int q = 0; q < N; ++q) count += v[q] >= f ? 1 : 0;
+        if (__reduce_add_sync(0xffffffffu, count) >= k) u = with;
+    }
+    if (u < 0x00800000u) return minus_inf<float>();
+    if ((int)u >= 0) u |= (unsigned)((1ull << (32 - BITS)) - 1);  // a negative value's lower bits are 0 in itself
+    return __int_as_float((int)u < 0 ? (int)(u & 0x7fffffffu) : (int)~u);
 }
 
 // The first `want` values of the row that equal v, in index order, by one warp.
@@ -662,6 +683,8 @@ template <class T, class A, int L, int K>
 __global__ void __launch_bounds__(kNT, IsF64<A>::value ? 2 : K > 4 ? 3 : 4)
     held_kernel(const T* __restrict__ x, int64_t ld, Args<A> a) {
     constexpr int V = 16 / sizeof(T), E = (2 * (V - 1) + L - 1) / L, CAP = held_cand<A, V, L, K>();
+    static_assert(L == 32 || CAP < kCand, "groups within a warp hold every value as a candidate");
+    static_assert(K * V <= 64, "a bit a value");
     __shared__ Lists<A, CAP> shared[kNT / L];
     Lists<A, CAP>& g = shared[threadIdx.x / L];
     const int lane = threadIdx.x % L, top = a.top;
@@ -722,7 +745,14 @@ __global__ void __launch_bounds__(kNT, IsF64<A>::value ? 2 : K > 4 ? 3 : 4)
     if (in && !go)
         for (int j = lane; j < top; j += L) a.no_class(t, j, r.s != r.s ? r.s : A(0));
     if (top == 0 || (L == 32 ? !go : __all_sync(0xffffffffu, !go))) return;
-    const A bound = reached_in_group<A, L>(mine, top);
+    A bound;
+    if constexpr (L == 32 && K == 1 && !IsF64<A>::value) {
+        A p[V];
+        Pack<T>::unpack(v[0], p);
+        bound = top > sh.nv ? kth_of_warp<sizeof(T) == 4 ? 32 : 19>(p, widen<A>(last[0]), top) : reached_in_group<A, L>(mine, top);
+    } else {
+        bound = reached_in_group<A, L>(mine, top);
+    }
     // A bit for each value that is listed; then they are taken one a lane at a time.
     auto walk = [&](auto strict) {
         constexpr bool S = decltype(strict)::value;
@@ -1109,44 +1139,49 @@ __global__ void __launch_bounds__(kSmallNT, IsF64<A>::value || CW > 16 ? 4 : 8)
 template <class T, class A, int L>
 __global__ void __launch_bounds__(kNT, IsF64<A>::value ? 2 : 4)
     grad_kernel(const T* __restrict__ x, int64_t ld, T* __restrict__ out, int64_t ld_out, GradArgs<A> a) {
-    constexpr int V = 16 / sizeof(T), U = 4;
+    constexpr int V = 16 / sizeof(T), U = 4, S = L < 32 ? L : 32;
     __shared__ A own[kNT / L][kTop + 1];
     __shared__ int at[kNT / L][kTop + 1];
     const int lane = threadIdx.x % L, group = threadIdx.x / L;
-    const int64_t t = a.n - 1 - ((int64_t)blockIdx.x * (kNT / L) + group);
-    if (t < 0) return;  // the whole group
+    // from the last row to the first: the forward left the last ones in L2
+    const int64_t back = (int64_t)blockIdx.x * (kNT / L) + group;
+    if (L >= 32 && back >= a.n) return;  // the whole group
+    const bool in = back < a.n;
+    const int64_t t = in ? a.n - 1 - back : 0;
     const T* row = x + t * ld;
     T* to = out + t * ld_out;
-    const RowShape<T> sh(row, (int)a.c);
+    const RowShape<T> sh(row, in ? (int)a.c : 0);
     const bool whole = alike(row, to);
     const int y = a.labels.p ? a.labels.in(t, a.c) : 0;
     const A l = a.lse[t], g_lp = a.g_lp ? a.g_lp[t] : A(0);
     A gh = a.g_entropy ? a.g_entropy[t] : A(0), h = a.g_entropy ? a.entropy[t] : A(0);
-    const bool dead = y < 0 || l == minus_inf<A>();
+    const bool dead = !in || y < 0 || l == minus_inf<A>();
     const int top = dead ? 0 : a.top, named = dead ? 0 : a.top + (a.g_lp ? 1 : 0);
-    // places are at most 33, threads at least 32
-    A sum = A(0);
-    if (top) {
+    A sum = top || dead ? A(0) : g_lp;
+    if (a.top) {
         for (int j = lane; j < named; j += L) {
             const int64_t i = j < top ? a.id(t * top + j) : (int64_t)y;
-            const bool in = i >= 0 && i < a.c;
-            at[group][j] = in ? (int)i : -1;
-            own[group][j] = in ? (j < top ? a.g_top[t * top + j] : g_lp) : A(0);
+            const bool is = i >= 0 && i < a.c;
+            at[group][j] = is ? (int)i : -1;
+            own[group][j] = is ? (j < top ? a.g_top[t * top + j] : g_lp) : A(0);
         }
         group_sync<L>();
-        const int w = threadIdx.x & 31;
-        sum = w < named ? own[group][w] : A(0);
-        if (w == 0 && named > 32) sum += own[group][32];
+        if (top) {
+            sum = A(0);
+            for (int j = threadIdx.x % S; j < named; j += S) sum += own[group][j];
+        }
+        __syncwarp();
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    } else if (!dead) {
-        sum = g_lp;
+        for (int o = S / 2; o > 0; o >>= 1) {
+            const A other = __shfl_xor_sync(0xffffffffu, sum, o);
+            if (top) sum += other;
+        }
     }
     if (dead) gh = A(0);
     const bool none = sum == A(0) && gh == A(0);
     const Slope<A> slope{l, gh == A(0) ? sum : sum + gh * h, gh};
-    if (lane < sh.edges) {
-        const int j = sh.edge(lane);
+    for (int i = lane; i < sh.edges; i += L) {
+        const int j = sh.edge(i);
         to[j] = narrow<T>(none ? A(0) : slope.of(widen<A>(row[j])));
     }
     for (int j0 = lane; j0 < sh.nv; j0 += L * U) {
@@ -1170,8 +1205,8 @@ __global__ void __launch_bounds__(kNT, IsF64<A>::value ? 2 : 4)
                 store16<T, A>(to + sh.head + (int64_t)(j0 + u * L) * V, p, whole);
             }
     }
-    if (named == 0) return;
     group_sync<L>();  // the places' values come after all others
+    if (named == 0) return;
     if (top == 0) {
         if (lane == 0) to[y] = narrow<T>(g_lp + (none ? A(0) : slope.of(widen<A>(row[y]))));
         return;
@@ -1303,10 +1338,17 @@ void grad_launch(int device, const T* x, int64_t ld, T* out, int64_t ld_out, con
         constexpr int L = decltype(l)::value;
         grad_kernel<T, A, L><<<(unsigned)ceil_div(a.n, kNT / L), kNT, 0, s>>>(x, ld, out, ld_out, a);
     };
-    if (a.c / Pack<T>::N >= 1024)
-        go(std::integral_constant<int, kNT>{});
-    else
+    const int64_t nv = a.c / Pack<T>::N;
+    // 8, 16, 32, 64 lanes a row, with five best classes: 400000 x 100 bf16 102, 180, 365, 686 us,
+    // 200000 x 1003 158, 174, 248, 407, 100000 x 2000 154, 145, 165, 218
+    if (nv <= 160)
+        go(std::integral_constant<int, 8>{});
+    else if (nv <= 512)
+        go(std::integral_constant<int, 16>{});
+    else if (nv < 1024)
         go(std::integral_constant<int, 32>{});
+    else
+        go(std::integral_constant<int, kNT>{});
 }
 
 }  // namespace

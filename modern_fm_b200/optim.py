@@ -134,6 +134,8 @@ class AdamW:
             (t["n_rows"] - 1) * t["ld"] + t["d"])) for t, p in zip(table, self.params) if p.numel())
         if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
             raise ValueError("parameters must not overlap")
+        self._some_by_rows, self._codes = any(rows), table["dtype"].copy()
+        self._table_at = table.ctypes.data
         self.state = self._states(size, master_size, n_steps, state, master)
         self._lay_out(master)
         new = self.params[0].new_zeros
@@ -222,24 +224,28 @@ class AdamW:
     def _gradients(self, grads):
         """Writes the gradients' addresses into the table; the tensors to be held."""
         table = self._table
-        if True not in self._by_rows and None not in map(type, grads) and all(
-                isinstance(g, torch.Tensor) for g in grads):
-            # every tensor has one: a few passes over the list instead of a loop's body
-            kinds = list(map(attrgetter("dtype"), grads))
-            if list(map(attrgetter("shape"), grads)) != self._shapes:
-                raise ValueError("every gradient must have its parameter's shape")
-            if not all(map(torch.Tensor.is_contiguous, grads)):
-                raise ValueError("gradients must be contiguous")
-            if set(map(torch.Tensor.get_device, grads)) != {self._device}:
-                raise ValueError("every gradient must be a CUDA tensor on the parameters' device")
-            if kinds != self._kinds:
-                for i, (k, p) in enumerate(zip(kinds, self._kinds)):
-                    self._check_kind(i, k, p)
-                table["grad_dtype"] = [_STORAGE[k] for k in kinds]
-            else:
-                table["grad_dtype"] = table["dtype"]
-            table["grad"] = list(map(torch.Tensor.data_ptr, grads))
-            return grads
+        if not self._some_by_rows:
+            # every one a tensor: a few passes over the list instead of a loop's body
+            try:
+                at = list(map(torch.Tensor.data_ptr, grads))
+            except TypeError:
+                at = None
+            if at is not None:
+                if list(map(attrgetter("shape"), grads)) != self._shapes:
+                    raise ValueError("every gradient must have its parameter's shape")
+                if not all(map(torch.Tensor.is_contiguous, grads)):
+                    raise ValueError("gradients must be contiguous")
+                if set(map(torch.Tensor.get_device, grads)) != {self._device}:
+                    raise ValueError("every gradient must be a CUDA tensor on the parameters' device")
+                kinds = list(map(attrgetter("dtype"), grads))
+                if kinds != self._kinds:
+                    for i, (k, p) in enumerate(zip(kinds, self._kinds)):
+                        self._check_kind(i, k, p)
+                    table["grad_dtype"] = [_STORAGE[k] for k in kinds]
+                else:
+                    table["grad_dtype"] = self._codes
+                table["grad"] = at
+                return grads
         held = []
         for i, g in enumerate(grads):
             t = table[i]
@@ -277,7 +283,7 @@ class AdamW:
             self._check_kind(i, g.dtype, self._kinds[i])
             t["grad"], t["grad_dtype"] = g.data_ptr(), _STORAGE[g.dtype]
             held.append(g)
-        if any(h.get_device() != self._device or not h.is_cuda for h in held):
+        if any(h.get_device() != self._device for h in held):
             raise ValueError("every gradient must be a CUDA tensor on the parameters' device")
         return held
 
@@ -318,6 +324,6 @@ class AdamW:
             with ctx:
                 norm = self._work.new_empty((), dtype=self._wide)
         _fail(_lib.lib().mfm_adamw_step_device(
-            self._device, self._table.ctypes.data, len(self.params), ct.byref(h),
+            self._device, self._table_at, len(self.params), ct.byref(h),
             self.state.step.data_ptr(), _ptr(norm), self._work.data_ptr(), self._work.numel(), s))
         return norm
