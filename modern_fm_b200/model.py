@@ -182,6 +182,18 @@ class DeviceModel:
         return label_logprobs(self.scores_device(indptr, indices, data, stream), labels, bounds,
                               stream)
 
+    def label_alternatives_device(self, indptr, indices, data, labels=None, top: int = 0,
+                                  stream=None):
+        """What this model's class scores say of each row (``preference.label_alternatives`` of
+        ``scores_device``): its label's log-probability and rank, the entropy, and the ``top``
+        best classes with their log-probabilities."""
+        from .preference import label_alternatives
+
+        if self.n_classes < 2:
+            raise ValueError("label alternatives need a model with n_classes >= 2")
+        return label_alternatives(self.scores_device(indptr, indices, data, stream), labels, top,
+                                  stream)
+
     def close(self):
         if getattr(self, "_h", None):
             _lib.lib().mfm_model_free(self._h)

@@ -1,13 +1,14 @@
-"""Losses of class scores by the log-probabilities of their labels
-(mfm_label_logprobs_*, mfm_preference_loss_device, mfm_policy_loss_device in the
-C ABI).
+"""Losses of class scores by the log-probabilities of their labels, and what else a row
+of scores says (mfm_label_logprobs_*, mfm_preference_loss_device,
+mfm_policy_loss_device, mfm_label_alternatives_* in the C ABI).
 
 The softmax models' class scores (``DeviceModel.predict_device`` with n_classes
 >= 2, or any (n_tokens, n_classes) matrix) are a policy over the classes. These
 calls give the log-probability of each row's label, the paired preference loss
-over sequences of rows against a reference, and the clipped policy loss with a
-KL term, each with the gradient of the scores; the engine's own losses
-(logistic, squared, softmax) exist inside ``fit`` and in ``evaluate``.
+over sequences of rows against a reference, the clipped policy loss with a KL
+term, and the label's rank, the entropy and the best classes, each with the
+gradient of the scores; the engine's own losses (logistic, squared, softmax) exist
+inside ``fit`` and in ``evaluate``.
 
 All calls take CUDA tensors on one device, run on ``stream`` (a
 torch.cuda.Stream, default the current one of that device) and neither

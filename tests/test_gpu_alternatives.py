@@ -347,3 +347,19 @@ def test_streams_and_graphs(n, c):
         graph.replay()
     for graph, out in graphs:
         assert all(torch.equal(a, b) for a, b in zip(want, out))
+
+
+@pytest.mark.parametrize("dtype", ["float32-float64", "float64", "float32"])
+def test_resident_model(dtype):
+    """The alternatives of a resident model's own scores."""
+    from test_gpu_model_policy import _case, _csr, _model
+
+    X, w0, w, V, R, fid, rng = _case(3, "fm", 7)
+    labels = torch.from_numpy(rng.integers(-1, 7, size=X.shape[0])).cuda()
+    with _model("fm", 7, dtype, X, w0, w, V, R, fid) as m:
+        csr = _csr(X, dtype)
+        _check(m.scores_device(*csr), labels, 4, m.label_alternatives_device(*csr, labels, top=4))
+        _check(m.scores_device(*csr), None, 0, m.label_alternatives_device(*csr))
+    X, w0, w, V, R, fid, rng = _case(3, "fm", 1)
+    with _model("fm", 1, dtype, X, w0, w, V, R, fid) as m, pytest.raises(ValueError, match="n_classes >= 2"):
+        m.label_alternatives_device(*_csr(X, dtype))
