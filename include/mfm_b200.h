@@ -632,7 +632,8 @@ typedef struct {
 
 /* One step; *step goes up by one. With max_norm >= 0 the norm |grad_scale| sqrt(sum of
  * squares of all gradients) goes to norm (float64 if any tensor is F64, else float32);
- * where it is not finite nothing else is written. workspace: 256-byte aligned,
+ * where it is not finite (float64: or beyond 1e154, whose squares are not) nothing else
+ * is written. workspace: 256-byte aligned,
  * mfm_adamw_workspace_bytes() bytes, zero before the first step, kept from step to step;
  * two steps that may run at the same time need two. */
 int64_t mfm_adamw_workspace_bytes(void);

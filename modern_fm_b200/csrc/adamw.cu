@@ -6,11 +6,12 @@
 // with s = grad_scale min(1, max_norm / norm). t is the device's own count, so that a
 // captured step goes on; a table's rows have one each (the engine's lazy Adam).
 //
-// One pass over p, g, m, v: bound by HBM (28 bytes a value with float32 everything, 10
-// with 16-bit values and 8-bit moments). All tensors of one kind of types are one
-// launch: their descriptions travel in the kernel's parameters, and persistent blocks
-// walk chunks of kChunk values across them. A norm is one launch more, whose last block
-// leaves the factor s.
+// One pass over p, g, m, v: bound by HBM (28 bytes a value with float32 everything: 332 M values
+// 1.49 ms, 6.2 TB/s), but for 8-bit moments (10 bytes a value of 16 bits): those are bound by the
+// integer pipe, which decodes and encodes (184 M values 444 us, 4.2 TB/s; 68 instructions a
+// value, half of them its). All tensors of one kind of types are one launch: their
+// descriptions travel in the kernel's parameters, and persistent blocks walk chunks across
+// them. A norm is one launch more, whose last block leaves the factor s.
 #include "vecio.cuh"
 
 #include <algorithm>
@@ -33,7 +34,7 @@ constexpr unsigned kNormBlocks = 1024;      // the most, each with its sum in th
 // m has a sign and 7 bits (15 octaves), v 8 bits (31 octaves: it holds squares). Scales
 // are powers of two, so a value that stays is encoded as itself whatever its block's
 // largest does.
-constexpr unsigned kHalfStep = (1u << 19) + 64;  // see m_code
+constexpr unsigned kHalfStep = (1u << 19) + 64;  // what `code` adds to m, of which it says why
 template <bool SIGNED>
 struct Code {
     static constexpr unsigned kMost = SIGNED ? 127 : 255, kReach = SIGNED ? 15 : 31;
@@ -150,22 +151,14 @@ __device__ __forceinline__ bool last_block(unsigned* done) {
 }
 
 // Squares are added in 32 bits over a thread's values of a chunk, and in 64 bits from
-// there; values whose squares leave the 32-bit range are squared in 64.
-template <class G>
-__device__ __forceinline__ double square_sum(const G* g, int64_t n, int64_t base) {
-    using A = typename Arith<G>::type;
-    A v[kPer], s = A(0), big = A(0);
+// there; values whose squares leave the 32-bit range are squared in 64. `bits`: not 0 where
+// any value is not.
+template <class A>
+__device__ __forceinline__ double square_sum(const A (&v)[kPer], unsigned bits) {
+    A s = A(0);
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) {
-        const int64_t e = base + j * kNT;
-        v[j] = e < n ? widen<A>(g[e]) : A(0);
-    }
-#pragma unroll
-    for (int j = 0; j < kPer; ++j) {
-        s += v[j] * v[j];
-        big = fmax(big, fabs(v[j]));
-    }
-    if (!IsF64<A>::value && (!(s < A(1e37)) || (s < A(1e-25) && big > A(0)))) {
+    for (int j = 0; j < kPer; ++j) s += v[j] * v[j];
+    if (!IsF64<A>::value && (!(s < A(1e37)) || (s < A(1e-25) && bits != 0))) {
         double w = 0.0;
 #pragma unroll
         for (int j = 0; j < kPer; ++j) w += (double)v[j] * (double)v[j];
@@ -173,11 +166,55 @@ __device__ __forceinline__ double square_sum(const G* g, int64_t n, int64_t base
     }
     return (double)s;
 }
+// A thread's share of the values [base, n) of a chunk of R kChunk: R times eight neighbouring ones,
+// all on their way at once, where the array begins at a vector and the chunk is whole; else every
+// kNT-th.
+template <class G, int R>
+__device__ __forceinline__ double square_sum(const G* g, int64_t n, int64_t base) {
+    using A = typename Arith<G>::type;
+    constexpr int V = Pack<G>::N, W = kPer / V;
+    double sum = 0.0;
+    if ((uintptr_t)g % 16 == 0 && base + R * kChunk <= n) {
+        uint4 r[R][W];
+#pragma unroll
+        for (int i = 0; i < R; ++i)
+#pragma unroll
+            for (int q = 0; q < W; ++q) r[i][q] = *reinterpret_cast<const uint4*>(g + base + i * kChunk + threadIdx.x * kPer + q * V);
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            A v[kPer];
+            unsigned bits = 0;
+#pragma unroll
+            for (int q = 0; q < W; ++q) {
+                A p[V];
+                Pack<G>::unpack(r[i][q], p);
+                bits |= r[i][q].x | r[i][q].y | r[i][q].z | r[i][q].w;
+#pragma unroll
+                for (int c = 0; c < V; ++c) v[q * V + c] = p[c];
+            }
+            sum += square_sum(v, bits);
+        }
+        return sum;
+    }
+    for (int64_t b = base; b < n && b < base + R * kChunk; b += kChunk) {
+        A v[kPer];
+        unsigned bits = 0;
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) {
+            const int64_t e = b + threadIdx.x + j * kNT;
+            v[j] = e < n ? widen<A>(g[e]) : A(0);
+            bits |= v[j] != A(0);
+        }
+        sum += square_sum(v, bits);
+    }
+    return sum;
+}
 
-// Sums of squares by block; the last block of the last launch (`finish`) adds them, in
+// Sums of squares by block, R chunks at a time where there are many, bound by HBM (184 M float32
+// values 110 us, 6.7 TB/s; bfloat16 60 us, 97 with R = 1); the last block of the last launch (`finish`) adds them, in
 // block order, to the norm and the gradients' factor. A norm that is not finite leaves
 // NaN there, and the step does nothing.
-template <int N>
+template <int N, int R>
 __global__ void __launch_bounds__(kNT)
     norm_kernel(const __grid_constant__ Summands<N> list, int n_of, int64_t chunks, Work* work,
                 int part_at, bool finish, const __grid_constant__ Hyper h, int norm64, void* norm) {
@@ -193,16 +230,16 @@ __global__ void __launch_bounds__(kNT)
             const int64_t used = *s.count;
             n = (used < 0 ? 0 : used > n ? n : used) * s.d;
         }
-        const int64_t base = (c - s.first) * kChunk + threadIdx.x;
+        const int64_t base = (c - s.first) * (R * kChunk);
         if (base >= n) continue;
         if (s.dtype == MFM_DTYPE_F64)
-            a += square_sum((const double*)s.p, n, base);
+            a += square_sum<double, R>((const double*)s.p, n, base);
         else if (s.dtype == MFM_DTYPE_F32)
-            a += square_sum((const float*)s.p, n, base);
+            a += square_sum<float, R>((const float*)s.p, n, base);
         else if (s.dtype == MFM_DTYPE_BF16)
-            a += square_sum((const __nv_bfloat16*)s.p, n, base);
+            a += square_sum<__nv_bfloat16, R>((const __nv_bfloat16*)s.p, n, base);
         else
-            a += square_sum((const __half*)s.p, n, base);
+            a += square_sum<__half, R>((const __half*)s.p, n, base);
     }
     a = block_sum(a, sm);
     if (threadIdx.x == 0) work->part[part_at + blockIdx.x] = a;
@@ -639,7 +676,10 @@ __device__ __forceinline__ int64_t row_of(const Table& s, int64_t slot, int64_t 
     return r < s.n_rows && r > before && r >= 0 ? r : -1;
 }
 
-// L lanes a row, a value a lane or (EIGHTS) eight neighbouring ones. A key outside the table, or not above the one before it, is left out.
+// L lanes a row, a value a lane or (EIGHTS) eight neighbouring ones: gathers of a few sectors a
+// row and array, bound by their latency where a batch touches few rows (55000 x 16 float32: 7.5 us
+// of kernel against 3.9 us of bytes; 14500 x 1024 bfloat16 48 us with 8-bit moments against
+// 27.5, 63 us with float32 ones against 54.5).
 template <class P, class G, bool MASTER, int BITS, class K, bool EIGHTS, int L>
 __global__ void __launch_bounds__(kNT, EIGHTS ? 3 : 4)
     adamw_rows_kernel(const __grid_constant__ Table s, Work* work, bool clipped, bool count,
@@ -878,8 +918,10 @@ extern "C" int mfm_adamw_step_device(int device, const mfm_adamw_tensor* tensors
             int part = 0;
             for (size_t l = 0; l < launches; ++l) {
                 const size_t lo = l * kNormMany, hi = std::min(all.size(), lo + kNormMany);
-                auto go = [&](auto most) {
-                    constexpr int N = decltype(most)::value;
+                int64_t values = 0;
+                for (size_t q = lo; q < hi; ++q) values += (tensors[all[q]].keys ? tensors[all[q]].n_keys : 1) * tensors[all[q]].d;
+                auto go = [&](auto most, auto rounds) {
+                    constexpr int N = decltype(most)::value, R = decltype(rounds)::value;
                     static thread_local Summands<N> list;
                     int64_t chunks = 0;
                     for (size_t q = lo; q < hi; ++q) {
@@ -887,16 +929,22 @@ extern "C" int mfm_adamw_step_device(int device, const mfm_adamw_tensor* tensors
                         const int64_t rows = t.keys ? t.n_keys : 1;
                         list.of[q - lo] = Summand{t.grad, t.keys ? t.n_keys : t.d, t.keys ? t.count : nullptr,
                                                   chunk(chunks), t.keys ? (int)t.d : 1, t.grad_dtype};
-                        chunks += ceil_div(rows * t.d, kChunk);
+                        chunks += ceil_div(rows * t.d, R * kChunk);
                     }
                     const unsigned grid = (unsigned)std::max<int64_t>(1, std::min<int64_t>({chunks, (int64_t)share, (int64_t)sm_count(device) * 6}));
-                    launch(norm_kernel<N>, grid, list, (int)(hi - lo), chunks, work, part, l + 1 == launches, h, wide ? 1 : 0, norm);
+                    launch(norm_kernel<N, R>, grid, list, (int)(hi - lo), chunks, work, part, l + 1 == launches, h, wide ? 1 : 0, norm);
                     part += (int)grid;
                 };
-                if (hi - lo <= kNormFew)
-                    go(std::integral_constant<int, kNormFew>{});
+                auto size = [&](auto rounds) {
+                    if (hi - lo <= kNormFew)
+                        go(std::integral_constant<int, kNormFew>{}, rounds);
+                    else
+                        go(std::integral_constant<int, kNormMany>{}, rounds);
+                };
+                if (values >= 4 * 6 * kChunk * sm_count(device))
+                    size(std::integral_constant<int, 4>{});
                 else
-                    go(std::integral_constant<int, kNormMany>{});
+                    size(std::integral_constant<int, 1>{});
             }
         }
         // dense tensors: as many of one kind as a launch carries

@@ -10,7 +10,9 @@ All tensors are CUDA tensors on one device. A step runs on ``stream`` (a
 torch.cuda.Stream, default the current one of that device) and neither synchronises
 nor copies to the host, and the step count lives on the device, so a step can be
 captured into a CUDA graph. Parameters are written in place, without a trace in
-torch's autograd. Every sum has a fixed order: results are bitwise reproducible.
+torch's autograd. Every sum has a fixed order: results are bitwise reproducible. An
+``AdamW`` and its state are made on the current stream, and stepped by one thread and
+on one stream at a time.
 """
 
 from __future__ import annotations
@@ -302,8 +304,9 @@ class AdamW:
 
         Every gradient is multiplied by ``grad_scale`` and, with ``max_norm``, by
         ``min(1, max_norm / norm)``, norm being that of all scaled gradients together; it is
-        returned (0-dim, in the arithmetic type). A norm that is not finite leaves parameters,
-        state and step count as they were. Without ``max_norm`` returns None.
+        returned (0-dim, in the arithmetic type). A norm that is not finite (or a float64 one
+        beyond 1e154, whose squares are not) leaves parameters, state and step count as they
+        were. Without ``max_norm`` returns None.
         """
         grads = list(grads)
         if len(grads) != len(self.params):

@@ -245,6 +245,27 @@ def test_moments_in_8_bits(kind, grad, off, master):
                 assert bool((fits | small).all())
 
 
+@pytest.mark.parametrize("kind,master", [("bf16", False), ("f32", False), ("f16", True)])
+def test_large_tensors_in_8_bits(kind, master):
+    """More than a block's share of chunks, in several tensors that end anywhere: parameters to
+    their bounds, moments to a step of their codes and 2^-14 of their block's largest."""
+    sizes = [17_000_003, 40, 9_000_031, 1 << 20]
+    ps = _tensors(sizes, kind, 13)
+    opt = AdamW(ps, lr=1e-3, weight_decay=0.1, state_bits=8, master=master)
+    for t in (1, 2):
+        gs = [torch.randn_like(p) * 0.02 for p in ps]
+        before = _now(opt, t)
+        opt.step(gs)
+        _check(opt, before, gs, 1e-3, [0.1] * 4)
+        m, v = opt.moments()
+        for i, n in enumerate(sizes):
+            want, _ = _want(before[i][0], gs[i].double(), before[i][1], before[i][2], t, 1e-3, 0.1, 1e-8)
+            for flat, x in ((m, want[1]), (v, want[2])):
+                whole = torch.nn.functional.pad(x.abs(), (0, -n % 32)).view(-1, 32).amax(1).repeat_interleave(32)[:n]
+                assert bool(((opt.view(flat, i).double() - x).abs() <= x.abs() / 8 + 2.0**-14 * whole).all())
+        del before, m, v
+
+
 def test_rounding_of_v_keeps_its_average():
     """A thousand steps' worth of values, each moved by less than half a step of its code: their
     mean moves as v does. v's values after one step lie on two codes a step h apart, up with
