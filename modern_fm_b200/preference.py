@@ -160,24 +160,25 @@ def label_alternatives(logits, labels=None, top: int = 0, stream=None) -> LabelA
     dev = _one_device(logits, labels)
     s, ctx = _on(stream, dev)
     _hold(stream, logits, labels)
-    some = 0 if labels is None else n
-    with ctx:  # one allocation for each type
+    some, kind = (0, torch.int64) if labels is None else (n, labels.dtype)
+    lps = ranks = ids = None
+    with ctx:
         values = logits.new_empty(some + n * (2 + top), dtype=wide)
-        ids = logits.new_empty(some + n * top, dtype=torch.int64 if l64 else torch.int32)
-    at, size, ids_at = values.data_ptr(), values.element_size(), ids.data_ptr()
-    own = None if labels is None else at
-    rank_at = None if labels is None else ids_at
+        if labels is not None:
+            ranks = torch.empty_like(labels)
+        if top:
+            ids = logits.new_empty((n, top), dtype=kind)
+    at, size = values.data_ptr(), values.element_size()
     _fail(_lib.lib().mfm_label_alternatives_device(
-        code, dev, p, ld, n, c, l64, _ptr(labels), top, own, at + size * some,
-        at + size * (some + n), rank_at, ids_at + (8 if l64 else 4) * some if top else None,
-        at + size * (some + 2 * n) if top else None, s))
-    lp, lse, entropy, lps = values.split_with_sizes((some, n, n, n * top))
-    ranks, ids = ids.split_with_sizes((some, n * top))
-    if labels is None:
-        lp = ranks = None
-    if not top:
-        return LabelAlternatives(lp, lse, entropy, ranks, None, None)
-    return LabelAlternatives(lp, lse, entropy, ranks, ids.view(n, top), lps.view(n, top))
+        code, dev, p, ld, n, c, l64, _ptr(labels), top, at if some else None, at + size * some,
+        at + size * (some + n), _ptr(ranks), _ptr(ids), at + size * (some + 2 * n) if top else None,
+        s))
+    if top:
+        lp, lse, entropy, lps = values.split_with_sizes((some, n, n, n * top))
+        lps = lps.view(n, top)
+    else:
+        lp, lse, entropy = values.split_with_sizes((some, n, n))
+    return LabelAlternatives(None if labels is None else lp, lse, entropy, ranks, ids, lps)
 
 
 def label_alternatives_grad(logits, lse, entropy=None, labels=None, grad_logprobs=None,
