@@ -475,26 +475,68 @@ struct Key<double> {
         return r;
     }
 };
-// How many of n keys come before `me`.
-template <class A>
-__device__ __forceinline__ int place_of(const Key<A>* keys, int n, const Key<A>& me) {
+// The same of a 16-bit value of a row of at most 2^16, in half the bits.
+template <class T>
+struct ShortKey {
+    unsigned k;
+    ShortKey() = default;
+    __device__ __forceinline__ ShortKey(float v, int i) {
+        const T t = narrow<T>(v + 0.0f);  // -0 is 0; exact
+        const unsigned b = *reinterpret_cast<const unsigned short*>(&t);
+        k = (b & 0x8000u ? ~b << 16 : (b | 0x8000u) << 16) | (0xffffu - (unsigned)i);
+    }
+    static __device__ __forceinline__ ShortKey none() {
+        ShortKey r;
+        r.k = 0;
+        return r;
+    }
+    __device__ __forceinline__ bool before(const ShortKey& o) const { return k > o.k; }
+    __device__ __forceinline__ float value() const {
+        const unsigned h = k >> 16;
+        const unsigned short b = (unsigned short)(h & 0x8000u ? h & 0x7fffu : ~h);
+        return widen<float>(*reinterpret_cast<const T*>(&b));
+    }
+    __device__ __forceinline__ int index() const { return (int)(0xffffu - (k & 0xffffu)); }
+    __device__ __forceinline__ ShortKey across(int lanes) const {
+        ShortKey r;
+        r.k = __shfl_xor_sync(0xffffffffu, k, lanes);
+        return r;
+    }
+};
+
+// How many of the keys of a list come before `me`: `n` of them, and up to kPad that are none behind
+// them, so that whole vectors can be read.
+constexpr int kPad = 4;
+template <class KT>
+__device__ __forceinline__ int place_of(const KT* keys, int n, const KT& me) {
     int place = 0;
-#pragma unroll 4
-    for (int o = 0; o < n; ++o) place += keys[o].before(me) ? 1 : 0;
+    if constexpr (sizeof(KT) == 4) {
+        for (int o = 0; o < n; o += 4) {
+            const uint4 k = *reinterpret_cast<const uint4*>(keys + o);
+            place += (k.x > me.k ? 1 : 0) + (k.y > me.k ? 1 : 0) + (k.z > me.k ? 1 : 0) + (k.w > me.k ? 1 : 0);
+        }
+    } else if constexpr (sizeof(KT) == 8) {
+        for (int o = 0; o < n; o += 4) {
+            const ulonglong2 a = *reinterpret_cast<const ulonglong2*>(keys + o), b = *reinterpret_cast<const ulonglong2*>(keys + o + 2);
+            place += (a.x > me.k ? 1 : 0) + (a.y > me.k ? 1 : 0) + (b.x > me.k ? 1 : 0) + (b.y > me.k ? 1 : 0);
+        }
+    } else {
+        for (int o = 0; o < n; ++o) place += keys[o].before(me) ? 1 : 0;
+    }
     return place;
 }
 
 constexpr int kSegments = 16;  // of a thread's vectors, each with its largest value
 
 // What a group shares.
-template <class A, int CAP>
+template <class KT, int CAP>
 struct Lists {
+    alignas(16) KT cand[CAP + kPad];
+    KT best[kTop];  // the answer
     int count, listed;
-    Key<A> best[kTop];  // the answer
-    Key<A> cand[CAP];
 };
 template <class A, int L>
-struct Shared : Lists<A, kCand> {
+struct Shared : Lists<Key<A>, kCand> {
     A m[L / 32], s[L / 32], d[L / 32];
     A one[L / 32], every[L / 32];
     int rank[L / 32];
@@ -558,6 +600,20 @@ __device__ __forceinline__ A reached_in_group(A v, int a) {
     return at;
 }
 
+// What k of a warp's 64 values reach, two a lane: the k-th largest, which is the least of the
+// larger ones of the i-th of the one half and the (k - 1 - i)-th of the other.
+template <class A>
+__device__ __forceinline__ A reached_of_two(A a, A b, int k) {
+    const int lane = threadIdx.x & 31;
+    a = sorted_lanes(a);
+    b = sorted_lanes(b);
+    const A other = __shfl_sync(0xffffffffu, b, k - 1 - lane & 31);
+    A least = lane < k ? fmax(a, other) : (A)INFINITY;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) least = fmin(least, __shfl_xor_sync(0xffffffffu, least, o));
+    return least;
+}
+
 // The k-th largest of a warp's values, N and one more a lane, by its bits from the highest on:
 // for rows of fewer vectors than the places that are asked for, where the lanes' largest say
 // nothing. BITS: the upper bits in which the values differ.
@@ -578,8 +634,8 @@ __device__ __forceinline__ float kth_of_warp(const float (&v)[N], float one, int
 }
 
 // The first `want` values of the row that equal v, in index order, by one warp.
-template <class T, class A>
-__device__ __noinline__ void first_equal(const T* row, int c, A v, int want, Key<A>* to) {
+template <class T, class A, class KT>
+__device__ __noinline__ void first_equal(const T* row, int c, A v, int want, KT* to) {
     const int lane = threadIdx.x & 31;
     int found = 0;
     for (int64_t j0 = 0; j0 < c && found < want; j0 += 32 * 8) {
@@ -600,7 +656,7 @@ __device__ __noinline__ void first_equal(const T* row, int c, A v, int want, Key
         before += found - mine;
         for (int q = 0; q < 8; ++q)
             if (bits >> q & 1) {
-                if (before < want) to[before] = Key<A>(v, (int)(j0 + lane * 8 + q));
+                if (before < want) to[before] = KT(v, (int)(j0 + lane * 8 + q));
                 ++before;
             }
         found += all;
@@ -609,19 +665,19 @@ __device__ __noinline__ void first_equal(const T* row, int c, A v, int want, Key
 
 // The first `top` values one at a time, each the first behind the one before, by a group: for
 // rows of which a few threads hold most of the large values.
-template <class T, class A, int L>
-__device__ __noinline__ void one_by_one(const T* row, int c, int top, Key<A>* parts, Key<A>* to) {
+template <class T, class A, int L, class KT>
+__device__ __noinline__ void one_by_one(const T* row, int c, int top, KT* parts, KT* to) {
     const int lane = threadIdx.x % L;
-    Key<A> last;
+    KT last;
     for (int place = 0; place < top; ++place) {
-        Key<A> best = Key<A>::none();
+        KT best = KT::none();
         for (int64_t j = lane; j < c; j += L) {
-            const Key<A> o(widen<A>(row[j]), (int)j);
+            const KT o(widen<A>(row[j]), (int)j);
             if ((place == 0 || last.before(o)) && o.before(best)) best = o;
         }
 #pragma unroll
         for (int s = 16; s > 0; s >>= 1) {
-            const Key<A> o = best.across(s);
+            const KT o = best.across(s);
             if (o.before(best)) best = o;
         }
         if (L > 32) {
@@ -636,11 +692,35 @@ __device__ __noinline__ void one_by_one(const T* row, int c, int top, Key<A>* pa
     }
 }
 
-// The places of a group's candidates among each other: the first `top` to g.best.
-template <class A, int L, int CAP>
-__device__ __forceinline__ void places(Lists<A, CAP>& g, int count, int top) {
-    for (int q = threadIdx.x % L; q < count; q += L) {
-        const Key<A> me = g.cand[q];
+// The places of a group's candidates among each other: the first `top` to g.best. A warp sorts
+// short keys that its lanes hold; others are counted against each other, n comparisons a key
+// (200000 x 1003 float16, 32 best of which 110 candidates: 1085 us with 64-bit keys, 795 with short).
+template <int L, class KT, int CAP>
+__device__ __forceinline__ void places(Lists<KT, CAP>& g, int count, int top) {
+    const int lane = threadIdx.x % L;
+    if constexpr (L == 32 && sizeof(KT) == 4) {
+        if (count <= 32) {
+            unsigned k = lane < count ? g.cand[lane].k : 0;
+            auto stage = [&](int size) {
+#pragma unroll
+                for (int j = size / 2; j > 0; j /= 2) {
+                    const unsigned o = __shfl_xor_sync(0xffffffffu, k, j);
+                    k = ((lane & j) == 0) == ((lane & size) == 0) ? max(k, o) : min(k, o);
+                }
+            };
+            stage(2);
+            stage(4);
+            stage(8);
+            if (count > 8) stage(16);
+            if (count > 16) stage(32);
+            if (lane < min(top, count)) g.best[lane].k = k;
+            return;
+        }
+    }
+    for (int j = lane; j < kPad; j += L) g.cand[count + j] = KT::none();
+    group_sync<L>();
+    for (int q = lane; q < count; q += L) {
+        const KT me = g.cand[q];
         const int place = place_of(g.cand, count, me);
         if (place < top) g.best[place] = me;
     }
@@ -649,12 +729,12 @@ __device__ __forceinline__ void places(Lists<A, CAP>& g, int count, int top) {
 // The first `top` of a row's c values in their order to g.best, by the group. `bound`: what at
 // least `top` of them reach. `walk(strict)` lists the values that reach it (strict: that are above it) as
 // candidates and says how many there are, or, where that is more than fit, that it is.
-template <class T, class A, int L, class W>
-__device__ __forceinline__ void choose(Lists<A, kCand>& g, const T* row, int c, int top, A bound, W&& walk) {
+template <class T, class A, int L, class KT, class W>
+__device__ __forceinline__ void choose(Lists<KT, kCand>& g, const T* row, int c, int top, A bound, W&& walk) {
     if (bound != minus_inf<A>()) {
         const int count = walk(std::false_type{});
         if (count <= kCand) {
-            places<A, L>(g, count, top);
+            places<L>(g, count, top);
             return;
         }
     }
@@ -662,7 +742,7 @@ __device__ __forceinline__ void choose(Lists<A, kCand>& g, const T* row, int c, 
     // of those that are equal.
     const int count = walk(std::true_type{});
     if (count <= kCand) {
-        places<A, L>(g, count, top);
+        places<L>(g, count, top);
         if (count < top && threadIdx.x % L < 32) first_equal(row, c, bound, top - count, g.best + count);
         return;
     }
@@ -702,8 +782,9 @@ __global__ void __launch_bounds__(kNT, IsF64<A>::value ? 2 : K > 4 ? 3 : 4)
     constexpr int V = 16 / sizeof(T), E = (2 * (V - 1) + L - 1) / L, CAP = held_cand<A, V, L, K>();
     static_assert(L == 32 || CAP < kCand, "groups within a warp hold every value as a candidate");
     static_assert(K * V <= 64, "a bit a value");
-    __shared__ Lists<A, CAP> shared[kNT / L];
-    Lists<A, CAP>& g = shared[threadIdx.x / L];
+    using KT = std::conditional_t<sizeof(T) == 2, ShortKey<T>, Key<A>>;
+    __shared__ Lists<KT, CAP> shared[kNT / L];
+    Lists<KT, CAP>& g = shared[threadIdx.x / L];
     const int lane = threadIdx.x % L, top = a.top;
     const int64_t t = (int64_t)blockIdx.x * (kNT / L) + threadIdx.x / L;
     const int y = t < a.n ? a.label(t) : -1;
@@ -767,6 +848,21 @@ __global__ void __launch_bounds__(kNT, IsF64<A>::value ? 2 : K > 4 ? 3 : 4)
         A p[V];
         Pack<T>::unpack(v[0], p);
         bound = top > sh.nv ? kth_of_warp<sizeof(T) == 4 ? 32 : 19>(p, widen<A>(last[0]), top) : reached_in_group<A, L>(mine, top);
+    } else if constexpr (L == 32 && K > 1) {
+        // With as many places as lanes the lanes' largest reach far down; two a lane reach half as
+        // far (200000 x 1003 float16, 32 best: 795 us by one, 331 by two; 16 best: 257 and 266).
+        if (top > 16) {
+            A first = minus_inf<A>(), second = minus_inf<A>();
+#pragma unroll
+            for (int i = 0; i < K; ++i)
+                if (i < K / 2)
+                    first = fmax(first, Pack<T>::top(v[i]));
+                else
+                    second = fmax(second, Pack<T>::top(v[i]));
+            bound = reached_of_two(first, fmax(second, widen<A>(last[0])), top);
+        } else {
+            bound = reached_in_group<A, L>(mine, top);
+        }
     } else {
         bound = reached_in_group<A, L>(mine, top);
     }
@@ -791,7 +887,7 @@ __global__ void __launch_bounds__(kNT, IsF64<A>::value ? 2 : K > 4 ? 3 : 4)
             const A e = widen<A>(last[i]);
             const bool hit = go && lane + i * L < sh.edges && (S ? e > bound : e >= bound);
             const unsigned hits = __ballot_sync(0xffffffffu, hit) & group;
-            if (hit) g.cand[count + __popc(hits & before_me)] = Key<A>(e, sh.edge(lane + i * L));
+            if (hit) g.cand[count + __popc(hits & before_me)] = KT(e, sh.edge(lane + i * L));
             count += __popc(hits);
         }
         for (;;) {
@@ -800,7 +896,7 @@ __global__ void __launch_bounds__(kNT, IsF64<A>::value ? 2 : K > 4 ? 3 : 4)
             if (hits >> (threadIdx.x & 31) & 1) {
                 const int q = __ffsll((long long)bits) - 1, i = sh.head + (lane + q / V * L) * V + q % V;
                 const int to = count + __popc(hits & before_me);
-                if (to < CAP) g.cand[to] = Key<A>(widen<A>(row[i]), i);
+                if (to < CAP) g.cand[to] = KT(widen<A>(row[i]), i);
                 bits &= bits - 1;
             }
             count += __popc(hits);
@@ -809,7 +905,7 @@ __global__ void __launch_bounds__(kNT, IsF64<A>::value ? 2 : K > 4 ? 3 : 4)
         return count;
     };
     if constexpr (CAP < kCand || L < 32)
-        places<A, L>(g, walk(std::false_type{}), top);  // every value fits
+        places<L>(g, walk(std::false_type{}), top);  // every value fits
     else
         choose<T, A, L>(g, row, (int)a.c, top, bound, walk);
     __syncwarp();
@@ -1012,7 +1108,7 @@ __global__ void __launch_bounds__(kNT, IsF64<A>::value ? 2 : 4)
                 group_sync<L>();
                 for (int q = lane; q < count; q += L) {
                     const Key<A> me = g.cand[q];
-                    const int place = place_of(g.cand, count, me);
+                    const int place = place_of(g.cand, count, me);  // eight times as many: whole vectors
                     if (place < top && !me.is_none()) {
                         a.id(a.top_ids, t * top + place, me.index());
                         a.top_lp[t * top + place] = (me.value() - off) - ls;
