@@ -44,8 +44,8 @@ extern "C" {
  * keeps float64 parameters for the whole fit in F32_F64, as the reference
  * does (python/modern_fm/_backend.py:116-130). */
 enum { MFM_DTYPE_F64 = 0, MFM_DTYPE_F32 = 1, MFM_DTYPE_F32_F64 = 2 };
-/* Storage types of the embedding and preference entry points only (float32
- * arithmetic, results rounded once); every other entry point rejects them. */
+/* Storage types of the embedding, class-score and AdamW entry points only
+ * (float32 arithmetic, results rounded once); every other one rejects them. */
 enum { MFM_DTYPE_BF16 = 3, MFM_DTYPE_F16 = 4 };
 enum { MFM_MODEL_FM = 0, MFM_MODEL_FFM = 1, MFM_MODEL_FWFM = 2 };
 enum { MFM_LOSS_LOGISTIC = 0, MFM_LOSS_SQUARED = 1 };

@@ -16,7 +16,7 @@ LIB_PATH = os.path.join(PKG, "libmfm_b200.so")
 MFM_OK = 0
 MFM_ERR_INVALID, MFM_ERR_UNSUPPORTED = -1, -2
 MFM_DTYPE_F64, MFM_DTYPE_F32, MFM_DTYPE_F32_F64 = 0, 1, 2
-MFM_DTYPE_BF16, MFM_DTYPE_F16 = 3, 4  # embedding and preference entry points only
+MFM_DTYPE_BF16, MFM_DTYPE_F16 = 3, 4  # embedding, class-score and AdamW calls only
 MFM_MODEL_FM, MFM_MODEL_FFM, MFM_MODEL_FWFM = 0, 1, 2
 DTYPES = {"float64": MFM_DTYPE_F64, "f64": MFM_DTYPE_F64, "float32": MFM_DTYPE_F32,
           "f32": MFM_DTYPE_F32, "float32-float64": MFM_DTYPE_F32_F64,

@@ -516,6 +516,33 @@ def test_on_another_stream():
     assert all(torch.equal(x, y) for x, y in zip((m, v), a.moments()))
 
 
+def test_two_on_two_streams():
+    """Steps of two optimizers in flight at once, and from two threads."""
+    import threading
+
+    pairs = [(_model("bf16", 8, True), _model("bf16", 8, True)), (_model("f32", 32, False), _model("f32", 32, False))]
+    streams = [torch.cuda.Stream() for _ in pairs]
+    grads = [[_grads(kind, t) for t in range(20)] for kind in ("bf16", "f32")]
+    torch.cuda.synchronize()
+    for (a, _), gs in zip(pairs, grads):
+        for g in gs:
+            a.step(g, max_norm=0.7)
+    torch.cuda.synchronize()
+
+    def run(opt, gs, stream):
+        for g in gs:
+            opt.step(g, max_norm=0.7, stream=stream)
+
+    threads = [threading.Thread(target=run, args=(b, gs, s)) for (_, b), gs, s in zip(pairs, grads, streams)]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    torch.cuda.synchronize()
+    for a, b in pairs:
+        assert all(torch.equal(x, y) for x, y in zip(_all(a), _all(b)))
+
+
 def test_empty_tensors():
     ps = [torch.zeros(0, device="cuda"), torch.ones(3, device="cuda"), torch.zeros(0, 5, device="cuda")]
     opt = AdamW(ps, by_rows=[False, False, True])

@@ -218,6 +218,23 @@ def test_best_classes_in_the_hands_of_few_threads(n, c, kind, offset):
             break
 
 
+@pytest.mark.parametrize("c", [520, 1000, 2040])
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("share", [4, 16])
+def test_best_classes_in_the_hands_of_few_lanes(c, kind, share):
+    """Rows that lanes hold in registers: 4 or 16 of 32 lanes have all large values, more than
+    are listed as candidates, or less; some of them equal."""
+    g = torch.Generator().manual_seed(c + share)
+    v = 128 // torch.finfo(TYPES[kind]).bits
+    big = (torch.arange(c) // v) % 32 < share
+    x = torch.where(big, 50.0 + torch.rand(20, c, generator=g) * 8, torch.randn(20, c, generator=g))
+    x[10:] = x[10:].round()
+    x = x.to(TYPES[kind]).cuda()
+    y = torch.randint(0, c, (20,), generator=g).cuda()
+    for top in (1, 7, 16, 17, 32):
+        _check(x, y, top)
+
+
 @pytest.mark.parametrize("c", [10, 32, 100, 1000, 5003, 50001])
 @pytest.mark.parametrize("kind", list(TYPES))
 def test_not_finite(c, kind):
