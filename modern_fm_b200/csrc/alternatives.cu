@@ -34,6 +34,7 @@ namespace {
 constexpr int kNT = 256;
 constexpr int kSmallC = 32;    // classes that a thread takes by itself
 constexpr int kSmallNT = 128;
+constexpr int kMany = 64;      // candidates that a few lanes rank
 constexpr int kTop = 32;       // the most classes that are listed
 constexpr int kCand = 288;     // candidates of a row: the vectors of kTop threads (256 values) and the row's edges
 
@@ -543,12 +544,12 @@ struct Shared : Lists<Key<A>, kCand> {
     A most[kSegments][L];  // of each of a thread's segments
 };
 
-// The 32 lanes' values in falling order.
-template <class A>
+// The values of each group of L lanes in falling order.
+template <class A, int L = 32>
 __device__ __forceinline__ A sorted_lanes(A v) {
-    const int lane = threadIdx.x & 31;
+    const int lane = threadIdx.x % L;
 #pragma unroll
-    for (int k = 2; k <= 32; k *= 2)
+    for (int k = 2; k <= L; k *= 2)
 #pragma unroll
         for (int j = k / 2; j > 0; j /= 2) {
             const A o = __shfl_xor_sync(0xffffffffu, v, j);
@@ -583,40 +584,63 @@ __device__ __forceinline__ void reached(double v, int a, int b, double& at_a, do
     at_a = __shfl_sync(0xffffffffu, v, a - 1);
     at_b = __shfl_sync(0xffffffffu, v, b - 1);
 }
-// The same of each group of L lanes, by maxima.
+// The same of each group of L lanes.
 template <class A, int L>
 __device__ __forceinline__ A reached_in_group(A v, int a) {
-    A at = minus_inf<A>();
-    if constexpr (L == 32) {
+    A at;
+    if constexpr (L == 32)
         reached(v, a, a, at, at);
-    } else {
-        for (int i = 0; i < a; ++i) {
-            at = v;
-#pragma unroll
-            for (int o = L / 2; o > 0; o >>= 1) at = fmax(at, __shfl_xor_sync(0xffffffffu, at, o));
-            if (v == at) v = minus_inf<A>();
-        }
-    }
+    else
+        at = __shfl_sync(0xffffffffu, sorted_lanes<A, L>(v), a - 1, L);
     return at;
 }
 
-// What k of a warp's 64 values reach, two a lane: the k-th largest, which is the least of the
-// larger ones of the i-th of the one half and the (k - 1 - i)-th of the other.
-template <class A>
+// What k <= kTop of a group's 2 L values reach, two a lane: the k-th largest, which is the least of
+// the larger ones of the i-th of the one half and the (k - 1 - i)-th of the other.
+template <class A, int L>
 __device__ __forceinline__ A reached_of_two(A a, A b, int k) {
-    const int lane = threadIdx.x & 31;
-    a = sorted_lanes(a);
-    b = sorted_lanes(b);
-    const A other = __shfl_sync(0xffffffffu, b, k - 1 - lane & 31);
-    A least = lane < k ? fmax(a, other) : (A)INFINITY;
+    const int lane = threadIdx.x % L, j = k - 1 - lane;
+    a = sorted_lanes<A, L>(a);
+    b = sorted_lanes<A, L>(b);
+    const A other = __shfl_sync(0xffffffffu, b, j & (L - 1), L);
+    A least = j < 0 ? (A)INFINITY : j < L ? fmax(a, other) : a;
+    if (L < 32) {
+        const A behind = __shfl_sync(0xffffffffu, b, (k - 1 - L) & (L - 1), L);  // beside none of the one half
+        if (k > L) least = fmin(least, behind);
+    }
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) least = fmin(least, __shfl_xor_sync(0xffffffffu, least, o));
+    for (int o = L / 2; o > 0; o >>= 1) least = fmin(least, __shfl_xor_sync(0xffffffffu, least, o));
     return least;
 }
 
+// The vectors of a row of c values of which it has at least so many, wherever it begins.
+template <int V>
+__host__ __device__ constexpr int fewest_vectors(int64_t c) {
+    return (int)(c - (V - 1)) / V;
+}
+
+// The least value of the type above v.
+template <class T>
+__device__ __forceinline__ float above(float v) {
+    if constexpr (sizeof(T) == 4) {
+        const int b = __float_as_int(v);
+        return v == 0.0f ? __int_as_float(1) : __int_as_float(b < 0 ? b - 1 : b + 1);
+    } else {
+        const T t = narrow<T>(v);
+        const unsigned short b = *reinterpret_cast<const unsigned short*>(&t);
+        const unsigned short up = v == 0.0f ? 1 : b & 0x8000 ? b - 1 : b + 1;
+        return widen<float>(*reinterpret_cast<const T*>(&up));
+    }
+}
+template <class T>
+__device__ __forceinline__ double above(double v) {
+    const long long b = __double_as_longlong(v);
+    return v == 0.0 ? __longlong_as_double(1) : __longlong_as_double(b < 0 ? b - 1 : b + 1);
+}
+
 // The k-th largest of a warp's values, N and one more a lane, by its bits from the highest on:
-// for rows of fewer vectors than the places that are asked for, where the lanes' largest say
-// nothing. BITS: the upper bits in which the values differ.
+// for rows of few vectors beside the places that are asked for, where the lanes' largest say
+// little. BITS: the upper bits in which the values differ.
 template <int BITS, int N>
 __device__ __forceinline__ float kth_of_warp(const float (&v)[N], float one, int k) {
     unsigned u = 0;
@@ -843,28 +867,42 @@ __global__ void __launch_bounds__(kNT, IsF64<A>::value ? 2 : K > 4 ? 3 : 4)
     if (in && !go)
         for (int j = lane; j < top; j += L) a.no_class(t, j, r.s != r.s ? r.s : A(0));
     if (top == 0 || (L == 32 ? !go : __all_sync(0xffffffffu, !go))) return;
-    A bound;
-    if constexpr (L == 32 && K == 1 && !IsF64<A>::value) {
-        A p[V];
-        Pack<T>::unpack(v[0], p);
-        bound = top > sh.nv ? kth_of_warp<sizeof(T) == 4 ? 32 : 19>(p, widen<A>(last[0]), top) : reached_in_group<A, L>(mine, top);
-    } else if constexpr (L == 32 && K > 1) {
-        // With as many places as lanes the lanes' largest reach far down; two a lane reach half as
-        // far (200000 x 1003 float16, 32 best: 795 us by one, 331 by two; 16 best: 257 and 266).
-        if (top > 16) {
-            A first = minus_inf<A>(), second = minus_inf<A>();
+    // Of the largest values of the lanes (up to half as many places as lanes), or of two a lane: with
+    // as many places as lanes one a lane reaches far down (200000 x 1003 float16, 32 best: 795 us by
+    // one, 331 by two; 16 best: 257 and 266). Where the row may have fewer than that, or hardly more,
+    // by bits in a warp (400000 x 128 bfloat16, 32 best: 650 us, by two a lane 850), and in fewer lanes not
+    // at all: its values are few enough to be listed. The warp's rows go one way, whose vectors may
+    // differ by one: `fewest` of them.
+    A bound = minus_inf<A>();
+    const int fewest = fewest_vectors<V>(a.c);
+    if (L == 32 && K > 1 ? top <= 16 : L < 32 && top <= L / 2 && top <= fewest) {
+        bound = reached_in_group<A, L>(mine, top);
+    } else if (L == 32 && K > 1 || top <= (L < 32 ? 2 * min(fewest, L) : fewest * 3 / 2)) {
+        A first = minus_inf<A>(), second = minus_inf<A>();
 #pragma unroll
-            for (int i = 0; i < K; ++i)
+        for (int i = 0; i < K; ++i) {
+            if constexpr (L == 32 && K > 1) {
                 if (i < K / 2)
                     first = fmax(first, Pack<T>::top(v[i]));
                 else
                     second = fmax(second, Pack<T>::top(v[i]));
-            bound = reached_of_two(first, fmax(second, widen<A>(last[0])), top);
-        } else {
-            bound = reached_in_group<A, L>(mine, top);
+            } else {
+                A p[V];
+                Pack<T>::unpack(v[i], p);
+#pragma unroll
+                for (int q = 0; q < V / 2; ++q) {
+                    first = fmax(first, p[q]);
+                    second = fmax(second, p[V / 2 + q]);
+                }
+            }
         }
-    } else {
-        bound = reached_in_group<A, L>(mine, top);
+#pragma unroll
+        for (int i = 0; i < E; ++i) second = fmax(second, widen<A>(last[i]));
+        bound = reached_of_two<A, L>(first, second, top);
+    } else if constexpr (L == 32 && K == 1 && !IsF64<A>::value) {
+        A p[V];
+        Pack<T>::unpack(v[0], p);
+        bound = kth_of_warp<sizeof(T) == 4 ? 32 : 19>(p, widen<A>(last[0]), top);
     }
     // A bit for each value that is listed; then they are taken one a lane at a time.
     auto walk = [&](auto strict) {
@@ -875,13 +913,7 @@ __global__ void __launch_bounds__(kNT, IsF64<A>::value ? 2 : K > 4 ? 3 : 4)
 #pragma unroll
         for (int i = 0; i < K; ++i) bits |= (uint64_t)Bits<T, S>::of(v[i], bound) << (i * V);
         int count = 0;
-        // the -infinity behind the row's end reaches a bound of -infinity
-        if (!go)
-            bits = 0;
-        else if (!S && bound == minus_inf<A>())
-#pragma unroll
-            for (int i = 0; i < K; ++i)
-                if (lane + i * L >= sh.nv) bits &= ~(((1ull << V) - 1) << (i * V));
+        if (!go) bits = 0;
 #pragma unroll
         for (int i = 0; i < E; ++i) {
             const A e = widen<A>(last[i]);
@@ -904,10 +936,31 @@ __global__ void __launch_bounds__(kNT, IsF64<A>::value ? 2 : K > 4 ? 3 : 4)
         __syncwarp();
         return count;
     };
-    if constexpr (CAP < kCand || L < 32)
-        places<L>(g, walk(std::false_type{}), top);  // every value fits
-    else
+    if constexpr (CAP < kCand) {
+        // Every value fits. Where many reach the bound (ties), and where it is -infinity, those
+        // above it are listed, and the first of its equals.
+        const A equal = bound;
+        bool over = bound == minus_inf<A>();
+        if (over) bound = above<T>(bound);
+        int count = walk(std::false_type{});
+        const bool many = !over && count > kMany;
+        if (__any_sync(0xffffffffu, many)) {
+            if (many) bound = above<T>(bound);
+            over |= many;
+            count = walk(std::false_type{});
+        }
+        places<L>(g, count, top);
+        const int more = go && over && count < top ? top - count : 0;
+        if (__any_sync(0xffffffffu, more > 0))
+            for (int o = 0; o < 32; o += L) {
+                const int want = __shfl_sync(0xffffffffu, more, o), from = __shfl_sync(0xffffffffu, count, o);
+                const A v = __shfl_sync(0xffffffffu, equal, o);
+                const int64_t of = __shfl_sync(0xffffffffu, t, o);
+                if (want > 0) first_equal(x + of * ld, (int)a.c, v, want, shared[threadIdx.x / 32 * (32 / L) + o / L].best + from);
+            }
+    } else {
         choose<T, A, L>(g, row, (int)a.c, top, bound, walk);
+    }
     __syncwarp();
     if (go)
         for (int j = lane; j < top; j += L) {
@@ -1398,10 +1451,13 @@ void rows_launch(int device, const T* x, int64_t ld, const Args<A>& a, cudaStrea
         allow_smem(k, device, bytes, asked, "row shared memory");
         k<<<(unsigned)ceil_div(a.n, kNT / L), kNT, bytes, s>>>(x, ld, a);
     };
-    // several rows a warp where that leaves enough lanes for the bound
-    if (nv <= 16 && a.top <= 5)
+    // Several rows a warp where their lanes are enough for the bound, or the values few enough to
+    // be ranked without one. bfloat16 by 8, 16 and 32 lanes a row: 400000 x 100, 10 best 162, 238,
+    // 428 us; 16 best 489, 285, 465; 24 best 795 by 16, 640 by 32; 400000 x 40, 16 best 213, 350, 580;
+    // 200000 x 250, 24 best 199 by 16, 228 by 32, 28 best 311 and 254.
+    if (nv <= 16 && (a.top <= 10 || a.c <= 64))
         held(integral_constant<int, 8>{}, integral_constant<int, 2>{});
-    else if (nv <= 32 && a.top <= 8)
+    else if (nv <= 32 && (a.top <= min(24, 2 * fewest_vectors<Pack<T>::N>(a.c)) || a.c <= 64))
         held(integral_constant<int, 16>{}, integral_constant<int, 2>{});
     else if (nv <= 32)
         held(integral_constant<int, 32>{}, integral_constant<int, 1>{});

@@ -235,6 +235,41 @@ def test_best_classes_in_the_hands_of_few_lanes(c, kind, share):
         _check(x, y, top)
 
 
+@pytest.mark.parametrize("c", [33, 39, 64, 65, 100, 127, 128, 135, 200, 256, 263])
+@pytest.mark.parametrize("kind", list(TYPES))
+def test_short_rows_of_every_kind_beside_each_other(c, kind):
+    """Several rows share a warp, each in a way of its own: plain, with ties, all equal, with few
+    classes or none left, masked by their label, with signed zeros; at every place within 16 bytes."""
+    g = torch.Generator().manual_seed(c)
+    x = torch.randn(96, c, generator=g) * 2.5
+    for i in range(0, 96, 2):  # neighbours differ
+        what = i // 2 % 8
+        if what == 0:
+            x[i] = x[i].round()
+        elif what == 1:
+            x[i] = float(x[i, 0])
+        elif what == 2:
+            x[i, torch.randperm(c, generator=g)[3:]] = -math.inf
+        elif what == 3:
+            x[i] = -math.inf
+        elif what == 4:
+            x[i, ::2] = -math.inf
+        elif what == 5:
+            x[i] = torch.where(x[i] > 1.5, x[i], torch.where(x[i] > 0, 0.0, -0.0))
+        elif what == 6:
+            x[i] = torch.finfo(torch.float16).min
+        else:
+            x[i, :8] += 20
+    y = torch.randint(0, c, (96,), generator=g)
+    y[5::17] = -100
+    pitch = c + 1
+    flat = torch.full((96 * pitch,), 99.0, dtype=TYPES[kind], device="cuda")
+    rows = flat.as_strided((96, c), (pitch, 1))
+    rows.copy_(x.to(TYPES[kind]))
+    for top in (1, 4, 5, 8, 9, 10, 11, 16, 17, 20, 24, 25, 32):
+        _check(rows, y.cuda(), top)
+
+
 @pytest.mark.parametrize("c", [10, 32, 100, 1000, 5003, 50001])
 @pytest.mark.parametrize("kind", list(TYPES))
 def test_not_finite(c, kind):
