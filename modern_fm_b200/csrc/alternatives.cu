@@ -14,7 +14,7 @@
 // (reductions, logarithm, the order of its best) costs its warp some 500 instructions. Rows are
 // worked on in three ways:
 //  * up to kSmallC classes: a thread per row (small_kernel, small_grad_kernel);
-//  * rows of up to 256 vectors of 16 bytes: 8 to 32 lanes hold the row in registers
+//  * rows of up to 256 vectors of 16 bytes: 4 to 32 lanes hold the row in registers
 //    (held_kernel);
 //  * longer ones: 32 to 256 threads scan the row with a running maximum, eight blocks of a
 //    cluster where rows are few (scan_kernel); the gradient is elementwise (grad_kernel).
@@ -36,6 +36,7 @@ constexpr int kSmallC = 32;    // classes that a thread takes by itself
 constexpr int kSmallNT = 128;
 constexpr int kMany = 64;      // candidates that a few lanes rank
 constexpr int kTop = 32;       // the most classes that are listed
+constexpr int kFew = 9;        // candidates a lane of a group within a warp
 constexpr int kCand = 288;     // candidates of a row: the vectors of kTop threads (256 values) and the row's edges
 
 // x - off where its exponential is not 0, or so low that it is: 0 times it stays 0. (The
@@ -700,7 +701,7 @@ __device__ __noinline__ void one_by_one(const T* row, int c, int top, KT* parts,
             if ((place == 0 || last.before(o)) && o.before(best)) best = o;
         }
 #pragma unroll
-        for (int s = 16; s > 0; s >>= 1) {
+        for (int s = min(L, 32) / 2; s > 0; s >>= 1) {
             const KT o = best.across(s);
             if (o.before(best)) best = o;
         }
@@ -792,19 +793,16 @@ __device__ __forceinline__ bool finish(const Args<A>& a, int64_t t, A xy, const 
     return true;
 }
 
-// Rows of up to L K vectors: L lanes each, the row in their registers. Bound by issue slots, 600
-// instructions a row of 1000 values and 400 to 700 more for its 5 or 16 best: 200000 x 1003 float16
-// 132, 207, 260 us without, with 5 and with 16 (401 MB: 61 us). The row behind one prefetched by
-// persistent warps: 148, 235, 296 us, for a block an SM less. Several rows a warp share what a row
-// costs: 400000 x 100 bf16 54 us with eight lanes a row, 101 with sixteen.
-template <class A, int V, int L, int K>
-constexpr int held_cand() { return L * K * V + 2 * (V - 1) < kCand ? L * K * V + 2 * (V - 1) : kCand; }
-
+// Rows of up to L K vectors: L lanes each, the row in their registers. Bound by issue slots, most of
+// them what a row costs its warp once: 200000 x 1003 float16 131, 208, 258 us without, with 5 and
+// with 16 best by a warp a row, 107, 172, 229 by half a warp (401 MB: 61 us). The row behind one
+// prefetched by persistent warps: 148, 235, 296 us instead of 131, 208, 258, for a block an SM less.
 template <class T, class A, int L, int K>
 __global__ void __launch_bounds__(kNT, IsF64<A>::value ? 2 : K > 4 ? 3 : 4)
     held_kernel(const T* __restrict__ x, int64_t ld, Args<A> a) {
-    constexpr int V = 16 / sizeof(T), E = (2 * (V - 1) + L - 1) / L, CAP = held_cand<A, V, L, K>();
-    static_assert(L == 32 || CAP < kCand, "groups within a warp hold every value as a candidate");
+    constexpr int V = 16 / sizeof(T), E = (2 * (V - 1) + L - 1) / L;
+    constexpr int ALL = L * K * V + 2 * (V - 1), CAP = ALL < kFew * L ? ALL : kFew * L;  // values, candidates
+    static_assert(kFew * 32 == kCand, "a warp's list is that of the longer rows");
     static_assert(K * V <= 64, "a bit a value");
     using KT = std::conditional_t<sizeof(T) == 2, ShortKey<T>, Key<A>>;
     __shared__ Lists<KT, CAP> shared[kNT / L];
@@ -887,13 +885,8 @@ __global__ void __launch_bounds__(kNT, IsF64<A>::value ? 2 : K > 4 ? 3 : 4)
                 else
                     second = fmax(second, Pack<T>::top(v[i]));
             } else {
-                A p[V];
-                Pack<T>::unpack(v[i], p);
-#pragma unroll
-                for (int q = 0; q < V / 2; ++q) {
-                    first = fmax(first, p[q]);
-                    second = fmax(second, p[V / 2 + q]);
-                }
+                first = fmax(first, Pack<T>::top(make_uint4(v[i].x, v[i].y, v[i].x, v[i].y)));
+                second = fmax(second, Pack<T>::top(make_uint4(v[i].z, v[i].w, v[i].z, v[i].w)));
             }
         }
 #pragma unroll
@@ -936,27 +929,35 @@ __global__ void __launch_bounds__(kNT, IsF64<A>::value ? 2 : K > 4 ? 3 : 4)
         __syncwarp();
         return count;
     };
-    if constexpr (CAP < kCand) {
-        // Every value fits. Where many reach the bound (ties), and where it is -infinity, those
-        // above it are listed, and the first of its equals.
+    if constexpr (L < 32 || CAP == ALL) {
+        // Where many reach the bound (ties), and where it is -infinity, those above it are listed,
+        // and the first of its equals; where these do not fit, one is found at a time.
         const A equal = bound;
         bool over = bound == minus_inf<A>();
         if (over) bound = above<T>(bound);
         int count = walk(std::false_type{});
-        const bool many = !over && count > kMany;
+        const bool many = !over && count > min(kMany, CAP);
         if (__any_sync(0xffffffffu, many)) {
             if (many) bound = above<T>(bound);
             over |= many;
             count = walk(std::false_type{});
         }
-        places<L>(g, count, top);
+        places<L>(g, min(count, CAP), top);
+        if constexpr (CAP < ALL) {
+            const bool beyond = go && count > CAP;
+            if (__any_sync(0xffffffffu, beyond)) {
+                __syncwarp();
+                one_by_one<T, A, L>(row, (int)a.c, top, g.cand, beyond ? g.best : g.cand);
+            }
+        }
         const int more = go && over && count < top ? top - count : 0;
         if (__any_sync(0xffffffffu, more > 0))
             for (int o = 0; o < 32; o += L) {
                 const int want = __shfl_sync(0xffffffffu, more, o), from = __shfl_sync(0xffffffffu, count, o);
                 const A v = __shfl_sync(0xffffffffu, equal, o);
                 const int64_t of = __shfl_sync(0xffffffffu, t, o);
-                if (want > 0) first_equal(x + of * ld, (int)a.c, v, want, shared[threadIdx.x / 32 * (32 / L) + o / L].best + from);
+                if (want > 0)
+                    first_equal(x + of * ld, (int)a.c, v, want, shared[threadIdx.x / 32 * (32 / L) + o / L].best + from);
             }
     } else {
         choose<T, A, L>(g, row, (int)a.c, top, bound, walk);
@@ -1451,14 +1452,29 @@ void rows_launch(int device, const T* x, int64_t ld, const Args<A>& a, cudaStrea
         allow_smem(k, device, bytes, asked, "row shared memory");
         k<<<(unsigned)ceil_div(a.n, kNT / L), kNT, bytes, s>>>(x, ld, a);
     };
-    // Several rows a warp where their lanes are enough for the bound, or the values few enough to
-    // be ranked without one. bfloat16 by 8, 16 and 32 lanes a row: 400000 x 100, 10 best 162, 238,
-    // 428 us; 16 best 489, 285, 465; 24 best 795 by 16, 640 by 32; 400000 x 40, 16 best 213, 350, 580;
-    // 200000 x 250, 24 best 199 by 16, 228 by 32, 28 best 311 and 254.
-    if (nv <= 16 && (a.top <= 10 || a.c <= 64))
+    // As few lanes a row as are enough for the bound, two values each, or for ranking the values of a
+    // short row without one (of double values as few as shared memory has lists for). By lanes, us
+    // without best classes, with 5, 10, 16, 24:
+    //   400000 x 100 bfloat16   4: 38, 92, 379   8: 55, 119, 162, 489   16: 10 best 238, 16 285, 24 795   32: 428, 465, 640
+    //   200000 x 250 bfloat16   8: 38, 74, 95, 475   16: 58, 105, 121, 144, 198   32: 16 best 207, 24 228
+    //   200000 x 500 float16    8: 61, 103, 131   16: 68, 119, 139, 162, 223   32: 111, 180, 207, 225, 248
+    //   200000 x 1003 float16   16: 107, 172, 199, 229, 304   32: 131, 208, 238, 258, 287
+    constexpr int kFour = IsF64<A>::value ? 8 : 4, kEight = IsF64<A>::value ? 16 : 8;
+    const int top = a.top, two = 2 * fewest_vectors<Pack<T>::N>(a.c);
+    if (nv <= 16 && top <= 5)
+        held(integral_constant<int, kFour>{}, integral_constant<int, 16 / kFour>{});
+    else if (nv <= 16 && (top <= 12 || a.c <= 64))
         held(integral_constant<int, 8>{}, integral_constant<int, 2>{});
-    else if (nv <= 32 && (a.top <= min(24, 2 * fewest_vectors<Pack<T>::N>(a.c)) || a.c <= 64))
+    else if (nv <= 32 && top <= 12)
+        held(integral_constant<int, kEight>{}, integral_constant<int, 32 / kEight>{});
+    else if (nv <= 32 && (top <= min(24, two) || a.c <= 64))
         held(integral_constant<int, 16>{}, integral_constant<int, 2>{});
+    else if (nv > 32 && nv <= 64 && top <= 10)
+        held(integral_constant<int, kEight>{}, integral_constant<int, 64 / kEight>{});
+    else if (nv > 32 && nv <= 64 && top <= 24)
+        held(integral_constant<int, 16>{}, integral_constant<int, 4>{});
+    else if (nv > 64 && nv <= 128 && top <= 20)
+        held(integral_constant<int, 16>{}, integral_constant<int, 8>{});
     else if (nv <= 32)
         held(integral_constant<int, 32>{}, integral_constant<int, 1>{});
     else if (nv <= 64)

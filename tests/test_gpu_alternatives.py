@@ -235,6 +235,27 @@ def test_best_classes_in_the_hands_of_few_lanes(c, kind, share):
         _check(x, y, top)
 
 
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("vectors", [16, 30, 62, 125])
+@pytest.mark.parametrize("share,lanes", [(1, 4), (3, 8), (6, 16)])
+def test_best_classes_in_the_hands_of_few_lanes_of_a_group(vectors, kind, share, lanes):
+    """The same of rows that share a warp, beside rows without: what a group lists may run over in
+    some of them, among all values or among those above the ties."""
+    g = torch.Generator().manual_seed(vectors + share)
+    v = 128 // torch.finfo(TYPES[kind]).bits
+    c = vectors * v
+    big = (torch.arange(c) // v) % lanes < share
+    x = torch.where(big, 50.0 + torch.rand(41, c, generator=g) * 8, torch.randn(41, c, generator=g))
+    x[10:20] = x[10:20].round()
+    x[20:24] = torch.where(big, 9.0, 4.0)
+    x[24:28, ~big] = -math.inf
+    x[1::3] = torch.randn(14, c, generator=g)
+    x = x.to(TYPES[kind]).cuda()
+    y = torch.randint(0, c, (41,), generator=g).cuda()
+    for top in (1, 5, 10, 12, 20, 24, 32):
+        _check(x, y, top)
+
+
 @pytest.mark.parametrize("c", [33, 39, 64, 65, 100, 127, 128, 135, 200, 256, 263])
 @pytest.mark.parametrize("kind", list(TYPES))
 def test_short_rows_of_every_kind_beside_each_other(c, kind):
