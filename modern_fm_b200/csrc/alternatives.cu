@@ -1527,9 +1527,12 @@ void grad_launch(int device, const T* x, int64_t ld, T* out, int64_t ld_out, con
         grad_kernel<T, A, L><<<(unsigned)ceil_div(a.n, kNT / L), kNT, 0, s>>>(x, ld, out, ld_out, a);
     };
     const int64_t nv = a.c / Pack<T>::N;
-    // 8, 16, 32, 64 lanes a row, with five best classes: 400000 x 100 bf16 102, 180, 365, 686 us,
-    // 200000 x 1003 158, 174, 248, 407, 100000 x 2000 154, 145, 165, 218
-    if (nv <= 160)
+    // 4, 8, 16, 32, 64 lanes a row, with five best classes: 400000 x 100 bf16 68, 102, 180, 365, 686 us
+    // (160 MB: 24), 200000 x 250 59, 66; 200000 x 500 95, 92, 200000 x 1003 192, 158, 174, 248, 407;
+    // 100000 x 2000 by 8 154, 145, 165, 218
+    if (nv <= 32)
+        go(std::integral_constant<int, 4>{});
+    else if (nv <= 160)
         go(std::integral_constant<int, 8>{});
     else if (nv <= 512)
         go(std::integral_constant<int, 16>{});
